@@ -404,6 +404,117 @@ int wkv_prefill_gqa_shared(const wkv_cache_t *cache, const void *key, int64_t ke
                            int32_t max_query_len, int32_t max_seq_len, float scale, int32_t workgroups,
                            void *workspace, int64_t workspace_bytes, const float *sinks, void *stream);
 
+/* ---- a step of drafted tokens --------------------------------------------
+ * Several drafted tokens per sequence verified in one step (speculative
+ * decoding): a tree of continuations, or one chain. Node i of a sequence's
+ * n_b nodes has a parent among its nodes, parents[..] < i (anything else: the
+ * node follows the cached context directly). The nodes are stored in the cache
+ * in node order behind the context, at positions L .. L + n_b - 1, whatever their
+ * depth; after verification wkv_compact moves the accepted path's together. */
+#define WKV_TREE_MAX_WORDS 4   /* 64-node words of a tree mask: at most 256 nodes per sequence */
+#define WKV_TREE_MAX_DEPTH 64  /* nodes of an accepted path */
+#define WKV_STEP_MAX_BATCH 2048
+
+/* A step's block tables, slots, positions and tree masks from the request
+ * lengths, on the GPU. Sequence b holds held_blocks[b] blocks (the leading
+ * entries of its table row) and seq_lens[b] cached tokens and brings
+ * new_lens[b] tokens; free_blocks[taken .. num_free) are the blocks to give (taken: one int
+ * in device memory). In batch order, each sequence gets the blocks that
+ * its tokens need beyond those it holds, written behind them in its row.
+ * A sequence is refused, and gets nothing, when its blocks pass max_blocks_per_seq,
+ * its rows pass max_tokens, its nodes pass 64 * mask_words, or it needs blocks and
+ * those asked for by it and the sequences before it (refused ones
+ * included) are more than are free: *refused counts them.
+ *   context_lens[b]    seq_lens[b] + new_lens[b]; seq_lens[b] without new tokens;
+ *                      0 for a refused sequence, whose rows then attend to nothing
+ *   cu_seqlens_q[B+1]  sums of new_lens, at most max_tokens
+ *   slot_mapping, positions [max_tokens]   of token j of sequence b in row
+ *                      cu_seqlens_q[b] + j: its slot and its position, seq_lens[b]
+ *                      + j, or with a tree seq_lens[b] + the node's depth; -1 for
+ *                      rows of refused sequences and past the last (and a slot
+ *                      of -1 where the table holds no block)
+ *   tree_mask [max_tokens, mask_words]  mask_words > 0 (a tree; parents
+ *                      [max_tokens]): bit j % 64 of word j / 64 is node j, itself or an ancestor
+ *   held_out [B], taken_out   the state after the step (may be held_blocks and taken)
+ * Negative lengths count as 0. At most WKV_STEP_MAX_BATCH sequences; context_lens
+ * is no input. Replaces the engine's per-step slot mapping and block tables,
+ * made on the host (reached through llm.generate, engine.py:887). */
+int wkv_extend_tables(int32_t *block_table, int64_t bt_stride, int32_t max_blocks_per_seq, const int32_t *held_blocks,
+                      const int32_t *seq_lens, const int32_t *new_lens, int32_t batch, int32_t block_size,
+                      const int32_t *free_blocks, int32_t num_free, const int32_t *taken, int32_t max_tokens,
+                      const int32_t *parents, int32_t mask_words, int32_t *held_out, int32_t *taken_out,
+                      int32_t *context_lens, int32_t *cu_seqlens_q, int64_t *slot_mapping, int64_t *positions,
+                      int64_t *tree_mask, int32_t *refused, void *stream);
+
+/* Rotary positions over q [num_tokens, num_q_heads, head_dim] and k [num_tokens,
+ * num_k_heads, head_dim] (either may have no heads): pair i of every head is
+ * turned by the angle t = positions[token] * inv_freq[i] (float64; any sign),
+ *   y_a = scale (x_a cos t - x_b sin t),  y_b = scale (x_b cos t + x_a sin t),
+ * pair i being dims (2 i, 2 i + 1) if interleaved, else (i, i + rotary_dim / 2);
+ * dims from rotary_dim on are copied. inverse: t negated, the transpose (the gradient of
+ * the forward call). dtype 0 = fp32, 1 = bf16, 2 = fp16; the last dim
+ * contiguous, strides in elements; an output is its input (in place) or does not overlap it.
+ * Computed in float32 from angles reduced in float64. Replaces the engine's rotary
+ * embedding, which the reference patches for one model
+ * (wavelet/inference/deepseek_v4.py:15-126). */
+#define WKV_ROTARY_MAX_DIM 512
+int wkv_rotary(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_stride_h, void *q_out, int64_t qo_stride_t,
+               int64_t qo_stride_h, int32_t num_q_heads, const void *k, int64_t k_stride_t, int64_t k_stride_h,
+               void *k_out, int64_t ko_stride_t, int64_t ko_stride_h, int32_t num_k_heads, int32_t head_dim,
+               const int64_t *positions, const double *inv_freq, int32_t rotary_dim, int32_t interleaved,
+               int32_t inverse, float scale, int64_t num_tokens, void *stream);
+
+/* Attention of drafted tokens over the paged cache: wkv_prefill_gqa with a mask
+ * in the place of the causal one. Row j of sequence b's n_b = cu_seqlens_q[b+1] -
+ * cu_seqlens_q[b] new tokens attends to the seq_lens[b] - n_b cached tokens
+ * before them, and to new token i where bit i of its tree_mask row ([num rows, mask_words]
+ * int64) is set; a row that sees nothing gives zeros. Keys of a table
+ * entry outside the cache are seen by no row. key / value / slot_mapping, q, out,
+ * sinks (NULL = none) and the table arguments as for wkv_prefill_gqa; num_tokens
+ * rows are appended. At most 64 * mask_words new tokens per sequence are seen.
+ * A non-finite value at a key that a row does not see leaves the row as it is.
+ * workspace: wkv_tree_workspace_size() bytes for the same geometry, max_seq_len clipped
+ * to the block-table width; without one (NULL) a sequence's keys are not cut over workgroups.
+ * No counterpart in the reference, whose engine verifies drafted tokens inside
+ * llm.generate (engine.py:887). */
+int64_t wkv_tree_workspace_size(int32_t batch, int32_t kv_dtype, int32_t num_kv_heads, int32_t num_q_heads,
+                                int32_t head_dim, int32_t max_query_len, int32_t max_seq_len);
+
+int wkv_tree_gqa(const wkv_cache_t *cache, const void *key, int64_t key_stride_t, int64_t key_stride_h,
+                 const void *value, int64_t value_stride_t, int64_t value_stride_h, const int64_t *slot_mapping,
+                 int64_t num_tokens, const void *q, int64_t q_stride_t, int64_t q_stride_h, void *out,
+                 int64_t out_stride_t, int64_t out_stride_h, int32_t num_q_heads, const int32_t *cu_seqlens_q,
+                 const int32_t *seq_lens, const int32_t *block_table, int64_t bt_stride, int32_t max_blocks_per_seq,
+                 int32_t batch, int32_t max_query_len, int32_t max_seq_len, const int64_t *tree_mask,
+                 int32_t mask_words, float scale, void *workspace, int64_t workspace_bytes, const float *sinks,
+                 void *stream);
+
+/* The accepted path of a verified tree. draft_tokens, parents and target_tokens
+ * [num rows]: a node's own token, its parent, and the token that the model sampled after
+ * it. Node 0 (the token of the step before, always right) is accepted; from an
+ * accepted node the path goes on to its first child whose token is the
+ * one sampled after it, up to max_depth nodes. path [B, max_depth]: the accepted nodes,
+ * then -1; accepted [B] their number; next_tokens [B] the token sampled
+ * after the last; seq_lens_out[b] = seq_lens[b] + accepted[b] (may be seq_lens).
+ * A sequence without rows, or refused (context_lens[b] <= 0), accepts nothing (next -1). A
+ * sequence's first 256 nodes count. No counterpart in the reference (inside llm.generate). */
+int wkv_accept_tree(const int64_t *draft_tokens, const int32_t *parents, const int64_t *target_tokens,
+                    const int32_t *cu_seqlens_q, const int32_t *seq_lens, const int32_t *context_lens, int32_t batch,
+                    int32_t max_depth, int32_t *accepted, int32_t *path, int64_t *next_tokens, int32_t *seq_lens_out,
+                    void *stream);
+
+/* Moves an accepted path's keys and values together, in place: for j <
+ * accepted[b] the token at position seq_lens[b] + path[b, j] of sequence b goes to position seq_lens[b]
+ * + j (seq_lens: the lengths before the step). All are read before any is
+ * written. path [B, path_len] rises from path[b, j] >= j; tokens that keep their place
+ * are not touched. fp8: the moved tokens' exact values are appended as
+ * wkv_append_fp8 codes them (a block begun at its first slot starts afresh).
+ * Positions without a block move nothing. Blocks that are written must belong to one
+ * sequence. No counterpart in the reference (inside llm.generate). */
+int wkv_compact(const wkv_cache_t *cache, const int32_t *block_table, int64_t bt_stride, int32_t max_blocks_per_seq,
+                const int32_t *seq_lens, const int32_t *path, int32_t path_len, const int32_t *accepted, int32_t batch,
+                void *stream);
+
 /* Token sampler: the step after decode, producing what the engine records per
  * generated token -- the token, its processed logprob and the sampling mask
  * (llm.generate with logprobs_mode="processed_logprobs" and

@@ -16,6 +16,12 @@ Public surface (a drop-in for the KV path of the reference's inference engine):
   sharing for GRPO groups;
 * ``KVPool`` -- all layers' caches plus the block manager, with the engine's
   sleep / wake_up lifecycle and KV metrics;
+* ``paged_tree_gqa`` -- attention of a tree of drafted tokens over the cache,
+  and around it: ``extend_tables`` (a step's blocks, slots, positions and tree
+  masks on the GPU), ``accept_tree`` (the path that the sampled tokens
+  agree with) and ``PagedKVCache.compact`` (its keys and values moved together);
+* ``apply_rotary`` / ``rotary_frequencies`` -- rotary positions of queries and
+  keys, with gradients;
 * ``sample`` -- the token sampler after decode (temperature, min_p, top_k,
   top_p, repetition penalty; processed logprobs and the sampling mask).
 
@@ -27,24 +33,33 @@ a ``KVPool`` and the ``"wavelet_paged"`` attention implementation.
 """
 
 from .attention import (decode_order, decode_plan, grouped_decode_order, paged_decode_gqa, paged_decode_gqa_grouped,
-                        paged_decode_mla, prefill_gqa)
+                        paged_decode_mla, paged_tree_gqa, prefill_gqa)
 from .blocks import BlockManager
 from .cache import MLALatentCache, PagedKVCache, validate_group_prefix, validate_tables
 from .pool import KVPool
+from .rotary import apply_rotary, rotary_frequencies
 from .sampler import sample
+from .step import Accepted, StepMaps, accept_tree, extend_tables
 
 __all__ = [
+    "Accepted",
     "BlockManager",
     "KVPool",
     "MLALatentCache",
     "PagedKVCache",
+    "StepMaps",
+    "accept_tree",
+    "apply_rotary",
     "decode_order",
     "grouped_decode_order",
     "decode_plan",
+    "extend_tables",
     "paged_decode_gqa",
     "paged_decode_gqa_grouped",
     "paged_decode_mla",
+    "paged_tree_gqa",
     "prefill_gqa",
+    "rotary_frequencies",
     "sample",
     "validate_group_prefix",
     "validate_tables",

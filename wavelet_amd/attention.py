@@ -16,7 +16,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .cache import KV_DTYPES, MLALatentCache, PagedKVCache, _require_cuda, _slots, _stream, _token_rows, check_tables
+from .cache import KV_DTYPES, MLALatentCache, PagedKVCache, _on, _require_cuda, _slots, _stream, _token_rows, check_tables
 
 _workspaces: dict[tuple[int, int], torch.Tensor] = {}
 
@@ -396,6 +396,93 @@ def prefill_gqa(
     else:
         rc = lib.wkv_prefill_gqa(*args, _stream(dev))
     _lib.check(rc, "prefill_gqa")
+    return out
+
+
+def paged_tree_gqa(
+    q: torch.Tensor,
+    cache: PagedKVCache,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    tree_mask: torch.Tensor,
+    scale: float,
+    *,
+    key: torch.Tensor | None = None,
+    value: torch.Tensor | None = None,
+    slot_mapping: torch.Tensor | None = None,
+    max_query_len: int | None = None,
+    max_seq_len: int | None = None,
+    out: torch.Tensor | None = None,
+    sinks: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of drafted tokens over the cache: ``q [T, Hq, D]`` bf16 -> ``[T, Hq, D]`` bf16.
+
+    ``prefill_gqa`` with a mask in the place of the causal one: of sequence ``b``'s ``seq_lens[b]`` tokens
+    the last ``n_b = cu_seqlens_q[b+1] - cu_seqlens_q[b]`` are drafted (rows of ``q``; at most ``64 W``); row
+    ``j`` attends to every token before them, and to drafted token ``i`` where bit ``i % 64`` of ``tree_mask[row, i // 64]``
+    (int64 ``[T, W]``, ``W`` up to 4) is set -- its own and its ancestors', as ``extend_tables``
+    makes them; any other mask does. A row that sees nothing gives zeros. ``key`` / ``value`` / ``slot_mapping``
+    (appended first), ``max_query_len``, ``max_seq_len``, ``out`` and ``sinks`` as for ``prefill_gqa``.
+    A row's last bits may depend on the other sequences of the call.
+    """
+    if not isinstance(cache, PagedKVCache):
+        raise ValueError("cache must be a PagedKVCache")
+    dev = cache.device
+    block_table, seq_lens = check_tables(block_table, seq_lens, dev, cache.block_size)
+    batch = seq_lens.shape[0]
+    _require_cuda(cu_seqlens_q, "cu_seqlens_q", dev)
+    if cu_seqlens_q.dtype != torch.int32 or cu_seqlens_q.dim() != 1 or cu_seqlens_q.shape[0] != batch + 1:
+        raise ValueError(f"cu_seqlens_q must be int32 [{batch + 1}]")
+    cu_seqlens_q = cu_seqlens_q.contiguous()
+    if q.dim() != 3:
+        raise ValueError("q must be [T, Hq, D]")
+    tokens, hq = q.shape[0], q.shape[1]
+    q = _query(q, "q", (hq, cache.head_dim), dev)
+    _require_cuda(tree_mask, "tree_mask", dev)
+    if tree_mask.dtype != torch.int64 or tree_mask.dim() != 2 or tree_mask.shape[0] != tokens \
+            or not 1 <= tree_mask.shape[1] <= 4:
+        raise ValueError(f"tree_mask must be int64 [{tokens}, 1 to 4] (got {tree_mask.dtype} {tuple(tree_mask.shape)})")
+    tree_mask = tree_mask.contiguous()
+    append = key is not None or value is not None or slot_mapping is not None
+    if append:
+        if key is None or value is None or slot_mapping is None:
+            raise ValueError("appending needs key, value and slot_mapping together")
+        shape = (cache.num_kv_heads, cache.head_dim)
+        key = _token_rows(key, "key", shape, dev)
+        value = _token_rows(value, "value", shape, dev)
+        if key.shape[0] != tokens or value.shape[0] != tokens:
+            raise ValueError(f"key/value must hold the {tokens} drafted tokens")
+        slot_mapping = _slots(slot_mapping, tokens, dev)
+    if out is None:
+        out = torch.empty((tokens, hq, cache.head_dim), dtype=torch.bfloat16, device=dev)
+    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (tokens, hq, cache.head_dim) or out.stride(2) != 1 \
+            or out.device != dev:
+        raise ValueError(f"out must be a bfloat16 [T, Hq, D] tensor on {dev} with a contiguous last dim")
+    sinks = _sinks(sinks, hq, dev)
+    if tokens == 0 or batch == 0:
+        return out
+    if max_query_len is None:
+        max_query_len = int((cu_seqlens_q[1:] - cu_seqlens_q[:-1]).max().item())
+    msl = min(_max_len(seq_lens, max_seq_len), block_table.shape[1] * cache.block_size)
+    lib = _lib.load()
+    need = lib.wkv_tree_workspace_size(batch, KV_DTYPES[cache.kv_dtype], cache.num_kv_heads, hq, cache.head_dim,
+                                       int(max_query_len), msl)
+    # partials of contexts cut over workgroups: from the caching allocator on the call's own stream
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    if append:
+        head = (key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0), value.stride(1),
+                slot_mapping.data_ptr(), tokens)
+    else:
+        head = (None, 0, 0, None, 0, 0, None, 0)
+    with _on(dev):
+        rc = lib.wkv_tree_gqa(
+            ctypes.byref(cache.descriptor()), *head, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0),
+            out.stride(1), hq, cu_seqlens_q.data_ptr(), seq_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+            block_table.shape[1], batch, int(max_query_len), msl, tree_mask.data_ptr(), tree_mask.shape[1], float(scale),
+            ws.data_ptr() if ws is not None else None, need if ws is not None else 0,
+            sinks.data_ptr() if sinks is not None else None, _stream(dev))
+    _lib.check(rc, "paged_tree_gqa")
     return out
 
 

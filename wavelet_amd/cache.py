@@ -21,6 +21,7 @@ layout-independent contract.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -32,6 +33,16 @@ KV_DTYPES = {"bf16": _lib.WKV_KV_BF16, "fp8_e4m3": _lib.WKV_KV_FP8_E4M3}
 
 def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """The device made current for a launch (a launch goes to the current one); nothing where it is already."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
 
 
 def _require_cuda(t: torch.Tensor, name: str, device: torch.device) -> None:
@@ -230,6 +241,31 @@ class PagedKVCache:
         m = block_mapping.contiguous()
         rc = _lib.load().wkv_copy_blocks(ctypes.byref(self.descriptor()), m.data_ptr(), m.shape[0], _stream(self.device))
         _lib.check(rc, "copy_blocks")
+
+    def compact(self, block_table: torch.Tensor, seq_lens: torch.Tensor, path: torch.Tensor,
+                accepted: torch.Tensor) -> None:
+        """Move an accepted path's tokens together: of sequence ``b``, position ``seq_lens[b] + path[b, j]`` to
+        ``seq_lens[b] + j`` for ``j < accepted[b]``, in place, K and V.
+
+        ``seq_lens`` int32 ``[B]`` are the lengths before the step; ``path [B, P]`` int32 (``P`` up to 64) and
+        ``accepted [B]`` int32 come from ``accept_tree``: a rising path, ``path[b, j] >= j``. Tokens that keep
+        their place are not touched; fp8 caches encode the others again as ``append`` does. The written
+        blocks must be the sequence's own (``BlockManager`` copies shared ones before a step writes them).
+        """
+        block_table, seq_lens = check_tables(block_table, seq_lens, self.device, self.block_size)
+        batch = seq_lens.shape[0]
+        _require_cuda(path, "path", self.device)
+        _require_cuda(accepted, "accepted", self.device)
+        if path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != batch or not 1 <= path.shape[1] <= 64:
+            raise ValueError(f"path must be int32 [{batch}, 1 to 64] (got {path.dtype} {tuple(path.shape)})")
+        if accepted.dtype != torch.int32 or tuple(accepted.shape) != (batch,):
+            raise ValueError(f"accepted must be int32 [{batch}] (got {accepted.dtype} {tuple(accepted.shape)})")
+        path, accepted = path.contiguous(), accepted.contiguous()
+        with _on(self.device):
+            rc = _lib.load().wkv_compact(ctypes.byref(self.descriptor()), block_table.data_ptr(), block_table.stride(0),
+                                         block_table.shape[1], seq_lens.data_ptr(), path.data_ptr(), path.shape[1],
+                                         accepted.data_ptr(), batch, _stream(self.device))
+        _lib.check(rc, "compact")
 
 
 class MLALatentCache:

@@ -152,24 +152,6 @@ struct LdsTile {
 // bf16) after the wait and before the barrier of the step: its V tile of
 // step s and its K tile of step s + 1. The attention arithmetic is the bf16
 // one. LDS: 64 KB bf16 plus 8 + 8 KB staging at d=128.
-// Division of a non-negative int by a divisor known on the host, in a handful
-// of scalar instructions (a runtime division takes some 40 vector ones, and
-// half a dozen of them stood in a row before a workgroup's first load: a
-// 60-token prompt's launch 8.5 us, 8.0 without them). m = min(floor(2^32 / d), 2^32 - 1) gives a quotient at
-// most one too small for every x below 2^31.
-struct FastDiv {
-  uint32_t m;
-  int d;
-};
-
-static FastDiv fast_div(int d) {
-  return FastDiv{d == 1 ? 0xffffffffu : static_cast<uint32_t>((1ull << 32) / static_cast<uint32_t>(d)), d};
-}
-
-__device__ __forceinline__ int operator/(int x, const FastDiv &f) {
-  const int q = static_cast<int>(__umulhi(static_cast<uint32_t>(x), f.m));
-  return q + (x - q * f.d >= f.d ? 1 : 0);
-}
 
 // How a launch covers its work (prefill_grid, on the host).
 struct PrefillGrid {
@@ -337,14 +319,6 @@ __device__ __forceinline__ const PrefillArgs &prefill_args() {
   auto p = __builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(p));
   return *(const PrefillArgs *)(p);
-}
-
-// A float at an address that every lane shares, by a scalar load: the compiler
-// takes the pointers of the argument struct as writable in the key loop, and a
-// vector load there counts with the copies in flight and waits for them (a
-// 512-token fp8 prompt at 32/8 heads 23.2 us so, 21.8 with scalar loads).
-__device__ __forceinline__ float load_scalar(const float *p) {
-  return *reinterpret_cast<const __attribute__((address_space(4))) float *>(reinterpret_cast<uintptr_t>(p));
 }
 
 // SHARED: workgroups share the launch's steps evenly (PrefillGrid::W), else one per unit group.
