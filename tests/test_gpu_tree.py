@@ -150,6 +150,41 @@ def test_wide_trees_and_long_contexts(cuda, kv, d):
 
 
 @pytest.mark.parametrize("kv", ["bf16", "fp8_e4m3"])
+@pytest.mark.parametrize("batch,longest", [(300, 700), (40, 2000), (3, 9000), (1, 600), (1, 4200)])
+def test_lines_of_steps(cuda, kv, batch, longest):
+    """The steps of all sequences shared between the workgroups: several sequences to a workgroup, several
+    workgroups to a sequence, sequences without tokens and without drafts among them."""
+    rng = np.random.default_rng(batch + longest)
+    ctx, new = rng.integers(0, longest // 3, batch), rng.integers(0, 12, batch)
+    ctx[rng.integers(0, batch)], new[rng.integers(0, batch)] = longest, 64
+    new[new.sum() == 0] = 3
+    c = Case(cuda, f"line{kv}{batch}{longest}", 8, 4, 128, 16, ctx, new, kv)
+    c.run("line")
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8_e4m3"])
+def test_parts_of_which_a_row_sees_nothing_or_nan(cuda, kv):
+    """Workgroups whose whole share of a context lies in blocks outside the cache, and ones where every key is NaN."""
+    c = Case(cuda, f"parts{kv}", 4, 2, 128, 16, [3000, 3000, 3000], [20, 20, 20], kv)
+    c._append(c.kn, c.vn, c.slots)
+    nan = c.w.block_tables[1, 40:180]
+    if kv == "bf16":
+        c.k[nan] = 0x7FC0
+    else:
+        c.k[nan] = 0x7F
+    c.upload()
+    bt = c.w.block_tables.copy()
+    bt[0, 3:150] = -1
+    bt[2, 60:] = c.w.num_blocks  # the drafted tokens' too
+    q, cache, _, sl, cu, mask, scale = c.args()
+    out = paged.bf16_to_f32(bits_of(paged_tree_gqa(q, cache, c.dev(bt), sl, cu, mask, scale)))
+    ref = c.ref(block_table=bt)
+    assert np.isnan(ref[20:40]).all() and np.isnan(out[20:40]).all()
+    check_attention(out[:20], ref[:20], "context without blocks")
+    check_attention(out[40:], ref[40:], "drafts without blocks")
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8_e4m3"])
 def test_chain_is_the_prefill(cuda, kv):
     c = Case(cuda, f"chain{kv}", 16, 8, 128, 16, [100, 0, 1500], [7, 40, 64], kv)
     c.mask = np.concatenate([tree.masks(np.arange(-1, n - 1), 1) for n in c.new])

@@ -7,34 +7,45 @@
 //
 // Work: the rows of one (sequence, KV head), node by node with the G heads of a
 // node together, are taken 32 at a time by a wave (a unit: the columns of its
-// 32x32x16 MFMAs), four units to a workgroup, so that up to 128 rows share one
-// read of the keys. 64-key steps are copied to LDS by LDS-DMA, a 16-key tile
-// by each wave, NS steps in flight; a wave without rows only copies. Long
-// contexts are cut into chunks of whole steps over workgroups (each sequence's
-// steps spread evenly over its chunks), whose fp32 partials a second kernel
-// merges by log-sum-exp.
-// Bound by reading K and V once: at 128 rows a step's 64 MFMAs of a SIMD pair
-// take as long as its 32 KB at the chip's read rate, below that the memory is
-// what lasts.
+// 32x32x16 MFMAs), four units to a workgroup (a row group), so that up to 128
+// rows share one read of the keys. Keys go in steps of 64, copied to LDS by
+// LDS-DMA, a 16-key tile by each wave; a wave without rows only copies. The
+// steps of all row groups form one line that the workgroups share evenly
+// (tree_prefix), whatever the mix of lengths; a row group cut between workgroups
+// leaves fp32 partials that a second kernel merges by log-sum-exp.
 //
-// fp8 caches stay in their codes in LDS; a wave widens its operands as it reads
-// them (exact) and applies the power-of-two scales to the scores (K) and the
-// probabilities (V).
+// Bound by reading K and V once for up to 64 rows of bf16, by the MFMAs past that and in
+// fp8. Measured with the append of the drafted tokens, 32 query and 8 KV heads of 128:
+// 64 sequences of 2,000 tokens with 8 drafted each, bf16, 186 us (5.9 TB/s; a chunk of each
+// sequence per workgroup, with cached reads: 206); 5 sequences of 700 to 15,000 tokens
+// with 40 to 64 drafted, fp8, 70 us (386 TFLOP/s; chunks: 172); 4 of 8,192 with 128 drafted
+// 110 us in bf16 and 102 in fp8 (630 and 676 TFLOP/s; chunks: 109 and 107). What a step
+// costs beside its MFMAs is mostly the issue of its copies (1 KB per instruction).
 //
-// Masked keys: scores are -inf after scaling (a step's window of the row's mask
-// as 64 bits), so that neither the scale's sign nor a NaN key matters. A masked
+// Software pipeline, one barrier per step: while a wave finishes step s
+// (probabilities, PV products) it scores step s + 1, so that the matrix unit
+// and the VALU work at the same time. At the barrier of step s every wave's V of
+// step s and K of step s + 1 have landed; their slots before (two each) take V of
+// step s + 1 and K of step s + 2. fp8 tiles land as codes in their bf16 tile's place and
+// are widened there, at their block's scale (exact), by the wave that copied them.
+//
+// Masked keys: scores are set to -inf after scaling (a step's window of the row's
+// mask, 64 bits), so that neither the scale's sign nor a NaN key matters. A masked
 // probability is 0, but 0 times a V that is not finite is NaN: in steps that
-// mask anything a tile with such a V is added key by key, to the rows that see the key.
+// mask anything, such a V goes apart, to the rows that see its key.
 #include <cmath>
+#include <type_traits>
 
 #include "gqa_tiles.h"
 #include "lds_dma.h"
 
 namespace wkv {
 
+typedef __attribute__((__vector_size__(2 * sizeof(uint16_t)))) uint16_t u16x2;
+
 constexpr int kTreeWaves = 4;
 constexpr int kTreeRows = 32 * kTreeWaves;  // rows of a workgroup
-constexpr int kTreeCus = 256;
+constexpr int kTreeShare = 512;             // workgroups that share a launch's steps: two per CU
 
 struct TreeArgs {
   const uint8_t *kc, *vc;
@@ -47,108 +58,257 @@ struct TreeArgs {
   int64_t bt_stride;
   const int64_t *mask;
   int words;
-  int Mb, max_seq, Hkv, G, BS, nb;
-  FastDiv by_BS, by_G, by_Hkv, by_chunks;
-  int items;        // (sequence, KV head) x chunks
-  int chunks;       // most chunks of a sequence
-  int chunk_steps;  // most 64-key steps of one
-  int units;        // units per (sequence, KV head) at the longest query
+  int batch, Mb, max_seq, Hkv, G, BS, nb;
+  FastDiv by_BS, by_G;
+  int share;   // workgroups that share the line; 0: one per row group
+  int groups;  // row groups per (sequence, KV head) at the longest query
+  int stream;  // blocks are read by one sequence
   float scale_log2;
   float *part;
   const float *sinks;
 };
 
-// The chunks of a sequence of L tokens: as many as its steps need at chunk_steps
-// each, the steps spread evenly over them.
-struct TreeChunks {
-  int n, per;
-};
-__device__ __forceinline__ TreeChunks tree_chunks(int L, int chunk_steps, int steps) {
-  TreeChunks c;
-  c.n = (steps + chunk_steps - 1) / chunk_steps;
-  c.per = c.n > 0 ? (steps + c.n - 1) / c.n : 0;
-  c.n = __builtin_amdgcn_readfirstlane(c.n);
-  c.per = __builtin_amdgcn_readfirstlane(c.per);
-  return c;
+// The kernel's arguments, read again from the kernel-argument segment (the
+// pointer is opaque to the compiler): held across the loop over row groups they
+// would spill scalar registers into the key loop.
+__device__ __forceinline__ const TreeArgs &tree_args() {
+  auto p = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const TreeArgs *)(p);
 }
 
-// A unit's partial of a chunk: D / 32 x 4 runs of 64 lanes x 4 fp32 (the output
-// accumulators as the lanes hold them), then the 32 rows' reference maxima (log2
-// domain) and sums.
+// A sequence's share of the line, per KV head: `groups` row groups of `steps` steps each
+// (a sequence without keys counts one: its rows are written all the same).
+struct TreeSeq {
+  int qlen, L, steps, groups;
+};
+__device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &a, int b) {
+  TreeSeq s;
+  s.qlen = a.cu_q[b + 1] - a.cu_q[b];
+  s.L = a.seq_lens[b];
+  s.L = s.L < a.max_seq ? s.L : a.max_seq;
+  s.steps = s.L > 0 ? (s.L + 63) >> 6 : 1;
+  s.groups = s.qlen > 0 ? (s.qlen * a.G + kTreeRows - 1) / kTreeRows : 0;
+  return s;
+}
+
+// The line: KV head by KV head, sequence by sequence, row group by row group,
+// step by step. Every workgroup forms its prefix itself: each thread adds up a
+// run of `per` sequences; pfx[t] (LDS) is the sum before thread t's run. Returns the
+// steps of one KV head.
+constexpr int kTreeThreads = 64 * kTreeWaves;
+__device__ __forceinline__ int tree_prefix(const TreeArgs &a, int *pfx, int *red, int per) {
+  int mine = 0;
+  for (int b = threadIdx.x * per; b < a.batch && b < static_cast<int>(threadIdx.x + 1) * per; ++b) {
+    const TreeSeq s = tree_seq(a, b);
+    mine += s.steps * s.groups;
+  }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(incl, o, 64);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 63) red[wave] = incl;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int w = 0; w < kTreeWaves; ++w) {
+    if (w == wave) pfx[threadIdx.x] = total + incl - mine;
+    total += red[w];
+  }
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(total);
+}
+
+// How many workgroups share a line of T steps: all of the grid, two per CU, with
+// at least four steps each. bf16, 32 query and 8 KV heads of 128, us for 512 / 256 /
+// 128 workgroups: eight shares' worth of steps each and more (sequences of 300 to
+// 24,000 tokens) 68 / 85 / 125; 64 sequences of 600 to 2,000 tokens 41 / 46 / 62;
+// one of 4,096 tokens (one step each / two / four) 32.5 / 26.7 / 26.8.
+__device__ __forceinline__ int tree_workgroups(int T) {
+  const int w = (T / 4) & ~7;
+  return w < 8 ? 8 : (w < kTreeShare ? w : kTreeShare);
+}
+
+// T steps over W workgroups: T / W each, one more for the first T % W (W <= T).
+// The host keeps T below 2^31.
+struct TreeShare {
+  int each, more;
+  __device__ __forceinline__ int begin(int w) const { return w * each + (w < more ? w : more); }
+  __device__ __forceinline__ int of(int x) const {  // the workgroup of step x
+    const int y = x - more * (each + 1);
+    return y < 0 ? x / (each + 1) : more + y / each;
+  }
+};
+
+// A unit's partial: D / 32 x 4 runs of 64 lanes x 4 fp32 (the output accumulators
+// as the lanes hold them), then the 32 rows' reference maxima (log2 domain) and
+// sums. Workgroup w owns slots 2 w (the row group that its share begins in) and
+// 2 w + 1 (a later one), four units each. Behind them, per workgroup of the grid, in how many
+// parts the row group is whose first one it left (0: none), and a record of it.
 template <int D>
-constexpr int tree_part_floats() {
+__host__ __device__ constexpr int tree_part_floats() {
   return 32 * D + 64;
 }
-
-template <int D, bool FP8>
-constexpr int tree_steps_in_lds() {
-  return (FP8 ? 1 : 2) * D >= 256 ? 2 : 4;
+struct TreeRec {
+  int slot;  // of the first part
+  int next;  // of the others, two apart: the first slots of the workgroups behind
+  int b, kvh, group;
+  int pad[3];
+};
+template <int D>
+__device__ __forceinline__ int *tree_counts(float *part) {
+  return reinterpret_cast<int *>(part + static_cast<int64_t>(kTreeShare) * 2 * kTreeWaves * tree_part_floats<D>());
+}
+template <int D>
+__device__ __forceinline__ TreeRec *tree_records(float *part) {
+  return reinterpret_cast<TreeRec *>(tree_counts<D>(part) + kTreeShare);
 }
 
-template <int D, bool FP8, int NS>
-__global__ __launch_bounds__(64 * kTreeWaves, 2) void tree_gqa_kernel(TreeArgs a) {
+// Eight e4m3fn codes (bytes of lo, then hi) times a power-of-two scale as
+// eight bf16 values (exact: every such product is a bf16 value).
+__device__ __forceinline__ u32x4 codes_to_bf16(uint32_t lo, uint32_t hi, float sc) {
+  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, sc, false)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, sc, true)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, sc, false)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, sc, true))};
+}
+
+// SHARED: the workgroups share the line; else one row group each.
+template <int D, bool FP8, bool SHARED>
+__global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kernel_args) {
   constexpr int ESZ = FP8 ? 1 : 2;
-  constexpr int TB = D * 16 * ESZ;  // bytes of a 16-key tile's K, and of its V
-  constexpr int NC = TB / 1024;     // 1 KB copies of each
-  constexpr int DV = D / 64;        // bf16 V copies per token octet
-  __shared__ __attribute__((aligned(16))) uint8_t ldsk[NS * 4 * TB];
-  __shared__ __attribute__((aligned(16))) uint8_t ldsv[NS * 4 * TB];
-  __shared__ __attribute__((aligned(16))) int s_ok[NS][4];          // the tile holds keys
-  __shared__ __attribute__((aligned(16))) float s_ks[NS][4], s_vs[NS][4];  // fp8: its block's scales
-  __shared__ uint64_t s_mask[kTreeRows][WKV_TREE_MAX_WORDS];
+  constexpr int TB = D * 16 * 2;         // bytes of a 16-key tile's K, and of its V, as bf16
+  constexpr int NC = D * 16 * ESZ / 1024;  // 1 KB copies of each
+  constexpr int DV = D / 64;             // bf16 V copies per token octet
+  // bf16 tiles as the MFMAs read them: K [D / 8 chunks][16 tokens][16 bytes] as the
+  // cache holds it, V [2 token octets][D rows][8 tokens]. fp8 codes land at their tile's
+  // start: K [D / 16 chunks][16 tokens][16 bytes], V [D rows][16 tokens].
+  __shared__ __attribute__((aligned(16))) uint8_t ldsk[2 * 4 * TB];
+  __shared__ __attribute__((aligned(16))) uint8_t ldsv[2 * 4 * TB];
+  __shared__ __attribute__((aligned(16))) int s_ok[4][4];  // by step: the tile holds keys
+  __shared__ TreeShare s_share;                            // SHARED: how the line is shared, and
+  __shared__ int s_place;                                  // this workgroup's place among those that do
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int lane = threadIdx.x & 63, n = lane & 31, hh = lane >> 5;
-
-  // The row groups of one item stand eight workgroups apart: on one XCD, whose
-  // L2 then serves their keys.
-  const int item = static_cast<int>(blockIdx.y) * 8 + static_cast<int>(blockIdx.x & 7);
-  const int rb = static_cast<int>(blockIdx.x >> 3);
-  if (item >= a.items) return;
-  const int bc = item / a.by_Hkv, kvh = item - bc * a.Hkv;
-  const int b = bc / a.by_chunks, chunk = bc - b * a.chunks;
-  const int q0 = a.cu_q[b], qlen = a.cu_q[b + 1] - q0;
-  int L = a.seq_lens[b];
-  L = L < a.max_seq ? L : a.max_seq;
+  // The lane, for code off the hot path: what is formed from it stays there (hoisted
+  // out of the key loop it would be spilled, and a reload waits for the copies in flight).
+  auto lane_here = [&]() __attribute__((always_inline)) {
+    int l = lane;
+    asm volatile("" : "+v"(l));
+    return l;
+  };
+  const int id = blockIdx.x;
+  int b, kvh, rg, s_begin = 0;
+  bool later = false;  // SHARED: past the share's first row group
+  int steps_left = 0;  // SHARED: of this workgroup's share
+  if constexpr (SHARED) {
+    const TreeArgs &a = tree_args();
+    int *pfx = reinterpret_cast<int *>(ldsk);
+    const int per = (a.batch + kTreeThreads - 1) / kTreeThreads;
+    const int line = tree_prefix(a, pfx, pfx + kTreeThreads, per);
+    const int T = line * a.Hkv;
+    if (threadIdx.x == 0) tree_counts<D>(a.part)[id] = 0;
+    // XCD i mod 8 takes a contiguous eighth of the line, whose workgroups read the same keys.
+    int W = tree_workgroups(T);
+    const int w = (id & 7) * (W / 8) + id / 8;
+    if (id >= W) return;
+    W = T < W ? T : W;
+    if (w >= W) return;
+    TreeShare share;
+    share.each = T / W;
+    share.more = T - share.each * W;
+    int y = share.begin(w);
+    steps_left = share.begin(w + 1) - y;
+    kvh = y / line;
+    y -= kvh * line;
+    int lo = 0, hi = kTreeThreads;  // the last run that begins at or before y (empty runs share their successor's sum)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (pfx[mid] <= y) lo = mid; else hi = mid;
+    }
+    y -= pfx[lo];
+    for (b = lo * per;; ++b) {  // the run holds y
+      const TreeSeq s = tree_seq(a, b);
+      const int c = s.steps * s.groups;
+      if (y < c || b + 1 >= a.batch) {
+        rg = y / s.steps;
+        s_begin = y - rg * s.steps;
+        break;
+      }
+      y -= c;
+    }
+    if (threadIdx.x == 0) {  // (read after the barriers of a row group)
+      s_share = share;
+      s_place = w;
+    }
+  } else {
+    // The row groups of one item stand eight workgroups apart: on one XCD, whose
+    // L2 then serves their keys.
+    const TreeArgs &a = kernel_args;
+    const int oct = id / (8 * a.groups), r = id - oct * 8 * a.groups;
+    rg = r >> 3;
+    const int item = 8 * oct + (r & 7);
+    if (item >= a.batch * a.Hkv) return;
+    b = item / a.Hkv;
+    kvh = item - b * a.Hkv;
+  }
+  for (;;) {  // SHARED: the row groups of the share; else one
+  const TreeArgs &a = tree_args();
+  b = __builtin_amdgcn_readfirstlane(b);
+  kvh = __builtin_amdgcn_readfirstlane(kvh);
+  rg = __builtin_amdgcn_readfirstlane(rg);
+  s_begin = __builtin_amdgcn_readfirstlane(s_begin);
+  const TreeSeq sq = tree_seq(a, b);
+  const int L = __builtin_amdgcn_readfirstlane(sq.L), qlen = __builtin_amdgcn_readfirstlane(sq.qlen);
+  const int all_steps = __builtin_amdgcn_readfirstlane(sq.steps);
+  const int groups = __builtin_amdgcn_readfirstlane(sq.groups);
+  if (rg < groups) {  // else no row: the whole workgroup goes on together
+  int take = all_steps - s_begin;
+  if constexpr (SHARED) {
+    take = __builtin_amdgcn_readfirstlane(steps_left < take ? steps_left : take);
+    __syncthreads();  // the LDS of the row group before (or of the prefix) is free
+  }
+  const bool partial = SHARED && take < all_steps;
+  const int q0 = __builtin_amdgcn_readfirstlane(a.cu_q[b]);
   const int G = a.G;
   const int rows = qlen * G;
-  if (qlen <= 0 || rb * kTreeRows >= rows) return;
-  const int unit = rb * kTreeWaves + wave;
+  const int unit = rg * kTreeWaves + wave;
   const bool active = 32 * unit < rows;  // uniform
-  const int row = 32 * unit + n;
-  const bool has_row = row < rows;
-  const int node = has_row ? row / a.by_G : 0;
-  const int h = kvh * G + (has_row ? row - node * G : 0);
-  uint16_t *const op = a.out + static_cast<int64_t>(q0 + node) * a.o_st + static_cast<int64_t>(h) * a.o_sh;
-  if (L <= 0) {  // nothing to attend to
-    if (chunk == 0 && has_row)
-#pragma unroll
-      for (int d = 0; d < D; d += 8) *reinterpret_cast<u32x2 *>(op + d + 4 * hh) = u32x2{0u, 0u};
-    return;
-  }
-  const int all_steps = (L + 63) >> 6;
-  const TreeChunks tc = tree_chunks(L, a.chunk_steps, all_steps);
-  if (chunk >= tc.n) return;  // the whole workgroup
-  const int s0 = chunk * tc.per;
-  const int s1 = s0 + tc.per < all_steps ? s0 + tc.per : all_steps;
+  // Row 32 unit + i of the sequence: its node and query head (of the last row for those past it).
+  struct Row {
+    int node, h;
+    bool real;
+  };
+  const FastDiv by_G = a.by_G;
+  auto row_of = [&](int i) __attribute__((always_inline)) {
+    Row r;
+    const int row = 32 * unit + i;
+    r.real = row < rows;
+    const int x = r.real ? row : rows - 1;
+    r.node = x / by_G;
+    r.h = kvh * G + x - r.node * G;
+    return r;
+  };
   const int ctx = L - qlen;  // the first drafted token's position
+  const int s0 = s_begin, s1 = L > 0 ? s_begin + take : s_begin;
 
   // Q^T operand j: lane l holds d = 16 j + 8 (l / 32) .. + 7 of row l % 32.
   bf16x8 qb[D / 16];
   {
-    const uint16_t *qp = a.q + static_cast<int64_t>(q0 + node) * a.q_st + static_cast<int64_t>(h) * a.q_sh;
+    const Row r = row_of(n);
+    const uint16_t *qp = a.q + static_cast<int64_t>(q0 + r.node) * a.q_st + static_cast<int64_t>(r.h) * a.q_sh;
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) {
       u32x4 w = *reinterpret_cast<const u32x4 *>(qp + 16 * j + 8 * hh);
-      if (!has_row) w = u32x4{0u, 0u, 0u, 0u};
+      if (!r.real) w = u32x4{0u, 0u, 0u, 0u};
       qb[j] = __builtin_bit_cast(bf16x8, w);
     }
   }
-  if (64 * s1 > ctx && hh == 0) {  // (read by this wave's own lanes)
-    const int64_t *mp = a.mask + static_cast<int64_t>(q0 + node) * a.words;
-#pragma unroll
-    for (int w = 0; w < WKV_TREE_MAX_WORDS; ++w)
-      s_mask[32 * wave + n][w] = has_row && w < a.words ? static_cast<uint64_t>(mp[w]) : 0ull;
-  }
+  const int64_t *const masks = a.mask + static_cast<int64_t>(q0) * a.words;
+  const int words = a.words;
 
   floatx16 o[D / 32];
 #pragma unroll
@@ -160,53 +320,67 @@ __global__ __launch_bounds__(64 * kTreeWaves, 2) void tree_gqa_kernel(TreeArgs a
   // Copies. Piece p = 64 k + l of a tile's K or V goes to LDS offset 16 p. K: chunk p / 16,
   // token p % 16, as the cache holds it. bf16 V: row p % D of token octet p / D;
   // fp8 V: row p.
-  const int BS = a.BS, region = D * BS * ESZ;
-  const uint32_t lane_k = static_cast<uint32_t>(((lane >> 4) * BS + (lane & 15)) * 16);
-  const uint32_t lane_v = static_cast<uint32_t>(lane * BS * ESZ);
+  const int BS = a.BS, region = D * BS * ESZ, Hkv = a.Hkv, nb = a.nb, Mb = a.Mb;
+  const uint8_t *const kc = a.kc, *const vc = a.vc;
+  const float *const ksc = a.ksc, *const vsc = a.vsc;
+  const float scale_log2 = a.scale_log2;
+  const bool stream = a.stream != 0 && groups == 1;  // uniform: nothing reads these keys again
   const uint32_t ldsk0 = lds_addr(ldsk), ldsv0 = lds_addr(ldsv);
   const int32_t *const btrow = a.bt + b * a.bt_stride;
-  const int key_w = 64 * s0 + 16 * wave;
-  int bix = key_w / a.by_BS;
-  int o0 = key_w - bix * BS;
-  const int dbix = 64 / a.by_BS, do0 = 64 - dbix * BS;
-  int wbase = bix;  // the window: lane i holds the id of block wbase + i
-  int win = load_i32_drained(btrow, wbase + lane, a.Mb);
-  uint32_t issued = 0;  // a bit per step, the last one lowest: this wave copied a tile of it
-  auto issue = [&](int s, int slot) {
-    issued <<= 1;
+  const FastDiv by_BS = a.by_BS;
+  int bix = 64 * s0 / by_BS;  // the block of the next step's first key, and its place there
+  int o0 = 64 * s0 - bix * BS;
+  const int dbix = 64 / by_BS, do0 = 64 - dbix * BS;
+  const int n_blocks = (L + BS - 1) / by_BS;
+  // The window: lane i holds the id of block wbase + i. `clean` until a window holds
+  // a block that is none (every wave has the same windows).
+  int wbase = bix, win;
+  bool clean = true;
+  auto open_window = [&]() __attribute__((always_inline)) {
+    wbase = bix;
+    const int l = lane_here();
+    win = load_i32_drained(btrow, wbase + l, Mb);
+    clean = clean && !__any(wbase + l < n_blocks && !(win >= 0 && win < nb));
+  };
+  open_window();
+  int64_t vbase = 0;  // of the wave's tile of the step whose K went out last: its V
+  bool v_ok = false;
+  float ks_next = 1.f, vs_next = 1.f, vs_land = 1.f;  // fp8 scales: last K issued, its V, the V that lands next
+  bool k_land = false, v_land = false;                // fp8: a tile of this wave's to widen
+  // K of the wave's tile of step s into K slot s & 1
+  auto issue_k = [&](int s) __attribute__((always_inline)) {
     bool ok = s < s1 && 64 * s + 16 * wave < L;  // uniform
+    // (the window holds the next step's blocks too, so that `clean` speaks for it a step ahead;
+    // at most once per 56 blocks: its wait drains the copies in flight)
+    if (s < s1 && bix - wbase > 56) open_window();
     if (ok) {
-      if (bix - wbase >= 64) {  // at most once per 64 blocks (its wait drains the copies in flight)
-        wbase = bix;
-        win = load_i32_drained(btrow, wbase + lane, a.Mb);
-      }
-      const int blk = __builtin_amdgcn_readlane(win, bix - wbase);
-      ok = blk >= 0 && blk < a.nb;
+      const int ahead = (o0 + 16 * wave) / by_BS, off = o0 + 16 * wave - ahead * BS;
+      const int blk = __builtin_amdgcn_readlane(win, bix + ahead - wbase);
+      ok = blk >= 0 && blk < nb;
       if (ok) {
-        const int64_t rb_ = static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(blk * a.Hkv + kvh)) *
-                                                 static_cast<uint32_t>(region));
+        const int64_t rb = static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(blk * Hkv + kvh)) *
+                                                static_cast<uint32_t>(region));
+        vbase = rb + off * ESZ;
         if constexpr (FP8) {
-          const float ks = load_scalar(a.ksc + blk * a.Hkv + kvh), vs = load_scalar(a.vsc + blk * a.Hkv + kvh);
-          if (lane == 0) {
-            s_ks[slot][wave] = ks;
-            s_vs[slot][wave] = vs;
-          }
+          ks_next = load_scalar(ksc + blk * Hkv + kvh);
+          vs_next = load_scalar(vsc + blk * Hkv + kvh);
         }
-        uint32_t kst = static_cast<uint32_t>(64 * BS), vst = static_cast<uint32_t>((FP8 ? 64 : 128) * BS);
-        asm volatile("" : "+s"(kst), "+s"(vst));
-        const __amdgpu_buffer_rsrc_t kr =
-            __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(a.kc + rb_ + o0 * 16), 0, region, kRawBufferWord3);
-        const uint32_t tile = static_cast<uint32_t>((4 * slot + wave) * TB);
-        buffer_copy16_run_to_lds<NC>(kr, lane_k, kst - 1024u, ldsk0 + tile);
-        const __amdgpu_buffer_rsrc_t vr =
-            __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(a.vc + rb_ + o0 * ESZ), 0, region, kRawBufferWord3);
-#pragma unroll
-        for (int k = 0; k < NC; ++k)
-          buffer_copy16_to_lds(vr, lane_v, FP8 ? vst * k : vst * (k % DV) + 16 * (k / DV), ldsv0 + tile + 1024 * k);
-        issued |= 1;
+        const int l = lane_here();
+        const uint32_t lane_k = static_cast<uint32_t>(((l >> 4) * BS + (l & 15)) * 16);
+        uint32_t kst = static_cast<uint32_t>(64 * BS);
+        asm volatile("" : "+s"(kst));
+        const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t *>(wave_uniform(kc + rb + off * 16)), 0, region, kRawBufferWord3);
+        const uint32_t dst = __builtin_amdgcn_readfirstlane(ldsk0 + static_cast<uint32_t>((4 * (s & 1) + wave) * TB));
+        if (stream)
+          buffer_copy16_run_to_lds_nt<NC>(kr, lane_k, kst - 1024u, dst);
+        else
+          buffer_copy16_run_to_lds<NC>(kr, lane_k, kst - 1024u, dst);
       }
     }
-    if (lane == 0) s_ok[slot][wave] = ok ? 1 : 0;
+    v_ok = ok;
+    k_land = ok;
+    if (lane == 0) s_ok[s & 3][wave] = ok ? 1 : 0;
     o0 += do0;
     bix += dbix;
     if (o0 >= BS) {
@@ -214,16 +388,70 @@ __global__ __launch_bounds__(64 * kTreeWaves, 2) void tree_gqa_kernel(TreeArgs a
       ++bix;
     }
   };
-  // Until the copies of all but the last NS - 2 steps issued have landed (this wave's).
-  auto wait_step = [&]() {
-    const int later = __builtin_popcount(issued & ((1u << (NS - 2)) - 1u));  // uniform
-    if (NS > 2 && later >= 1) {
-      if (NS > 3 && later >= 2)
-        wait_vmcnt<(NS > 3 ? 4 * NC : 0)>();
-      else
-        wait_vmcnt<(NS > 2 ? 2 * NC : 0)>();
-    } else {
-      wait_vmcnt<0>();
+  // V of the wave's tile of step s (whose K went out last) into V slot s & 1
+  auto issue_v = [&](int s) __attribute__((always_inline)) {
+    v_land = v_ok;
+    if (v_ok) {
+      vs_land = vs_next;
+      const uint32_t lane_v = static_cast<uint32_t>(lane_here() * BS * ESZ);
+      uint32_t vst = static_cast<uint32_t>((FP8 ? 64 : 128) * BS);
+      asm volatile("" : "+s"(vst));
+      const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint8_t *>(wave_uniform(vc + vbase)), 0, region, kRawBufferWord3);
+      const uint32_t dst = __builtin_amdgcn_readfirstlane(ldsv0 + static_cast<uint32_t>((4 * (s & 1) + wave) * TB));
+      auto off = [&](int k) { return FP8 ? vst * k : vst * (k % DV) + 16 * (k / DV); };
+      if (stream) {
+#pragma unroll
+        for (int k = 0; k < NC; ++k) buffer_copy16_to_lds_nt(vr, lane_v, off(k), dst + 1024 * k);
+      } else {
+#pragma unroll
+        for (int k = 0; k < NC; ++k) buffer_copy16_to_lds(vr, lane_v, off(k), dst + 1024 * k);
+      }
+    }
+  };
+  // fp8: this wave's landed codes widened in their place. Piece p = 64 i + l of K: chunk
+  // p / 16 (16 d) of token p % 16 -> bf16 chunks 2 (p / 16), + 1; of V: row p -> octets
+  // 0, 1 of the row. (All of a tile's reads come before its writes: a wave's LDS accesses keep their order.)
+  auto widen = [&](int s, auto do_v, auto do_k) __attribute__((always_inline)) {  // V of step s, K of step s + 1
+    uint8_t *const tv = ldsv + (4 * (s & 1) + wave) * TB;
+    uint8_t *const tk = ldsk + (4 * ((s + 1) & 1) + wave) * TB;
+    u32x4 wv[D / 64], wk[D / 64];
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      if (do_v) wv[i] = *reinterpret_cast<const u32x4 *>(tv + (64 * i + lane) * 16);
+      if (do_k) wk[i] = *reinterpret_cast<const u32x4 *>(tk + (64 * i + lane) * 16);
+    }
+    asm volatile("" ::: "memory");  // (a lane's writes go over what others read)
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      const int p = 64 * i + lane;
+      if (do_v) {
+        *reinterpret_cast<u32x4 *>(tv + p * 16) = codes_to_bf16(wv[i][0], wv[i][1], vs_land);
+        *reinterpret_cast<u32x4 *>(tv + (D + p) * 16) = codes_to_bf16(wv[i][2], wv[i][3], vs_land);
+      }
+      if (do_k) {
+        uint8_t *d = tk + ((2 * (p >> 4)) * 16 + (p & 15)) * 16;
+        *reinterpret_cast<u32x4 *>(d) = codes_to_bf16(wk[i][0], wk[i][1], ks_next);
+        *reinterpret_cast<u32x4 *>(d + 256) = codes_to_bf16(wk[i][2], wk[i][3], ks_next);
+      }
+    }
+  };
+  // V of step s and K of step s + 1 as the products read them. A tile without keys
+  // (past the last, or of no block) is masked; its V is zeros, as 0 times what may stand there is not.
+  auto land = [&](int s) __attribute__((always_inline)) {
+    if (!v_land) {  // uniform
+      const int l = lane_here();
+      u32x4 *t = reinterpret_cast<u32x4 *>(ldsv + (4 * (s & 1) + wave) * TB);
+#pragma unroll
+      for (int i = 0; i < TB / 1024; ++i) t[64 * i + l] = u32x4{0u, 0u, 0u, 0u};
+    }
+    if constexpr (FP8) {
+      if (v_land && k_land) {  // uniform: both tiles' reads ahead of the conversions
+        widen(s, std::true_type{}, std::true_type{});
+      } else {
+        if (v_land) widen(s, std::true_type{}, std::false_type{});
+        if (k_land) widen(s, std::false_type{}, std::true_type{});
+      }
     }
   };
 
@@ -231,103 +459,84 @@ __global__ __launch_bounds__(64 * kTreeWaves, 2) void tree_gqa_kernel(TreeArgs a
   // l is key 16 (r / 8) + 8 (l / 32) + r % 8 of the half: the PV operand as it stands.
   const int kn = (n & 16) | (((n >> 2) & 3) == 1 ? (n & 3) + 8 : ((n >> 2) & 3) == 2 ? (n & 3) + 4 : (n & 15));
   const bf16x2 ones = __builtin_bit_cast(bf16x2, 0x3F803F80u);
+  uint32_t pw[4][4];  // PV operands of the step being finished: packed bf16 probabilities
 
-  // V operand: row 32 c + n, the tokens 8 hh .. + 7 of tile t of a slot, as bf16.
-  auto v_operand = [&](int slot, int t, int c) {
-    const uint8_t *lv = ldsv + (4 * slot + t) * TB;
-    if constexpr (FP8) {
-      const u32x2 w = *reinterpret_cast<const u32x2 *>(lv + (32 * c + n) * 16 + 8 * hh);
-      return __builtin_bit_cast(u32x4, fp8x8_to_bf16x8(w[0], w[1]));
-    } else {
-      return *reinterpret_cast<const u32x4 *>(lv + (hh * D + 32 * c + n) * 16);
-    }
-  };
-  // V of row d, token e of tile t
-  auto v_value = [&](int slot, int t, int d, int e) {
-    const uint8_t *lv = ldsv + (4 * slot + t) * TB;
-    if constexpr (FP8)
-      return __builtin_amdgcn_cvt_f32_fp8(lv[d * 16 + e], 0);
-    else
-      return bf16_bits_to_f32(*reinterpret_cast<const uint16_t *>(lv + ((e >> 3) * D + d) * 16 + 2 * (e & 7)));
-  };
-
-  auto attend = [&](int s, int slot) {
-    const int kb = 64 * s;
-    floatx16 x0, x1;
+  // S^T of step s into (x0, x1)
+  auto qk = [&](int s, floatx16 &x0, floatx16 &x1) __attribute__((always_inline)) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) x0[r] = x1[r] = 0.f;
-    {
-      const uint8_t *lk = ldsk + (4 * slot + (kn >> 4)) * TB + (kn & 15) * 16;
+    const uint8_t *lk = ldsk + ((s & 1) * 4 + (kn >> 4)) * TB + (kn & 15) * 16;
 #pragma unroll
-      for (int j = 0; j < D / 16; ++j) {
-        bf16x8 a0, a1;
-        if constexpr (FP8) {
-          const u32x2 w0 = *reinterpret_cast<const u32x2 *>(lk + j * 256 + 8 * hh);
-          const u32x2 w1 = *reinterpret_cast<const u32x2 *>(lk + 2 * TB + j * 256 + 8 * hh);
-          a0 = fp8x8_to_bf16x8(w0[0], w0[1]);
-          a1 = fp8x8_to_bf16x8(w1[0], w1[1]);
-        } else {
-          a0 = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(lk + (2 * j + hh) * 256));
-          a1 = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(lk + 2 * TB + (2 * j + hh) * 256));
-        }
-        x0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a0, qb[j], x0, 0, 0, 0);
-        x1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1, qb[j], x1, 0, 0, 0);
+    for (int j = 0; j < D / 16; ++j) {
+      const bf16x8 a0 = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(lk + (2 * j + hh) * 256));
+      const bf16x8 a1 = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(lk + 2 * TB + (2 * j + hh) * 256));
+      x0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a0, qb[j], x0, 0, 0, 0);
+      x1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1, qb[j], x1, 0, 0, 0);
+    }
+  };
+  // The tiles of step s that hold keys, a bit each.
+  auto tiles = [&](int s) __attribute__((always_inline)) {
+    const u32x4 w = *reinterpret_cast<const u32x4 *>(s_ok[s & 3]);
+    return __builtin_amdgcn_readfirstlane(w[0] | w[1] << 1 | w[2] << 2 | w[3] << 3);
+  };
+  // The keys of step s that this lane's row sees, a bit each.
+  auto window = [&](int s, uint32_t ok) __attribute__((always_inline)) {
+    const int kb = 64 * s, first = kb - ctx;  // the node of the step's first key
+    uint64_t seen = ~0ull;
+    if (first > -64) {
+      const Row r = row_of(lane_here() & 31);
+      auto word = [&](int i) __attribute__((always_inline)) {
+        return r.real && i < words ? static_cast<uint64_t>(masks[r.node * words + i]) : 0ull;
+      };
+      if (first < 0) {
+        seen = ((1ull << -first) - 1ull) | (word(0) << -first);
+      } else {
+        const int w = first >> 6, sh = first & 63;
+        seen = word(w) >> sh;
+        if (sh) seen |= word(w + 1) << (64 - sh);
       }
     }
-    const u32x4 okw = *reinterpret_cast<const u32x4 *>(s_ok[slot]);
-    float mul[4], vsc[4];
+    const int left = L - kb;
+    if (left < 64) seen &= (1ull << left) - 1ull;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      mul[t] = FP8 ? a.scale_log2 * s_ks[slot][t] : a.scale_log2;
-      vsc[t] = FP8 ? s_vs[slot][t] : 1.f;
-    }
-    // exponents against the reference maximum
+    for (int t = 0; t < 4; ++t)
+      if (!(ok >> t & 1)) seen &= ~(0xFFFFull << (16 * t));
+    return seen;
+  };
+  // Exponents against the reference maximum (0 before the first seen key).
+  auto expo = [&](floatx16 &x0, floatx16 &x1) __attribute__((always_inline)) {
     const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      x0[r] = __builtin_fmaf(x0[r], mul[r >> 3], -m_use);
-      x1[r] = __builtin_fmaf(x1[r], mul[2 + (r >> 3)], -m_use);
+      x0[r] = __builtin_fmaf(x0[r], scale_log2, -m_use);
+      x1[r] = __builtin_fmaf(x1[r], scale_log2, -m_use);
     }
-    const uint32_t ok = __builtin_amdgcn_readfirstlane(okw[0] | okw[1] << 1 | okw[2] << 2 | okw[3] << 3);
-    const bool masked = ok != 15u || kb + 64 > ctx;  // uniform
-    uint64_t seen = ~0ull;                           // key kb + i is seen by this lane's row
-    if (masked) {
-      const int first = kb - ctx;  // the node of the step's first key
-      if (first <= -64) {
-      } else if (first < 0) {
-        seen = ((1ull << -first) - 1ull) | (s_mask[32 * wave + n][0] << -first);
-      } else {
-        const int w = first >> 6, sh = first & 63;
-        const uint64_t lo = w < WKV_TREE_MAX_WORDS ? s_mask[32 * wave + n][w & 3] : 0ull;
-        const uint64_t hi = w + 1 < WKV_TREE_MAX_WORDS ? s_mask[32 * wave + n][(w + 1) & 3] : 0ull;
-        seen = sh ? (lo >> sh) | (hi << (64 - sh)) : lo;
-      }
-      const int left = L - kb;
-      if (left < 64) seen &= (1ull << left) - 1ull;
+  };
+  auto hide = [&](uint64_t seen, floatx16 &x0, floatx16 &x1) __attribute__((always_inline)) {
+    const uint64_t v = seen >> (8 * (lane_here() >> 5));
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-        if (!(ok >> t & 1)) seen &= ~(0xFFFFull << (16 * t));
-      const uint64_t v = seen >> (8 * hh);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        if (!(v >> (16 * (r >> 3) + (r & 7)) & 1)) x0[r] = -INFINITY;
-        if (!(v >> (32 + 16 * (r >> 3) + (r & 7)) & 1)) x1[r] = -INFINITY;
-      }
+    for (int r = 0; r < 16; ++r) {
+      if (!(v >> (16 * (r >> 3) + (r & 7)) & 1)) x0[r] = -INFINITY;
+      if (!(v >> (32 + 16 * (r >> 3) + (r & 7)) & 1)) x1[r] = -INFINITY;
     }
+  };
+  auto largest = [&](const floatx16 &x0, const floatx16 &x1) __attribute__((always_inline)) {
     float mt0 = fmaxf(x0[0], x0[1]), mt1 = fmaxf(x1[0], x1[1]);
 #pragma unroll
     for (int r = 2; r < 16; r += 2) {
       mt0 = fmaxf(fmaxf(mt0, x0[r]), x0[r + 1]);
       mt1 = fmaxf(fmaxf(mt1, x1[r]), x1[r + 1]);
     }
-    float mt = fmaxf(mt0, mt1);
-    {
-      const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
-      mt = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-    }
+    const float mt = fmaxf(mt0, mt1);
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
+    return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+  };
+  // The rare move of the reference maximum (after the PV products of the steps before).
+  auto rescale = [&](float mt, floatx16 &x0, floatx16 &x1) __attribute__((always_inline)) {
     const bool unset = m_ref == -INFINITY;
     const bool move = unset ? mt > -INFINITY : mt > SOFTMAX_TAU;
-    if (__any(move)) {  // rare after the first step
+    if (__any(move)) {
+      asm volatile("");  // stays a branch: a step seldom has it
       const float sh = move ? mt : 0.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -336,121 +545,231 @@ __global__ __launch_bounds__(64 * kTreeWaves, 2) void tree_gqa_kernel(TreeArgs a
       }
       const float corr = move && !unset ? fast_exp2(-sh) : 1.f;
       l_part *= corr;
-      if (move) m_ref = m_use + sh;
+      if (move) m_ref = unset ? sh : m_ref + sh;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[c][r] *= corr;
     }
-    // probabilities, their sum and the PV operands
+  };
+  // Probabilities, packed as the PV operands, and the sum of the rounded ones.
+  auto probs = [&](floatx16 &x0, floatx16 &x1) __attribute__((always_inline)) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       x0[r] = fast_exp2(x0[r]);
       x1[r] = fast_exp2(x1[r]);
     }
-    uint32_t pw[4][4];
     float ps = 0.f;
-    if constexpr (FP8) {
-      float p0 = 0.f;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        ps += x0[r];
-        p0 += x1[r];
-      }
-      ps += p0;
-    }
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const floatx16 &sv = t < 2 ? x0 : x1;
       const int e0 = 8 * (t & 1);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if constexpr (FP8) {
-          pw[t][i] = pack_bf16x2(sv[e0 + 2 * i] * vsc[t], sv[e0 + 2 * i + 1] * vsc[t]);
-        } else {  // the sum of the rounded probabilities that the products take
-          pw[t][i] = pack_bf16x2(sv[e0 + 2 * i], sv[e0 + 2 * i + 1]);
-          ps = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pw[t][i]), ones, ps, false);
-        }
+        pw[t][i] = pack_bf16x2(sv[e0 + 2 * i], sv[e0 + 2 * i + 1]);
+        ps = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pw[t][i]), ones, ps, false);
       }
     }
     l_part += ps;
-    if (!masked) {
+  };
+  // P V^T of step s
+  auto pv = [&](int s) __attribute__((always_inline)) {
+    const uint8_t *lv = ldsv + (s & 1) * 4 * TB + (hh * D + n) * 16;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const bf16x8 pb = __builtin_bit_cast(bf16x8, (u32x4{pw[t][0], pw[t][1], pw[t][2], pw[t][3]}));
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c)
-          o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v_operand(slot, t, c)), pb, o[c], 0,
-                                                         0, 0);
-      }
-      return;
-    }
-#pragma unroll 1
     for (int t = 0; t < 4; ++t) {
-      const int left = L - kb - 16 * t;
-      if (left <= 0 || !(ok >> t & 1)) continue;  // uniform
-      u32x4 pt = t == 0   ? u32x4{pw[0][0], pw[0][1], pw[0][2], pw[0][3]}
-                 : t == 1 ? u32x4{pw[1][0], pw[1][1], pw[1][2], pw[1][3]}
-                 : t == 2 ? u32x4{pw[2][0], pw[2][1], pw[2][2], pw[2][3]}
-                          : u32x4{pw[3][0], pw[3][1], pw[3][2], pw[3][3]};
-      // slots past the last token may hold anything: zeros in their place
-      u32x4 real;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        real[i] = (8 * hh + 2 * i < left ? 0xFFFFu : 0u) | (8 * hh + 2 * i + 1 < left ? 0xFFFF0000u : 0u);
-      u32x4 w[D / 32];
-      bool odd = false;  // a V that is not finite
+      const bf16x8 pb = __builtin_bit_cast(bf16x8, (u32x4{pw[t][0], pw[t][1], pw[t][2], pw[t][3]}));
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
-        w[c] = v_operand(slot, t, c) & real;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          odd = odd || (w[c][i] & 0x7F80u) == 0x7F80u || (w[c][i] & 0x7F800000u) == 0x7F800000u;
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(lv + t * TB + 32 * c * 16);
+        o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w), pb, o[c], 0, 0, 0);
       }
-      if (!__any(odd)) {
-        const bf16x8 pb = __builtin_bit_cast(bf16x8, pt);
+    }
+  };
+  // The same of a step that masks: slots past the last token (they may hold
+  // anything) as zeros. V that are not finite are zeros there too, and are added
+  // to the rows that see their keys: as many +inf, -inf or both (a NaN) as products of
+  // where they stand with what is seen count.
+  auto pv_masked = [&](int s) __attribute__((always_inline)) {
+    const int l = lane_here(), n = l & 31, hh = l >> 5;
+    const uint8_t *const lv = ldsv + (s & 1) * 4 * TB + (hh * D + n) * 16;
+    bool odd = false;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int left = L - 64 * s - 16 * t;
+      if (left <= 0) continue;  // uniform
+      u32x4 w[D / 32];
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) w[c] = *reinterpret_cast<const u32x4 *>(lv + t * TB + 32 * c * 16);
+      if (left < 16) {  // uniform
 #pragma unroll
         for (int c = 0; c < D / 32; ++c)
-          o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w[c]), pb, o[c], 0, 0, 0);
-      } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            w[c][i] &= (8 * hh + 2 * i < left ? 0xFFFFu : 0u) | (8 * hh + 2 * i + 1 < left ? 0xFFFF0000u : 0u);
+      }
+      u16x2 most = {0, 0};  // largest magnitude bits
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w[c][i] & 0x7FFF7FFFu));
+      if (__any(most[0] >= 0x7F80u || most[1] >= 0x7F80u)) {
+        odd = true;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            w[c][i] &= ((w[c][i] & 0x7F80u) == 0x7F80u ? 0u : 0xFFFFu) |
+                       ((w[c][i] & 0x7F800000u) == 0x7F800000u ? 0u : 0xFFFF0000u);
+      }
+      const bf16x8 pb = __builtin_bit_cast(bf16x8, (u32x4{pw[t][0], pw[t][1], pw[t][2], pw[t][3]}));
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c)
+        o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w[c]), pb, o[c], 0, 0, 0);
+    }
+    if (!odd) return;  // uniform
+    const uint64_t seen = window(s, tiles(s)) >> (8 * hh);
 #pragma unroll 1
-        for (int e = 0; e < 16 && e < left; ++e) {
-          const uint32_t word = (e & 7) < 2 ? pt[0] : (e & 7) < 4 ? pt[1] : (e & 7) < 6 ? pt[2] : pt[3];
-          const uint32_t got = __shfl(word, n + 32 * (e >> 3), 64);
-          const float p = bf16_bits_to_f32((e & 1) ? got >> 16 : got & 0xFFFFu);
-          if (seen >> (16 * t + e) & 1) {
+    for (int t = 0; t < 4; ++t) {
+      u32x4 vis;  // 1 where the row sees the key
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
+      for (int i = 0; i < 4; ++i)
+        vis[i] = (seen >> (16 * t + 2 * i) & 1 ? 0x3F80u : 0u) | (seen >> (16 * t + 2 * i + 1) & 1 ? 0x3F800000u : 0u);
 #pragma unroll
-              for (int r = 0; r < 16; ++r)
-                o[c][r] = __builtin_fmaf(p, v_value(slot, t, 32 * c + 8 * (r >> 2) + 4 * hh + (r & 3), e), o[c][r]);
-              __builtin_amdgcn_sched_barrier(0);  // (few loads at a time: this path must not cost the others registers)
-            }
+      for (int c = 0; c < D / 32; ++c) {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(lv + t * TB + 32 * c * 16);
+#pragma unroll
+        for (int sign = 0; sign < 2; ++sign) {  // 1 where V is a NaN or the infinity of this sign
+          const uint32_t inf = sign ? 0xFF80u : 0x7F80u;
+          u32x4 is;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t lo = w[i] & 0xFFFFu, hi = w[i] >> 16;
+            is[i] = ((lo & 0x7FFFu) > 0x7F80u || lo == inf ? 0x3F80u : 0u) |
+                    ((hi & 0x7FFFu) > 0x7F80u || hi == inf ? 0x3F800000u : 0u);
           }
+          floatx16 x;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[r] = 0.f;
+          x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, is), __builtin_bit_cast(bf16x8, vis), x,
+                                                      0, 0, 0);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[c][r] += x[r] > 0.f ? (sign ? -INFINITY : INFINITY) : 0.f;
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
   };
 
+  // The copies' turn of step s, and the next ones on their way.
+  auto turn = [&](int s) __attribute__((always_inline)) {
+    wait_vmcnt<0>();  // this wave's copies of step s's V and step s + 1's K
+    land(s);
+    barrier_lds();    // ... every wave's; every wave is done with step s - 1
+    issue_v(s + 1);
+    issue_k(s + 2);
+  };
+  // Step s finished while step s + 1 is scored, both of whole tiles of the context.
+  auto body = [&](int s, floatx16 &c0, floatx16 &c1, floatx16 &n0, floatx16 &n1) __attribute__((always_inline)) {
+    turn(s);
+    if (!active) return;  // uniform
+    qk(s + 1, n0, n1);
+    probs(c0, c1);
+    // keeps the probabilities in this block
+    asm volatile("" ::"v"(l_part), "v"(pw[0][0]), "v"(pw[0][1]), "v"(pw[0][2]), "v"(pw[0][3]), "v"(pw[1][0]),
+                 "v"(pw[1][1]), "v"(pw[1][2]), "v"(pw[1][3]), "v"(pw[2][0]), "v"(pw[2][1]), "v"(pw[2][2]),
+                 "v"(pw[2][3]), "v"(pw[3][0]), "v"(pw[3][1]), "v"(pw[3][2]), "v"(pw[3][3]));
+    // the score products of step s + 1 interleaved with step s's probabilities
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);  // LDS reads, four ahead
 #pragma unroll
-  for (int i = 0; i < NS - 1; ++i) issue(s0 + i, i);
-  int slot = 0;
-  for (int s = s0; s < s1; ++s) {
-    wait_step();    // this wave's tile of step s
-    barrier_lds();  // every wave's; every wave is done with step s - 1, whose slot takes step s + NS - 1
-    const int next = slot == 0 ? NS - 1 : slot - 1;
-    issue(s + NS - 1, next);
-    if (active) attend(s, slot);
-    slot = slot + 1 == NS ? 0 : slot + 1;
+    for (int i = 0; i < 2 * D / 16; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+      if (i + 4 < 2 * D / 16) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
+      __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);  // VALU
+    }
+    expo(n0, n1);
+    const float mt = largest(n0, n1);
+    pv(s);
+    // step s's PV products interleaved with step s + 1's exponents
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int i = 0; i < 4 * D / 32; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (i + 4 < 4 * D / 32) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+    }
+    rescale(mt, n0, n1);
+  };
+
+  if (s1 > s0) {
+    issue_k(s0);
+    if constexpr (FP8) {
+      wait_vmcnt<0>();
+      if (k_land) widen(s0 - 1, std::false_type{}, std::true_type{});
+    }
+    issue_v(s0);
+    issue_k(s0 + 1);
+    if constexpr (!FP8) {  // K of step s0 landed: at most its V and the next K on their way
+      if (k_land) wait_vmcnt<2 * NC>(); else wait_vmcnt<NC>();
+      if (!v_land) wait_vmcnt<0>();  // (no tile of step s0)
+    }
+    barrier_lds();
+    floatx16 a0, a1;
+    auto score = [&](int s) __attribute__((always_inline)) {
+      qk(s, a0, a1);
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);  // LDS reads four ahead of their MFMAs, not all at once
+#pragma unroll
+      for (int i = 0; i < 2 * D / 16; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (i + 4 < 2 * D / 16) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      expo(a0, a1);
+      const uint32_t ok = tiles(s);
+      if (ok != 15u || 64 * s + 64 > ctx) {  // uniform
+        hide(window(s, ok), a0, a1);
+      }
+      rescale(largest(a0, a1), a0, a1);
+    };
+    if (active) score(s0);
+    // Steps of context alone, in pairs: what a pair scores, steps s + 1 and s + 2, is of
+    // windows opened before it.
+    int s = s0;
+    {
+      floatx16 b0, b1;
+      const int ends = (ctx >> 6) < s1 ? (ctx >> 6) : s1;
+      for (; s + 2 < ends && clean; s += 2) {
+        body(s, a0, a1, b0, b1);
+        body(s + 1, b0, b1, a0, a1);
+      }
+      if (s + 1 < ends && clean) {
+        body(s, a0, a1, b0, b1);
+        ++s;
+        a0 = b0;
+        a1 = b1;
+      }
+    }
+    // The others, one at a time.
+#pragma unroll 1
+    for (; s < s1; ++s) {
+      turn(s);
+      if (!active) continue;  // uniform
+      probs(a0, a1);
+      pv_masked(s);
+      if (s + 1 < s1) score(s + 1);
+    }
   }
-  if (!active) return;
+  const TreeArgs &ae = tree_args();
+  if (active) {
+  const int lane = lane_here(), n = lane & 31, hh = lane >> 5;
   float l = l_part;
   {
     const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
     l = __uint_as_float(x[0]) + __uint_as_float(x[1]);
   }
-  if (tc.n > 1) {  // uniform
-    float *pp = a.part + ((static_cast<int64_t>(b * a.Hkv + kvh) * a.units + unit) * a.chunks + chunk) * tree_part_floats<D>();
+  if (partial) {  // uniform
+    const int64_t slot = 2 * s_place + (later ? 1 : 0);
+    float *pp = ae.part + (slot * kTreeWaves + wave) * tree_part_floats<D>();
 #pragma unroll
     for (int c = 0; c < D / 32; ++c)
 #pragma unroll
@@ -461,10 +780,11 @@ __global__ __launch_bounds__(64 * kTreeWaves, 2) void tree_gqa_kernel(TreeArgs a
       pp[32 * D + n] = m_ref;
       pp[32 * D + 32 + n] = l;
     }
-  } else if (has_row) {
+  } else if (const Row r = row_of(n); r.real) {
     const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-    if (a.sinks != nullptr) l += exp2f(a.sinks[h] * 1.4426950408889634f - m_use);
+    if (ae.sinks != nullptr) l += exp2f(ae.sinks[r.h] * 1.4426950408889634f - m_use);
     const float inv = l != 0.f ? 1.f / l : 0.f;
+    uint16_t *const op = ae.out + static_cast<int64_t>(q0 + r.node) * ae.o_st + static_cast<int64_t>(r.h) * ae.o_sh;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c)
 #pragma unroll
@@ -473,82 +793,136 @@ __global__ __launch_bounds__(64 * kTreeWaves, 2) void tree_gqa_kernel(TreeArgs a
             u32x2{pack_bf16x2(o[c][4 * g] * inv, o[c][4 * g + 1] * inv),
                   pack_bf16x2(o[c][4 * g + 2] * inv, o[c][4 * g + 3] * inv)};
   }
-}
-
-// Log-sum-exp merge of a unit's chunks: one wave per unit and 32 output columns.
-// A sequence of one chunk was finished by the attention kernel.
-template <int D>
-__global__ __launch_bounds__(64) void tree_merge_kernel(TreeArgs a) {
-  constexpr int PF = tree_part_floats<D>();
-  const int lane = threadIdx.x, n = lane & 31, hh = lane >> 5;
-  const int unit = blockIdx.x, c = blockIdx.z;
-  const int kvh = blockIdx.y % a.Hkv, b = blockIdx.y / a.Hkv;
-  const int q0 = a.cu_q[b], qlen = a.cu_q[b + 1] - q0;
-  int L = a.seq_lens[b];
-  L = L < a.max_seq ? L : a.max_seq;
-  const int rows = qlen * a.G;
-  if (qlen <= 0 || L <= 0 || 32 * unit >= rows) return;
-  const int chunks = tree_chunks(L, a.chunk_steps, (L + 63) >> 6).n;
-  if (chunks <= 1) return;
-  const float *p = a.part + (static_cast<int64_t>(b * a.Hkv + kvh) * a.units + unit) * a.chunks * PF;
-  float M = -INFINITY;
-#pragma unroll 4
-  for (int i = 0; i < chunks; ++i) M = fmaxf(M, p[i * static_cast<int64_t>(PF) + 32 * D + n]);
-  const int row = 32 * unit + n;
-  const bool has_row = row < rows;
-  const int node = has_row ? row / a.by_G : 0, h = kvh * a.G + (has_row ? row - node * a.G : 0);
-  const float m_use = M == -INFINITY ? 0.f : M;
-  float l = 0.f;
-  floatx4 acc[4];
-#pragma unroll
-  for (int g = 0; g < 4; ++g) acc[g] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int i = 0; i < chunks; ++i) {
-    const float *ps = p + i * static_cast<int64_t>(PF);
-    const float w = exp2f(ps[32 * D + n] - m_use);  // 0 for a chunk of which the row saw no key
-    l += w * ps[32 * D + 32 + n];
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const floatx4 x = *reinterpret_cast<const floatx4 *>(ps + ((4 * c + g) * 64 + lane) * 4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[g][e] += w * x[e];
+  }
+  if constexpr (SHARED) {
+    if (partial && s_begin == 0 && threadIdx.x == 0) {  // the group's first part (and the last of this share)
+      const TreeShare share = s_share;
+      const int w = s_place;
+      const int w1 = share.of(share.begin(w + 1) + (all_steps - take) - 1);  // the workgroup of the group's last step
+      tree_counts<D>(ae.part)[id] = w1 - w + 1;
+      tree_records<D>(ae.part)[id] = TreeRec{2 * w + (later ? 1 : 0), 2 * (w + 1), b, kvh, rg, {0, 0, 0}};
+    }
+    steps_left -= take;
+    later = true;
+  }
+  }
+  if constexpr (!SHARED) {
+    break;
+  } else {
+    if (steps_left <= 0) break;
+    s_begin = 0;
+    const TreeArgs &an = tree_args();
+    if (++rg >= groups) {
+      rg = 0;
+      if (++b == an.batch) {
+        b = 0;
+        if (++kvh == an.Hkv) break;  // never with steps left
+      }
     }
   }
-  if (!has_row) return;
-  if (a.sinks != nullptr) l += exp2f(a.sinks[h] * 1.4426950408889634f - m_use);
-  const float inv = l != 0.f ? 1.f / l : 0.f;
-  uint16_t *op = a.out + static_cast<int64_t>(q0 + node) * a.o_st + static_cast<int64_t>(h) * a.o_sh;
+  }
+}
+
+// Log-sum-exp merge of the cut row groups' parts. A wave takes 8 output columns
+// of a unit at a time, of the records that name a group in turn over the grid's waves:
+// each wave finds them by itself in the list of the part counts. (A workgroup per
+// record instead, three quarters of which are empty, cost 8 us for their dispatch alone.)
+constexpr int kMergeGroups = 1024;
+template <int D>
+__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
+  constexpr int PF = tree_part_floats<D>();
+  constexpr int CG = D / 8;  // column groups
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int lane = threadIdx.x & 63, n = lane & 31, hh = lane >> 5;
+  const int *counts = tree_counts<D>(a.part);
+  uint64_t named[kTreeShare / 64];
+  int total = 0;
 #pragma unroll
-  for (int g = 0; g < 4; ++g)
-    *reinterpret_cast<u32x2 *>(op + 32 * c + 8 * g + 4 * hh) =
-        u32x2{pack_bf16x2(acc[g][0] * inv, acc[g][1] * inv), pack_bf16x2(acc[g][2] * inv, acc[g][3] * inv)};
+  for (int i = 0; i < kTreeShare / 64; ++i) named[i] = __ballot(counts[64 * i + lane] > 0);
+#pragma unroll
+  for (int i = 0; i < kTreeShare / 64; ++i) total += __builtin_popcountll(named[i]);
+  total *= kTreeWaves * CG;
+  for (int item = blockIdx.x * 4 + wave; item < total; item += kMergeGroups * 4) {
+    int k = item / (kTreeWaves * CG), id = 0;  // the k-th record that names a group
+    uint64_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < kTreeShare / 64; ++i) {
+      const int c = __builtin_popcountll(named[i]);
+      if (k >= 0 && k < c) {
+        id = 64 * i;
+        bits = named[i];
+        for (; k > 0; --k) bits &= bits - 1;
+        k = 0;
+      }
+      k -= c;
+    }
+    id = __builtin_amdgcn_readfirstlane(id + __builtin_ctzll(bits));
+    const int unit = item / CG % kTreeWaves, cg = item % CG;
+    const int parts = __builtin_amdgcn_readfirstlane(counts[id]);
+    const TreeRec rec = tree_records<D>(a.part)[id];
+    const int q0 = a.cu_q[rec.b], rows = (a.cu_q[rec.b + 1] - q0) * a.G;
+    const int row = 32 * (rec.group * kTreeWaves + unit) + n;
+    const float *p0 = a.part + (static_cast<int64_t>(rec.slot) * kTreeWaves + unit) * PF;
+    const float *pn = a.part + (static_cast<int64_t>(rec.next) * kTreeWaves + unit) * PF;
+    constexpr int64_t step = 2 * kTreeWaves * PF;
+    if (row - n >= rows) continue;
+    float M = -INFINITY, l = 0.f;
+    floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+    constexpr int N = 8;  // parts in flight: a long group has tens
+    for (int i0 = 0; i0 < parts; i0 += N) {
+      float m[N], s[N];
+      floatx4 x[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        m[j] = -INFINITY;
+        if (i0 + j < parts) {  // uniform
+          const float *ps = i0 + j == 0 ? p0 : pn + (i0 + j - 1) * step;
+          m[j] = ps[32 * D + n];
+          s[j] = ps[32 * D + 32 + n];
+          x[j] = *reinterpret_cast<const floatx4 *>(ps + (cg * 64 + lane) * 4);
+        }
+      }
+      float top = M;
+#pragma unroll
+      for (int j = 0; j < N; ++j) top = fmaxf(top, m[j]);
+      const float m_use = top == -INFINITY ? 0.f : top;
+      const float was = exp2f(M - m_use);  // 0 while no part saw a key
+      l *= was;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] *= was;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        if (i0 + j < parts) {
+          const float w = exp2f(m[j] - m_use);  // 0 for a part of which the row saw no key
+          l += w * s[j];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] += w * x[j][e];
+        }
+      }
+      M = top;
+    }
+    if (row >= rows) continue;
+    const int node = row / a.by_G, h = rec.kvh * a.G + row - node * a.G;
+    const float m_use = M == -INFINITY ? 0.f : M;
+    if (a.sinks != nullptr) l += exp2f(a.sinks[h] * 1.4426950408889634f - m_use);
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    uint16_t *op = a.out + static_cast<int64_t>(q0 + node) * a.o_st + static_cast<int64_t>(h) * a.o_sh;
+    *reinterpret_cast<u32x2 *>(op + 8 * cg + 4 * hh) =
+        u32x2{pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv)};
+  }
 }
 
-// How a launch covers its work.
-struct TreePlan {
-  int units;        // per (sequence, KV head) at the longest query
-  int row_groups;   // workgroups of them
-  int chunks, chunk_steps;
-};
-
-// Chunks: enough workgroups for two per CU, of at least four steps each.
-static TreePlan tree_plan(int batch, int Hkv, int G, int max_query_len, int max_seq, bool cut) {
-  TreePlan p;
-  p.units = static_cast<int>((static_cast<int64_t>(max_query_len) * G + 31) / 32);
-  p.row_groups = (p.units + kTreeWaves - 1) / kTreeWaves;
-  const int steps = (max_seq + 63) / 64;
-  const int64_t wgs = static_cast<int64_t>(batch) * Hkv * p.row_groups;
-  int64_t chunks = cut ? (2 * kTreeCus + wgs - 1) / wgs : 1;
-  const int most = steps / 4 > 1 ? steps / 4 : 1;
-  if (chunks > most) chunks = most;
-  p.chunk_steps = static_cast<int>((steps + chunks - 1) / chunks);
-  if (p.chunk_steps < 1) p.chunk_steps = 1;
-  p.chunks = steps > 0 ? (steps + p.chunk_steps - 1) / p.chunk_steps : 1;
-  return p;
+// The workgroups that share a launch (0: one per row group): contexts of at most
+// eight steps are not cut (8 sequences of up to 300 tokens, with the merge's launch:
+// 22 us whole, 26 cut), and a line of 2^31 steps is not formed.
+static int tree_sharing(int batch, int Hkv, int G, int max_query_len, int max_seq) {
+  const int64_t steps = (static_cast<int64_t>(max_seq) + 63) / 64;
+  const int64_t groups = (static_cast<int64_t>(max_query_len) * G + kTreeRows - 1) / kTreeRows;
+  return steps > 8 && groups * batch <= INT32_MAX / (steps * Hkv) ? kTreeShare : 0;
 }
 
-static int64_t tree_workspace(const TreePlan &p, int batch, int Hkv, int D) {
-  return p.chunks > 1 ? static_cast<int64_t>(batch) * Hkv * p.units * p.chunks * (32 * D + 64) * 4 : 0;
+static int64_t tree_workspace(int share, int D) {
+  return share > 0 ? static_cast<int64_t>(share) * (2 * kTreeWaves * (32 * D + 64) * 4 + 4 + sizeof(TreeRec)) : 0;
 }
 
 }  // namespace wkv
@@ -563,8 +937,8 @@ extern "C" int64_t wkv_tree_workspace_size(int32_t batch, int32_t kv_dtype, int3
       static_cast<int64_t>(max_query_len) * (num_q_heads / num_kv_heads) > (1 << 24))
     return -1;
   if (batch == 0 || max_query_len == 0) return 0;
-  const TreePlan p = tree_plan(batch, num_kv_heads, num_q_heads / num_kv_heads, max_query_len, max_seq_len, true);
-  return tree_workspace(p, batch, num_kv_heads, head_dim);
+  return tree_workspace(
+      tree_sharing(batch, num_kv_heads, num_q_heads / num_kv_heads, max_query_len, max_seq_len), head_dim);
 }
 
 extern "C" int wkv_tree_gqa(const wkv_cache_t *cache, const void *key, int64_t key_stride_t, int64_t key_stride_h,
@@ -612,26 +986,59 @@ extern "C" int wkv_tree_gqa(const wkv_cache_t *cache, const void *key, int64_t k
   WKV_CHECK_ARG(static_cast<int64_t>(max_query_len) * G <= (1 << 24), "max_query_len * query heads per KV head too large");
   const int64_t table_tokens = static_cast<int64_t>(max_blocks_per_seq) * BS;
   const int max_seq = max_seq_len < table_tokens ? max_seq_len : static_cast<int>(table_tokens);
-  const TreePlan p = tree_plan(batch, Hkv, G, max_query_len, max_seq, workspace != nullptr);
-  const int64_t need = tree_workspace(p, batch, Hkv, D);
+  const int share = workspace != nullptr ? tree_sharing(batch, Hkv, G, max_query_len, max_seq) : 0;
+  const int64_t need = tree_workspace(share, D);
   if (need > 0)
     WKV_CHECK_ARG(aligned16(workspace) && workspace_bytes >= need, "workspace too small: need %lld bytes, got %lld",
                   (long long)need, (long long)workspace_bytes);
-  const int64_t items = static_cast<int64_t>(batch) * p.chunks * Hkv;
-  WKV_CHECK_ARG(items <= 8 * 65535 && static_cast<int64_t>(batch) * Hkv <= 65535, "too many sequences and KV heads");
+  const int64_t items = static_cast<int64_t>(batch) * Hkv;
+  const int groups = static_cast<int>((static_cast<int64_t>(max_query_len) * G + kTreeRows - 1) / kTreeRows);
+  const int64_t n_wg = share > 0 ? share : (items + 7) / 8 * 8 * groups;
+  WKV_CHECK_ARG(n_wg <= INT32_MAX / kTreeThreads, "too many sequences, KV heads and drafted tokens");
   rc = append();
   if (rc) return rc;
-  const TreeArgs a{static_cast<const uint8_t *>(cache->k), static_cast<const uint8_t *>(cache->v), cache->k_scale,
-                   cache->v_scale, static_cast<const uint16_t *>(q), q_stride_t, q_stride_h,
-                   static_cast<uint16_t *>(out), out_stride_t, out_stride_h, cu_seqlens_q, seq_lens, block_table,
-                   bt_stride, tree_mask, mask_words, max_blocks_per_seq, max_seq, Hkv, G, BS,
-                   static_cast<int>(cache->num_blocks), fast_div(BS), fast_div(G), fast_div(Hkv), fast_div(p.chunks),
-                   static_cast<int>(items), p.chunks, p.chunk_steps, p.units, scale * 1.4426950408889634f,
-                   static_cast<float *>(workspace), sinks};
-  const dim3 grid(static_cast<unsigned>(8 * p.row_groups), static_cast<unsigned>((items + 7) / 8));
+  TreeArgs a{};
+  a.kc = static_cast<const uint8_t *>(cache->k);
+  a.vc = static_cast<const uint8_t *>(cache->v);
+  a.ksc = cache->k_scale;
+  a.vsc = cache->v_scale;
+  a.q = static_cast<const uint16_t *>(q);
+  a.q_st = q_stride_t;
+  a.q_sh = q_stride_h;
+  a.out = static_cast<uint16_t *>(out);
+  a.o_st = out_stride_t;
+  a.o_sh = out_stride_h;
+  a.cu_q = cu_seqlens_q;
+  a.seq_lens = seq_lens;
+  a.bt = block_table;
+  a.bt_stride = bt_stride;
+  a.mask = tree_mask;
+  a.words = mask_words;
+  a.batch = batch;
+  a.Mb = max_blocks_per_seq;
+  a.max_seq = max_seq;
+  a.Hkv = Hkv;
+  a.G = G;
+  a.BS = BS;
+  a.nb = static_cast<int>(cache->num_blocks);
+  a.by_BS = fast_div(BS);
+  a.by_G = fast_div(G);
+  a.share = share;
+  a.groups = groups;
+  a.stream = (cache->flags & WKV_CACHE_SHARED_BLOCKS) == 0;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.part = static_cast<float *>(workspace);
+  a.sinks = sinks;
+  const dim3 grid(static_cast<unsigned>(n_wg));
   auto s = static_cast<hipStream_t>(stream);
   const bool fp8 = cache->kv_dtype == WKV_KV_FP8_E4M3;
-#define WKV_TREE(Dv, F8) tree_gqa_kernel<Dv, F8, tree_steps_in_lds<Dv, F8>()><<<grid, 64 * kTreeWaves, 0, s>>>(a)
+#define WKV_TREE(Dv, F8)                                                        \
+  do {                                                                          \
+    if (share > 0)                                                              \
+      tree_gqa_kernel<Dv, F8, true><<<grid, kTreeThreads, 0, s>>>(a);           \
+    else                                                                        \
+      tree_gqa_kernel<Dv, F8, false><<<grid, kTreeThreads, 0, s>>>(a);          \
+  } while (0)
   if (D == 128) {
     if (fp8) WKV_TREE(128, true); else WKV_TREE(128, false);
   } else {
@@ -639,12 +1046,11 @@ extern "C" int wkv_tree_gqa(const wkv_cache_t *cache, const void *key, int64_t k
   }
 #undef WKV_TREE
   WKV_CHECK_LAUNCH("tree attention");
-  if (p.chunks > 1) {
-    const dim3 mgrid(static_cast<unsigned>(p.units), static_cast<unsigned>(batch * Hkv), static_cast<unsigned>(D / 32));
+  if (share > 0) {
     if (D == 128)
-      tree_merge_kernel<128><<<mgrid, 64, 0, s>>>(a);
+      tree_merge_kernel<128><<<kMergeGroups, 256, 0, s>>>(a);
     else
-      tree_merge_kernel<64><<<mgrid, 64, 0, s>>>(a);
+      tree_merge_kernel<64><<<kMergeGroups, 256, 0, s>>>(a);
     WKV_CHECK_LAUNCH("tree attention merge");
   }
   return WKV_OK;
