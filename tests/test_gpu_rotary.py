@@ -147,6 +147,42 @@ def test_rotary_backward_twice_and_captured(cuda):
         assert torch.equal(out, apply_rotary(x, None, pos, freq)[0])
 
 
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("r", [128, 72])
+def test_rotary_of_many_rows_is_that_of_few(cuda, r, inter):
+    """A batch far larger than the caches gives the bits of its parts turned alone."""
+    tokens = 7003
+    gen = torch.Generator(device=cuda).manual_seed(r)
+    q, k = (torch.randn((tokens, h, 128), generator=gen, device=cuda).to(torch.bfloat16) for h in (32, 8))
+    pos = torch.randint(0, 40000, (tokens,), generator=gen, device=cuda)
+    freq, scale = rotary_frequencies(r, 1e6, device=cuda)
+    gq, gk = apply_rotary(q, k, pos, freq, interleaved=inter, scale=scale)
+    for i in range(0, tokens, 1500):
+        rows = slice(i, min(i + 1500, tokens))
+        wq, wk = apply_rotary(q[rows], k[rows], pos[rows], freq, interleaved=inter, scale=scale)
+        assert torch.equal(gq[rows], wq) and torch.equal(gk[rows], wk)
+
+
+@pytest.mark.parametrize("need_q,need_k,use_q,use_k", [(True, True, True, False), (True, True, False, True),
+                                                       (True, False, True, True), (False, True, True, True)])
+def test_rotary_gradient_of_one_alone(cuda, need_q, need_k, use_q, use_k):
+    """The transpose's rows for what needs a gradient; nothing for a result that is not used."""
+    gen = torch.Generator(device=cuda).manual_seed(3)
+    q, k = (torch.randn((5, h, 64), generator=gen, device=cuda) for h in (4, 2))
+    gq, gk = (torch.randn((5, h, 64), generator=gen, device=cuda) for h in (4, 2))
+    pos, (freq, _) = torch.arange(5, device=cuda) * 100, rotary_frequencies(64, device=cuda)
+    q.requires_grad_(need_q), k.requires_grad_(need_k)
+    yq, yk = apply_rotary(q, k, pos, freq)
+    loss = sum((y * g).sum() for y, g, use in ((yq, gq, use_q), (yk, gk, use_k)) if use)
+    loss.backward()
+    wq, wk = apply_rotary(gq, gk, pos, freq, inverse=True)
+    for x, want, got_any in ((q, wq, need_q and use_q), (k, wk, need_k and use_k)):
+        if got_any:
+            assert torch.equal(x.grad, want)
+        else:
+            assert x.grad is None or not x.grad.any()
+
+
 def test_rotary_refusals(cuda):
     q, k = torch.zeros((3, 2, 64), device=cuda), torch.zeros((3, 1, 64), device=cuda)
     pos, freq = torch.arange(3, device=cuda), _freq(64, 1e4, cuda)

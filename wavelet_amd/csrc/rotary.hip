@@ -9,12 +9,13 @@
 // tokens enough for the chip). Its lanes form the token's angles once, a pair
 // each, and leave the sines and cosines in LDS for every head; a lane then
 // turns units of V pairs, two 16-byte loads and two stores where the layout
-// allows, four units in flight. Angles are taken in float64, in turns, and
+// allows, some units in flight. Angles are taken in float64, in turns, and
 // reduced there: float32 would lose a position of 131,072 at frequency 1 to
 // 2^-7 of a radian. Sines and products are float32, one rounding to the
 // type at the end.
-// Bound by HBM past some thousand tokens, by the launch and one round trip for
-// a single one.
+// Bound by HBM past some thousand tokens (16,384 tokens of 40 heads of 128, bf16, in
+// either layout: 55 us, 6.1 TB/s), by the launch and one round trip for a single one
+// (3.4 us).
 #include <cmath>
 
 #include "wkv_common.h"
@@ -48,9 +49,12 @@ __device__ __forceinline__ float to_f32(T x) {
   return static_cast<float>(x);
 }
 
-// INTER: pair i is dims (2 i, 2 i + 1), else (i, i + half). A unit is V pairs:
-// two runs of V elements, adjacent (INTER, and what is only copied) or half apart.
-template <class T, int V, bool INTER>
+// INTER: pair i is dims (2 i, 2 i + 1), else (i, i + half). A unit is V pairs
+// in two runs of V elements: half apart, or (INTER, and what is only copied) half
+// the units apart, so that the lanes' runs follow each other; single elements
+// (V = 1) of an INTER pair are adjacent.
+// FAR: rows read past the caches.
+template <class T, int V, bool INTER, bool FAR>
 __global__ __launch_bounds__(64 * kRotaryWaves) void rotary_kernel(RotaryArgs a) {
   typedef __attribute__((__vector_size__(V * sizeof(T)))) T Vec;
   __shared__ float2 turn[kRotaryWaves][kRotaryMaxPairs];
@@ -71,11 +75,11 @@ __global__ __launch_bounds__(64 * kRotaryWaves) void rotary_kernel(RotaryArgs a)
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   const int n = heads * a.units.d;
-  constexpr int N = 4;  // units of a lane in flight
+  constexpr int N = FAR ? 2 : 4;  // units of a lane in flight (FAR: 4 take 8% more of the time, 1 14%)
   for (int i0 = 0; i0 < n; i0 += 64 * N) {
     Vec x0[N], x1[N];
     T *y0[N], *y1[N];
-    int first[N];  // the unit's first pair
+    int first[N], second[N];  // the runs' first pairs
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const int i = i0 + 64 * k + lane;
@@ -86,22 +90,23 @@ __global__ __launch_bounds__(64 * kRotaryWaves) void rotary_kernel(RotaryArgs a)
         const int hr = h < a.Hq ? h : h - a.Hq;
         int e0, e1;
         if (INTER) {
-          first[k] = V * u;
-          e0 = 2 * V * u;
-          e1 = e0 + V;
+          e0 = V > 1 ? V * u : 2 * u;
+          e1 = V > 1 ? V * (u + a.units.d) : 2 * u + 1;
+          first[k] = e0 / 2;
+          second[k] = e1 / 2;
         } else if (u < a.turned) {
-          first[k] = V * u;
-          e0 = V * u;
+          first[k] = e0 = V * u;
           e1 = e0 + a.half;
         } else {
           first[k] = a.half;
-          e0 = 2 * a.half + 2 * V * (u - a.turned);
-          e1 = e0 + V;
+          e0 = 2 * a.half + V * (u - a.turned);
+          e1 = e0 + V * (a.units.d - a.turned);
         }
         const T *x = static_cast<const T *>(r.x) + t * r.xt + hr * r.xh;
         T *y = static_cast<T *>(r.y) + t * r.yt + hr * r.yh;
-        x0[k] = *reinterpret_cast<const Vec *>(x + e0);
-        x1[k] = *reinterpret_cast<const Vec *>(x + e1);
+        const Vec *p0 = reinterpret_cast<const Vec *>(x + e0), *p1 = reinterpret_cast<const Vec *>(x + e1);
+        x0[k] = FAR ? __builtin_nontemporal_load(p0) : *p0;
+        x1[k] = FAR ? __builtin_nontemporal_load(p1) : *p1;
         y0[k] = y + e0;
         y1[k] = y + e1;
       }
@@ -109,20 +114,33 @@ __global__ __launch_bounds__(64 * kRotaryWaves) void rotary_kernel(RotaryArgs a)
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       if (y0[k] == nullptr) continue;
-      if (first[k] < a.half) {
+      auto turn_pair = [&](int i, T &xa, T &xb) __attribute__((always_inline)) {
+        const float2 cs = turn[wave][i];
+        const float fa = to_f32(xa), fb = to_f32(xb);
+        xa = static_cast<T>(fa * cs.x - fb * cs.y);
+        xb = static_cast<T>(fb * cs.x + fa * cs.y);
+      };
+      auto turn_runs = [&](int m, int w, int i) __attribute__((always_inline)) {  // elements m of x0 and w of x1
+        T xa = x0[k][m], xb = x1[k][w];
+        turn_pair(i, xa, xb);
+        x0[k][m] = xa;
+        x1[k][w] = xb;
+      };
+      auto turn_run = [&](Vec &x, int i0) __attribute__((always_inline)) {  // a run's adjacent pairs
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          // the pair's places among the unit's 2 V elements
-          const int m = INTER ? 2 * v : v, w = INTER ? 2 * v + 1 : V + v;
-          const int i = first[k] + v;
-          if (INTER && i >= a.half) continue;  // (a unit past the turned pairs' end is partly copied)
-          const float2 cs = turn[wave][i];
-          const float xa = to_f32(m < V ? x0[k][m % V] : x1[k][m % V]);
-          const float xb = to_f32(w < V ? x0[k][w % V] : x1[k][w % V]);
-          const T ya = static_cast<T>(xa * cs.x - xb * cs.y), yb = static_cast<T>(xb * cs.x + xa * cs.y);
-          if (m < V) x0[k][m % V] = ya; else x1[k][m % V] = ya;
-          if (w < V) x0[k][w % V] = yb; else x1[k][w % V] = yb;
+        for (int v = 0; v < V / 2; ++v) {
+          T xa = x[2 * v], xb = x[2 * v + 1];
+          if (i0 + v < a.half) turn_pair(i0 + v, xa, xb);
+          x[2 * v] = xa;
+          x[2 * v + 1] = xb;
         }
+      };
+      if (INTER && V > 1) {
+        if (first[k] < a.half) turn_run(x0[k], first[k]);  // (a run past the turned pairs' end is partly copied)
+        if (second[k] < a.half) turn_run(x1[k], second[k]);
+      } else if (first[k] < a.half) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) turn_runs(v, v, first[k] + v);
       }
       *reinterpret_cast<Vec *>(y0[k]) = x0[k];
       *reinterpret_cast<Vec *>(y1[k]) = x1[k];
@@ -143,14 +161,12 @@ static int rotary_width(int esz, int D, int half, bool inter, const RotaryRows *
 }
 
 template <class T, bool INTER>
-static void launch_rotary(const RotaryArgs &a, int v, dim3 grid, hipStream_t s) {
-  constexpr int B = 64 * kRotaryWaves;
-  if constexpr (sizeof(T) == 2) {
-    if (v == 8) return rotary_kernel<T, 8, INTER><<<grid, B, 0, s>>>(a);
-  }
-  if (v == 4) return rotary_kernel<T, 4, INTER><<<grid, B, 0, s>>>(a);
-  if (v == 2) return rotary_kernel<T, 2, INTER><<<grid, B, 0, s>>>(a);
-  rotary_kernel<T, 1, INTER><<<grid, B, 0, s>>>(a);
+static void launch_rotary(const RotaryArgs &a, int v, bool far, dim3 grid, hipStream_t s) {
+  constexpr int B = 64 * kRotaryWaves, W = 16 / sizeof(T);
+  if (v == W) return far ? rotary_kernel<T, W, INTER, true><<<grid, B, 0, s>>>(a) : rotary_kernel<T, W, INTER, false><<<grid, B, 0, s>>>(a);
+  if (W > 4 && v == 4) return rotary_kernel<T, 4, INTER, false><<<grid, B, 0, s>>>(a);
+  if (v == 2) return rotary_kernel<T, 2, INTER, false><<<grid, B, 0, s>>>(a);
+  rotary_kernel<T, 1, INTER, false><<<grid, B, 0, s>>>(a);
 }
 
 }  // namespace wkv
@@ -216,13 +232,16 @@ extern "C" int wkv_rotary(int32_t dtype, const void *q, int64_t q_stride_t, int6
   a.per = (H + split - 1) / split;
   const dim3 grid(static_cast<unsigned>((num_tokens + kRotaryWaves - 1) / kRotaryWaves),
                   static_cast<unsigned>((H + a.per - 1) / a.per));
+  // Rows far larger than the caches are read past them (32 query and 8 key heads of
+  // 128, bf16, near / far: 4,096 tokens 16.0 / 18.6 us, 6,144 26.4 / 24.9, 16,384 69 / 55).
+  const bool far = static_cast<int64_t>(num_tokens) * H * head_dim * esz >= (64 << 20);
   auto s = static_cast<hipStream_t>(stream);
   if (dtype == 0) {
-    if (inter) launch_rotary<float, true>(a, v, grid, s); else launch_rotary<float, false>(a, v, grid, s);
+    if (inter) launch_rotary<float, true>(a, v, far, grid, s); else launch_rotary<float, false>(a, v, far, grid, s);
   } else if (dtype == 1) {
-    if (inter) launch_rotary<__bf16, true>(a, v, grid, s); else launch_rotary<__bf16, false>(a, v, grid, s);
+    if (inter) launch_rotary<__bf16, true>(a, v, far, grid, s); else launch_rotary<__bf16, false>(a, v, far, grid, s);
   } else {
-    if (inter) launch_rotary<_Float16, true>(a, v, grid, s); else launch_rotary<_Float16, false>(a, v, grid, s);
+    if (inter) launch_rotary<_Float16, true>(a, v, far, grid, s); else launch_rotary<_Float16, false>(a, v, far, grid, s);
   }
   WKV_CHECK_LAUNCH("rotary");
   return WKV_OK;

@@ -110,31 +110,25 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: dict 
     return torch.tensor(freq, dtype=torch.float64, device=dev), scale
 
 
-def _rows(x: torch.Tensor, name: str, like: torch.Tensor) -> torch.Tensor:
-    if not isinstance(x, torch.Tensor) or x.dim() != 3 or x.dtype != like.dtype or x.device != like.device \
-            or x.shape[0] != like.shape[0] or x.shape[2] != like.shape[2]:
-        raise ValueError(f"{name} must be {like.dtype} [{like.shape[0]}, heads, {like.shape[2]}] on {like.device}")
-    return x if x.stride(2) == 1 else x.contiguous()
-
-
 def _launch(q, k, positions, inv_freq, interleaved: bool, scale: float, inverse: bool, out):
     """One launch over checked tensors (k may be None)."""
-    qi = _rows(q, "q", q)
-    ki = None if k is None else _rows(k, "k", q)
-    if out is None:
-        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    else:
-        qo, ko = out
+    qi = q if q.stride(2) == 1 else q.contiguous()
+    qo = torch.empty_like(qi, memory_format=torch.contiguous_format) if out is None else out[0]
+    tokens, hq, d = qi.shape
+    st, sh, _ = qi.stride()
+    ot, oh, _ = qo.stride()
+    ko = None
     if k is None:
         tail = (None, 0, 0, None, 0, 0, 0)
     else:
-        tail = (ki.data_ptr(), ki.stride(0), ki.stride(1), ko.data_ptr(), ko.stride(0), ko.stride(1), k.shape[1])
-    with _on(q.device):
+        ki = k if k.stride(2) == 1 else k.contiguous()
+        ko = torch.empty_like(ki, memory_format=torch.contiguous_format) if out is None else out[1]
+        tail = (ki.data_ptr(), *ki.stride()[:2], ko.data_ptr(), *ko.stride()[:2], ki.shape[1])
+    dev = q.device
+    with _on(dev):
         rc = _lib.load().wkv_rotary(
-            _DTYPES[q.dtype], qi.data_ptr(), qi.stride(0), qi.stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1),
-            q.shape[1], *tail, q.shape[2], positions.data_ptr(), inv_freq.data_ptr(), 2 * inv_freq.shape[0],
-            int(interleaved), int(inverse), float(scale), q.shape[0], _stream(q.device))
+            _DTYPES[q.dtype], qi.data_ptr(), st, sh, qo.data_ptr(), ot, oh, hq, *tail, d, positions.data_ptr(),
+            inv_freq.data_ptr(), 2 * inv_freq.shape[0], interleaved, inverse, scale, tokens, _stream(dev))
     _lib.check(rc, "apply_rotary")
     return qo, ko
 
@@ -147,14 +141,25 @@ class _Rotary(torch.autograd.Function):
     def forward(ctx, q, k, positions, inv_freq, interleaved, scale, inverse):
         ctx.save_for_backward(positions, inv_freq)
         ctx.how = (interleaved, scale, inverse)
+        ctx.set_materialize_grads(False)
         return _launch(q, k, positions, inv_freq, interleaved, scale, inverse, None)
 
     @staticmethod
     def backward(ctx, gq, gk):
-        positions, inv_freq = ctx.saved_tensors
-        interleaved, scale, inverse = ctx.how
-        gq, gk = _Rotary.apply(gq, gk, positions, inv_freq, interleaved, scale, not inverse)
+        gq, gk = (g if need else None for g, need in zip((gq, gk), ctx.needs_input_grad))
+        lone = gk if gq is None else None  # k's alone
+        if gq is not None or gk is not None:
+            interleaved, scale, inverse = ctx.how
+            turn = _Rotary.apply if torch.is_grad_enabled() else _launch_back
+            gq, gk = turn(gq if lone is None else lone, gk if lone is None else None, *ctx.saved_tensors, interleaved,
+                          scale, not inverse)
+        if lone is not None:
+            gq, gk = None, gq
         return gq, gk, None, None, None, None, None
+
+
+def _launch_back(*args):
+    return _launch(*args, None)
 
 
 def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, *,
