@@ -14,7 +14,7 @@
 // 2^-7 of a radian. Sines and products are float32, one rounding to the
 // type at the end.
 // Bound by HBM past some thousand tokens (16,384 tokens of 40 heads of 128, bf16, in
-// either layout: 55 us, 6.1 TB/s), by the launch and one round trip for a single one
+// either layout: 61 us, 5.5 TB/s), by the launch and one round trip for a single one
 // (3.4 us).
 #include <cmath>
 
@@ -53,7 +53,7 @@ __device__ __forceinline__ float to_f32(T x) {
 // in two runs of V elements: half apart, or (INTER, and what is only copied) half
 // the units apart, so that the lanes' runs follow each other; single elements
 // (V = 1) of an INTER pair are adjacent.
-// FAR: rows read past the caches.
+// FAR: rows read and written past the caches.
 template <class T, int V, bool INTER, bool FAR>
 __global__ __launch_bounds__(64 * kRotaryWaves) void rotary_kernel(RotaryArgs a) {
   typedef __attribute__((__vector_size__(V * sizeof(T)))) T Vec;
@@ -142,8 +142,13 @@ __global__ __launch_bounds__(64 * kRotaryWaves) void rotary_kernel(RotaryArgs a)
 #pragma unroll
         for (int v = 0; v < V; ++v) turn_runs(v, v, first[k] + v);
       }
-      *reinterpret_cast<Vec *>(y0[k]) = x0[k];
-      *reinterpret_cast<Vec *>(y1[k]) = x1[k];
+      if (FAR) {
+        __builtin_nontemporal_store(x0[k], reinterpret_cast<Vec *>(y0[k]));
+        __builtin_nontemporal_store(x1[k], reinterpret_cast<Vec *>(y1[k]));
+      } else {
+        *reinterpret_cast<Vec *>(y0[k]) = x0[k];
+        *reinterpret_cast<Vec *>(y1[k]) = x1[k];
+      }
     }
   }
 }
@@ -232,8 +237,9 @@ extern "C" int wkv_rotary(int32_t dtype, const void *q, int64_t q_stride_t, int6
   a.per = (H + split - 1) / split;
   const dim3 grid(static_cast<unsigned>((num_tokens + kRotaryWaves - 1) / kRotaryWaves),
                   static_cast<unsigned>((H + a.per - 1) / a.per));
-  // Rows far larger than the caches are read past them (32 query and 8 key heads of
-  // 128, bf16, near / far: 4,096 tokens 16.0 / 18.6 us, 6,144 26.4 / 24.9, 16,384 69 / 55).
+  // Rows far larger than the caches go past them (32 query and 8 key heads of 128,
+  // bf16, near / far: 4,096 tokens 16.0 / 18.6 us, 16,384 into new memory 72 / 61, 32,768
+  // 131 / 117; stored near, 16,384 take 65 into new memory and 55 into memory just written).
   const bool far = static_cast<int64_t>(num_tokens) * H * head_dim * esz >= (64 << 20);
   auto s = static_cast<hipStream_t>(stream);
   if (dtype == 0) {
