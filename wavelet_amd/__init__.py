@@ -20,6 +20,8 @@ Public surface (a drop-in for the KV path of the reference's inference engine):
   and around it: ``extend_tables`` (a step's blocks, slots, positions and tree
   masks on the GPU), ``accept_tree`` (the path that the sampled tokens
   agree with) and ``PagedKVCache.compact`` (its keys and values moved together);
+  ``KVPool.lend`` / ``settle`` -- the blocks and lengths of such steps, lent to
+  the device and taken back (``StepState``);
 * ``apply_rotary`` / ``rotary_frequencies`` -- rotary positions of queries and
   keys, with gradients;
 * ``sample`` -- the token sampler after decode (temperature, min_p, top_k,
@@ -27,7 +29,7 @@ Public surface (a drop-in for the KV path of the reference's inference engine):
 
 Also, by module: ``wavelet_amd.plan`` -- a whole decode or prompt step over
 every layer, built once and launched per step (``DecodeStep``,
-``MLADecodeStep``, ``PrefillStep``), and ``GraphDecodeStep``, the decode step
+``MLADecodeStep``, ``PrefillStep``, ``TreeStep``), and ``GraphDecodeStep``, the decode step
 captured in one HIP graph; ``wavelet_amd.hf`` -- a transformers ``Cache`` over
 a ``KVPool`` and the ``"wavelet_paged"`` attention implementation.
 """
@@ -39,7 +41,7 @@ from .cache import MLALatentCache, PagedKVCache, validate_group_prefix, validate
 from .pool import KVPool
 from .rotary import apply_rotary, rotary_frequencies
 from .sampler import sample
-from .step import Accepted, StepMaps, accept_tree, extend_tables
+from .step import Accepted, StepMaps, StepState, accept_tree, extend_tables
 
 __all__ = [
     "Accepted",
@@ -48,6 +50,7 @@ __all__ = [
     "MLALatentCache",
     "PagedKVCache",
     "StepMaps",
+    "StepState",
     "accept_tree",
     "apply_rotary",
     "decode_order",

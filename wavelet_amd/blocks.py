@@ -37,6 +37,14 @@ class _Seq:
     length: int = 0
 
 
+@dataclass
+class Loan:
+    """Blocks lent to the device for the next steps of some sequences (``BlockManager.lend``)."""
+
+    seq_ids: list
+    blocks: list[int]  # in the order in which they are to be taken
+
+
 class BlockManager:
     """Allocates physical KV blocks to sequences; one table per sequence."""
 
@@ -55,6 +63,7 @@ class BlockManager:
         self._free: deque[int] = deque(range(self.num_blocks))
         self._ref = np.zeros(self.num_blocks, dtype=np.int64)
         self._seqs: dict[object, _Seq] = {}
+        self._lent: set = set()  # sequences whose tables the device extends (``lend``)
         self._index: dict[bytes, int] = {}  # full-block chain hash -> block id
         self._hash_of: dict[int, bytes] = {}  # block id -> its chain hash (indexed blocks)
         self._evictable: OrderedDict[int, None] = OrderedDict()  # indexed blocks with ref 0, LRU first
@@ -169,6 +178,7 @@ class BlockManager:
     def share_prefix(self, src_seq, dst_seqs, n_blocks: int | None) -> None:
         """New sequences ``dst_seqs`` start with ``src_seq``'s first ``n_blocks`` blocks (all if None)."""
         src = self._seqs[src_seq]
+        self._own(src_seq)
         n = len(src.blocks) if n_blocks is None else int(n_blocks)
         if n > len(src.blocks):
             raise ValueError(f"{src_seq!r} has only {len(src.blocks)} blocks")
@@ -193,6 +203,7 @@ class BlockManager:
         need = 0
         for sid in seq_ids:
             seq = self._seqs[sid]
+            self._own(sid)
             if self.max_model_len is not None and seq.length + num_tokens > self.max_model_len:
                 raise ValueError(f"sequence {sid!r} at {seq.length} tokens cannot take {num_tokens} more: "
                                  f"max_model_len is {self.max_model_len}")
@@ -247,6 +258,84 @@ class BlockManager:
         """Blocks ``append_slots(seq_ids, num_tokens)`` would take from the free pool."""
         return self._append_plan(list(seq_ids), int(num_tokens))
 
+    # -- tables extended on the device ------------------------------------------
+    def _own(self, seq_id) -> None:
+        if seq_id in self._lent:
+            raise ValueError(f"the device extends the table of sequence {seq_id!r}: settle its loan first")
+
+    def lend(self, seq_ids, num_blocks: int) -> tuple[Loan, list[tuple[int, int]]]:
+        """Take ``num_blocks`` free blocks for the device to extend these sequences' tables with
+        (``extend_tables``), over any number of steps, until ``settle``.
+
+        Also returns the copy-on-write pairs to apply first (as ``append_slots``): each sequence's
+        partly filled last block becomes its own. Until it is settled the manager neither changes
+        nor frees these sequences. Raises MemoryError, before any state moves, when too few blocks are free.
+        """
+        seq_ids, num_blocks = list(seq_ids), int(num_blocks)
+        if num_blocks < 0:
+            raise ValueError(f"num_blocks must be non-negative (got {num_blocks})")
+        if len(set(seq_ids)) != len(seq_ids):
+            raise ValueError("a sequence is listed twice")
+        held: dict[int, int] = {}  # shared partly filled block -> references left
+        copies = []
+        for sid in seq_ids:
+            seq = self._seqs[sid]
+            self._own(sid)
+            if seq.length % self.block_size:
+                last = seq.blocks[seq.length // self.block_size]
+                refs = held.get(last, int(self._ref[last]))
+                if refs > 1:
+                    copies.append(seq)
+                    held[last] = refs - 1
+        need = num_blocks + len(copies)
+        if need > self.num_free_blocks:
+            raise MemoryError(f"out of KV cache blocks: the loan needs {need}, {self.num_free_blocks} are free")
+        cow = []
+        for seq in copies:
+            at = seq.length // self.block_size
+            last, fresh = seq.blocks[at], self._take()
+            cow.append((last, fresh))
+            self._release(last)
+            seq.blocks[at] = fresh
+        loan = Loan(seq_ids, [self._take() for _ in range(num_blocks)])
+        self._lent.update(seq_ids)
+        return loan, cow
+
+    def settle(self, loan: Loan, block_table, held_blocks, seq_lens) -> None:
+        """Take over what the device made of a loan: row ``i`` of ``block_table`` (its first ``held_blocks[i]``
+        entries) and ``seq_lens[i]`` are sequence ``loan.seq_ids[i]``'s table and length; lent blocks that no
+        length needs go back to the free pool. Raises ValueError, before any state moves, for tables
+        that do not continue the sequences' own with lent blocks, each used once."""
+        tables, held, lens = (np.asarray(x, dtype=np.int64) for x in (block_table, held_blocks, seq_lens))
+        n = len(loan.seq_ids)
+        if tables.ndim != 2 or not len(tables) == len(held) == len(lens) == n:
+            raise ValueError(f"the loan is of {n} sequences")
+        if any(sid not in self._lent for sid in loan.seq_ids):
+            raise ValueError("the loan is settled already")
+        unused = set(loan.blocks)
+        if len(unused) != len(loan.blocks):
+            raise ValueError("the loan names a block twice")
+        kept = []
+        for i, sid in enumerate(loan.seq_ids):
+            seq = self._seqs[sid]
+            have = len(seq.blocks)
+            if not have <= held[i] <= tables.shape[1] or not seq.length <= lens[i] <= held[i] * self.block_size:
+                raise ValueError(f"sequence {sid!r}: {int(held[i])} blocks and {int(lens[i])} tokens do not continue "
+                                 f"its {have} and {seq.length}")
+            row = tables[i, :held[i]].tolist()
+            if row[:have] != seq.blocks or not unused.issuperset(row[have:]) or len(set(row[have:])) != held[i] - have:
+                raise ValueError(f"sequence {sid!r}: its table is not its own blocks and lent ones")
+            need = max(-(-int(lens[i]) // self.block_size), have)
+            unused.difference_update(row[have:])
+            kept.append(row[:need])
+        used = {b for row, sid in zip(kept, loan.seq_ids) for b in row[len(self._seqs[sid].blocks):]}
+        for row, sid, length in zip(kept, loan.seq_ids, lens.tolist()):
+            self._seqs[sid].blocks, self._seqs[sid].length = row, length
+        for b in loan.blocks:
+            if b not in used:
+                self._release(b)
+        self._lent.difference_update(loan.seq_ids)
+
     def any_shared(self, seq_ids) -> bool:
         """Whether any block of these sequences is held by more than one sequence: a
         decode step over them then reads such blocks more than once, and should keep
@@ -259,6 +348,8 @@ class BlockManager:
 
     def free(self, seq_id) -> None:
         """Release a finished sequence's blocks (indexed prompt blocks stay matchable)."""
+        if seq_id in self._seqs:
+            self._own(seq_id)
         seq = self._seqs.pop(seq_id)
         for b in reversed(seq.blocks):
             self._release(b)

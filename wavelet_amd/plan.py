@@ -23,7 +23,8 @@ import torch
 
 from . import _lib
 from .attention import _workspace, decode_plan
-from .cache import KV_DTYPES, PagedKVCache, _require_cuda, check_tables
+from .cache import KV_DTYPES, PagedKVCache, _on, _require_cuda, _stream, check_tables
+from .step import MAX_DEPTH, MAX_NODES, Accepted, StepState, accept_tree, new_step_maps
 
 
 # Smallest B * Hkv * max_seq_len (token-heads) for which DecodeStep orders
@@ -462,3 +463,126 @@ class PrefillStep:
     def run(self) -> None:
         for layer in range(len(self.calls)):
             self.step_layer(layer)
+
+
+class TreeStep:
+    """A step of drafted tokens for every layer, whose lengths stay on the device.
+
+    ``state`` (``KVPool.lend``) holds the sequences' tables and lengths. A step is ``begin()`` -- sequence
+    ``b``'s ``new_lens[b]`` tokens, node 0 the last token sampled and behind it what was drafted, get
+    blocks, slots, positions and tree masks (``extend_tables``) --, then ``step_layer(l)`` for every
+    layer once its ``q[l]`` ``[T, Hq, D]``, ``key[l]`` / ``value[l]`` ``[T, Hkv, D]`` are there: queries and keys
+    are turned in place by their positions (``inv_freq`` from ``rotary_frequencies``; None: they come
+    turned), keys and values appended, and ``out[l]`` is their attention over context and tree
+    (``paged_tree_gqa``) --, then ``finish()`` once ``target_tokens`` holds what was sampled after every
+    node: the path that agrees is accepted (``accept_tree``), its keys and values move together in every layer's
+    cache (``compact``) and ``state.seq_lens`` moves on. ``maps`` and ``accepted`` are the step's results;
+    ``accepted.next_tokens`` are the next step's first nodes.
+
+    ``new_lens [B]``, ``parents [T]`` (int32), ``draft_tokens [T]``, ``target_tokens [T]`` (int64) and the
+    layers' buffers are refilled in place between steps. ``max_nodes`` (a multiple of 64 up to 256) and
+    ``max_seq_len`` bound the trees and the lengths with them, ``max_depth`` the accepted path. ``shared_blocks``
+    is the read policy (None: each cache's default; ``KVPool.decode_shares_blocks``). Nothing is allocated
+    after the constructor and everything runs on the current stream: the three calls can be
+    captured in graphs; steps of one plan, or of plans over one state, must not overlap.
+    """
+
+    def __init__(self, caches: list[PagedKVCache], q: list[torch.Tensor], key: list[torch.Tensor],
+                 value: list[torch.Tensor], out: list[torch.Tensor], state: StepState, new_lens: torch.Tensor,
+                 parents: torch.Tensor, draft_tokens: torch.Tensor, target_tokens: torch.Tensor, scale: float,
+                 max_nodes: int, max_seq_len: int, max_depth: int, *, inv_freq: torch.Tensor | None = None,
+                 rotary_scale: float = 1.0, interleaved: bool = False, shared_blocks: bool | None = None) -> None:
+        if not caches:
+            raise ValueError("no layers")
+        if not len(q) == len(key) == len(value) == len(out) == len(caches):
+            raise ValueError("q, key, value and out need one tensor per layer")
+        dev = self.device = caches[0].device
+        if any(c.block_size != state.block_size or c.device != dev for c in caches):
+            raise ValueError(f"the caches must have the state's blocks of {state.block_size} tokens, on {dev}")
+        check_tables(state.block_table, state.seq_lens, dev, state.block_size, strict=True)
+        if not 0 < max_nodes <= MAX_NODES or max_nodes % 64:
+            raise ValueError(f"max_nodes must be a multiple of 64 up to {MAX_NODES} (got {max_nodes})")
+        if not 1 <= max_depth <= MAX_DEPTH:
+            raise ValueError(f"max_depth must be in [1, {MAX_DEPTH}] (got {max_depth})")
+        T, batch = parents.shape[0], state.block_table.shape[0]
+        for name, t, n, dtype in (("new_lens", new_lens, batch, torch.int32), ("parents", parents, T, torch.int32),
+                                  ("draft_tokens", draft_tokens, T, torch.int64),
+                                  ("target_tokens", target_tokens, T, torch.int64)):
+            if t.dtype != dtype or tuple(t.shape) != (n,) or not t.is_contiguous() or t.device != dev:
+                raise ValueError(f"{name} must be a contiguous {dtype} [{n}] tensor on {dev}")
+        if inv_freq is not None and (inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.device != dev
+                                     or not inv_freq.is_contiguous()):
+            raise ValueError(f"inv_freq must be a contiguous float64 vector on {dev}")
+        self.state, self.new_lens, self.parents = state, new_lens, parents
+        self.draft_tokens, self.target_tokens = draft_tokens, target_tokens
+        self.max_nodes, self.max_depth = int(max_nodes), int(max_depth)
+        self.caches = list(caches)
+        self._live = _Live(caches)
+        m = self.maps = new_step_maps(batch, T, max_nodes, dev)._replace(held_blocks=state.held_blocks, taken=state.taken)
+        self.accepted = Accepted(torch.zeros(batch, dtype=torch.int32, device=dev),
+                                 torch.full((batch, max_depth), -1, dtype=torch.int32, device=dev),
+                                 torch.zeros(batch, dtype=torch.int64, device=dev),
+                                 torch.zeros(batch, dtype=torch.int32, device=dev))
+        self.lib = lib = _lib.load()
+        need = max(lib.wkv_tree_workspace_size(batch, KV_DTYPES[c.kv_dtype], c.num_kv_heads, qq.shape[1], c.head_dim,
+                                               min(max_nodes, T), int(max_seq_len)) for c, qq in zip(caches, q))
+        if need < 0:
+            raise ValueError("invalid tree attention geometry")
+        self.workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+        bt = state.block_table
+        self.calls = []
+        for layer, (cache, qq, kk, vv, oo) in enumerate(zip(caches, q, key, value, out)):
+            hq, d = qq.shape[1], cache.head_dim
+            for name, t, shape in (("q", qq, (T, hq, d)), ("out", oo, (T, hq, d)), ("key", kk, (T, cache.num_kv_heads, d)),
+                                   ("value", vv, (T, cache.num_kv_heads, d))):
+                if t.dtype != torch.bfloat16 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != dev:
+                    raise ValueError(f"layer {layer}: {name} must be a contiguous bfloat16 {shape} tensor on {dev}")
+            rotary = None
+            if inv_freq is not None:
+                if not 0 < 2 * inv_freq.shape[0] <= d:
+                    raise ValueError(f"layer {layer}: inv_freq turns {2 * inv_freq.shape[0]} of {d} dims")
+                rotary = (1, *(x for t in (qq, kk) for x in (t.data_ptr(), t.stride(0), t.stride(1)) * 2 + (t.shape[1],)),
+                          d, m.positions.data_ptr(), inv_freq.data_ptr(), 2 * inv_freq.shape[0], int(interleaved), 0,
+                          ctypes.c_float(rotary_scale), T)
+            attend = (ctypes.byref(cache.descriptor(shared_blocks)), kk.data_ptr(), kk.stride(0), kk.stride(1),
+                      vv.data_ptr(), vv.stride(0), vv.stride(1), m.slot_mapping.data_ptr(), T, qq.data_ptr(), qq.stride(0),
+                      qq.stride(1), oo.data_ptr(), oo.stride(0), oo.stride(1), hq, m.cu_seqlens_q.data_ptr(),
+                      m.context_lens.data_ptr(), bt.data_ptr(), bt.stride(0), bt.shape[1], batch, min(max_nodes, T),
+                      min(int(max_seq_len), bt.shape[1] * cache.block_size), m.tree_mask.data_ptr(), m.tree_mask.shape[1],
+                      ctypes.c_float(scale), self.workspace.data_ptr() if need > 0 else None, max(need, 0), None)
+            self.calls.append((rotary, attend))
+        self._keep = (q, key, value, out, inv_freq)
+
+    def begin(self) -> None:
+        """The step's blocks, slots, positions and masks."""
+        self.state.extend(self.new_lens, self.parents.shape[0], parents=self.parents, max_nodes=self.max_nodes,
+                          out=self.maps)
+
+    def step_layer(self, layer: int) -> None:
+        """One layer's rotation, append and attention."""
+        self._live.check(layer)
+        rotary, attend = self.calls[layer]
+        with _on(self.device):
+            stream = _stream(self.device)
+            if rotary is not None:
+                rc = self.lib.wkv_rotary(*rotary, stream)
+                if rc:
+                    _lib.check(rc, f"rotary layer {layer}")
+            rc = self.lib.wkv_tree_gqa(*attend, stream)
+            if rc:
+                _lib.check(rc, f"tree attention layer {layer}")
+
+    def run(self) -> None:
+        """``step_layer`` of every layer."""
+        for layer in range(len(self.calls)):
+            self.step_layer(layer)
+
+    def finish(self) -> None:
+        """Accept what agrees with ``target_tokens``, move its keys and values together, and the lengths on."""
+        self._live.check_all()
+        m, s, a = self.maps, self.state, self.accepted
+        accept_tree(self.draft_tokens, self.parents, self.target_tokens, m.cu_seqlens_q, s.seq_lens, m.context_lens,
+                    self.max_depth, out=a)
+        for cache in self.caches:
+            cache.compact(s.block_table, s.seq_lens, a.path, a.accepted)
+        s.seq_lens.copy_(a.seq_lens)

@@ -21,6 +21,7 @@ import torch
 
 from .blocks import BlockManager
 from .cache import MLALatentCache, PagedKVCache
+from .step import StepState
 
 
 # Device memory a pool sized from the engine's knobs leaves unclaimed beyond
@@ -171,6 +172,29 @@ class KVPool:
         slots, cow = self.blocks.append_slots(seq_ids, num_tokens)
         self.copy_blocks(cow)
         return torch.from_numpy(slots).to(self.device)
+
+    def lend(self, seq_ids, num_blocks: int, *, width: int | None = None) -> StepState:
+        """The sequences' tables and lengths on the device, with ``num_blocks`` free blocks to extend them by there
+        (``BlockManager.lend``), for steps whose token counts the host does not know (``StepState``,
+        ``TreeStep``). A partly filled block that is shared is copied first. ``width`` (blocks per table) defaults to
+        ``max_blocks_per_seq``, without a ``max_model_len`` to the longest table and the loan."""
+        seq_ids = list(seq_ids)
+        longest = max((len(self.blocks.blocks_of(s)) for s in seq_ids), default=0)
+        if width is None:
+            width = self.blocks.max_blocks_per_seq or longest + int(num_blocks)
+        if not seq_ids or width < max(longest, 1):
+            raise ValueError(f"a loan needs sequences and tables of at least {max(longest, 1)} blocks")
+        loan, cow = self.blocks.lend(seq_ids, num_blocks)
+        self.copy_blocks(cow)
+        table, lens = self.blocks.tables(seq_ids, width)
+        held = np.array([len(self.blocks.blocks_of(s)) for s in seq_ids], dtype=np.int32)
+        dev = self.device
+        return StepState(*(torch.from_numpy(x).to(dev) for x in (
+            table, held, lens, np.array(loan.blocks, dtype=np.int32), np.zeros(1, dtype=np.int32))), self.block_size, loan)
+
+    def settle(self, state: StepState) -> None:
+        """Hand a loan's tables and lengths back to the block manager (waits for the device)."""
+        self.blocks.settle(state.loan, *(x.cpu().numpy() for x in (state.block_table, state.held_blocks, state.seq_lens)))
 
     def decode_shares_blocks(self, seq_ids) -> bool:
         """The read policy of a decode step over ``seq_ids``: True when some block is held by

@@ -10,6 +10,7 @@ instead, in one launch (or two) per step for every layer.
 
 from __future__ import annotations
 
+from dataclasses import dataclass
 from typing import NamedTuple
 
 import torch
@@ -44,11 +45,36 @@ class Accepted(NamedTuple):
     seq_lens: torch.Tensor     # [B] int32
 
 
+@dataclass
+class StepState:
+    """The sequences of the next steps as the device carries them on (``KVPool.lend``): ``extend`` gives a
+    step's tokens their blocks and slots, an accepted path's lengths go back into ``seq_lens``, and
+    ``KVPool.settle`` hands tables and lengths to the block manager."""
+
+    block_table: torch.Tensor  # [B, M] int32
+    held_blocks: torch.Tensor  # [B] int32
+    seq_lens: torch.Tensor     # [B] int32
+    free_blocks: torch.Tensor  # [F] int32
+    taken: torch.Tensor        # [1] int32
+    block_size: int
+    loan: object = None        # the block manager's
+
+    def extend(self, new_lens: torch.Tensor, max_tokens: int, *, parents: torch.Tensor | None = None,
+               max_nodes: int = 0, out: StepMaps | None = None) -> StepMaps:
+        """``extend_tables`` of this state, in place (``held_blocks`` and ``taken`` of the result are the state's)."""
+        if out is None:
+            out = new_step_maps(self.block_table.shape[0], max_tokens, max_nodes, self.block_table.device)
+        return extend_tables(self.block_table, self.held_blocks, self.seq_lens, new_lens, self.free_blocks, self.taken,
+                             self.block_size, max_tokens, parents=parents, max_nodes=max_nodes,
+                             out=out._replace(held_blocks=self.held_blocks, taken=self.taken))
+
+
 def _vector(x: torch.Tensor, name: str, n: int | None, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    if isinstance(x, torch.Tensor) and x.device == device and x.dtype == dtype and x.dim() == 1 \
+            and (n is None or x.shape[0] == n):
+        return x.contiguous()
     _require_cuda(x, name, device)
-    if x.dtype != dtype or x.dim() != 1 or (n is not None and x.shape[0] != n):
-        raise ValueError(f"{name} must be {dtype} [{'n' if n is None else n}] (got {x.dtype} {tuple(x.shape)})")
-    return x.contiguous()
+    raise ValueError(f"{name} must be {dtype} [{'n' if n is None else n}] (got {x.dtype} {tuple(x.shape)})")
 
 
 def _outputs(out, kinds, device: torch.device, what: str):
@@ -68,6 +94,14 @@ def _new_outputs(longs: tuple[int, ...], ints: tuple[int, ...], device: torch.de
     room += room & 1
     *a, b = torch.empty(sum(longs) + room // 2, dtype=torch.int64, device=device).split_with_sizes((*longs, room // 2))
     return a, b.view(torch.int32).split_with_sizes((*ints, room - sum(ints)))
+
+
+def new_step_maps(batch: int, max_tokens: int, max_nodes: int, device: torch.device) -> StepMaps:
+    """Tensors for ``extend_tables``'s ``out``."""
+    words = max_nodes // 64
+    (slots, positions, mask), (context, cu, held, refused, taken, _) = _new_outputs(
+        (max_tokens, max_tokens, max_tokens * words), (batch, batch + 1, batch, 1, 1), device)
+    return StepMaps(context, cu, slots, positions, mask.view(max_tokens, words) if words else None, refused, held, taken)
 
 
 def extend_tables(block_table: torch.Tensor, held_blocks: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch.Tensor,
@@ -119,10 +153,7 @@ def extend_tables(block_table: torch.Tensor, held_blocks: torch.Tensor, seq_lens
         parents = _vector(parents, "parents", max_tokens, torch.int32, dev)
     words = max_nodes // 64
     if out is None:
-        (slots, positions, mask), (context, cu, held_after, refused, taken_after, _) = _new_outputs(
-            (max_tokens, max_tokens, max_tokens * words), (batch, batch + 1, batch, 1, 1), dev)
-        m = StepMaps(context, cu, slots, positions, mask.view(max_tokens, words) if words else None, refused, held_after,
-                     taken_after)
+        m = new_step_maps(batch, max_tokens, max_nodes, dev)
     else:
         m = StepMaps(*_outputs(out, (("context_lens", (batch,), torch.int32), ("cu_seqlens_q", (batch + 1,), torch.int32),
                                      ("slot_mapping", (max_tokens,), torch.int64), ("positions", (max_tokens,), torch.int64),
