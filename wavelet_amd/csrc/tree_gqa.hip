@@ -318,8 +318,8 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
   float m_ref = -INFINITY, l_part = 0.f;  // reference maximum (-inf until a key is seen), this lane's share of the sum
 
   // Copies. Piece p = 64 k + l of a tile's K or V goes to LDS offset 16 p. K: chunk p / 16,
-  // token p % 16, as the cache holds it. bf16 V: row p % D of token octet p / D;
-  // fp8 V: row p.
+  // token p % 16, as the cache holds it. bf16 V: row p / 2, its token octets in turn (octet 1
+  // first in every second four rows, for the banks); fp8 V: row p.
   const int BS = a.BS, region = D * BS * ESZ, Hkv = a.Hkv, nb = a.nb, Mb = a.Mb;
   const uint8_t *const kc = a.kc, *const vc = a.vc;
   const float *const ksc = a.ksc, *const vsc = a.vsc;
@@ -393,20 +393,17 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
     v_land = v_ok;
     if (v_ok) {
       vs_land = vs_next;
-      const uint32_t lane_v = static_cast<uint32_t>(lane_here() * BS * ESZ);
-      uint32_t vst = static_cast<uint32_t>((FP8 ? 64 : 128) * BS);
+      const int l = lane_here();
+      const uint32_t lane_v = static_cast<uint32_t>(FP8 ? l * BS : (l >> 1) * BS * 2 + 16 * ((l ^ l >> 3) & 1));
+      uint32_t vst = static_cast<uint32_t>(64 * BS);
       asm volatile("" : "+s"(vst));
       const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(
           const_cast<uint8_t *>(wave_uniform(vc + vbase)), 0, region, kRawBufferWord3);
       const uint32_t dst = __builtin_amdgcn_readfirstlane(ldsv0 + static_cast<uint32_t>((4 * (s & 1) + wave) * TB));
-      auto off = [&](int k) { return FP8 ? vst * k : vst * (k % DV) + 16 * (k / DV); };
-      if (stream) {
-#pragma unroll
-        for (int k = 0; k < NC; ++k) buffer_copy16_to_lds_nt(vr, lane_v, off(k), dst + 1024 * k);
-      } else {
-#pragma unroll
-        for (int k = 0; k < NC; ++k) buffer_copy16_to_lds(vr, lane_v, off(k), dst + 1024 * k);
-      }
+      if (stream)
+        buffer_copy16_run_to_lds_nt<NC>(vr, lane_v, vst - 1024u, dst);
+      else
+        buffer_copy16_run_to_lds<NC>(vr, lane_v, vst - 1024u, dst);
     }
   };
   // fp8: this wave's landed codes widened in their place. Piece p = 64 i + l of K: chunk
@@ -426,8 +423,10 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
     for (int i = 0; i < D / 64; ++i) {
       const int p = 64 * i + lane;
       if (do_v) {
-        *reinterpret_cast<u32x4 *>(tv + p * 16) = codes_to_bf16(wv[i][0], wv[i][1], vs_land);
-        *reinterpret_cast<u32x4 *>(tv + (D + p) * 16) = codes_to_bf16(wv[i][2], wv[i][3], vs_land);
+        uint8_t *d = tv + p * 32;
+        const int first = 4 * (p & 4);  // where the row's octet 0 goes
+        *reinterpret_cast<u32x4 *>(d + first) = codes_to_bf16(wv[i][0], wv[i][1], vs_land);
+        *reinterpret_cast<u32x4 *>(d + 16 - first) = codes_to_bf16(wv[i][2], wv[i][3], vs_land);
       }
       if (do_k) {
         uint8_t *d = tk + ((2 * (p >> 4)) * 16 + (p & 15)) * 16;
@@ -574,13 +573,13 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
   };
   // P V^T of step s
   auto pv = [&](int s) __attribute__((always_inline)) {
-    const uint8_t *lv = ldsv + (s & 1) * 4 * TB + (hh * D + n) * 16;
+    const uint8_t *lv = ldsv + (s & 1) * 4 * TB + n * 32 + 16 * (hh ^ ((n >> 2) & 1));
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const bf16x8 pb = __builtin_bit_cast(bf16x8, (u32x4{pw[t][0], pw[t][1], pw[t][2], pw[t][3]}));
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(lv + t * TB + 32 * c * 16);
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(lv + t * TB + 1024 * c);
         o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w), pb, o[c], 0, 0, 0);
       }
     }
@@ -591,7 +590,7 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
   // where they stand with what is seen count.
   auto pv_masked = [&](int s) __attribute__((always_inline)) {
     const int l = lane_here(), n = l & 31, hh = l >> 5;
-    const uint8_t *const lv = ldsv + (s & 1) * 4 * TB + (hh * D + n) * 16;
+    const uint8_t *const lv = ldsv + (s & 1) * 4 * TB + n * 32 + 16 * (hh ^ ((n >> 2) & 1));
     bool odd = false;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -599,7 +598,7 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
       if (left <= 0) continue;  // uniform
       u32x4 w[D / 32];
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) w[c] = *reinterpret_cast<const u32x4 *>(lv + t * TB + 32 * c * 16);
+      for (int c = 0; c < D / 32; ++c) w[c] = *reinterpret_cast<const u32x4 *>(lv + t * TB + 1024 * c);
       if (left < 16) {  // uniform
 #pragma unroll
         for (int c = 0; c < D / 32; ++c)
@@ -637,7 +636,7 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
         vis[i] = (seen >> (16 * t + 2 * i) & 1 ? 0x3F80u : 0u) | (seen >> (16 * t + 2 * i + 1) & 1 ? 0x3F800000u : 0u);
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(lv + t * TB + 32 * c * 16);
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(lv + t * TB + 1024 * c);
 #pragma unroll
         for (int sign = 0; sign < 2; ++sign) {  // 1 where V is a NaN or the infinity of this sign
           const uint32_t inf = sign ? 0xFF80u : 0x7F80u;
