@@ -9,18 +9,21 @@
 // node together, are taken 32 at a time by a wave (a unit: the columns of its
 // 32x32x16 MFMAs), four units to a workgroup (a row group), so that up to 128
 // rows share one read of the keys. Keys go in steps of 64, copied to LDS by
-// LDS-DMA, a 16-key tile by each wave; a wave without rows only copies. The
+// LDS-DMA, a 16-key tile by each wave. A row group of at most two units has two waves
+// on each, for 32 keys of every step each, and joins them in LDS; in a larger one a
+// wave without rows only copies. The
 // steps of all row groups form one line that the workgroups share evenly
 // (tree_prefix), whatever the mix of lengths; a row group cut between workgroups
 // leaves fp32 partials that a second kernel merges by log-sum-exp.
 //
-// Bound by reading K and V once for up to 64 rows of bf16, by the MFMAs past that and in
-// fp8. Measured with the append of the drafted tokens, 32 query and 8 KV heads of 128:
-// 64 sequences of 2,000 tokens with 8 drafted each, bf16, 186 us (5.9 TB/s; a chunk of each
-// sequence per workgroup, with cached reads: 206); 5 sequences of 700 to 15,000 tokens
-// with 40 to 64 drafted, fp8, 70 us (386 TFLOP/s; chunks: 172); 4 of 8,192 with 128 drafted
-// 110 us in bf16 and 102 in fp8 (630 and 676 TFLOP/s; chunks: 109 and 107). What a step
-// costs beside its MFMAs is mostly the issue of its copies (1 KB per instruction).
+// Bound by reading K and V once for up to 64 rows of bf16, by the step's own chain
+// (products, exponents, the copies' issue, a barrier) past that and in fp8. Measured, 32 query and
+// 8 KV heads of 128: 64 sequences of 4,096 tokens with 16 drafted each, bf16, 183 us
+// (6.0 TB/s; a chunk of each sequence per workgroup, with cached reads: 206); 6 of 3,000 to 24,000
+// with 5 to 63 drafted, 28 and 4 heads, fp8, 65 us (411 TFLOP/s; chunks: 172); 64 of 4,096
+// with 8 drafted, fp8, with their append, 121 us (4.5 TB/s; with one wave per unit 140); 4 of
+// 8,192 with 128 drafted and their append 107 us in bf16 and 102 in fp8 (646 and 678 TFLOP/s; the
+// matrix unit is busy 41% of the time, the VALU 37%).
 //
 // Software pipeline, one barrier per step: while a wave finishes step s
 // (probabilities, PV products) it scores step s + 1, so that the matrix unit
@@ -176,20 +179,20 @@ __device__ __forceinline__ u32x4 codes_to_bf16(uint32_t lo, uint32_t hi, float s
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, sc, true))};
 }
 
-// SHARED: the workgroups share the line; else one row group each.
-template <int D, bool FP8, bool SHARED>
+// The workgroups share the line (a.share of them), or take one row group each.
+template <int D, bool FP8>
 __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kernel_args) {
   constexpr int ESZ = FP8 ? 1 : 2;
-  constexpr int TB = D * 16 * 2;         // bytes of a 16-key tile's K, and of its V, as bf16
+  constexpr int TB = D * 16 * 2;           // bytes of a 16-key tile's K, and of its V, as bf16
   constexpr int NC = D * 16 * ESZ / 1024;  // 1 KB copies of each
-  constexpr int DV = D / 64;             // bf16 V copies per token octet
   // bf16 tiles as the MFMAs read them: K [D / 8 chunks][16 tokens][16 bytes] as the
-  // cache holds it, V [2 token octets][D rows][8 tokens]. fp8 codes land at their tile's
-  // start: K [D / 16 chunks][16 tokens][16 bytes], V [D rows][16 tokens].
+  // cache holds it, V [D rows][2 token octets][8 tokens] (the octets swapped in every second
+  // four rows). fp8 codes land at their tile's start: K [D / 16 chunks][16 tokens][16 bytes],
+  // V [D rows][16 tokens].
   __shared__ __attribute__((aligned(16))) uint8_t ldsk[2 * 4 * TB];
   __shared__ __attribute__((aligned(16))) uint8_t ldsv[2 * 4 * TB];
   __shared__ __attribute__((aligned(16))) int s_ok[4][4];  // by step: the tile holds keys
-  __shared__ TreeShare s_share;                            // SHARED: how the line is shared, and
+  __shared__ TreeShare s_share;                            // how the line is shared, and
   __shared__ int s_place;                                  // this workgroup's place among those that do
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int lane = threadIdx.x & 63, n = lane & 31, hh = lane >> 5;
@@ -202,9 +205,9 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
   };
   const int id = blockIdx.x;
   int b, kvh, rg, s_begin = 0;
-  bool later = false;  // SHARED: past the share's first row group
-  int steps_left = 0;  // SHARED: of this workgroup's share
-  if constexpr (SHARED) {
+  bool later = false;  // past the share's first row group
+  int steps_left;      // of this workgroup's share
+  if (kernel_args.share > 0) {
     const TreeArgs &a = tree_args();
     int *pfx = reinterpret_cast<int *>(ldsk);
     const int per = (a.batch + kTreeThreads - 1) / kTreeThreads;
@@ -254,8 +257,11 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
     if (item >= a.batch * a.Hkv) return;
     b = item / a.Hkv;
     kvh = item - b * a.Hkv;
+    const TreeSeq s = tree_seq(a, b);
+    if (rg >= s.groups) return;
+    steps_left = s.steps;
   }
-  for (;;) {  // SHARED: the row groups of the share; else one
+  for (;;) {  // the row groups of the share
   const TreeArgs &a = tree_args();
   b = __builtin_amdgcn_readfirstlane(b);
   kvh = __builtin_amdgcn_readfirstlane(kvh);
@@ -266,16 +272,17 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
   const int all_steps = __builtin_amdgcn_readfirstlane(sq.steps);
   const int groups = __builtin_amdgcn_readfirstlane(sq.groups);
   if (rg < groups) {  // else no row: the whole workgroup goes on together
-  int take = all_steps - s_begin;
-  if constexpr (SHARED) {
-    take = __builtin_amdgcn_readfirstlane(steps_left < take ? steps_left : take);
-    __syncthreads();  // the LDS of the row group before (or of the prefix) is free
-  }
-  const bool partial = SHARED && take < all_steps;
+  const int whole = all_steps - s_begin;
+  const int take = __builtin_amdgcn_readfirstlane(steps_left < whole ? steps_left : whole);
+  __syncthreads();  // the LDS of the row group before (or of the prefix) is free
+  const bool partial = take < all_steps;
   const int q0 = __builtin_amdgcn_readfirstlane(a.cu_q[b]);
   const int G = a.G;
   const int rows = qlen * G;
-  const int unit = rg * kTreeWaves + wave;
+  // With one or two units, two waves share each: every step's first 32 keys are the one's, the others the other's.
+  const bool split = rows - 32 * kTreeWaves * rg <= 64;  // uniform
+  const int part = split ? wave >> 1 : 0;
+  const int unit = rg * kTreeWaves + (split ? wave & 1 : wave);
   const bool active = 32 * unit < rows;  // uniform
   // Row 32 unit + i of the sequence: its node and query head (of the last row for those past it).
   struct Row {
@@ -460,17 +467,19 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
   const bf16x2 ones = __builtin_bit_cast(bf16x2, 0x3F803F80u);
   uint32_t pw[4][4];  // PV operands of the step being finished: packed bf16 probabilities
 
-  // S^T of step s into (x0, x1)
-  auto qk = [&](int s, floatx16 &x0, floatx16 &x1) __attribute__((always_inline)) {
+  // S^T of step s into (x0, x1); of 32 keys (not WHOLE) into x0
+  auto qk = [&](int s, floatx16 &x0, floatx16 &x1, auto WHOLE) __attribute__((always_inline)) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) x0[r] = x1[r] = 0.f;
-    const uint8_t *lk = ldsk + ((s & 1) * 4 + (kn >> 4)) * TB + (kn & 15) * 16;
+    const uint8_t *lk = ldsk + ((s & 1) * 4 + 2 * (WHOLE ? 0 : part) + (kn >> 4)) * TB + (kn & 15) * 16;
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) {
       const bf16x8 a0 = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(lk + (2 * j + hh) * 256));
-      const bf16x8 a1 = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(lk + 2 * TB + (2 * j + hh) * 256));
       x0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a0, qb[j], x0, 0, 0, 0);
-      x1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1, qb[j], x1, 0, 0, 0);
+      if constexpr (WHOLE) {
+        const bf16x8 a1 = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(lk + 2 * TB + (2 * j + hh) * 256));
+        x1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1, qb[j], x1, 0, 0, 0);
+      }
     }
   };
   // The tiles of step s that hold keys, a bit each.
@@ -503,35 +512,36 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
     return seen;
   };
   // Exponents against the reference maximum (0 before the first seen key).
-  auto expo = [&](floatx16 &x0, floatx16 &x1) __attribute__((always_inline)) {
+  auto expo = [&](floatx16 &x0, floatx16 &x1, auto WHOLE) __attribute__((always_inline)) {
     const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       x0[r] = __builtin_fmaf(x0[r], scale_log2, -m_use);
-      x1[r] = __builtin_fmaf(x1[r], scale_log2, -m_use);
+      if constexpr (WHOLE) x1[r] = __builtin_fmaf(x1[r], scale_log2, -m_use);
     }
   };
-  auto hide = [&](uint64_t seen, floatx16 &x0, floatx16 &x1) __attribute__((always_inline)) {
-    const uint64_t v = seen >> (8 * (lane_here() >> 5));
+  auto hide = [&](uint64_t seen, floatx16 &x0, floatx16 &x1, auto WHOLE) __attribute__((always_inline)) {
+    const uint64_t v = seen >> (8 * (lane_here() >> 5) + (WHOLE ? 0 : 32 * part));
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       if (!(v >> (16 * (r >> 3) + (r & 7)) & 1)) x0[r] = -INFINITY;
-      if (!(v >> (32 + 16 * (r >> 3) + (r & 7)) & 1)) x1[r] = -INFINITY;
+      if constexpr (WHOLE)
+        if (!(v >> (32 + 16 * (r >> 3) + (r & 7)) & 1)) x1[r] = -INFINITY;
     }
   };
-  auto largest = [&](const floatx16 &x0, const floatx16 &x1) __attribute__((always_inline)) {
-    float mt0 = fmaxf(x0[0], x0[1]), mt1 = fmaxf(x1[0], x1[1]);
+  auto largest = [&](const floatx16 &x0, const floatx16 &x1, auto WHOLE) __attribute__((always_inline)) {
+    float mt = fmaxf(x0[0], x0[1]), mt1 = fmaxf(x1[0], x1[1]);
 #pragma unroll
     for (int r = 2; r < 16; r += 2) {
-      mt0 = fmaxf(fmaxf(mt0, x0[r]), x0[r + 1]);
-      mt1 = fmaxf(fmaxf(mt1, x1[r]), x1[r + 1]);
+      mt = fmaxf(fmaxf(mt, x0[r]), x0[r + 1]);
+      if constexpr (WHOLE) mt1 = fmaxf(fmaxf(mt1, x1[r]), x1[r + 1]);
     }
-    const float mt = fmaxf(mt0, mt1);
+    if constexpr (WHOLE) mt = fmaxf(mt, mt1);
     const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
     return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
   };
   // The rare move of the reference maximum (after the PV products of the steps before).
-  auto rescale = [&](float mt, floatx16 &x0, floatx16 &x1) __attribute__((always_inline)) {
+  auto rescale = [&](float mt, floatx16 &x0, floatx16 &x1, auto WHOLE) __attribute__((always_inline)) {
     const bool unset = m_ref == -INFINITY;
     const bool move = unset ? mt > -INFINITY : mt > SOFTMAX_TAU;
     if (__any(move)) {
@@ -540,7 +550,7 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         x0[r] -= sh;
-        x1[r] -= sh;
+        if constexpr (WHOLE) x1[r] -= sh;
       }
       const float corr = move && !unset ? fast_exp2(-sh) : 1.f;
       l_part *= corr;
@@ -552,15 +562,15 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
     }
   };
   // Probabilities, packed as the PV operands, and the sum of the rounded ones.
-  auto probs = [&](floatx16 &x0, floatx16 &x1) __attribute__((always_inline)) {
+  auto probs = [&](floatx16 &x0, floatx16 &x1, auto WHOLE) __attribute__((always_inline)) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       x0[r] = fast_exp2(x0[r]);
-      x1[r] = fast_exp2(x1[r]);
+      if constexpr (WHOLE) x1[r] = fast_exp2(x1[r]);
     }
     float ps = 0.f;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < (WHOLE ? 4 : 2); ++t) {
       const floatx16 &sv = t < 2 ? x0 : x1;
       const int e0 = 8 * (t & 1);
 #pragma unroll
@@ -572,10 +582,10 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
     l_part += ps;
   };
   // P V^T of step s
-  auto pv = [&](int s) __attribute__((always_inline)) {
-    const uint8_t *lv = ldsv + (s & 1) * 4 * TB + n * 32 + 16 * (hh ^ ((n >> 2) & 1));
+  auto pv = [&](int s, auto WHOLE) __attribute__((always_inline)) {
+    const uint8_t *lv = ldsv + ((s & 1) * 4 + 2 * (WHOLE ? 0 : part)) * TB + n * 32 + 16 * (hh ^ ((n >> 2) & 1));
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < (WHOLE ? 4 : 2); ++t) {
       const bf16x8 pb = __builtin_bit_cast(bf16x8, (u32x4{pw[t][0], pw[t][1], pw[t][2], pw[t][3]}));
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
@@ -588,13 +598,14 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
   // anything) as zeros. V that are not finite are zeros there too, and are added
   // to the rows that see their keys: as many +inf, -inf or both (a NaN) as products of
   // where they stand with what is seen count.
-  auto pv_masked = [&](int s) __attribute__((always_inline)) {
+  auto pv_masked = [&](int s, auto WHOLE) __attribute__((always_inline)) {
     const int l = lane_here(), n = l & 31, hh = l >> 5;
-    const uint8_t *const lv = ldsv + (s & 1) * 4 * TB + n * 32 + 16 * (hh ^ ((n >> 2) & 1));
+    const int t0 = WHOLE ? 0 : 2 * part;
+    const uint8_t *const lv = ldsv + ((s & 1) * 4 + t0) * TB + n * 32 + 16 * (hh ^ ((n >> 2) & 1));
     bool odd = false;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int left = L - 64 * s - 16 * t;
+    for (int t = 0; t < (WHOLE ? 4 : 2); ++t) {
+      const int left = L - 64 * s - 16 * (t0 + t);
       if (left <= 0) continue;  // uniform
       u32x4 w[D / 32];
 #pragma unroll
@@ -627,9 +638,9 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
         o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w[c]), pb, o[c], 0, 0, 0);
     }
     if (!odd) return;  // uniform
-    const uint64_t seen = window(s, tiles(s)) >> (8 * hh);
+    const uint64_t seen = window(s, tiles(s)) >> (8 * hh + 16 * t0);
 #pragma unroll 1
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < (WHOLE ? 4 : 2); ++t) {
       u32x4 vis;  // 1 where the row sees the key
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -669,38 +680,43 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
     issue_k(s + 2);
   };
   // Step s finished while step s + 1 is scored, both of whole tiles of the context.
-  auto body = [&](int s, floatx16 &c0, floatx16 &c1, floatx16 &n0, floatx16 &n1) __attribute__((always_inline)) {
+  auto body = [&](int s, floatx16 &c0, floatx16 &c1, floatx16 &n0, floatx16 &n1, auto WHOLE) __attribute__((always_inline)) {
     turn(s);
     if (!active) return;  // uniform
-    qk(s + 1, n0, n1);
-    probs(c0, c1);
+    qk(s + 1, n0, n1, WHOLE);
+    probs(c0, c1, WHOLE);
     // keeps the probabilities in this block
-    asm volatile("" ::"v"(l_part), "v"(pw[0][0]), "v"(pw[0][1]), "v"(pw[0][2]), "v"(pw[0][3]), "v"(pw[1][0]),
-                 "v"(pw[1][1]), "v"(pw[1][2]), "v"(pw[1][3]), "v"(pw[2][0]), "v"(pw[2][1]), "v"(pw[2][2]),
-                 "v"(pw[2][3]), "v"(pw[3][0]), "v"(pw[3][1]), "v"(pw[3][2]), "v"(pw[3][3]));
+    if constexpr (WHOLE)
+      asm volatile("" ::"v"(l_part), "v"(pw[0][0]), "v"(pw[0][1]), "v"(pw[0][2]), "v"(pw[0][3]), "v"(pw[1][0]),
+                   "v"(pw[1][1]), "v"(pw[1][2]), "v"(pw[1][3]), "v"(pw[2][0]), "v"(pw[2][1]), "v"(pw[2][2]),
+                   "v"(pw[2][3]), "v"(pw[3][0]), "v"(pw[3][1]), "v"(pw[3][2]), "v"(pw[3][3]));
+    else
+      asm volatile("" ::"v"(l_part), "v"(pw[0][0]), "v"(pw[0][1]), "v"(pw[0][2]), "v"(pw[0][3]), "v"(pw[1][0]),
+                   "v"(pw[1][1]), "v"(pw[1][2]), "v"(pw[1][3]));
     // the score products of step s + 1 interleaved with step s's probabilities
+    constexpr int QK = (WHOLE ? 2 : 1) * D / 16, PV = (WHOLE ? 4 : 2) * D / 32;  // products
     __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);  // LDS reads, four ahead
 #pragma unroll
-    for (int i = 0; i < 2 * D / 16; ++i) {
+    for (int i = 0; i < QK; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
-      if (i + 4 < 2 * D / 16) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
+      if (i + 4 < QK) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
       __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);  // VALU
     }
-    expo(n0, n1);
-    const float mt = largest(n0, n1);
-    pv(s);
+    expo(n0, n1, WHOLE);
+    const float mt = largest(n0, n1, WHOLE);
+    pv(s, WHOLE);
     // step s's PV products interleaved with step s + 1's exponents
     __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-    for (int i = 0; i < 4 * D / 32; ++i) {
+    for (int i = 0; i < PV; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      if (i + 4 < 4 * D / 32) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      if (i + 4 < PV) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
     }
-    rescale(mt, n0, n1);
+    rescale(mt, n0, n1, WHOLE);
   };
 
-  if (s1 > s0) {
+  auto keys = [&](auto WHOLE) __attribute__((always_inline)) {
     issue_k(s0);
     if constexpr (FP8) {
       wait_vmcnt<0>();
@@ -713,22 +729,23 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
       if (!v_land) wait_vmcnt<0>();  // (no tile of step s0)
     }
     barrier_lds();
+    constexpr int QK = (WHOLE ? 2 : 1) * D / 16;
     floatx16 a0, a1;
     auto score = [&](int s) __attribute__((always_inline)) {
-      qk(s, a0, a1);
+      qk(s, a0, a1, WHOLE);
       __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);  // LDS reads four ahead of their MFMAs, not all at once
 #pragma unroll
-      for (int i = 0; i < 2 * D / 16; ++i) {
+      for (int i = 0; i < QK; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        if (i + 4 < 2 * D / 16) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        if (i + 4 < QK) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
-      expo(a0, a1);
+      expo(a0, a1, WHOLE);
       const uint32_t ok = tiles(s);
       if (ok != 15u || 64 * s + 64 > ctx) {  // uniform
-        hide(window(s, ok), a0, a1);
+        hide(window(s, ok), a0, a1, WHOLE);
       }
-      rescale(largest(a0, a1), a0, a1);
+      rescale(largest(a0, a1, WHOLE), a0, a1, WHOLE);
     };
     if (active) score(s0);
     // Steps of context alone, in pairs: what a pair scores, steps s + 1 and s + 2, is of
@@ -738,11 +755,11 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
       floatx16 b0, b1;
       const int ends = (ctx >> 6) < s1 ? (ctx >> 6) : s1;
       for (; s + 2 < ends && clean; s += 2) {
-        body(s, a0, a1, b0, b1);
-        body(s + 1, b0, b1, a0, a1);
+        body(s, a0, a1, b0, b1, WHOLE);
+        body(s + 1, b0, b1, a0, a1, WHOLE);
       }
       if (s + 1 < ends && clean) {
-        body(s, a0, a1, b0, b1);
+        body(s, a0, a1, b0, b1, WHOLE);
         ++s;
         a0 = b0;
         a1 = b1;
@@ -753,13 +770,48 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
     for (; s < s1; ++s) {
       turn(s);
       if (!active) continue;  // uniform
-      probs(a0, a1);
-      pv_masked(s);
+      probs(a0, a1, WHOLE);
+      pv_masked(s, WHOLE);
       if (s + 1 < s1) score(s + 1);
+    }
+  };
+  if (s1 > s0) {
+    if (split) keys(std::false_type{}); else keys(std::true_type{});
+  }
+  bool writes = active;
+  if (split) {  // the second part's waves hand theirs to the first's
+    barrier_lds();
+    float *const jo = reinterpret_cast<float *>(unit & 1 ? ldsv : ldsk);
+    const int l = lane_here();
+    if (active && part == 1) {
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<floatx4 *>(jo + ((4 * c + g) * 64 + l) * 4) =
+              floatx4{o[c][4 * g], o[c][4 * g + 1], o[c][4 * g + 2], o[c][4 * g + 3]};
+      jo[32 * D + l] = m_ref;
+      jo[32 * D + 64 + l] = l_part;
+    }
+    barrier_lds();
+    writes = active && part == 0;
+    if (writes) {
+      const float mb = jo[32 * D + l], m = fmaxf(m_ref, mb), m_use = m == -INFINITY ? 0.f : m;
+      const float wa = fast_exp2(m_ref - m_use), wb = fast_exp2(mb - m_use);  // 0 of a part that saw no key
+      l_part = l_part * wa + jo[32 * D + 64 + l] * wb;
+      m_ref = m;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const floatx4 x = *reinterpret_cast<const floatx4 *>(jo + ((4 * c + g) * 64 + l) * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[c][4 * g + e] = o[c][4 * g + e] * wa + x[e] * wb;
+        }
     }
   }
   const TreeArgs &ae = tree_args();
-  if (active) {
+  if (writes) {
   const int lane = lane_here(), n = lane & 31, hh = lane >> 5;
   float l = l_part;
   {
@@ -793,30 +845,24 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
                   pack_bf16x2(o[c][4 * g + 2] * inv, o[c][4 * g + 3] * inv)};
   }
   }
-  if constexpr (SHARED) {
-    if (partial && s_begin == 0 && threadIdx.x == 0) {  // the group's first part (and the last of this share)
-      const TreeShare share = s_share;
-      const int w = s_place;
-      const int w1 = share.of(share.begin(w + 1) + (all_steps - take) - 1);  // the workgroup of the group's last step
-      tree_counts<D>(ae.part)[id] = w1 - w + 1;
-      tree_records<D>(ae.part)[id] = TreeRec{2 * w + (later ? 1 : 0), 2 * (w + 1), b, kvh, rg, {0, 0, 0}};
-    }
-    steps_left -= take;
-    later = true;
+  if (partial && s_begin == 0 && threadIdx.x == 0) {  // the group's first part (and the last of this share)
+    const TreeShare share = s_share;
+    const int w = s_place;
+    const int w1 = share.of(share.begin(w + 1) + (all_steps - take) - 1);  // the workgroup of the group's last step
+    tree_counts<D>(ae.part)[id] = w1 - w + 1;
+    tree_records<D>(ae.part)[id] = TreeRec{2 * w + (later ? 1 : 0), 2 * (w + 1), b, kvh, rg, {0, 0, 0}};
   }
+  steps_left -= take;
+  later = true;
   }
-  if constexpr (!SHARED) {
-    break;
-  } else {
-    if (steps_left <= 0) break;
-    s_begin = 0;
-    const TreeArgs &an = tree_args();
-    if (++rg >= groups) {
-      rg = 0;
-      if (++b == an.batch) {
-        b = 0;
-        if (++kvh == an.Hkv) break;  // never with steps left
-      }
+  if (steps_left <= 0) break;
+  s_begin = 0;
+  const TreeArgs &an = tree_args();
+  if (++rg >= groups) {
+    rg = 0;
+    if (++b == an.batch) {
+      b = 0;
+      if (++kvh == an.Hkv) break;  // never with steps left
     }
   }
   }
@@ -1031,13 +1077,7 @@ extern "C" int wkv_tree_gqa(const wkv_cache_t *cache, const void *key, int64_t k
   const dim3 grid(static_cast<unsigned>(n_wg));
   auto s = static_cast<hipStream_t>(stream);
   const bool fp8 = cache->kv_dtype == WKV_KV_FP8_E4M3;
-#define WKV_TREE(Dv, F8)                                                        \
-  do {                                                                          \
-    if (share > 0)                                                              \
-      tree_gqa_kernel<Dv, F8, true><<<grid, kTreeThreads, 0, s>>>(a);           \
-    else                                                                        \
-      tree_gqa_kernel<Dv, F8, false><<<grid, kTreeThreads, 0, s>>>(a);          \
-  } while (0)
+#define WKV_TREE(Dv, F8) tree_gqa_kernel<Dv, F8><<<grid, kTreeThreads, 0, s>>>(a)
   if (D == 128) {
     if (fp8) WKV_TREE(128, true); else WKV_TREE(128, false);
   } else {
