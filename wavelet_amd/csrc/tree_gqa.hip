@@ -187,7 +187,7 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
   constexpr int NC = D * 16 * ESZ / 1024;  // 1 KB copies of each
   // bf16 tiles as the MFMAs read them: K [D / 8 chunks][16 tokens][16 bytes] as the
   // cache holds it, V [D rows][2 token octets][8 tokens] (the octets swapped in every second
-  // four rows). fp8 codes land at their tile's start: K [D / 16 chunks][16 tokens][16 bytes],
+  // eight rows). fp8 codes land at their tile's start: K [D / 16 chunks][16 tokens][16 bytes],
   // V [D rows][16 tokens].
   __shared__ __attribute__((aligned(16))) uint8_t ldsk[2 * 4 * TB];
   __shared__ __attribute__((aligned(16))) uint8_t ldsv[2 * 4 * TB];
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
 
   // Copies. Piece p = 64 k + l of a tile's K or V goes to LDS offset 16 p. K: chunk p / 16,
   // token p % 16, as the cache holds it. bf16 V: row p / 2, its token octets in turn (octet 1
-  // first in every second four rows, for the banks); fp8 V: row p.
+  // first in every second eight rows, for the banks); fp8 V: row p.
   const int BS = a.BS, region = D * BS * ESZ, Hkv = a.Hkv, nb = a.nb, Mb = a.Mb;
   const uint8_t *const kc = a.kc, *const vc = a.vc;
   const float *const ksc = a.ksc, *const vsc = a.vsc;
@@ -401,7 +401,7 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
     if (v_ok) {
       vs_land = vs_next;
       const int l = lane_here();
-      const uint32_t lane_v = static_cast<uint32_t>(FP8 ? l * BS : (l >> 1) * BS * 2 + 16 * ((l ^ l >> 3) & 1));
+      const uint32_t lane_v = static_cast<uint32_t>(FP8 ? l * BS : (l >> 1) * BS * 2 + 16 * ((l ^ l >> 4) & 1));
       uint32_t vst = static_cast<uint32_t>(64 * BS);
       asm volatile("" : "+s"(vst));
       const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(
@@ -431,7 +431,7 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
       const int p = 64 * i + lane;
       if (do_v) {
         uint8_t *d = tv + p * 32;
-        const int first = 4 * (p & 4);  // where the row's octet 0 goes
+        const int first = 2 * (p & 8);  // where the row's octet 0 goes
         *reinterpret_cast<u32x4 *>(d + first) = codes_to_bf16(wv[i][0], wv[i][1], vs_land);
         *reinterpret_cast<u32x4 *>(d + 16 - first) = codes_to_bf16(wv[i][2], wv[i][3], vs_land);
       }
@@ -583,7 +583,7 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
   };
   // P V^T of step s
   auto pv = [&](int s, auto WHOLE) __attribute__((always_inline)) {
-    const uint8_t *lv = ldsv + ((s & 1) * 4 + 2 * (WHOLE ? 0 : part)) * TB + n * 32 + 16 * (hh ^ ((n >> 2) & 1));
+    const uint8_t *lv = ldsv + ((s & 1) * 4 + 2 * (WHOLE ? 0 : part)) * TB + n * 32 + 16 * (hh ^ ((n >> 3) & 1));
 #pragma unroll
     for (int t = 0; t < (WHOLE ? 4 : 2); ++t) {
       const bf16x8 pb = __builtin_bit_cast(bf16x8, (u32x4{pw[t][0], pw[t][1], pw[t][2], pw[t][3]}));
@@ -601,7 +601,7 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
   auto pv_masked = [&](int s, auto WHOLE) __attribute__((always_inline)) {
     const int l = lane_here(), n = l & 31, hh = l >> 5;
     const int t0 = WHOLE ? 0 : 2 * part;
-    const uint8_t *const lv = ldsv + ((s & 1) * 4 + t0) * TB + n * 32 + 16 * (hh ^ ((n >> 2) & 1));
+    const uint8_t *const lv = ldsv + ((s & 1) * 4 + t0) * TB + n * 32 + 16 * (hh ^ ((n >> 3) & 1));
     bool odd = false;
 #pragma unroll
     for (int t = 0; t < (WHOLE ? 4 : 2); ++t) {
