@@ -14,6 +14,9 @@ Modules
 ``oracle.paged``  slot-mapped append (bf16 / fp8 with per-(block, head)
                   scales), block-table gather, GQA and MLA paged decode
                   attention (attention.py:81-96; wavelet/kernels/patch.py:173-196).
+``oracle.tree``   a step of drafted tokens: rotation, step tables, tree attention,
+                  the accepted path and the move of its keys and values (pinned in
+                  tests/test_tree_oracle.py).
 
 How each function is pinned (tests/test_oracle.py)
 -------------------------------------------------

@@ -11,7 +11,8 @@
 // new block's tokens as one run, with the append kernel's own run (one wave a
 // run): the block's earlier codes are encoded again where its scale grows.
 // Bound by two round trips to memory and the launch: the bytes of a step (64
-// sequences x 8 tokens x 8 heads) are 4 MB.
+// sequences x 8 tokens x 8 heads) are 4 MB. That step in bf16 5.5 us; 33 sequences x up
+// to 12 tokens x 4 heads in fp8 10.8 us, half of it the runs of the append rule.
 #include "kv_append_dev.h"
 
 namespace wkv {

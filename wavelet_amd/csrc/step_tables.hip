@@ -2,7 +2,8 @@
 // tree masks from the request lengths (wkv_extend_tables), and the accepted
 // path of a verified tree (wkv_accept_tree). Both are bound by their launch and
 // a few dependent round trips, not by bytes: 16 bytes per token and 24 per
-// sequence.
+// sequence. 64 sequences with trees of 16 nodes 7.9 us, with 75,000 prompt tokens
+// 8.4 + 4.2 us (two launches); the paths of 256 trees of 64 nodes 4.0 us.
 #include "wkv_common.h"
 
 namespace wkv {
