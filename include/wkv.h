@@ -490,7 +490,7 @@ int wkv_tree_gqa(const wkv_cache_t *cache, const void *key, int64_t key_stride_t
                  void *stream);
 
 /* The accepted path of a verified tree. draft_tokens, parents and target_tokens
- * [num rows]: a node's own token, its parent, and the token that the model sampled after
+ * [num_tokens]: a node's own token, its parent, and the token that the model sampled after
  * it. Node 0 (the token of the step before, always right) is accepted; from an
  * accepted node the path goes on to its first child whose token is the
  * one sampled after it, up to max_depth nodes. path [B, max_depth]: the accepted nodes,
@@ -499,8 +499,8 @@ int wkv_tree_gqa(const wkv_cache_t *cache, const void *key, int64_t key_stride_t
  * A sequence without rows, or refused (context_lens[b] <= 0), accepts nothing (next -1). A
  * sequence's first 256 nodes count. No counterpart in the reference (inside llm.generate). */
 int wkv_accept_tree(const int64_t *draft_tokens, const int32_t *parents, const int64_t *target_tokens,
-                    const int32_t *cu_seqlens_q, const int32_t *seq_lens, const int32_t *context_lens, int32_t batch,
-                    int32_t max_depth, int32_t *accepted, int32_t *path, int64_t *next_tokens, int32_t *seq_lens_out,
+                    int64_t num_tokens, const int32_t *cu_seqlens_q, const int32_t *seq_lens,
+                    const int32_t *context_lens, int32_t batch, int32_t max_depth, int32_t *accepted, int32_t *path, int64_t *next_tokens, int32_t *seq_lens_out,
                     void *stream);
 
 /* Moves an accepted path's keys and values together, in place: for j <

@@ -183,6 +183,11 @@ def test_accept_without_rows_and_refusals(cuda):
     assert got.accepted.tolist() == [0, 0] and got.next_tokens.tolist() == [-1, -1] and got.seq_lens.tolist() == [3, 3]
     assert (got.path == -1).all()
     assert accept_tree(z, z.int(), z, cu[:1], i[:0], i[:0], 4).path.shape == (0, 4)
+    # rows that there are not (a longer step's cu_seqlens_q): nodes past the last are none
+    t = torch.tensor([5, 6, 7], device=cuda)
+    got = accept_tree(t, torch.tensor([-1, 0, 1], dtype=torch.int32, device=cuda), t + 1, cu + 100 * i.new_tensor([0, 1, 2]),
+                      i + 3, i + 9, 4)
+    assert got.accepted.tolist() == [3, 0] and got.next_tokens.tolist() == [8, -1] and got.path[0].tolist() == [0, 1, 2, -1]
     for bad in ((z.int(), z.int(), z, cu, i, i, 4), (z, z, z, cu, i, i, 4), (z, z.int(), z, cu, i[:1], i, 4),
                 (z, z.int(), z, cu, i, i, 0), (z, z.int(), z, cu, i, i, 65), (z, z.int(), z.cpu(), cu, i, i, 4)):
         with pytest.raises(ValueError):

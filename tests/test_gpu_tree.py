@@ -331,6 +331,26 @@ def test_on_another_stream(cuda):
     check_attention(paged.bf16_to_f32(bits_of(out)), c.ref(), "stream")
 
 
+def test_two_calls_at_once(cuda):
+    """Calls on two streams that share nothing but the queries give what each gives alone."""
+    a = Case(cuda, "both0", 8, 2, 128, 16, [6000, 900], [64, 40])
+    b = Case(cuda, "both1", 8, 2, 128, 16, [5000], [50])
+    alone = [paged_tree_gqa(*c.args(), **c.appended()) for c in (a, b)]
+    calls = [(c.args(), c.appended()) for c in (a, b)]
+    streams = [torch.cuda.Stream(cuda) for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, (args, new) in enumerate(calls):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(paged_tree_gqa(*args, max_query_len=64, max_seq_len=6100, **new))
+    torch.cuda.synchronize()
+    for want, outs in zip(alone, got):
+        for out in outs:
+            torch.testing.assert_close(out.float(), want.float(), atol=2e-2, rtol=1e-2)
+            assert torch.equal(out, outs[0])
+
+
 def test_refusals(cuda):
     c = Case(cuda, "refuse", 8, 2, 128, 16, [10], [4])
     names = ("q", "cache", "block_table", "seq_lens", "cu_seqlens_q", "tree_mask", "scale")

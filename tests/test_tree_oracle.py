@@ -245,9 +245,10 @@ def test_compact_refusals(kw):
 
 
 @host_only
-@pytest.mark.parametrize("kw", [dict(depth=0), dict(depth=65), dict(draft=None), dict(batch=-1), dict(out=None)])
+@pytest.mark.parametrize("kw", [dict(depth=0), dict(depth=65), dict(draft=None), dict(batch=-1), dict(out=None),
+                                dict(rows=-1), dict(rows=2**31)])
 def test_accept_refusals(kw):
-    a = dict(draft=P, parents=P, target=P, cu=P, lens=P, context=P, batch=2, depth=4, acc=P, path=P, nxt=P, out=P,
+    a = dict(draft=P, parents=P, target=P, rows=9, cu=P, lens=P, context=P, batch=2, depth=4, acc=P, path=P, nxt=P, out=P,
              stream=None)
     a.update(kw)
     assert _lib.load().wkv_accept_tree(*a.values()) == _lib.WKV_ERR_INVALID

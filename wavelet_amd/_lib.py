@@ -92,7 +92,7 @@ _SIGNATURES = {
                              c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_void_p,
                              c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p, c_int32,
                              c_float, c_void_p, c_int64, c_void_p, c_void_p]),
-    "wkv_accept_tree": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p,
+    "wkv_accept_tree": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p,
                                 c_void_p, c_void_p, c_void_p, c_void_p]),
     "wkv_compact": (c_int, [POINTER(WkvCache), c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_int32, c_void_p,
                             c_int32, c_void_p]),

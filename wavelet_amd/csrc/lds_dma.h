@@ -31,13 +31,6 @@ __device__ __forceinline__ void buffer_copy16_to_lds(__amdgpu_buffer_rsrc_t r, u
                "s"(soff)
                : "memory", "m0");
 }
-// The same with the non-temporal bit, for data read once.
-__device__ __forceinline__ void buffer_copy16_to_lds_nt(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff,
-                                                        uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds" ::"s"(lds), "v"(voff),
-               "s"(r), "s"(soff)
-               : "memory", "m0");
-}
 // NCP copies of 1 KB under one M0 write: copy k lands at lds + 1024 k. The
 // LDS address of a copy is M0 + its instruction offset + 16 x lane, and the
 // instruction offset (1024 k here) is added to the memory address as well, so
@@ -66,10 +59,10 @@ __device__ __forceinline__ void buffer_copy16_run_to_lds(__amdgpu_buffer_rsrc_t 
                  : "memory", "m0");
   }
 }
-// The same with the non-temporal bit.
+// The same with the non-temporal bit, for data read once.
 template <int NCP>
 __device__ __forceinline__ void buffer_copy16_run_to_lds_nt(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t sdelta,
-                                                         uint32_t lds) {
+                                                            uint32_t lds) {
   static_assert(NCP >= 1 && NCP <= 4, "instruction offsets below 4096");
   if constexpr (NCP == 1) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" ::"s"(lds), "v"(voff),

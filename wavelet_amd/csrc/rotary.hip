@@ -168,8 +168,9 @@ static int rotary_width(int esz, int D, int half, bool inter, const RotaryRows *
 template <class T, bool INTER>
 static void launch_rotary(const RotaryArgs &a, int v, bool far, dim3 grid, hipStream_t s) {
   constexpr int B = 64 * kRotaryWaves, W = 16 / sizeof(T);
-  if (v == W) return far ? rotary_kernel<T, W, INTER, true><<<grid, B, 0, s>>>(a) : rotary_kernel<T, W, INTER, false><<<grid, B, 0, s>>>(a);
-  if (W > 4 && v == 4) return rotary_kernel<T, 4, INTER, false><<<grid, B, 0, s>>>(a);
+  if (v == W && far) return rotary_kernel<T, W, INTER, true><<<grid, B, 0, s>>>(a);
+  if (v == W) return rotary_kernel<T, W, INTER, false><<<grid, B, 0, s>>>(a);
+  if (W > 4 && v == 4) return rotary_kernel<T, 4, INTER, false><<<grid, B, 0, s>>>(a);  // (narrower: never far)
   if (v == 2) return rotary_kernel<T, 2, INTER, false><<<grid, B, 0, s>>>(a);
   rotary_kernel<T, 1, INTER, false><<<grid, B, 0, s>>>(a);
 }

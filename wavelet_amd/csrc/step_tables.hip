@@ -212,7 +212,7 @@ __global__ __launch_bounds__(256) void tables_rows_kernel(TablesArgs a) {
 // lane i. Each step compares every node at once with the current one.
 __global__ __launch_bounds__(256) void accept_tree_kernel(const int64_t *__restrict__ draft,
                                                           const int32_t *__restrict__ parents,
-                                                          const int64_t *__restrict__ target,
+                                                          const int64_t *__restrict__ target, int rows,
                                                           const int32_t *__restrict__ cu, const int32_t *seq_lens,
                                                           const int32_t *__restrict__ context, int B, int max_depth,
                                                           int32_t *__restrict__ accepted, int32_t *__restrict__ path,
@@ -221,8 +221,8 @@ __global__ __launch_bounds__(256) void accept_tree_kernel(const int64_t *__restr
   const int b = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x * 4 + (threadIdx.x >> 6)));
   if (b >= B) return;
   const int lane = threadIdx.x & 63;
-  const int q0 = cu[b], L = max(seq_lens[b], 0);
-  int n = cu[b + 1] - q0;
+  const int q0 = min(max(cu[b], 0), rows), L = max(seq_lens[b], 0);
+  int n = min(cu[b + 1], rows) - q0;  // (none past the rows that there are)
   if (context[b] <= 0) n = 0;
   n = n < 64 * N ? n : 64 * N;
   int64_t d[N], t[N];
@@ -304,19 +304,21 @@ extern "C" int wkv_extend_tables(int32_t *block_table, int64_t bt_stride, int32_
 }
 
 extern "C" int wkv_accept_tree(const int64_t *draft_tokens, const int32_t *parents, const int64_t *target_tokens,
-                               const int32_t *cu_seqlens_q, const int32_t *seq_lens, const int32_t *context_lens,
-                               int32_t batch, int32_t max_depth, int32_t *accepted, int32_t *path, int64_t *next_tokens,
-                               int32_t *seq_lens_out, void *stream) {
+                               int64_t num_tokens, const int32_t *cu_seqlens_q, const int32_t *seq_lens,
+                               const int32_t *context_lens, int32_t batch, int32_t max_depth, int32_t *accepted,
+                               int32_t *path, int64_t *next_tokens, int32_t *seq_lens_out, void *stream) {
   WKV_CHECK_ARG(batch >= 0, "batch must be >= 0 (got %d)", batch);
   WKV_CHECK_ARG(max_depth > 0 && max_depth <= WKV_TREE_MAX_DEPTH, "max_depth must be in [1, %d] (got %d)",
                 WKV_TREE_MAX_DEPTH, max_depth);
+  WKV_CHECK_ARG(num_tokens >= 0 && num_tokens <= INT32_MAX, "num_tokens must be in [0, 2^31) (got %lld)",
+                (long long)num_tokens);
   if (batch == 0) return WKV_OK;
-  WKV_CHECK_ARG(draft_tokens && parents && target_tokens && cu_seqlens_q && seq_lens && context_lens && accepted &&
-                    path && next_tokens && seq_lens_out,
+  WKV_CHECK_ARG(((draft_tokens && parents && target_tokens) || num_tokens == 0) && cu_seqlens_q && seq_lens &&
+                    context_lens && accepted && path && next_tokens && seq_lens_out,
                 "an input or output is NULL");
   accept_tree_kernel<<<static_cast<unsigned>((batch + 3) / 4), 256, 0, static_cast<hipStream_t>(stream)>>>(
-      draft_tokens, parents, target_tokens, cu_seqlens_q, seq_lens, context_lens, batch, max_depth, accepted, path,
-      next_tokens, seq_lens_out);
+      draft_tokens, parents, target_tokens, static_cast<int>(num_tokens), cu_seqlens_q, seq_lens, context_lens, batch,
+      max_depth, accepted, path, next_tokens, seq_lens_out);
   WKV_CHECK_LAUNCH("accept tree");
   return WKV_OK;
 }

@@ -1022,7 +1022,8 @@ extern "C" int wkv_tree_gqa(const wkv_cache_t *cache, const void *key, int64_t k
   WKV_CHECK_ARG(cu_seqlens_q != nullptr && seq_lens != nullptr && block_table != nullptr,
                 "cu_seqlens_q / seq_lens / block_table is NULL");
   WKV_CHECK_ARG(max_blocks_per_seq > 0 && bt_stride >= max_blocks_per_seq, "bad block table geometry");
-  WKV_CHECK_ARG(max_query_len > 0 && max_seq_len >= 0, "max_query_len must be > 0 and max_seq_len >= 0");
+  WKV_CHECK_ARG(max_query_len > 0 && max_seq_len >= 0 && max_seq_len <= INT32_MAX - 256,
+                "max_query_len must be > 0 and max_seq_len in [0, 2^31 - 257]");
   WKV_CHECK_ARG(tree_mask != nullptr && reinterpret_cast<uintptr_t>(tree_mask) % 8 == 0, "tree_mask must be non-NULL int64");
   WKV_CHECK_ARG(mask_words >= 1 && mask_words <= WKV_TREE_MAX_WORDS, "mask_words must be in [1, %d] (got %d)",
                 WKV_TREE_MAX_WORDS, mask_words);

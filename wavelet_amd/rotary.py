@@ -174,7 +174,8 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     i + R / 2)``, or ``(2 i, 2 i + 1)`` if ``interleaved``; dims from ``R`` on stay as they are. Positions
     may be any, in any order (a drafted tree's depths; far ones keep their exact angle). ``inverse``
     turns back (the transpose, also by ``scale``). ``out``: the two results' tensors; ``out=(q, k)`` works in
-    place. Differentiable in ``q`` and ``k`` (not with ``out``). For an MLA layer, ``q_pe`` and ``k_pe[:, None]``.
+    place, other tensors share no memory with ``q`` and ``k``. Differentiable in ``q`` and ``k`` (not with
+    ``out``). For an MLA layer, ``q_pe`` and ``k_pe[:, None]``.
     """
     if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype not in _DTYPES:
         raise ValueError("q must be a bfloat16, float16 or float32 [T, Hq, D] tensor")

@@ -211,11 +211,9 @@ def accept_tree(draft_tokens: torch.Tensor, parents: torch.Tensor, target_tokens
                                "Accepted"))
     if batch == 0:
         return a
-    if rows == 0:  # nothing to point at: one node that no sequence has
-        draft, target, parents = cu.new_zeros(1, dtype=torch.int64), cu.new_zeros(1, dtype=torch.int64), cu.new_zeros(1)
     with _on(dev):
-        rc = _lib.load().wkv_accept_tree(draft.data_ptr(), parents.data_ptr(), target.data_ptr(), cu.data_ptr(),
-                                         lens.data_ptr(), context.data_ptr(), batch, max_depth,
+        rc = _lib.load().wkv_accept_tree(draft.data_ptr(), parents.data_ptr(), target.data_ptr(), rows,
+                                         cu.data_ptr(), lens.data_ptr(), context.data_ptr(), batch, max_depth,
                                          a.accepted.data_ptr(), a.path.data_ptr(), a.next_tokens.data_ptr(),
                                          a.seq_lens.data_ptr(), _stream(dev))
     _lib.check(rc, "accept_tree")
