@@ -97,32 +97,49 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &a, int b) {
 
 // The line: KV head by KV head, sequence by sequence, row group by row group,
 // step by step. Every workgroup forms its prefix itself: each thread adds up a
-// run of `per` sequences; pfx[t] (LDS) is the sum before thread t's run. Returns the
-// steps of one KV head.
+// run of `per` sequences; pfx[t] (LDS) is the sum before thread t's run, of steps or
+// (GROUPS) of row groups.
 constexpr int kTreeThreads = 64 * kTreeWaves;
-__device__ __forceinline__ int tree_prefix(const TreeArgs &a, int *pfx, int *red, int per) {
-  int mine = 0;
+struct TreeLine {
+  int steps, groups, longest;  // of one KV head; steps of the longest sequence
+};
+template <bool GROUPS>
+__device__ __forceinline__ TreeLine tree_prefix(const TreeArgs &a, int *pfx, int *red, int per) {
+  int steps = 0, groups = 0, longest = 0;
   for (int b = threadIdx.x * per; b < a.batch && b < static_cast<int>(threadIdx.x + 1) * per; ++b) {
     const TreeSeq s = tree_seq(a, b);
-    mine += s.steps * s.groups;
+    steps += s.steps * s.groups;
+    groups += s.groups;
+    if (s.groups > 0) longest = max(longest, s.steps);
   }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int mine = GROUPS ? groups : steps;
   int incl = mine;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const int y = __shfl_up(incl, o, 64);
     if (lane >= o) incl += y;
+    longest = max(longest, __shfl_xor(longest, o, 64));
+    if (!GROUPS) groups += __shfl_xor(groups, o, 64);
   }
-  if (lane == 63) red[wave] = incl;
+  if (lane == 63) {
+    red[wave] = incl;
+    red[kTreeWaves + wave] = groups;
+    red[2 * kTreeWaves + wave] = longest;
+  }
   __syncthreads();
   int total = 0;
+  groups = longest = 0;
 #pragma unroll
   for (int w = 0; w < kTreeWaves; ++w) {
     if (w == wave) pfx[threadIdx.x] = total + incl - mine;
     total += red[w];
+    groups += red[kTreeWaves + w];
+    longest = max(longest, red[2 * kTreeWaves + w]);
   }
   __syncthreads();
-  return __builtin_amdgcn_readfirstlane(total);
+  return TreeLine{__builtin_amdgcn_readfirstlane(total), __builtin_amdgcn_readfirstlane(GROUPS ? total : groups),
+                  __builtin_amdgcn_readfirstlane(longest)};
 }
 
 // How many workgroups share a line of T steps: all of the grid, two per CU, with
@@ -133,6 +150,20 @@ __device__ __forceinline__ int tree_prefix(const TreeArgs &a, int *pfx, int *red
 __device__ __forceinline__ int tree_workgroups(int T) {
   const int w = (T / 4) & ~7;
   return w < 8 ? 8 : (w < kTreeShare ? w : kTreeShare);
+}
+
+// Whether each of N row groups (T steps, the longest of `longest`) gets a workgroup of its own
+// instead: up to as many as run at once, when the longest takes less than an even share with
+// the partials that cutting leaves and the merge reads (of W shares and of N cuts). By
+// microseconds of a step alone on its CU, of one of two, and of a partial (D = 128). 64
+// sequences of 700 to 1,000 tokens, 16 drafted, 32 and 8 heads of 128: 67 us whole, 99 shared; 4
+// of 8,192 with 128 drafted 208 and 110.
+template <int D>
+__device__ __forceinline__ bool tree_whole(int T, int N, int longest, int W) {
+  constexpr float kAlone = 1.3f, kPair = 2.6f, kMerge = 4.f, kPart = 0.026f * D / 128;
+  if (N > kTreeShare) return false;
+  const float share = static_cast<float>(T) / W * (W > kTreeShare / 2 ? kPair : kAlone);
+  return longest * (N > kTreeShare / 2 ? kPair : kAlone) <= share + kMerge + kPart * (W + N);
 }
 
 // T steps over W workgroups: T / W each, one more for the first T % W (W <= T).
@@ -211,22 +242,30 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
     const TreeArgs &a = tree_args();
     int *pfx = reinterpret_cast<int *>(ldsk);
     const int per = (a.batch + kTreeThreads - 1) / kTreeThreads;
-    const int line = tree_prefix(a, pfx, pfx + kTreeThreads, per);
-    const int T = line * a.Hkv;
+    const TreeLine line = tree_prefix<false>(a, pfx, pfx + kTreeThreads, per);
+    const int T = line.steps * a.Hkv, N = line.groups * a.Hkv;
     if (threadIdx.x == 0) tree_counts<D>(a.part)[id] = 0;
     // XCD i mod 8 takes a contiguous eighth of the line, whose workgroups read the same keys.
     int W = tree_workgroups(T);
+    const bool whole = tree_whole<D>(T, N, line.longest, W);  // uniform
+    if (whole) W = (N + 7) & ~7;
     const int w = (id & 7) * (W / 8) + id / 8;
     if (id >= W) return;
-    W = T < W ? T : W;
+    const int points = whole ? N : T;  // of the line
+    W = points < W ? points : W;
     if (w >= W) return;
     TreeShare share;
-    share.each = T / W;
-    share.more = T - share.each * W;
+    share.each = points / W;
+    share.more = points - share.each * W;
     int y = share.begin(w);
     steps_left = share.begin(w + 1) - y;
-    kvh = y / line;
-    y -= kvh * line;
+    if (whole) {
+      __syncthreads();
+      tree_prefix<true>(a, pfx, pfx + kTreeThreads, per);
+    }
+    const int head = whole ? line.groups : line.steps;
+    kvh = y / head;
+    y -= kvh * head;
     int lo = 0, hi = kTreeThreads;  // the last run that begins at or before y (empty runs share their successor's sum)
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -235,10 +274,10 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
     y -= pfx[lo];
     for (b = lo * per;; ++b) {  // the run holds y
       const TreeSeq s = tree_seq(a, b);
-      const int c = s.steps * s.groups;
+      const int c = whole ? s.groups : s.steps * s.groups;
       if (y < c || b + 1 >= a.batch) {
-        rg = y / s.steps;
-        s_begin = y - rg * s.steps;
+        rg = whole ? y : y / s.steps;
+        if (whole) steps_left = s.steps; else s_begin = y - rg * s.steps;
         break;
       }
       y -= c;
@@ -958,12 +997,12 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
 }
 
 // The workgroups that share a launch (0: one per row group): contexts of at most
-// eight steps are not cut (8 sequences of up to 300 tokens, with the merge's launch:
-// 22 us whole, 26 cut), and a line of 2^31 steps is not formed.
+// twelve steps are not cut (one sequence of 600 tokens, with the merge's launch: 20.3 us
+// whole, 23.5 cut; of 900 tokens 26.2 and 23.5), and a line of 2^31 steps is not formed.
 static int tree_sharing(int batch, int Hkv, int G, int max_query_len, int max_seq) {
   const int64_t steps = (static_cast<int64_t>(max_seq) + 63) / 64;
   const int64_t groups = (static_cast<int64_t>(max_query_len) * G + kTreeRows - 1) / kTreeRows;
-  return steps > 8 && groups * batch <= INT32_MAX / (steps * Hkv) ? kTreeShare : 0;
+  return steps > 12 && groups * batch <= INT32_MAX / (steps * Hkv) ? kTreeShare : 0;
 }
 
 static int64_t tree_workspace(int share, int D) {
