@@ -14,7 +14,8 @@
 // wave without rows only copies. The
 // steps of all row groups form one line that the workgroups share evenly
 // (tree_prefix), whatever the mix of lengths; a row group cut between workgroups
-// leaves fp32 partials that a second kernel merges by log-sum-exp.
+// leaves fp32 partials that a second kernel merges by log-sum-exp. Row groups enough for the
+// chip and of like lengths stay whole instead, one to a workgroup (tree_whole).
 //
 // Bound by reading K and V once for up to 64 rows of bf16, by the step's own chain
 // (products, exponents, the copies' issue, a barrier) past that and in fp8. Measured, 32 query and
@@ -48,6 +49,7 @@ typedef __attribute__((__vector_size__(2 * sizeof(uint16_t)))) uint16_t u16x2;
 
 constexpr int kTreeWaves = 4;
 constexpr int kTreeRows = 32 * kTreeWaves;  // rows of a workgroup
+constexpr int kTreeMost = 2048;  // workgroups of a launch that may share
 constexpr int kTreeShare = 512;             // workgroups that share a launch's steps: two per CU
 
 struct TreeArgs {
@@ -101,16 +103,17 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &a, int b) {
 // (GROUPS) of row groups.
 constexpr int kTreeThreads = 64 * kTreeWaves;
 struct TreeLine {
-  int steps, groups, longest;  // of one KV head; steps of the longest sequence
+  int steps, groups, longest, seqs;  // of one KV head; steps of the longest sequence, sequences with rows
 };
 template <bool GROUPS>
 __device__ __forceinline__ TreeLine tree_prefix(const TreeArgs &a, int *pfx, int *red, int per) {
-  int steps = 0, groups = 0, longest = 0;
+  int steps = 0, groups = 0, longest = 0, seqs = 0;
   for (int b = threadIdx.x * per; b < a.batch && b < static_cast<int>(threadIdx.x + 1) * per; ++b) {
     const TreeSeq s = tree_seq(a, b);
     steps += s.steps * s.groups;
     groups += s.groups;
     if (s.groups > 0) longest = max(longest, s.steps);
+    seqs += s.groups > 0 ? 1 : 0;
   }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int mine = GROUPS ? groups : steps;
@@ -121,25 +124,28 @@ __device__ __forceinline__ TreeLine tree_prefix(const TreeArgs &a, int *pfx, int
     if (lane >= o) incl += y;
     longest = max(longest, __shfl_xor(longest, o, 64));
     if (!GROUPS) groups += __shfl_xor(groups, o, 64);
+    seqs += __shfl_xor(seqs, o, 64);
   }
   if (lane == 63) {
     red[wave] = incl;
     red[kTreeWaves + wave] = groups;
     red[2 * kTreeWaves + wave] = longest;
+    red[3 * kTreeWaves + wave] = seqs;
   }
   __syncthreads();
   int total = 0;
-  groups = longest = 0;
+  groups = longest = seqs = 0;
 #pragma unroll
   for (int w = 0; w < kTreeWaves; ++w) {
     if (w == wave) pfx[threadIdx.x] = total + incl - mine;
     total += red[w];
     groups += red[kTreeWaves + w];
     longest = max(longest, red[2 * kTreeWaves + w]);
+    seqs += red[3 * kTreeWaves + w];
   }
   __syncthreads();
   return TreeLine{__builtin_amdgcn_readfirstlane(total), __builtin_amdgcn_readfirstlane(GROUPS ? total : groups),
-                  __builtin_amdgcn_readfirstlane(longest)};
+                  __builtin_amdgcn_readfirstlane(longest), __builtin_amdgcn_readfirstlane(seqs)};
 }
 
 // How many workgroups share a line of T steps: all of the grid, two per CU, with
@@ -152,26 +158,29 @@ __device__ __forceinline__ int tree_workgroups(int T) {
   return w < 8 ? 8 : (w < kTreeShare ? w : kTreeShare);
 }
 
-// Whether each of N row groups (T steps, the longest of `longest`) gets a workgroup of its own
-// instead: up to as many as run at once, when the longest takes less than an even share with
-// the partials that cutting leaves and the merge reads (of W shares and of N cuts). By
-// microseconds of a step alone on its CU, of one of two, and of a partial (D = 128). 64
-// sequences of 700 to 1,000 tokens, 16 drafted, 32 and 8 heads of 128: 67 us whole, 99 shared; 4
-// of 8,192 with 128 drafted 208 and 110.
-template <int D>
-__device__ __forceinline__ bool tree_whole(int T, int N, int longest, int W) {
-  constexpr float kAlone = 1.3f, kPair = 2.6f, kMerge = 4.f, kPart = 0.026f * D / 128;
-  if (N > kTreeShare) return false;
-  const float share = static_cast<float>(T) / W * (W > kTreeShare / 2 ? kPair : kAlone);
-  return longest * (N > kTreeShare / 2 ? kPair : kAlone) <= share + kMerge + kPart * (W + N);
+// Whether each of N row groups (T steps, the longest of `longest`) gets a workgroup of its
+// own instead of even shares. Those cost the partials that cutting leaves and the merge reads,
+// another start, and the meeting of row groups of the same keys in the L2; whole groups
+// wait for the longest. By microseconds of a step alone on its CU, of one of two, and of a
+// partial. 32 and 8 heads of 128, bf16, whole / shared: 64 sequences of 700 to 1,000 tokens
+// with 16 drafted 71 / 99, 128 of 100 to 1,000 with 8 to 32 105 / 130, 64 of 4,000 to 8,000 with
+// 32 to 64 523 / 623, of 100 to 8,000 with 16 to 48 394 / 305 us.
+template <int D, bool FP8>
+__device__ __forceinline__ bool tree_whole(int T, int N, int longest, int items, int W) {
+  constexpr float kAlone = 1.3f, kPair = 2.6f, kCut = D == 128 ? 60.f : 40.f, kPart = 0.026f * D / 128;
+  const float line = static_cast<float>(T) / W * (W > kTreeShare / 2 ? kPair : kAlone);
+  if (N <= kTreeShare / 2) return longest * kAlone <= line + 9.f + kPart * (W + N);
+  const float mean = static_cast<float>(T) / N;
+  const float again = FP8 ? 0.f : 0.25f * line * (1.f - static_cast<float>(items) / N);
+  return (longest - mean) * kAlone + 0.3f * mean <= kCut + again;
 }
 
-// T steps over W workgroups: T / W each, one more for the first T % W (W <= T).
-// The host keeps T below 2^31.
+// The points of the line (steps, or whole row groups) over W workgroups: an even number each, one
+// more for the first (W at most the points, below 2^31).
 struct TreeShare {
   int each, more;
   __device__ __forceinline__ int begin(int w) const { return w * each + (w < more ? w : more); }
-  __device__ __forceinline__ int of(int x) const {  // the workgroup of step x
+  __device__ __forceinline__ int of(int x) const {  // the workgroup of point x
     const int y = x - more * (each + 1);
     return y < 0 ? x / (each + 1) : more + y / each;
   }
@@ -244,11 +253,12 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
     const int per = (a.batch + kTreeThreads - 1) / kTreeThreads;
     const TreeLine line = tree_prefix<false>(a, pfx, pfx + kTreeThreads, per);
     const int T = line.steps * a.Hkv, N = line.groups * a.Hkv;
-    if (threadIdx.x == 0) tree_counts<D>(a.part)[id] = 0;
+    if (threadIdx.x == 0 && id < kTreeShare) tree_counts<D>(a.part)[id] = 0;
     // XCD i mod 8 takes a contiguous eighth of the line, whose workgroups read the same keys.
     int W = tree_workgroups(T);
-    const bool whole = tree_whole<D>(T, N, line.longest, W);  // uniform
-    if (whole) W = (N + 7) & ~7;
+    const bool whole = N <= static_cast<int>(gridDim.x) &&
+                       tree_whole<D, FP8>(T, N, line.longest, line.seqs * a.Hkv, W);  // uniform
+    if (whole) W = (N + 7) & ~7;  // one each
     const int w = (id & 7) * (W / 8) + id / 8;
     if (id >= W) return;
     const int points = whole ? N : T;  // of the line
@@ -996,9 +1006,9 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
   }
 }
 
-// The workgroups that share a launch (0: one per row group): contexts of at most
-// twelve steps are not cut (one sequence of 600 tokens, with the merge's launch: 20.3 us
-// whole, 23.5 cut; of 900 tokens 26.2 and 23.5), and a line of 2^31 steps is not formed.
+// The workgroups that share a launch; 0: one per row group. Contexts of at most twelve steps are
+// not cut (one sequence of 600 tokens, with the merge's launch: 20.3 us whole, 23.5 cut; of
+// 900 tokens 26.2 and 23.5), and a line of 2^31 steps is not formed.
 static int tree_sharing(int batch, int Hkv, int G, int max_query_len, int max_seq) {
   const int64_t steps = (static_cast<int64_t>(max_seq) + 63) / 64;
   const int64_t groups = (static_cast<int64_t>(max_query_len) * G + kTreeRows - 1) / kTreeRows;
@@ -1078,7 +1088,9 @@ extern "C" int wkv_tree_gqa(const wkv_cache_t *cache, const void *key, int64_t k
                   (long long)need, (long long)workspace_bytes);
   const int64_t items = static_cast<int64_t>(batch) * Hkv;
   const int groups = static_cast<int>((static_cast<int64_t>(max_query_len) * G + kTreeRows - 1) / kTreeRows);
-  const int64_t n_wg = share > 0 ? share : (items + 7) / 8 * 8 * groups;
+  // (A shared launch may turn out to be of whole row groups: as many workgroups as there can be, to a limit.)
+  const int64_t most = (items * groups + 7) / 8 * 8;
+  const int64_t n_wg = share == 0 ? (items + 7) / 8 * 8 * groups : most < share ? share : most < kTreeMost ? most : kTreeMost;
   WKV_CHECK_ARG(n_wg <= INT32_MAX / kTreeThreads, "too many sequences, KV heads and drafted tokens");
   rc = append();
   if (rc) return rc;
