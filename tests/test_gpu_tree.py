@@ -163,6 +163,18 @@ def test_lines_of_steps(cuda, kv, batch, longest):
 
 
 @pytest.mark.parametrize("kv", ["bf16", "fp8_e4m3"])
+@pytest.mark.parametrize("longest", [1000, 14000])
+def test_many_row_groups(cuda, kv, longest):
+    """More row groups than workgroups run at once, of like lengths (whole, one to a workgroup) and with one far
+    longer (cut); sequences without drafts and with two row groups among them."""
+    rng = np.random.default_rng(longest)
+    ctx, new = rng.integers(800, 1000, 150), rng.integers(0, 6, 150)
+    ctx[77], new[[3, 100]] = longest, 65
+    c = Case(cuda, f"many{kv}{longest}", 8, 4, 64, 16, ctx, new, kv)
+    c.run("many")
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8_e4m3"])
 def test_parts_of_which_a_row_sees_nothing_or_nan(cuda, kv):
     """Workgroups whose whole share of a context lies in blocks outside the cache, and ones where every key is NaN."""
     c = Case(cuda, f"parts{kv}", 4, 2, 128, 16, [3000, 3000, 3000], [20, 20, 20], kv)

@@ -99,53 +99,53 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &a, int b) {
 
 // The line: KV head by KV head, sequence by sequence, row group by row group,
 // step by step. Every workgroup forms its prefix itself: each thread adds up a
-// run of `per` sequences; pfx[t] (LDS) is the sum before thread t's run, of steps or
-// (GROUPS) of row groups.
+// run of `per` sequences; pfx[t] (LDS) is the sum before thread t's run, of steps, and
+// pfx[kTreeThreads + t] of row groups.
 constexpr int kTreeThreads = 64 * kTreeWaves;
 struct TreeLine {
-  int steps, groups, longest, seqs;  // of one KV head; steps of the longest sequence, sequences with rows
+  int steps, groups, longest;  // of one KV head; steps of the longest sequence
 };
-template <bool GROUPS>
-__device__ __forceinline__ TreeLine tree_prefix(const TreeArgs &a, int *pfx, int *red, int per) {
-  int steps = 0, groups = 0, longest = 0, seqs = 0;
+__device__ __forceinline__ TreeLine tree_prefix(const TreeArgs &a, int *pfx, int per) {
+  int steps = 0, groups = 0, longest = 0;
   for (int b = threadIdx.x * per; b < a.batch && b < static_cast<int>(threadIdx.x + 1) * per; ++b) {
     const TreeSeq s = tree_seq(a, b);
     steps += s.steps * s.groups;
     groups += s.groups;
     if (s.groups > 0) longest = max(longest, s.steps);
-    seqs += s.groups > 0 ? 1 : 0;
   }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int mine = GROUPS ? groups : steps;
-  int incl = mine;
+  int *const red = pfx + 2 * kTreeThreads;
+  int sum = steps, sum_g = groups;  // inclusive
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(incl, o, 64);
-    if (lane >= o) incl += y;
-    longest = max(longest, __shfl_xor(longest, o, 64));
-    if (!GROUPS) groups += __shfl_xor(groups, o, 64);
-    seqs += __shfl_xor(seqs, o, 64);
+    const int y = __shfl_up(sum, o, 64), z = __shfl_up(sum_g, o, 64), m = __shfl_xor(longest, o, 64);
+    if (lane >= o) {
+      sum += y;
+      sum_g += z;
+    }
+    longest = max(longest, m);
   }
   if (lane == 63) {
-    red[wave] = incl;
-    red[kTreeWaves + wave] = groups;
+    red[wave] = sum;
+    red[kTreeWaves + wave] = sum_g;
     red[2 * kTreeWaves + wave] = longest;
-    red[3 * kTreeWaves + wave] = seqs;
   }
   __syncthreads();
-  int total = 0;
-  groups = longest = seqs = 0;
+  int before = 0, before_g = 0;
+  longest = 0;
 #pragma unroll
   for (int w = 0; w < kTreeWaves; ++w) {
-    if (w == wave) pfx[threadIdx.x] = total + incl - mine;
-    total += red[w];
-    groups += red[kTreeWaves + w];
+    if (w == wave) {
+      pfx[threadIdx.x] = before + sum - steps;
+      pfx[kTreeThreads + threadIdx.x] = before_g + sum_g - groups;
+    }
+    before += red[w];
+    before_g += red[kTreeWaves + w];
     longest = max(longest, red[2 * kTreeWaves + w]);
-    seqs += red[3 * kTreeWaves + w];
   }
   __syncthreads();
-  return TreeLine{__builtin_amdgcn_readfirstlane(total), __builtin_amdgcn_readfirstlane(GROUPS ? total : groups),
-                  __builtin_amdgcn_readfirstlane(longest), __builtin_amdgcn_readfirstlane(seqs)};
+  return TreeLine{__builtin_amdgcn_readfirstlane(before), __builtin_amdgcn_readfirstlane(before_g),
+                  __builtin_amdgcn_readfirstlane(longest)};
 }
 
 // How many workgroups share a line of T steps: all of the grid, two per CU, with
@@ -169,9 +169,9 @@ template <int D, bool FP8>
 __device__ __forceinline__ bool tree_whole(int T, int N, int longest, int items, int W) {
   constexpr float kAlone = 1.3f, kPair = 2.6f, kCut = D == 128 ? 60.f : 40.f, kPart = 0.026f * D / 128;
   const float line = static_cast<float>(T) / W * (W > kTreeShare / 2 ? kPair : kAlone);
-  if (N <= kTreeShare / 2) return longest * kAlone <= line + 9.f + kPart * (W + N);
+  if (N <= kTreeShare / 2) return longest * kAlone <= line + 6.f + kPart * (W + N);
   const float mean = static_cast<float>(T) / N;
-  const float again = FP8 ? 0.f : 0.25f * line * (1.f - static_cast<float>(items) / N);
+  const float again = FP8 || N <= items ? 0.f : 0.25f * line * (1.f - static_cast<float>(items) / N);
   return (longest - mean) * kAlone + 0.3f * mean <= kCut + again;
 }
 
@@ -249,15 +249,15 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
   int steps_left;      // of this workgroup's share
   if (kernel_args.share > 0) {
     const TreeArgs &a = tree_args();
-    int *pfx = reinterpret_cast<int *>(ldsk);
+    const int *pfx = reinterpret_cast<int *>(ldsk);
     const int per = (a.batch + kTreeThreads - 1) / kTreeThreads;
-    const TreeLine line = tree_prefix<false>(a, pfx, pfx + kTreeThreads, per);
+    const TreeLine line = tree_prefix(a, reinterpret_cast<int *>(ldsk), per);
     const int T = line.steps * a.Hkv, N = line.groups * a.Hkv;
     if (threadIdx.x == 0 && id < kTreeShare) tree_counts<D>(a.part)[id] = 0;
     // XCD i mod 8 takes a contiguous eighth of the line, whose workgroups read the same keys.
     int W = tree_workgroups(T);
     const bool whole = N <= static_cast<int>(gridDim.x) &&
-                       tree_whole<D, FP8>(T, N, line.longest, line.seqs * a.Hkv, W);  // uniform
+                       tree_whole<D, FP8>(T, N, line.longest, a.batch * a.Hkv, W);  // uniform
     if (whole) W = (N + 7) & ~7;  // one each
     const int w = (id & 7) * (W / 8) + id / 8;
     if (id >= W) return;
@@ -269,10 +269,7 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
     share.more = points - share.each * W;
     int y = share.begin(w);
     steps_left = share.begin(w + 1) - y;
-    if (whole) {
-      __syncthreads();
-      tree_prefix<true>(a, pfx, pfx + kTreeThreads, per);
-    }
+    if (whole) pfx += kTreeThreads;
     const int head = whole ? line.groups : line.steps;
     kvh = y / head;
     y -= kvh * head;
