@@ -500,8 +500,8 @@ int wkv_tree_gqa(const wkv_cache_t *cache, const void *key, int64_t key_stride_t
  * sequence's first 256 nodes count. No counterpart in the reference (inside llm.generate). */
 int wkv_accept_tree(const int64_t *draft_tokens, const int32_t *parents, const int64_t *target_tokens,
                     int64_t num_tokens, const int32_t *cu_seqlens_q, const int32_t *seq_lens,
-                    const int32_t *context_lens, int32_t batch, int32_t max_depth, int32_t *accepted, int32_t *path, int64_t *next_tokens, int32_t *seq_lens_out,
-                    void *stream);
+                    const int32_t *context_lens, int32_t batch, int32_t max_depth, int32_t *accepted, int32_t *path,
+                    int64_t *next_tokens, int32_t *seq_lens_out, void *stream);
 
 /* Moves an accepted path's keys and values together, in place: for j <
  * accepted[b] the token at position seq_lens[b] + path[b, j] of sequence b goes to position seq_lens[b]

@@ -19,12 +19,12 @@
 //
 // Bound by reading K and V once for up to 64 rows of bf16, by the step's own chain
 // (products, exponents, the copies' issue, a barrier) past that and in fp8. Measured, 32 query and
-// 8 KV heads of 128: 64 sequences of 4,096 tokens with 16 drafted each, bf16, 183 us
-// (6.0 TB/s; a chunk of each sequence per workgroup, with cached reads: 206); 6 of 3,000 to 24,000
-// with 5 to 63 drafted, 28 and 4 heads, fp8, 65 us (411 TFLOP/s; chunks: 172); 64 of 4,096
-// with 8 drafted, fp8, with their append, 121 us (4.5 TB/s; with one wave per unit 140); 4 of
-// 8,192 with 128 drafted and their append 107 us in bf16 and 102 in fp8 (646 and 678 TFLOP/s; the
-// matrix unit is busy 41% of the time, the VALU 37%).
+// 8 KV heads of 128, with the drafted tokens' append: 64 sequences of 4,096 tokens with 16 drafted
+// each, bf16, 184 us (6.0 TB/s; a chunk of each sequence per workgroup, with cached reads: 206); 6 of
+// 3,000 to 24,000 with 5 to 63 drafted, 28 and 4 heads, fp8, 65 to 69 us (400 TFLOP/s;
+// chunks: 172); 64 of 4,096 with 8 drafted, fp8, 116 us (4.7 TB/s; with one wave per unit
+// 137); 4 of 8,192 with 128 drafted 112 us in bf16 and 105 in fp8 (620 and 660 TFLOP/s; the matrix
+// unit is busy 41% of the time, the VALU 38%; chunks: 111 and 108).
 //
 // Software pipeline, one barrier per step: while a wave finishes step s
 // (probabilities, PV products) it scores step s + 1, so that the matrix unit
@@ -49,8 +49,8 @@ typedef __attribute__((__vector_size__(2 * sizeof(uint16_t)))) uint16_t u16x2;
 
 constexpr int kTreeWaves = 4;
 constexpr int kTreeRows = 32 * kTreeWaves;  // rows of a workgroup
-constexpr int kTreeMost = 2048;  // workgroups of a launch that may share
-constexpr int kTreeShare = 512;             // workgroups that share a launch's steps: two per CU
+constexpr int kTreeShare = 512;  // workgroups that share a launch's steps: two per CU
+constexpr int kTreeMost = 2048;  // of a launch that may share them or have one per row group
 
 struct TreeArgs {
   const uint8_t *kc, *vc;
@@ -65,7 +65,7 @@ struct TreeArgs {
   int words;
   int batch, Mb, max_seq, Hkv, G, BS, nb;
   FastDiv by_BS, by_G;
-  int share;   // workgroups that share the line; 0: one per row group
+  int share;   // workgroups that may share the line; 0: one per row group
   int groups;  // row groups per (sequence, KV head) at the longest query
   int stream;  // blocks are read by one sequence
   float scale_log2;
@@ -726,7 +726,8 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
     issue_k(s + 2);
   };
   // Step s finished while step s + 1 is scored, both of whole tiles of the context.
-  auto body = [&](int s, floatx16 &c0, floatx16 &c1, floatx16 &n0, floatx16 &n1, auto WHOLE) __attribute__((always_inline)) {
+  auto body = [&](int s, floatx16 &c0, floatx16 &c1, floatx16 &n0, floatx16 &n1, auto WHOLE)
+                  __attribute__((always_inline)) {
     turn(s);
     if (!active) return;  // uniform
     qk(s + 1, n0, n1, WHOLE);
@@ -1087,7 +1088,9 @@ extern "C" int wkv_tree_gqa(const wkv_cache_t *cache, const void *key, int64_t k
   const int groups = static_cast<int>((static_cast<int64_t>(max_query_len) * G + kTreeRows - 1) / kTreeRows);
   // (A shared launch may turn out to be of whole row groups: as many workgroups as there can be, to a limit.)
   const int64_t most = (items * groups + 7) / 8 * 8;
-  const int64_t n_wg = share == 0 ? (items + 7) / 8 * 8 * groups : most < share ? share : most < kTreeMost ? most : kTreeMost;
+  const int64_t n_wg = share == 0     ? (items + 7) / 8 * 8 * groups
+                       : most < share ? share
+                                      : (most < kTreeMost ? most : kTreeMost);
   WKV_CHECK_ARG(n_wg <= INT32_MAX / kTreeThreads, "too many sequences, KV heads and drafted tokens");
   rc = append();
   if (rc) return rc;
