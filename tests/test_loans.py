@@ -119,3 +119,10 @@ def test_pool_lends_and_settles():
         with pytest.raises(ValueError):
             pool.lend(**{"num_blocks": 1, **bad})
     assert pool.blocks.num_free_blocks == 32 - 3
+    for sid in (0, 1):
+        pool.blocks.free(sid)
+    pool.sleep()
+    pool.blocks.allocate(2, range(5))
+    with pytest.raises(RuntimeError, match="asleep"):
+        pool.lend([2], 1)
+    pool.blocks.append_slots([2])  # nothing is lent

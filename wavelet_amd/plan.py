@@ -518,18 +518,20 @@ class TreeStep:
         self.max_nodes, self.max_depth = int(max_nodes), int(max_depth)
         self.caches = list(caches)
         self._live = _Live(caches)
-        m = self.maps = new_step_maps(batch, T, max_nodes, dev)._replace(held_blocks=state.held_blocks, taken=state.taken)
+        m = self.maps = new_step_maps(batch, T, max_nodes, dev)._replace(held_blocks=state.held_blocks,
+                                                                         taken=state.taken)
         self.accepted = Accepted(torch.zeros(batch, dtype=torch.int32, device=dev),
                                  torch.full((batch, max_depth), -1, dtype=torch.int32, device=dev),
                                  torch.zeros(batch, dtype=torch.int64, device=dev),
                                  torch.zeros(batch, dtype=torch.int32, device=dev))
         self.lib = lib = _lib.load()
+        bt = state.block_table
+        longest = min(int(max_seq_len), bt.shape[1] * state.block_size)
         need = max(lib.wkv_tree_workspace_size(batch, KV_DTYPES[c.kv_dtype], c.num_kv_heads, qq.shape[1], c.head_dim,
-                                               min(max_nodes, T), int(max_seq_len)) for c, qq in zip(caches, q))
+                                               min(max_nodes, T), longest) for c, qq in zip(caches, q))
         if need < 0:
             raise ValueError("invalid tree attention geometry")
         self.workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-        bt = state.block_table
         self.calls = []
         for layer, (cache, qq, kk, vv, oo) in enumerate(zip(caches, q, key, value, out)):
             hq, d = qq.shape[1], cache.head_dim
@@ -548,8 +550,7 @@ class TreeStep:
                       vv.data_ptr(), vv.stride(0), vv.stride(1), m.slot_mapping.data_ptr(), T, qq.data_ptr(), qq.stride(0),
                       qq.stride(1), oo.data_ptr(), oo.stride(0), oo.stride(1), hq, m.cu_seqlens_q.data_ptr(),
                       m.context_lens.data_ptr(), bt.data_ptr(), bt.stride(0), bt.shape[1], batch, min(max_nodes, T),
-                      min(int(max_seq_len), bt.shape[1] * cache.block_size), m.tree_mask.data_ptr(), m.tree_mask.shape[1],
-                      ctypes.c_float(scale), self.workspace.data_ptr() if need > 0 else None, max(need, 0), None)
+                      longest, m.tree_mask.data_ptr(), m.tree_mask.shape[1], ctypes.c_float(scale), self.workspace.data_ptr() if need > 0 else None, max(need, 0), None)
             self.calls.append((rotary, attend))
         self._keep = (q, key, value, out, inv_freq)
 

@@ -178,6 +178,8 @@ class KVPool:
         (``BlockManager.lend``), for steps whose token counts the host does not know (``StepState``,
         ``TreeStep``). A partly filled block that is shared is copied first. ``width`` (blocks per table) defaults to
         ``max_blocks_per_seq``, without a ``max_model_len`` to the longest table and the loan."""
+        if self.asleep:
+            raise RuntimeError("the KV pool is asleep: call wake_up() first")
         seq_ids = list(seq_ids)
         longest = max((len(self.blocks.blocks_of(s)) for s in seq_ids), default=0)
         if width is None:
