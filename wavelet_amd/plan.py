@@ -535,22 +535,23 @@ class TreeStep:
         self.calls = []
         for layer, (cache, qq, kk, vv, oo) in enumerate(zip(caches, q, key, value, out)):
             hq, d = qq.shape[1], cache.head_dim
-            for name, t, shape in (("q", qq, (T, hq, d)), ("out", oo, (T, hq, d)), ("key", kk, (T, cache.num_kv_heads, d)),
-                                   ("value", vv, (T, cache.num_kv_heads, d))):
+            rows, kv_rows = (T, hq, d), (T, cache.num_kv_heads, d)
+            for name, t, shape in (("q", qq, rows), ("out", oo, rows), ("key", kk, kv_rows), ("value", vv, kv_rows)):
                 if t.dtype != torch.bfloat16 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != dev:
                     raise ValueError(f"layer {layer}: {name} must be a contiguous bfloat16 {shape} tensor on {dev}")
             rotary = None
             if inv_freq is not None:
                 if not 0 < 2 * inv_freq.shape[0] <= d:
                     raise ValueError(f"layer {layer}: inv_freq turns {2 * inv_freq.shape[0]} of {d} dims")
-                rotary = (1, *(x for t in (qq, kk) for x in (t.data_ptr(), t.stride(0), t.stride(1)) * 2 + (t.shape[1],)),
-                          d, m.positions.data_ptr(), inv_freq.data_ptr(), 2 * inv_freq.shape[0], int(interleaved), 0,
+                turned = (x for t in (qq, kk) for x in (t.data_ptr(), t.stride(0), t.stride(1)) * 2 + (t.shape[1],))
+                rotary = (1, *turned, d, m.positions.data_ptr(), inv_freq.data_ptr(), 2 * inv_freq.shape[0], int(interleaved), 0,
                           ctypes.c_float(rotary_scale), T)
             attend = (ctypes.byref(cache.descriptor(shared_blocks)), kk.data_ptr(), kk.stride(0), kk.stride(1),
-                      vv.data_ptr(), vv.stride(0), vv.stride(1), m.slot_mapping.data_ptr(), T, qq.data_ptr(), qq.stride(0),
-                      qq.stride(1), oo.data_ptr(), oo.stride(0), oo.stride(1), hq, m.cu_seqlens_q.data_ptr(),
-                      m.context_lens.data_ptr(), bt.data_ptr(), bt.stride(0), bt.shape[1], batch, min(max_nodes, T),
-                      longest, m.tree_mask.data_ptr(), m.tree_mask.shape[1], ctypes.c_float(scale), self.workspace.data_ptr() if need > 0 else None, max(need, 0), None)
+                      vv.data_ptr(), vv.stride(0), vv.stride(1), m.slot_mapping.data_ptr(), T, qq.data_ptr(),
+                      qq.stride(0), qq.stride(1), oo.data_ptr(), oo.stride(0), oo.stride(1), hq,
+                      m.cu_seqlens_q.data_ptr(), m.context_lens.data_ptr(), bt.data_ptr(), bt.stride(0), bt.shape[1],
+                      batch, min(max_nodes, T), longest, m.tree_mask.data_ptr(), m.tree_mask.shape[1],
+                      ctypes.c_float(scale), self.workspace.data_ptr() if need > 0 else None, need, None)
             self.calls.append((rotary, attend))
         self._keep = (q, key, value, out, inv_freq)
 

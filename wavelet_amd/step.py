@@ -84,7 +84,8 @@ def _outputs(out, kinds, device: torch.device, what: str):
     for o, (name, shape, dtype) in zip(out, kinds):
         if (o is None) != (shape is None) or o is not None and (
                 o.dtype != dtype or tuple(o.shape) != shape or not o.is_contiguous() or o.device != device):
-            raise ValueError(f"out.{name} must be " + ("None" if shape is None else f"a contiguous {dtype} {shape} tensor on {device}"))
+            raise ValueError(f"out.{name} must be " +
+                             ("None" if shape is None else f"a contiguous {dtype} {shape} tensor on {device}"))
     return out
 
 
