@@ -919,6 +919,8 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
 // of a unit at a time, of the records that name a group in turn over the grid's waves:
 // each wave finds them by itself in the list of the part counts. (A workgroup per
 // record instead, three quarters of which are empty, cost 8 us for their dispatch alone.)
+// 256 / 512 / 1,024 / 2,048 workgroups: 64 sequences of 100 to 8,000 tokens with 16 to 48 drafted
+// 333 / 313 / 304 / 303 us with their attention; a merge of nothing costs the same.
 constexpr int kMergeGroups = 1024;
 template <int D>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
