@@ -473,6 +473,8 @@ int wkv_rotary(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_strid
  * sinks (NULL = none) and the table arguments as for wkv_prefill_gqa; num_tokens
  * rows are appended. At most 64 * mask_words new tokens per sequence are seen.
  * A non-finite value at a key that a row does not see leaves the row as it is.
+ * Tokens past max_seq_len or the table's width are attended by no row; the new tokens' places
+ * follow from seq_lens all the same.
  * workspace: wkv_tree_workspace_size() bytes for the same geometry, max_seq_len clipped
  * to the block-table width; without one (NULL) a sequence's keys are not cut over workgroups.
  * No counterpart in the reference, whose engine verifies drafted tokens inside

@@ -83,14 +83,16 @@ __device__ __forceinline__ const TreeArgs &tree_args() {
 }
 
 // A sequence's share of the line, per KV head: `groups` row groups of `steps` steps each
-// (a sequence without keys counts one: its rows are written all the same).
+// (a sequence without keys counts one: its rows are written all the same). The drafted tokens are
+// the last of all its tokens; of those past max_seq no key is read.
 struct TreeSeq {
-  int qlen, L, steps, groups;
+  int qlen, ctx, L, steps, groups;  // rows, cached tokens, tokens that are read
 };
 __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &a, int b) {
   TreeSeq s;
   s.qlen = a.cu_q[b + 1] - a.cu_q[b];
   s.L = a.seq_lens[b];
+  s.ctx = s.L - s.qlen;
   s.L = s.L < a.max_seq ? s.L : a.max_seq;
   s.steps = s.L > 0 ? (s.L + 63) >> 6 : 1;
   s.groups = s.qlen > 0 ? (s.qlen * a.G + kTreeRows - 1) / kTreeRows : 0;
@@ -345,7 +347,8 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
     r.h = kvh * G + x - r.node * G;
     return r;
   };
-  const int ctx = L - qlen;  // the first drafted token's position
+  const int ctx = __builtin_amdgcn_readfirstlane(sq.ctx);  // the first drafted token's position
+  const int seen_by_all = ctx < L ? ctx : L;               // keys before it need no mask
   const int s0 = s_begin, s1 = L > 0 ? s_begin + take : s_begin;
 
   // Q^T operand j: lane l holds d = 16 j + 8 (l / 32) .. + 7 of row l % 32.
@@ -789,7 +792,7 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
       __builtin_amdgcn_sched_barrier(0);
       expo(a0, a1, WHOLE);
       const uint32_t ok = tiles(s);
-      if (ok != 15u || 64 * s + 64 > ctx) {  // uniform
+      if (ok != 15u || 64 * s + 64 > seen_by_all) {  // uniform
         hide(window(s, ok), a0, a1, WHOLE);
       }
       rescale(largest(a0, a1, WHOLE), a0, a1, WHOLE);
@@ -800,7 +803,7 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
     int s = s0;
     {
       floatx16 b0, b1;
-      const int ends = (ctx >> 6) < s1 ? (ctx >> 6) : s1;
+      const int ends = (seen_by_all >> 6) < s1 ? (seen_by_all >> 6) : s1;
       for (; s + 2 < ends && clean; s += 2) {
         body(s, a0, a1, b0, b1, WHOLE);
         body(s + 1, b0, b1, a0, a1, WHOLE);
