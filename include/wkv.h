@@ -446,6 +446,17 @@ int wkv_extend_tables(int32_t *block_table, int64_t bt_stride, int32_t max_block
                       int32_t *context_lens, int32_t *cu_seqlens_q, int64_t *slot_mapping, int64_t *positions,
                       int64_t *tree_mask, int32_t *refused, void *stream);
 
+/* The same with a limit: a sequence whose cached and new tokens together pass
+ * max_seq_len is refused too (the model's context limit, and the max_seq_len that the
+ * step's attention is given: the host does not know the lengths). */
+int wkv_extend_tables_limited(int32_t *block_table, int64_t bt_stride, int32_t max_blocks_per_seq,
+                              const int32_t *held_blocks, const int32_t *seq_lens, const int32_t *new_lens,
+                              int32_t batch, int32_t block_size, const int32_t *free_blocks, int32_t num_free,
+                              const int32_t *taken, int32_t max_tokens, int32_t max_seq_len, const int32_t *parents,
+                              int32_t mask_words, int32_t *held_out, int32_t *taken_out, int32_t *context_lens,
+                              int32_t *cu_seqlens_q, int64_t *slot_mapping, int64_t *positions, int64_t *tree_mask,
+                              int32_t *refused, void *stream);
+
 /* Rotary positions over q [num_tokens, num_q_heads, head_dim] and k [num_tokens,
  * num_k_heads, head_dim] (either may have no heads): pair i of every head is
  * turned by the angle t = positions[token] * inv_freq[i] (float64; any sign),

@@ -55,7 +55,7 @@ def masks(parents, words: int) -> np.ndarray:
 
 
 def extend_tables(block_table, held_blocks, seq_lens, new_lens, free_blocks, taken, block_size, max_tokens, *,
-                  parents=None, max_nodes=0):
+                  parents=None, max_nodes=0, max_seq_len=2**31 - 1):
     """The step's tables (see ``wavelet_amd.extend_tables``): a dict of its outputs, ``block_table`` a copy."""
     table = np.array(block_table, np.int32)
     b, width = table.shape
@@ -76,7 +76,7 @@ def extend_tables(block_table, held_blocks, seq_lens, new_lens, free_blocks, tak
         if n == 0:
             continue
         total = -(-int(length[i] + n) // block_size)
-        fits = total <= width and row <= max_tokens and (words == 0 or n <= max_nodes)
+        fits = total <= width and length[i] + n <= max_seq_len and row <= max_tokens and (words == 0 or n <= max_nodes)
         need = max(total - int(held[i]), 0) if fits else 0
         asked += need  # a sequence that is refused its blocks still stands in the queue
         if not fits or (need > 0 and asked > len(free_blocks)):

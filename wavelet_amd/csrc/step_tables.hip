@@ -20,7 +20,7 @@ struct TablesArgs {
   int width;
   const int32_t *held, *seq_lens, *new_lens, *free_blocks, *taken;
   int32_t num_free;
-  int B, BS, rows;
+  int B, BS, rows, limit;  // limit: cached and new tokens of a sequence
   const int32_t *parents;
   int words;
   int32_t *held_out, *taken_out, *context, *cu, *refused;
@@ -129,7 +129,7 @@ __global__ __launch_bounds__(kTablesThreads) void tables_plan_kernel(TablesArgs 
     row = min(row + min(static_cast<uint32_t>(n[k]), row_cap), row_cap);
     if (b == a.B - 1) s_cu[a.B] = static_cast<int>(min(row, static_cast<uint32_t>(a.rows)));
     const int64_t end = static_cast<int64_t>(L[k]) + n[k], total = (end + a.BS - 1) / a.BS;
-    fits[k] = n[k] > 0 && total <= a.width && end <= INT32_MAX && row <= static_cast<uint32_t>(a.rows) &&
+    fits[k] = n[k] > 0 && total <= a.width && end <= a.limit && row <= static_cast<uint32_t>(a.rows) &&
               (a.words == 0 || n[k] <= 64 * a.words);
     need[k] = fits[k] && total > held[k] ? min(static_cast<uint32_t>(total - held[k]), need_cap) : 0u;
     sum = min(sum + need[k], need_cap);
@@ -267,16 +267,18 @@ __global__ __launch_bounds__(256) void accept_tree_kernel(const int64_t *__restr
 
 using namespace wkv;
 
-extern "C" int wkv_extend_tables(int32_t *block_table, int64_t bt_stride, int32_t max_blocks_per_seq,
-                                 const int32_t *held_blocks, const int32_t *seq_lens, const int32_t *new_lens,
-                                 int32_t batch, int32_t block_size, const int32_t *free_blocks, int32_t num_free,
-                                 const int32_t *taken, int32_t max_tokens, const int32_t *parents, int32_t mask_words,
-                                 int32_t *held_out, int32_t *taken_out, int32_t *context_lens, int32_t *cu_seqlens_q,
-                                 int64_t *slot_mapping, int64_t *positions, int64_t *tree_mask, int32_t *refused,
-                                 void *stream) {
+extern "C" int wkv_extend_tables_limited(int32_t *block_table, int64_t bt_stride, int32_t max_blocks_per_seq,
+                                         const int32_t *held_blocks, const int32_t *seq_lens, const int32_t *new_lens,
+                                         int32_t batch, int32_t block_size, const int32_t *free_blocks,
+                                         int32_t num_free, const int32_t *taken, int32_t max_tokens,
+                                         int32_t max_seq_len, const int32_t *parents, int32_t mask_words,
+                                         int32_t *held_out, int32_t *taken_out, int32_t *context_lens,
+                                         int32_t *cu_seqlens_q, int64_t *slot_mapping, int64_t *positions,
+                                         int64_t *tree_mask, int32_t *refused, void *stream) {
   WKV_CHECK_ARG(batch > 0 && batch <= WKV_STEP_MAX_BATCH, "batch must be in [1, %d] (got %d)", WKV_STEP_MAX_BATCH, batch);
   WKV_CHECK_ARG(block_size > 0, "block_size must be positive (got %d)", block_size);
   WKV_CHECK_ARG(max_tokens >= 0 && max_tokens < INT32_MAX - 1024, "max_tokens must be in [0, 2^31 - 1025)");
+  WKV_CHECK_ARG(max_seq_len >= 0, "max_seq_len must be >= 0 (got %d)", max_seq_len);
   WKV_CHECK_ARG(num_free >= 0 && num_free < INT32_MAX - 1, "num_free must be in [0, 2^31 - 2)");
   WKV_CHECK_ARG(block_table != nullptr && max_blocks_per_seq > 0 && bt_stride >= max_blocks_per_seq,
                 "bad block table geometry");
@@ -290,8 +292,8 @@ extern "C" int wkv_extend_tables(int32_t *block_table, int64_t bt_stride, int32_
   WKV_CHECK_ARG(context_lens != seq_lens && context_lens != new_lens && context_lens != held_blocks,
                 "context_lens must not be one of the inputs");
   const TablesArgs a{block_table, bt_stride, max_blocks_per_seq, held_blocks, seq_lens, new_lens, free_blocks, taken,
-                     num_free, batch, block_size, max_tokens, parents, mask_words, held_out, taken_out, context_lens,
-                     cu_seqlens_q, refused, slot_mapping, positions, tree_mask};
+                     num_free, batch, block_size, max_tokens, max_seq_len, parents, mask_words, held_out, taken_out,
+                     context_lens, cu_seqlens_q, refused, slot_mapping, positions, tree_mask};
   auto s = static_cast<hipStream_t>(stream);
   if (max_tokens <= kTablesOwnRows) {
     tables_plan_kernel<true><<<1, kTablesThreads, 0, s>>>(a);
@@ -301,6 +303,19 @@ extern "C" int wkv_extend_tables(int32_t *block_table, int64_t bt_stride, int32_
   }
   WKV_CHECK_LAUNCH("extend tables");
   return WKV_OK;
+}
+
+extern "C" int wkv_extend_tables(int32_t *block_table, int64_t bt_stride, int32_t max_blocks_per_seq,
+                                 const int32_t *held_blocks, const int32_t *seq_lens, const int32_t *new_lens,
+                                 int32_t batch, int32_t block_size, const int32_t *free_blocks, int32_t num_free,
+                                 const int32_t *taken, int32_t max_tokens, const int32_t *parents, int32_t mask_words,
+                                 int32_t *held_out, int32_t *taken_out, int32_t *context_lens, int32_t *cu_seqlens_q,
+                                 int64_t *slot_mapping, int64_t *positions, int64_t *tree_mask, int32_t *refused,
+                                 void *stream) {
+  return wkv_extend_tables_limited(block_table, bt_stride, max_blocks_per_seq, held_blocks, seq_lens, new_lens, batch,
+                                   block_size, free_blocks, num_free, taken, max_tokens, INT32_MAX, parents, mask_words,
+                                   held_out, taken_out, context_lens, cu_seqlens_q, slot_mapping, positions, tree_mask,
+                                   refused, stream);
 }
 
 extern "C" int wkv_accept_tree(const int64_t *draft_tokens, const int32_t *parents, const int64_t *target_tokens,

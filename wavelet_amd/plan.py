@@ -481,7 +481,9 @@ class TreeStep:
 
     ``new_lens [B]``, ``parents [T]`` (int32), ``draft_tokens [T]``, ``target_tokens [T]`` (int64) and the
     layers' buffers are refilled in place between steps. ``max_nodes`` (a multiple of 64 up to 256) and
-    ``max_seq_len`` bound the trees and the lengths with them, ``max_depth`` the accepted path. ``shared_blocks``
+    ``max_seq_len`` bound the trees and the lengths with them -- a sequence that would pass either (or
+    ``state.max_seq_len``, or needs a block that is not there) is refused for the step: its rows give zeros
+    and nothing of it is accepted --, ``max_depth`` the accepted path. ``shared_blocks``
     is the read policy (None: each cache's default; ``KVPool.decode_shares_blocks``). Nothing is allocated
     after the constructor and everything runs on the current stream: the three calls can be
     captured in graphs; steps of one plan, or of plans over one state, must not overlap.
@@ -515,7 +517,7 @@ class TreeStep:
             raise ValueError(f"inv_freq must be a contiguous float64 vector on {dev}")
         self.state, self.new_lens, self.parents = state, new_lens, parents
         self.draft_tokens, self.target_tokens = draft_tokens, target_tokens
-        self.max_nodes, self.max_depth = int(max_nodes), int(max_depth)
+        self.max_nodes, self.max_depth, self.max_seq_len = int(max_nodes), int(max_depth), int(max_seq_len)
         self.caches = list(caches)
         self._live = _Live(caches)
         m = self.maps = new_step_maps(batch, T, max_nodes, dev)._replace(held_blocks=state.held_blocks,
@@ -558,7 +560,7 @@ class TreeStep:
     def begin(self) -> None:
         """The step's blocks, slots, positions and masks."""
         self.state.extend(self.new_lens, self.parents.shape[0], parents=self.parents, max_nodes=self.max_nodes,
-                          out=self.maps)
+                          max_seq_len=self.max_seq_len, out=self.maps)
 
     def step_layer(self, layer: int) -> None:
         """One layer's rotation, append and attention."""

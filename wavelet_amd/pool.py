@@ -177,7 +177,8 @@ class KVPool:
         """The sequences' tables and lengths on the device, with ``num_blocks`` free blocks to extend them by there
         (``BlockManager.lend``), for steps whose token counts the host does not know (``StepState``,
         ``TreeStep``). A partly filled block that is shared is copied first. ``width`` (blocks per table) defaults to
-        ``max_blocks_per_seq``, without a ``max_model_len`` to the longest table and the loan."""
+        ``max_blocks_per_seq``, without a ``max_model_len`` to the longest table and the loan; no step takes a
+        sequence past ``max_model_len``."""
         if self.asleep:
             raise RuntimeError("the KV pool is asleep: call wake_up() first")
         seq_ids = list(seq_ids)
@@ -192,7 +193,8 @@ class KVPool:
         held = np.array([len(self.blocks.blocks_of(s)) for s in seq_ids], dtype=np.int32)
         dev = self.device
         return StepState(*(torch.from_numpy(x).to(dev) for x in (
-            table, held, lens, np.array(loan.blocks, dtype=np.int32), np.zeros(1, dtype=np.int32))), self.block_size, loan)
+            table, held, lens, np.array(loan.blocks, dtype=np.int32), np.zeros(1, dtype=np.int32))), self.block_size, loan,
+            self.max_model_len)
 
     def settle(self, state: StepState) -> None:
         """Hand a loan's tables and lengths back to the block manager (waits for the device)."""

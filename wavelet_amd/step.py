@@ -21,6 +21,7 @@ from .cache import _on, _require_cuda, _stream
 MAX_BATCH = 2048  # WKV_STEP_MAX_BATCH
 MAX_NODES = 256   # 64 * WKV_TREE_MAX_WORDS
 MAX_DEPTH = 64    # WKV_TREE_MAX_DEPTH
+NO_LIMIT = 2**31 - 1  # of a sequence's length
 
 
 class StepMaps(NamedTuple):
@@ -49,7 +50,8 @@ class Accepted(NamedTuple):
 class StepState:
     """The sequences of the next steps as the device carries them on (``KVPool.lend``): ``extend`` gives a
     step's tokens their blocks and slots, an accepted path's lengths go back into ``seq_lens``, and
-    ``KVPool.settle`` hands tables and lengths to the block manager."""
+    ``KVPool.settle`` hands tables and lengths to the block manager. No step takes a sequence past
+    ``max_seq_len`` (the pool's ``max_model_len``; None: the tables' width alone is a limit)."""
 
     block_table: torch.Tensor  # [B, M] int32
     held_blocks: torch.Tensor  # [B] int32
@@ -58,15 +60,18 @@ class StepState:
     taken: torch.Tensor        # [1] int32
     block_size: int
     loan: object = None        # the block manager's
+    max_seq_len: int | None = None
 
     def extend(self, new_lens: torch.Tensor, max_tokens: int, *, parents: torch.Tensor | None = None,
-               max_nodes: int = 0, out: StepMaps | None = None) -> StepMaps:
-        """``extend_tables`` of this state, in place (``held_blocks`` and ``taken`` of the result are the state's)."""
+               max_nodes: int = 0, max_seq_len: int | None = None, out: StepMaps | None = None) -> StepMaps:
+        """``extend_tables`` of this state, in place (``held_blocks`` and ``taken`` of the result are the state's), up
+        to the state's ``max_seq_len`` or a lower one given here."""
+        limits = [x for x in (self.max_seq_len, max_seq_len) if x is not None]
         if out is None:
             out = new_step_maps(self.block_table.shape[0], max_tokens, max_nodes, self.block_table.device)
         return extend_tables(self.block_table, self.held_blocks, self.seq_lens, new_lens, self.free_blocks, self.taken,
                              self.block_size, max_tokens, parents=parents, max_nodes=max_nodes,
-                             out=out._replace(held_blocks=self.held_blocks, taken=self.taken))
+                             max_seq_len=min(limits, default=None), out=out._replace(held_blocks=self.held_blocks, taken=self.taken))
 
 
 def _vector(x: torch.Tensor, name: str, n: int | None, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
@@ -108,7 +113,8 @@ def _new_accepted(batch: int, max_depth: int, device: torch.device) -> Accepted:
 
 def extend_tables(block_table: torch.Tensor, held_blocks: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch.Tensor,
                   free_blocks: torch.Tensor, taken: torch.Tensor, block_size: int, max_tokens: int, *,
-                  parents: torch.Tensor | None = None, max_nodes: int = 0, out: StepMaps | None = None) -> StepMaps:
+                  parents: torch.Tensor | None = None, max_nodes: int = 0, max_seq_len: int | None = None,
+                  out: StepMaps | None = None) -> StepMaps:
     """A step's blocks, slots and positions from its lengths, without the host.
 
     Sequence ``b`` (of at most 2,048) holds ``held_blocks[b]`` blocks, the leading entries of row ``b`` of
@@ -116,7 +122,8 @@ def extend_tables(block_table: torch.Tensor, held_blocks: torch.Tensor, seq_lens
     tokens, and brings ``new_lens[b]`` tokens (int32 ``[B]`` each). In batch order, each gets the blocks its
     tokens need beyond those it holds, the next of ``free_blocks`` (int32 ``[F]``) past the first
     ``taken`` (int32 ``[1]``). A sequence is refused, wholly, when it has too few table entries, rows
-    (``max_tokens``) or nodes (``max_nodes``), or needs blocks once those asked for are more than are free.
+    (``max_tokens``) or nodes (``max_nodes``), would pass ``max_seq_len`` tokens (None: no limit), or needs
+    blocks once those asked for are more than are free.
 
     The result's rows are the step's tokens, sequence by sequence (``cu_seqlens_q``), ``max_tokens`` of
     them: each token's slot and position, -1 for a refused sequence's and past the last. With ``max_nodes``
@@ -147,6 +154,9 @@ def extend_tables(block_table: torch.Tensor, held_blocks: torch.Tensor, seq_lens
     max_tokens, max_nodes, block_size = int(max_tokens), int(max_nodes), int(block_size)
     if max_tokens < 0 or block_size <= 0:
         raise ValueError("max_tokens must be non-negative and block_size positive")
+    max_seq_len = NO_LIMIT if max_seq_len is None else min(int(max_seq_len), NO_LIMIT)
+    if max_seq_len < 0:
+        raise ValueError(f"max_seq_len must be non-negative (got {max_seq_len})")
     if max_nodes % 64 or not 0 <= max_nodes <= MAX_NODES:
         raise ValueError(f"max_nodes must be a multiple of 64 up to {MAX_NODES} (got {max_nodes})")
     if (parents is None) != (max_nodes == 0):
@@ -163,10 +173,10 @@ def extend_tables(block_table: torch.Tensor, held_blocks: torch.Tensor, seq_lens
                                      ("refused", (1,), torch.int32), ("held_blocks", (batch,), torch.int32),
                                      ("taken", (1,), torch.int32)), dev, "StepMaps"))
     with _on(dev):
-        rc = _lib.load().wkv_extend_tables(
+        rc = _lib.load().wkv_extend_tables_limited(
             block_table.data_ptr(), max(block_table.stride(0), width), width, held.data_ptr(), lens.data_ptr(),
             new.data_ptr(), batch, block_size, free.data_ptr() or None, free.shape[0], taken.data_ptr(), max_tokens,
-            parents.data_ptr() if words else None, words, m.held_blocks.data_ptr(), m.taken.data_ptr(),
+            max_seq_len, parents.data_ptr() if words else None, words, m.held_blocks.data_ptr(), m.taken.data_ptr(),
             m.context_lens.data_ptr(), m.cu_seqlens_q.data_ptr(), m.slot_mapping.data_ptr(), m.positions.data_ptr(),
             m.tree_mask.data_ptr() if words else None, m.refused.data_ptr(), _stream(dev))
     _lib.check(rc, "extend_tables")
