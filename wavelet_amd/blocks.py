@@ -43,6 +43,7 @@ class Loan:
 
     seq_ids: list
     blocks: list[int]  # in the order in which they are to be taken
+    settled: bool = False
 
 
 class BlockManager:
@@ -63,7 +64,7 @@ class BlockManager:
         self._free: deque[int] = deque(range(self.num_blocks))
         self._ref = np.zeros(self.num_blocks, dtype=np.int64)
         self._seqs: dict[object, _Seq] = {}
-        self._lent: set = set()  # sequences whose tables the device extends (``lend``)
+        self._lent: dict[object, Loan] = {}  # sequences whose tables the device extends (``lend``), and their loan
         self._index: dict[bytes, int] = {}  # full-block chain hash -> block id
         self._hash_of: dict[int, bytes] = {}  # block id -> its chain hash (indexed blocks)
         self._evictable: OrderedDict[int, None] = OrderedDict()  # indexed blocks with ref 0, LRU first
@@ -298,7 +299,7 @@ class BlockManager:
             self._release(last)
             seq.blocks[at] = fresh
         loan = Loan(seq_ids, [self._take() for _ in range(num_blocks)])
-        self._lent.update(seq_ids)
+        self._lent.update(dict.fromkeys(seq_ids, loan))
         return loan, cow
 
     def settle(self, loan: Loan, block_table, held_blocks, seq_lens) -> None:
@@ -310,8 +311,8 @@ class BlockManager:
         n = len(loan.seq_ids)
         if tables.ndim != 2 or not len(tables) == len(held) == len(lens) == n:
             raise ValueError(f"the loan is of {n} sequences")
-        if any(sid not in self._lent for sid in loan.seq_ids):
-            raise ValueError("the loan is settled already")
+        if loan.settled or any(self._lent.get(sid) is not loan for sid in loan.seq_ids):
+            raise ValueError("the loan is settled already, or not this manager's")
         unused = set(loan.blocks)
         if len(unused) != len(loan.blocks):
             raise ValueError("the loan names a block twice")
@@ -334,7 +335,9 @@ class BlockManager:
         for b in loan.blocks:
             if b not in used:
                 self._release(b)
-        self._lent.difference_update(loan.seq_ids)
+        for sid in loan.seq_ids:
+            del self._lent[sid]
+        loan.settled = True
 
     def any_shared(self, seq_ids) -> bool:
         """Whether any block of these sequences is held by more than one sequence: a
