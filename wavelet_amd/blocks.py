@@ -306,7 +306,8 @@ class BlockManager:
         """Take over what the device made of a loan: row ``i`` of ``block_table`` (its first ``held_blocks[i]``
         entries) and ``seq_lens[i]`` are sequence ``loan.seq_ids[i]``'s table and length; lent blocks that no
         length needs go back to the free pool. Raises ValueError, before any state moves, for tables
-        that do not continue the sequences' own with lent blocks, each used once."""
+        that do not continue the sequences' own with lent blocks, each used once, and for lengths past
+        ``max_model_len``."""
         tables, held, lens = (np.asarray(x, dtype=np.int64) for x in (block_table, held_blocks, seq_lens))
         n = len(loan.seq_ids)
         if tables.ndim != 2 or not len(tables) == len(held) == len(lens) == n:
@@ -323,6 +324,8 @@ class BlockManager:
             if not have <= held[i] <= tables.shape[1] or not seq.length <= lens[i] <= held[i] * self.block_size:
                 raise ValueError(f"sequence {sid!r}: {int(held[i])} blocks and {int(lens[i])} tokens do not continue "
                                  f"its {have} and {seq.length}")
+            if self.max_model_len is not None and lens[i] > self.max_model_len:
+                raise ValueError(f"sequence {sid!r}: {int(lens[i])} tokens are more than max_model_len {self.max_model_len}")
             row = tables[i, :held[i]].tolist()
             if row[:have] != seq.blocks or not unused.issuperset(row[have:]) or len(set(row[have:])) != held[i] - have:
                 raise ValueError(f"sequence {sid!r}: its table is not its own blocks and lent ones")
