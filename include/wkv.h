@@ -516,6 +516,14 @@ int wkv_accept_tree(const int64_t *draft_tokens, const int32_t *parents, const i
                     const int32_t *context_lens, int32_t batch, int32_t max_depth, int32_t *accepted, int32_t *path,
                     int64_t *next_tokens, int32_t *seq_lens_out, void *stream);
 
+/* The same, and pending [B] (NULL = none), the token that each sequence goes on
+ * with: next_tokens[b] where the sequence accepted anything, else left as it is (a
+ * sequence that a step refuses or leaves out keeps the token sampled before). */
+int wkv_accept_tree_pending(const int64_t *draft_tokens, const int32_t *parents, const int64_t *target_tokens,
+                            int64_t num_tokens, const int32_t *cu_seqlens_q, const int32_t *seq_lens,
+                            const int32_t *context_lens, int32_t batch, int32_t max_depth, int32_t *accepted,
+                            int32_t *path, int64_t *next_tokens, int32_t *seq_lens_out, int64_t *pending, void *stream);
+
 /* Moves an accepted path's keys and values together, in place: for j <
  * accepted[b] the token at position seq_lens[b] + path[b, j] of sequence b goes to position seq_lens[b]
  * + j (seq_lens: the lengths before the step). All are read before any is

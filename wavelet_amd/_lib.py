@@ -98,6 +98,8 @@ _SIGNATURES = {
                              c_float, c_void_p, c_int64, c_void_p, c_void_p]),
     "wkv_accept_tree": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p,
                                 c_void_p, c_void_p, c_void_p, c_void_p]),
+    "wkv_accept_tree_pending": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int32,
+                                        c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "wkv_compact": (c_int, [POINTER(WkvCache), c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_int32, c_void_p,
                             c_int32, c_void_p]),
     "wkv_mla_workspace_size": (c_int64, [c_int32, c_int32, c_int32, c_int32, c_int32]),

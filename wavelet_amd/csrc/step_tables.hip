@@ -216,7 +216,8 @@ __global__ __launch_bounds__(256) void accept_tree_kernel(const int64_t *__restr
                                                           const int32_t *__restrict__ cu, const int32_t *seq_lens,
                                                           const int32_t *__restrict__ context, int B, int max_depth,
                                                           int32_t *__restrict__ accepted, int32_t *__restrict__ path,
-                                                          int64_t *__restrict__ next, int32_t *len_out) {
+                                                          int64_t *__restrict__ next, int32_t *len_out,
+                                                          int64_t *__restrict__ pending) {
   constexpr int N = WKV_TREE_MAX_WORDS;
   const int b = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x * 4 + (threadIdx.x >> 6)));
   if (b >= B) return;
@@ -259,6 +260,7 @@ __global__ __launch_bounds__(256) void accept_tree_kernel(const int64_t *__restr
   if (lane == 0) {
     accepted[b] = count;
     next[b] = want;
+    if (pending != nullptr && count > 0) pending[b] = want;
     len_out[b] = L + count;
   }
 }
@@ -318,10 +320,11 @@ extern "C" int wkv_extend_tables(int32_t *block_table, int64_t bt_stride, int32_
                                    refused, stream);
 }
 
-extern "C" int wkv_accept_tree(const int64_t *draft_tokens, const int32_t *parents, const int64_t *target_tokens,
-                               int64_t num_tokens, const int32_t *cu_seqlens_q, const int32_t *seq_lens,
-                               const int32_t *context_lens, int32_t batch, int32_t max_depth, int32_t *accepted,
-                               int32_t *path, int64_t *next_tokens, int32_t *seq_lens_out, void *stream) {
+extern "C" int wkv_accept_tree_pending(const int64_t *draft_tokens, const int32_t *parents,
+                                       const int64_t *target_tokens, int64_t num_tokens, const int32_t *cu_seqlens_q,
+                                       const int32_t *seq_lens, const int32_t *context_lens, int32_t batch,
+                                       int32_t max_depth, int32_t *accepted, int32_t *path, int64_t *next_tokens,
+                                       int32_t *seq_lens_out, int64_t *pending, void *stream) {
   WKV_CHECK_ARG(batch >= 0, "batch must be >= 0 (got %d)", batch);
   WKV_CHECK_ARG(max_depth > 0 && max_depth <= WKV_TREE_MAX_DEPTH, "max_depth must be in [1, %d] (got %d)",
                 WKV_TREE_MAX_DEPTH, max_depth);
@@ -333,7 +336,15 @@ extern "C" int wkv_accept_tree(const int64_t *draft_tokens, const int32_t *paren
                 "an input or output is NULL");
   accept_tree_kernel<<<static_cast<unsigned>((batch + 3) / 4), 256, 0, static_cast<hipStream_t>(stream)>>>(
       draft_tokens, parents, target_tokens, static_cast<int>(num_tokens), cu_seqlens_q, seq_lens, context_lens, batch,
-      max_depth, accepted, path, next_tokens, seq_lens_out);
+      max_depth, accepted, path, next_tokens, seq_lens_out, pending);
   WKV_CHECK_LAUNCH("accept tree");
   return WKV_OK;
+}
+
+extern "C" int wkv_accept_tree(const int64_t *draft_tokens, const int32_t *parents, const int64_t *target_tokens,
+                               int64_t num_tokens, const int32_t *cu_seqlens_q, const int32_t *seq_lens,
+                               const int32_t *context_lens, int32_t batch, int32_t max_depth, int32_t *accepted,
+                               int32_t *path, int64_t *next_tokens, int32_t *seq_lens_out, void *stream) {
+  return wkv_accept_tree_pending(draft_tokens, parents, target_tokens, num_tokens, cu_seqlens_q, seq_lens, context_lens,
+                                 batch, max_depth, accepted, path, next_tokens, seq_lens_out, nullptr, stream);
 }

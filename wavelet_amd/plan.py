@@ -477,7 +477,8 @@ class TreeStep:
     (``paged_tree_gqa``) --, then ``finish()`` once ``target_tokens`` holds what was sampled after every
     node: the path that agrees is accepted (``accept_tree``), its keys and values move together in every layer's
     cache (``compact``) and ``state.seq_lens`` moves on. ``maps`` and ``accepted`` are the step's results;
-    ``accepted.next_tokens`` are the next step's first nodes.
+    ``state.next_tokens`` are the next step's first nodes: what was sampled after the accepted path, and what
+    it was for a sequence of which nothing was accepted (paused, ``new_lens`` 0, or refused).
 
     ``new_lens [B]``, ``parents [T]`` (int32), ``draft_tokens [T]``, ``target_tokens [T]`` (int64) and the
     layers' buffers are refilled in place between steps. ``max_nodes`` (a multiple of 64 up to 256) and
@@ -515,6 +516,10 @@ class TreeStep:
         if inv_freq is not None and (inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.device != dev
                                      or not inv_freq.is_contiguous()):
             raise ValueError(f"inv_freq must be a contiguous float64 vector on {dev}")
+        pending = state.next_tokens
+        if pending is not None and (pending.dtype != torch.int64 or tuple(pending.shape) != (batch,)
+                                    or not pending.is_contiguous() or pending.device != dev):
+            raise ValueError(f"state.next_tokens must be a contiguous int64 [{batch}] tensor on {dev}")
         self.state, self.new_lens, self.parents = state, new_lens, parents
         self.draft_tokens, self.target_tokens = draft_tokens, target_tokens
         self.max_nodes, self.max_depth, self.max_seq_len = int(max_nodes), int(max_depth), int(max_seq_len)
@@ -586,7 +591,7 @@ class TreeStep:
         self._live.check_all()
         m, s, a = self.maps, self.state, self.accepted
         accept_tree(self.draft_tokens, self.parents, self.target_tokens, m.cu_seqlens_q, s.seq_lens, m.context_lens,
-                    self.max_depth, out=a)
+                    self.max_depth, pending=s.next_tokens, out=a)
         for cache in self.caches:
             cache.compact(s.block_table, s.seq_lens, a.path, a.accepted)
         s.seq_lens.copy_(a.seq_lens)

@@ -178,7 +178,8 @@ class KVPool:
         (``BlockManager.lend``), for steps whose token counts the host does not know (``StepState``,
         ``TreeStep``). A partly filled block that is shared is copied first. ``width`` (blocks per table) defaults to
         ``max_blocks_per_seq``, without a ``max_model_len`` to the longest table and the loan; no step takes a
-        sequence past ``max_model_len``."""
+        sequence past ``max_model_len``. ``next_tokens`` of the result is -1 until the caller fills in what was
+        sampled last."""
         if self.asleep:
             raise RuntimeError("the KV pool is asleep: call wake_up() first")
         seq_ids = list(seq_ids)
@@ -194,7 +195,7 @@ class KVPool:
         dev = self.device
         return StepState(*(torch.from_numpy(x).to(dev) for x in (
             table, held, lens, np.array(loan.blocks, dtype=np.int32), np.zeros(1, dtype=np.int32))), self.block_size, loan,
-            self.max_model_len)
+            self.max_model_len, torch.full((len(seq_ids),), -1, dtype=torch.int64, device=dev))
 
     def settle(self, state: StepState) -> None:
         """Hand a loan's tables and lengths back to the block manager (waits for the device)."""

@@ -49,7 +49,8 @@ class Accepted(NamedTuple):
 @dataclass
 class StepState:
     """The sequences of the next steps as the device carries them on (``KVPool.lend``): ``extend`` gives a
-    step's tokens their blocks and slots, an accepted path's lengths go back into ``seq_lens``, and
+    step's tokens their blocks and slots, an accepted path's lengths go back into ``seq_lens`` and the token
+    sampled after it into ``next_tokens`` (a sequence that accepts nothing keeps its own), and
     ``KVPool.settle`` hands tables and lengths to the block manager. No step takes a sequence past
     ``max_seq_len`` (the pool's ``max_model_len``; None: the tables' width alone is a limit)."""
 
@@ -61,6 +62,7 @@ class StepState:
     block_size: int
     loan: object = None        # the block manager's
     max_seq_len: int | None = None
+    next_tokens: torch.Tensor | None = None  # [B] int64: sampled, not cached yet: node 0 of the next step's trees
 
     def extend(self, new_lens: torch.Tensor, max_tokens: int, *, parents: torch.Tensor | None = None,
                max_nodes: int = 0, max_seq_len: int | None = None, out: StepMaps | None = None) -> StepMaps:
@@ -185,7 +187,7 @@ def extend_tables(block_table: torch.Tensor, held_blocks: torch.Tensor, seq_lens
 
 def accept_tree(draft_tokens: torch.Tensor, parents: torch.Tensor, target_tokens: torch.Tensor,
                 cu_seqlens_q: torch.Tensor, seq_lens: torch.Tensor, context_lens: torch.Tensor, max_depth: int, *,
-                out: Accepted | None = None) -> Accepted:
+                pending: torch.Tensor | None = None, out: Accepted | None = None) -> Accepted:
     """The drafted tokens of a verified tree that agree with the sampled ones.
 
     ``draft_tokens [T]`` int64 and ``parents [T]`` int32 are the trees' nodes, sequence by sequence
@@ -195,7 +197,9 @@ def accept_tree(draft_tokens: torch.Tensor, parents: torch.Tensor, target_tokens
     it, up to ``max_depth`` (at most 64) nodes. ``next_tokens`` is what was sampled after the last.
     ``seq_lens`` are the lengths before the step, and the result's those with the accepted tokens
     (``out.seq_lens`` may be the argument); ``PagedKVCache.compact`` moves their keys and values there. A
-    sequence without nodes or with ``context_lens`` 0 (refused by ``extend_tables``) accepts nothing.
+    sequence without nodes or with ``context_lens`` 0 (refused by ``extend_tables``) accepts nothing
+    (``next_tokens`` -1). ``pending [B]`` int64, written in place: the token that each sequence goes on with,
+    ``next_tokens`` where anything was accepted, else what it was.
     """
     _require_cuda(cu_seqlens_q, "cu_seqlens_q", cu_seqlens_q.device if isinstance(cu_seqlens_q, torch.Tensor) else None)
     dev = cu_seqlens_q.device
@@ -214,6 +218,8 @@ def accept_tree(draft_tokens: torch.Tensor, parents: torch.Tensor, target_tokens
     max_depth = int(max_depth)
     if not 1 <= max_depth <= MAX_DEPTH:
         raise ValueError(f"max_depth must be in [1, {MAX_DEPTH}] (got {max_depth})")
+    if pending is not None and (_vector(pending, "pending", batch, torch.int64, dev) is not pending):
+        raise ValueError("pending must be contiguous (it is written in place)")
     if out is None:
         a = _new_accepted(batch, max_depth, dev)
     else:
@@ -223,9 +229,9 @@ def accept_tree(draft_tokens: torch.Tensor, parents: torch.Tensor, target_tokens
     if batch == 0:
         return a
     with _on(dev):
-        rc = _lib.load().wkv_accept_tree(draft.data_ptr(), parents.data_ptr(), target.data_ptr(), rows,
-                                         cu.data_ptr(), lens.data_ptr(), context.data_ptr(), batch, max_depth,
-                                         a.accepted.data_ptr(), a.path.data_ptr(), a.next_tokens.data_ptr(),
-                                         a.seq_lens.data_ptr(), _stream(dev))
+        rc = _lib.load().wkv_accept_tree_pending(
+            draft.data_ptr(), parents.data_ptr(), target.data_ptr(), rows, cu.data_ptr(), lens.data_ptr(),
+            context.data_ptr(), batch, max_depth, a.accepted.data_ptr(), a.path.data_ptr(), a.next_tokens.data_ptr(),
+            a.seq_lens.data_ptr(), pending.data_ptr() if pending is not None else None, _stream(dev))
     _lib.check(rc, "accept_tree")
     return a
