@@ -482,7 +482,8 @@ int wkv_rotary(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_strid
  * int64) is set; a row that sees nothing gives zeros. Keys of a table
  * entry outside the cache are seen by no row. key / value / slot_mapping, q, out,
  * sinks (NULL = none) and the table arguments as for wkv_prefill_gqa; num_tokens
- * rows are appended. At most 64 * mask_words new tokens per sequence are seen.
+ * rows are appended. At most 64 * mask_words new tokens per sequence are seen. Rows past
+ * max_query_len (if it is not 0) are computed too, a sequence's in turn: the bound shapes the launch.
  * A non-finite value at a key that a row does not see leaves the row as it is.
  * Tokens past max_seq_len or the table's width are attended by no row; the new tokens' places
  * follow from seq_lens all the same.

@@ -307,7 +307,10 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_gqa_kernel(TreeArgs kern
     kvh = item - b * a.Hkv;
     const TreeSeq s = tree_seq(a, b);
     if (rg >= s.groups) return;
-    steps_left = s.steps;
+    // (the last one takes those past the longest query that the launch was told of, too: a sequence
+    // that was refused for its many nodes has rows to clear)
+    const int64_t all = static_cast<int64_t>(rg + 1 == a.groups ? s.groups - rg : 1) * s.steps;
+    steps_left = all < INT32_MAX ? static_cast<int>(all) : INT32_MAX;
   }
   for (;;) {  // the row groups of the share
   const TreeArgs &a = tree_args();
