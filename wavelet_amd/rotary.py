@@ -13,6 +13,7 @@ from __future__ import annotations
 import math
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _lib
 from .cache import _on, _require_cuda, _stream
@@ -133,14 +134,22 @@ def _launch(q, k, positions, inv_freq, interleaved: bool, scale: float, inverse:
     return qo, ko
 
 
+def _dual(*tensors) -> bool:
+    """Whether any of them carries a tangent (forward-mode derivatives)."""
+    return _forward_ad._current_level >= 0 and any(
+        t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 class _Rotary(torch.autograd.Function):
     """The rotation is linear and its transpose turns the other way: the backward pass is the same launch
-    with the angles negated (and differentiable again)."""
+    with the angles negated (and differentiable again), a tangent's the launch itself."""
 
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, interleaved, scale, inverse):
         ctx.save_for_backward(positions, inv_freq)
+        ctx.save_for_forward(positions, inv_freq)
         ctx.how = (interleaved, scale, inverse)
+        ctx.heads = (q.shape[1], None if k is None else k.shape[1])
         ctx.set_materialize_grads(False)
         return _launch(q, k, positions, inv_freq, interleaved, scale, inverse, None)
 
@@ -150,12 +159,21 @@ class _Rotary(torch.autograd.Function):
         lone = gk if gq is None else None  # k's alone
         if gq is not None or gk is not None:
             interleaved, scale, inverse = ctx.how
-            turn = _Rotary.apply if torch.is_grad_enabled() else _launch_back
+            turn = _Rotary.apply if torch.is_grad_enabled() or _dual(gq, gk) else _launch_back
             gq, gk = turn(gq if lone is None else lone, gk if lone is None else None, *ctx.saved_tensors, interleaved,
                           scale, not inverse)
         if lone is not None:
             gq, gk = None, gq
         return gq, gk, None, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        some, k_heads = tk if tq is None else tq, ctx.heads[1]
+        if tq is None:  # (autograd takes no result without a tangent next to one with)
+            tq = some.new_zeros((some.shape[0], ctx.heads[0], some.shape[2]))
+        if tk is None and k_heads is not None:
+            tk = some.new_zeros((some.shape[0], k_heads, some.shape[2]))
+        return _launch(tq, tk, *ctx.saved_tensors, *ctx.how, None)
 
 
 def _launch_back(*args):
@@ -174,8 +192,8 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     i + R / 2)``, or ``(2 i, 2 i + 1)`` if ``interleaved``; dims from ``R`` on stay as they are. Positions
     may be any, in any order (a drafted tree's depths; far ones keep their exact angle). ``inverse``
     turns back (the transpose, also by ``scale``). ``out``: the two results' tensors; ``out=(q, k)`` works in
-    place, other tensors share no memory with ``q`` and ``k``. Differentiable in ``q`` and ``k`` (not with
-    ``out``). For an MLA layer, ``q_pe`` and ``k_pe[:, None]``.
+    place, other tensors share no memory with ``q`` and ``k``. Differentiable in ``q`` and ``k``, forward
+    mode too (not with ``out``). For an MLA layer, ``q_pe`` and ``k_pe[:, None]``.
     """
     if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype not in _DTYPES:
         raise ValueError("q must be a bfloat16, float16 or float32 [T, Hq, D] tensor")
@@ -193,7 +211,7 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not 0 < 2 * inv_freq.shape[0] <= d:
         raise ValueError(f"inv_freq must be float64 [R / 2] with R <= {d} (got {inv_freq.dtype} {tuple(inv_freq.shape)})")
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
-    grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
+    grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) or _dual(q, k)
     if out is None and grad:
         return _Rotary.apply(q, k, positions, inv_freq, bool(interleaved), float(scale), bool(inverse))
     if out is not None:
