@@ -531,7 +531,7 @@ int wkv_accept_tree_pending(const int64_t *draft_tokens, const int32_t *parents,
  * written. path [B, path_len] rises from path[b, j] >= j; tokens that keep their place
  * are not touched. fp8: the moved tokens' exact values are appended as
  * wkv_append_fp8 codes them (a block begun at its first slot starts afresh).
- * Positions without a block move nothing. Blocks that are written must belong to one
+ * Positions without a block move nothing, and nothing moves there. Blocks that are written must belong to one
  * sequence. No counterpart in the reference (inside llm.generate). */
 int wkv_compact(const wkv_cache_t *cache, const int32_t *block_table, int64_t bt_stride, int32_t max_blocks_per_seq,
                 const int32_t *seq_lens, const int32_t *path, int32_t path_len, const int32_t *accepted, int32_t batch,

@@ -127,16 +127,24 @@ def accept_tree(draft_tokens, parents, target_tokens, cu_seqlens_q, seq_lens, co
 
 def compact(k, v, k_scale, v_scale, block_table, seq_lens, path, accepted) -> None:
     """The tokens at positions ``seq_lens[i] + path[i, j]`` to ``seq_lens[i] + j``, in place: those that change
-    their place are read together, then appended (fp8: their exact values, as ``append_fp8`` codes them)."""
+    their place are read together, then appended (fp8: their exact values, as ``append_fp8`` codes them). One
+    whose old or new position has no block is left out."""
     bs = v.shape[-1]
     nb, h, d = v.shape[:3]
     for i in range(len(seq_lens)):
-        moved = [j for j in range(int(accepted[i])) if path[i, j] != j]
-        if not moved:
+        row = np.asarray(block_table[i])
+
+        def slot(p):
+            blk = int(row[p // bs]) if 0 <= p < len(row) * bs else -1
+            return blk * bs + p % bs if 0 <= blk < nb else -1
+
+        at = max(int(seq_lens[i]), 0)
+        places = [(slot(at + int(path[i, j])), slot(at + j)) for j in range(int(accepted[i]))
+                  if path[i, j] != j and path[i, j] >= 0]
+        places = np.array([p for p in places if min(p) >= 0]).reshape(-1, 2)
+        if not len(places):
             continue
-        slot = lambda p: int(block_table[i][p // bs]) * bs + p % bs  # noqa: E731
-        src = np.array([slot(int(seq_lens[i]) + int(path[i, j])) for j in moved])
-        dst = np.array([slot(int(seq_lens[i]) + j) for j in moved])
+        src, dst = places.T
         kl = np.ascontiguousarray(paged.k_logical(k)[src // bs, src % bs]).reshape(len(src), h, d)
         vl = np.ascontiguousarray(paged.v_logical(v)[src // bs, src % bs])
         if k_scale is None:

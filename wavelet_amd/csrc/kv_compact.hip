@@ -30,8 +30,9 @@ __global__ __launch_bounds__(64 * kCompactWaves) void compact_kernel(
   struct Place {
     int blk, off;  // block (-1: none) and offset in it
   };
-  __shared__ Place src[P], dst[P];
-  __shared__ int64_t slots[P];  // of the new places, for the fp8 runs
+  __shared__ Place src[P], dst[P];  // of the moved tokens that have both
+  __shared__ int64_t slots[P];      // of the new places, for the fp8 runs
+  __shared__ int moved;
   const int b = blockIdx.y, h = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -42,28 +43,37 @@ __global__ __launch_bounds__(64 * kCompactWaves) void compact_kernel(
   const int mine = lane < n ? path[static_cast<int64_t>(b) * path_len + lane] : lane;
   const uint64_t off = __ballot(mine != lane);
   if (off == 0) return;  // the whole workgroup
-  const int j0 = __builtin_ctzll(off);
-  const int m = n - j0;  // moved tokens: path entries j0 .. n - 1
+  const int j0 = __builtin_ctzll(off);  // path entries j0 .. n - 1 move
   const int32_t *row = bt + b * bt_stride;
   auto place = [&](int64_t pos) {
     if (pos < 0 || pos >= static_cast<int64_t>(Mb) * BS || pos > INT32_MAX) return Place{-1, 0};
     const int i = static_cast<int>(pos) / BS, blk = row[i];
     return blk >= 0 && blk < NB ? Place{blk, static_cast<int>(pos) - i * BS} : Place{-1, 0};
   };
-  if (wave == 0 && lane >= j0 && lane < n) {
-    const Place d = place(static_cast<int64_t>(L) + lane);
-    src[lane - j0] = mine >= 0 ? place(static_cast<int64_t>(L) + mine) : Place{-1, 0};
-    dst[lane - j0] = d;
-    slots[lane - j0] = static_cast<int64_t>(d.blk) * BS + d.off;
+  if (wave == 0) {  // uniform. What has no place before or after is left out, so that a block's tokens are one run.
+    Place d{-1, 0}, s{-1, 0};
+    if (lane >= j0 && lane < n && mine != lane) {
+      d = place(static_cast<int64_t>(L) + lane);
+      if (mine >= 0) s = place(static_cast<int64_t>(L) + mine);
+    }
+    const bool both = d.blk >= 0 && s.blk >= 0;
+    const uint64_t kept = __ballot(both);
+    if (both) {
+      const int t = __builtin_popcountll(kept & ((1ull << lane) - 1ull));
+      src[t] = s;
+      dst[t] = d;
+      slots[t] = static_cast<int64_t>(d.blk) * BS + d.off;
+    }
+    if (lane == 0) moved = __builtin_popcountll(kept);
   }
   auto region = [&](const Place &x) { return static_cast<int64_t>(x.blk) * H + h; };
   __syncthreads();
+  const int m = __builtin_amdgcn_readfirstlane(moved);
   constexpr int X = FP8 ? 16 : 8;  // elements of a K chunk
   constexpr int NC = D / X;
   for (int i = tid; i < m * NC; i += 64 * kCompactWaves) {
     const int t = i / NC, c = i % NC;
     const Place s = src[t];
-    if (s.blk < 0) continue;
     const u32x4 w = *reinterpret_cast<const u32x4 *>(kc + ((region(s) * NC + c) * BS + s.off) * 16);
     if constexpr (FP8) {
       const float sc = ks[region(s)];
@@ -84,7 +94,6 @@ __global__ __launch_bounds__(64 * kCompactWaves) void compact_kernel(
   for (int i = tid; i < m * D; i += 64 * kCompactWaves) {
     const int t = i / D, d = i % D;
     const Place s = src[t];
-    if (s.blk < 0) continue;
     const int64_t at = (region(s) * D + d) * BS + s.off;
     if constexpr (FP8)
       rv[t * KP + d] = static_cast<uint16_t>(f32_to_bf16_bits(e4m3_decode(vc[at]) * vs[region(s)]));
@@ -96,7 +105,6 @@ __global__ __launch_bounds__(64 * kCompactWaves) void compact_kernel(
     for (int i = tid; i < m * NC; i += 64 * kCompactWaves) {
       const int t = i / NC, c = i % NC;
       const Place s = dst[t];
-      if (s.blk < 0 || src[t].blk < 0) continue;
       *reinterpret_cast<u32x4 *>(kc + ((region(s) * NC + c) * BS + s.off) * 16) =
           *reinterpret_cast<const u32x4 *>(rk + t * KP + 8 * c);
     }
@@ -104,21 +112,16 @@ __global__ __launch_bounds__(64 * kCompactWaves) void compact_kernel(
     for (int i = tid; i < m * D; i += 64 * kCompactWaves) {
       const int t = i / D, d = i % D;
       const Place s = dst[t];
-      if (s.blk < 0 || src[t].blk < 0) continue;
       reinterpret_cast<uint16_t *>(vc)[(region(s) * D + d) * BS + s.off] = rv[t * KP + d];
     }
   } else {
-    // Runs: the new places by block, in turn over the waves. A run ends before a
-    // token whose old or new place is no slot (what stands there then is unspecified).
+    // Runs: the new places by block, in turn over the waves -- one run a block, as two waves
+    // at one block would race.
     int run = 0;
     for (int t = 0; t < m;) {  // uniform
       const int blk = __builtin_amdgcn_readfirstlane(dst[t].blk), first = __builtin_amdgcn_readfirstlane(dst[t].off);
-      if (blk < 0 || src[t].blk < 0) {
-        ++t;
-        continue;
-      }
       int r = 1;
-      while (t + r < m && first + r < BS && dst[t + r].blk == blk && src[t + r].blk >= 0) ++r;
+      while (t + r < m && dst[t + r].blk == blk) ++r;
       r = __builtin_amdgcn_readfirstlane(r);
       if (run % kCompactWaves == wave)
         fp8_append_run_kv<D>(kc, vc, ks, vs, rk, KP, 0, rv, KP, 0, slots, t, r, blk, first, h, H, BS);
