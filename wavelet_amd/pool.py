@@ -198,7 +198,10 @@ class KVPool:
             self.max_model_len, torch.full((len(seq_ids),), -1, dtype=torch.int64, device=dev))
 
     def settle(self, state: StepState) -> None:
-        """Hand a loan's tables and lengths back to the block manager (waits for the device)."""
+        """Hand a loan's tables and lengths back to the block manager (waits for the device: its steps may have run
+        on any stream)."""
+        if self.device.type == "cuda":
+            torch.cuda.synchronize(self.device)
         self.blocks.settle(state.loan, *(x.cpu().numpy() for x in (state.block_table, state.held_blocks, state.seq_lens)))
 
     def decode_shares_blocks(self, seq_ids) -> bool:
