@@ -43,6 +43,7 @@ class Loan:
 
     seq_ids: list
     blocks: list[int]  # in the order in which they are to be taken
+    copies: list[tuple]  # (sequence, place in its table, shared block, its own in the place of it)
     settled: bool = False
 
 
@@ -269,7 +270,7 @@ class BlockManager:
         (``extend_tables``), over any number of steps, until ``settle``.
 
         Also returns the copy-on-write pairs to apply first (as ``append_slots``): each sequence's
-        partly filled last block becomes its own. Until it is settled the manager neither changes
+        partly filled last block becomes its own. Until it is settled (or cancelled) the manager neither changes
         nor frees these sequences. Raises MemoryError, before any state moves, when too few blocks are free.
         """
         seq_ids, num_blocks = list(seq_ids), int(num_blocks)
@@ -286,21 +287,45 @@ class BlockManager:
                 last = seq.blocks[seq.length // self.block_size]
                 refs = held.get(last, int(self._ref[last]))
                 if refs > 1:
-                    copies.append(seq)
+                    copies.append(sid)
                     held[last] = refs - 1
         need = num_blocks + len(copies)
         if need > self.num_free_blocks:
             raise MemoryError(f"out of KV cache blocks: the loan needs {need}, {self.num_free_blocks} are free")
-        cow = []
-        for seq in copies:
+        made = []
+        for sid in copies:
+            seq = self._seqs[sid]
             at = seq.length // self.block_size
             last, fresh = seq.blocks[at], self._take()
-            cow.append((last, fresh))
+            made.append((sid, at, last, fresh))
             self._release(last)
             seq.blocks[at] = fresh
-        loan = Loan(seq_ids, [self._take() for _ in range(num_blocks)])
+        loan = Loan(seq_ids, [self._take() for _ in range(num_blocks)], made)
         self._lent.update(dict.fromkeys(seq_ids, loan))
-        return loan, cow
+        return loan, [(last, fresh) for _, _, last, fresh in made]
+
+    def _open(self, loan: Loan) -> None:
+        if loan.settled or any(self._lent.get(sid) is not loan for sid in loan.seq_ids):
+            raise ValueError("the loan is settled already, or not this manager's")
+
+    def _close(self, loan: Loan) -> None:
+        for sid in loan.seq_ids:
+            del self._lent[sid]
+        loan.settled = True
+
+    def cancel(self, loan: Loan, *, copied: bool = True) -> None:
+        """Take a loan back without a settlement: its blocks return to the free pool, its sequences keep the tables
+        and lengths that they have here. ``copied``: whether the copy-on-write pairs were applied (else the
+        sequences share those blocks again). The device must be done with the loan's steps."""
+        self._open(loan)
+        if not copied:
+            for sid, at, last, fresh in loan.copies:
+                self._seqs[sid].blocks[at] = last
+                self._ref[last] += 1
+                self._release(fresh)
+        for b in loan.blocks:
+            self._release(b)
+        self._close(loan)
 
     def settle(self, loan: Loan, block_table, held_blocks, seq_lens) -> None:
         """Take over what the device made of a loan: row ``i`` of ``block_table`` (its first ``held_blocks[i]``
@@ -312,8 +337,7 @@ class BlockManager:
         n = len(loan.seq_ids)
         if tables.ndim != 2 or not len(tables) == len(held) == len(lens) == n:
             raise ValueError(f"the loan is of {n} sequences")
-        if loan.settled or any(self._lent.get(sid) is not loan for sid in loan.seq_ids):
-            raise ValueError("the loan is settled already, or not this manager's")
+        self._open(loan)
         unused = set(loan.blocks)
         if len(unused) != len(loan.blocks):
             raise ValueError("the loan names a block twice")
@@ -338,9 +362,7 @@ class BlockManager:
         for b in loan.blocks:
             if b not in used:
                 self._release(b)
-        for sid in loan.seq_ids:
-            del self._lent[sid]
-        loan.settled = True
+        self._close(loan)
 
     def any_shared(self, seq_ids) -> bool:
         """Whether any block of these sequences is held by more than one sequence: a

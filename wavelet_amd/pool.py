@@ -189,19 +189,33 @@ class KVPool:
         if not seq_ids or width < max(longest, 1):
             raise ValueError(f"a loan needs sequences and tables of at least {max(longest, 1)} blocks")
         loan, cow = self.blocks.lend(seq_ids, num_blocks)
-        self.copy_blocks(cow)
-        table, lens = self.blocks.tables(seq_ids, width)
-        held = np.array([len(self.blocks.blocks_of(s)) for s in seq_ids], dtype=np.int32)
-        dev = self.device
-        return StepState(*(torch.from_numpy(x).to(dev) for x in (
-            table, held, lens, np.array(loan.blocks, dtype=np.int32), np.zeros(1, dtype=np.int32))), self.block_size, loan,
-            self.max_model_len, torch.full((len(seq_ids),), -1, dtype=torch.int64, device=dev))
+        try:
+            table, lens = self.blocks.tables(seq_ids, width)
+            held = np.array([len(self.blocks.blocks_of(s)) for s in seq_ids], dtype=np.int32)
+            dev = self.device
+            state = StepState(*(torch.from_numpy(x).to(dev) for x in (
+                table, held, lens, np.array(loan.blocks, dtype=np.int32), np.zeros(1, dtype=np.int32))), self.block_size,
+                loan, self.max_model_len, torch.full((len(seq_ids),), -1, dtype=torch.int64, device=dev))
+            self.copy_blocks(cow)
+        except BaseException:
+            self.blocks.cancel(loan, copied=False)
+            raise
+        return state
 
-    def settle(self, state: StepState) -> None:
-        """Hand a loan's tables and lengths back to the block manager (waits for the device: its steps may have run
-        on any stream)."""
+    def _wait(self) -> None:
+        """The device done (steps over a loan may have run on any stream)."""
         if self.device.type == "cuda":
             torch.cuda.synchronize(self.device)
+
+    def cancel(self, state: StepState) -> None:
+        """Take a loan back without its steps (``BlockManager.cancel``): the sequences are as before it."""
+        self._wait()
+        self.blocks.cancel(state.loan)
+
+    def settle(self, state: StepState) -> None:
+        """Hand a loan's tables and lengths back to the block manager (waits for the device). What cannot settle
+        raises ValueError and stays lent, for ``cancel``."""
+        self._wait()
         self.blocks.settle(state.loan, *(x.cpu().numpy() for x in (state.block_table, state.held_blocks, state.seq_lens)))
 
     def decode_shares_blocks(self, seq_ids) -> bool:
