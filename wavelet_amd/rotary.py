@@ -215,13 +215,17 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     if out is None and grad:
         return _Rotary.apply(q, k, positions, inv_freq, bool(interleaved), float(scale), bool(inverse))
     if out is not None:
-        if grad:
-            raise ValueError("out and gradients do not go together: detach q and k, or leave out")
         if len(out) != 2 or (out[1] is None) != (k is None):
             raise ValueError("out must hold the results' two tensors (None for no k)")
+        written = [o for o in out if o is not None]
+        if grad or torch.is_grad_enabled() and any(o.requires_grad for o in written) or _dual(*written):
+            raise ValueError("out and gradients do not go together: detach q, k and out, or leave out")
         for name, o, x in (("q", out[0], q), ("k", out[1], k)):
             if o is not None and (o.dtype != x.dtype or o.shape != x.shape or o.device != dev or o.stride(2) != 1
                                   or (o.shape[0] > 1 and o.stride(0) == 0) or (o.shape[1] > 1 and o.stride(1) == 0)):
                 raise ValueError(f"out for {name} must be {x.dtype} {tuple(x.shape)} on {dev} with its last dim contiguous "
                                  "and no row twice")
-    return _launch(q, k, positions, inv_freq, bool(interleaved), float(scale), bool(inverse), out)
+    result = _launch(q, k, positions, inv_freq, bool(interleaved), float(scale), bool(inverse), out)
+    if out is not None:
+        torch.autograd.graph.increment_version(written)  # what autograd saved of them is stale
+    return result
