@@ -499,6 +499,8 @@ class TreeStep:
             raise ValueError("no layers")
         if not len(q) == len(key) == len(value) == len(out) == len(caches):
             raise ValueError("q, key, value and out need one tensor per layer")
+        if any(not isinstance(c, PagedKVCache) for c in caches):
+            raise ValueError("a step of drafted tokens needs PagedKVCache layers")
         dev = self.device = caches[0].device
         if any(c.block_size != state.block_size or c.device != dev for c in caches):
             raise ValueError(f"the caches must have the state's blocks of {state.block_size} tokens, on {dev}")
