@@ -460,10 +460,10 @@ def paged_tree_gqa(
             or out.device != dev:
         raise ValueError(f"out must be a bfloat16 [T, Hq, D] tensor on {dev} with a contiguous last dim")
     sinks = _sinks(sinks, hq, dev)
-    if tokens == 0 or batch == 0:
+    if tokens == 0:
         return out
     if max_query_len is None:
-        max_query_len = int((cu_seqlens_q[1:] - cu_seqlens_q[:-1]).max().item())
+        max_query_len = int((cu_seqlens_q[1:] - cu_seqlens_q[:-1]).max().item()) if batch else 0
     msl = min(_max_len(seq_lens, max_seq_len), block_table.shape[1] * cache.block_size)
     lib = _lib.load()
     need = lib.wkv_tree_workspace_size(batch, KV_DTYPES[cache.kv_dtype], cache.num_kv_heads, hq, cache.head_dim,
