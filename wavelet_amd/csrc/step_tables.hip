@@ -20,9 +20,10 @@ struct TablesArgs {
   int width;
   const int32_t *held, *seq_lens, *new_lens, *free_blocks, *taken;
   int32_t num_free;
-  int B, BS, rows, limit;  // limit: cached and new tokens of a sequence
+  int B, BS, rows;
   const int32_t *parents;
   int words;
+  int limit;  // cached and new tokens of a sequence
   int32_t *held_out, *taken_out, *context, *cu, *refused;
   int64_t *slots, *positions, *masks;
 };
@@ -294,7 +295,7 @@ extern "C" int wkv_extend_tables_limited(int32_t *block_table, int64_t bt_stride
   WKV_CHECK_ARG(context_lens != seq_lens && context_lens != new_lens && context_lens != held_blocks,
                 "context_lens must not be one of the inputs");
   const TablesArgs a{block_table, bt_stride, max_blocks_per_seq, held_blocks, seq_lens, new_lens, free_blocks, taken,
-                     num_free, batch, block_size, max_tokens, max_seq_len, parents, mask_words, held_out, taken_out,
+                     num_free, batch, block_size, max_tokens, parents, mask_words, max_seq_len, held_out, taken_out,
                      context_lens, cu_seqlens_q, refused, slot_mapping, positions, tree_mask};
   auto s = static_cast<hipStream_t>(stream);
   if (max_tokens <= kTablesOwnRows) {
