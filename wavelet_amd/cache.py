@@ -251,7 +251,8 @@ class PagedKVCache:
 
         ``seq_lens`` int32 ``[B]`` are the lengths before the step; ``path [B, P]`` int32 (``P`` up to 64) and
         ``accepted [B]`` int32 come from ``accept_tree``: a rising path, ``path[b, j] >= j``. Tokens that keep
-        their place are not touched; fp8 caches encode the others again as ``append`` does. The written
+        their place are not touched; fp8 caches encode the others again as ``append`` does (each is then rounded
+        twice, and a block keeps the scale that a rejected token gave it until it is begun afresh). The written
         blocks must be the sequence's own (``BlockManager`` copies shared ones before a step writes them).
         """
         block_table, seq_lens = check_tables(block_table, seq_lens, self.device, self.block_size)

@@ -11,8 +11,13 @@
 // new block's tokens as one run, with the append kernel's own run (one wave a
 // run): the block's earlier codes are encoded again where its scale grows.
 // Bound by two round trips to memory and the launch: the bytes of a step (64
-// sequences x 8 tokens x 8 heads) are 4 MB. That step in bf16 5.5 us; 33 sequences x up
-// to 12 tokens x 4 heads in fp8 10.8 us, half of it the runs of the append rule.
+// sequences x 8 tokens x 8 heads) are 4 MB. That step in bf16 5.2 us; 33 sequences x up
+// to 12 tokens x 4 heads in fp8 10.0 us, half of it the runs of the append rule: a run is one wave's
+// chain of loads, maximum, scale and codes, and a path that fits one block is one run.
+//
+// fp8 costs accuracy that a bf16 cache does not: a moved token has been rounded twice (to
+// half a step of e4m3, 2^-4 of it, each time), and a block keeps the scale of the largest token that was
+// drafted into it, rejected ones too, until it is begun afresh -- as the append rule has it.
 #include "kv_append_dev.h"
 
 namespace wkv {
