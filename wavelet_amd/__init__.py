@@ -20,8 +20,8 @@ Public surface (a drop-in for the KV path of the reference's inference engine):
   and around it: ``extend_tables`` (a step's blocks, slots, positions and tree
   masks on the GPU), ``accept_tree`` (the path that the sampled tokens
   agree with) and ``PagedKVCache.compact`` (its keys and values moved together);
-  ``KVPool.lend`` / ``settle`` -- the blocks and lengths of such steps, lent to
-  the device and taken back (``StepState``);
+  ``KVPool.lend`` / ``settle`` / ``cancel`` -- the blocks and lengths of such steps,
+  lent to the device and taken back (``StepState``);
 * ``apply_rotary`` / ``rotary_frequencies`` -- rotary positions of queries and
   keys, with gradients;
 * ``sample`` -- the token sampler after decode (temperature, min_p, top_k,

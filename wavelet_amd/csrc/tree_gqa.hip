@@ -21,10 +21,11 @@
 // (products, exponents, the copies' issue, a barrier) past that and in fp8. Measured, 32 query and
 // 8 KV heads of 128, with the drafted tokens' append: 64 sequences of 4,096 tokens with 16 drafted
 // each, bf16, 184 us (6.0 TB/s; a chunk of each sequence per workgroup, with cached reads: 206); 6 of
-// 3,000 to 24,000 with 5 to 63 drafted, 28 and 4 heads, fp8, 65 to 69 us (400 TFLOP/s;
-// chunks: 172); 64 of 4,096 with 8 drafted, fp8, 116 us (4.7 TB/s; with one wave per unit
-// 137); 4 of 8,192 with 128 drafted 112 us in bf16 and 105 in fp8 (620 and 660 TFLOP/s; the matrix
-// unit is busy 41% of the time, the VALU 38%; chunks: 111 and 108).
+// 3,000 to 24,000 with 5 to 63 drafted, 28 and 4 heads, fp8, 67 to 72 us (400 TFLOP/s;
+// chunks: 172); 64 of 4,096 with 8 drafted, fp8, 120 us (4.5 TB/s; with one wave per unit
+// 137); 4 of 8,192 with 128 drafted 111 to 115 us in bf16 and 106 to 112 in fp8 (610 and 640 TFLOP/s; the
+// matrix unit is busy 41% of the time, the VALU 38%). Chunks took 111 and 108 there: even shares
+// gain nothing where the sequences are alike and wide.
 //
 // Software pipeline, one barrier per step: while a wave finishes step s
 // (probabilities, PV products) it scores step s + 1, so that the matrix unit
@@ -32,6 +33,12 @@
 // step s and K of step s + 1 have landed; their slots before (two each) take V of
 // step s + 1 and K of step s + 2. fp8 tiles land as codes in their bf16 tile's place and
 // are widened there, at their block's scale (exact), by the wave that copied them.
+//
+// Rounding: scores, exponents, maxima, sums, outputs in progress and partials are fp32. Probabilities
+// are rounded to bf16 for the PV product, as the prompt kernel has them (the bf16 MFMA is the fast one;
+// the sum is of the rounded ones, so that a row of equal values keeps them): each is off
+// by at most 2^-9 of itself, independently, which is an error the size of the bf16 output's own
+// rounding -- together sqrt(2) of it, 2.3e-3 of the result's norm against 1.7e-3 with fp32 probabilities.
 //
 // Masked keys: scores are set to -inf after scaling (a step's window of the row's
 // mask, 64 bits), so that neither the scale's sign nor a NaN key matters. A masked
@@ -164,9 +171,15 @@ __device__ __forceinline__ int tree_workgroups(int T) {
 // own instead of even shares. Those cost the partials that cutting leaves and the merge reads,
 // another start, and the meeting of row groups of the same keys in the L2; whole groups
 // wait for the longest. By microseconds of a step alone on its CU, of one of two, and of a
-// partial. 32 and 8 heads of 128, bf16, whole / shared: 64 sequences of 700 to 1,000 tokens
-// with 16 drafted 71 / 99, 128 of 100 to 1,000 with 8 to 32 105 / 130, 64 of 4,000 to 8,000 with
-// 32 to 64 523 / 623, of 100 to 8,000 with 16 to 48 394 / 305 us.
+// partial. Whole / shared, us (the one taken first):
+//   32 and 8 heads of 128, bf16: 64 sequences of 700 to 1,000 tokens with 16 drafted 71 / 99, 128 of
+//   100 to 1,000 with 8 to 32 105 / 130, 64 of 4,000 to 8,000 with 32 to 64 523 / 623; shared: 64
+//   of 100 to 8,000 with 16 to 48 305 / 394;
+//   the same heads, fp8: 64 of 700 to 1,000 43 / 69, 128 of 800 to 1,000 with 8 to 32 95 / 119; shared:
+//   64 of 4,000 to 8,000 with 32 to 64 521 / 556, of 100 to 8,000 with 16 to 48 249 / 349;
+//   14 and 2 heads of 64, bf16: 64 of 700 to 1,000 36 / 39, 128 of 1,000 to 1,400 with 8 to 32 50 / 56;
+//   shared: 64 of 4,000 to 8,000 with 32 to 64 138 / 169, of 100 to 8,000 with 16 to 48 91 / 155 (fp8:
+//   144 / 199 and 88 / 181).
 template <int D, bool FP8>
 __device__ __forceinline__ bool tree_whole(int T, int N, int longest, int items, int W) {
   constexpr float kAlone = 1.3f, kPair = 2.6f, kCut = D == 128 ? 60.f : 40.f, kPart = 0.026f * D / 128;
@@ -1013,8 +1026,10 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
 }
 
 // The workgroups that share a launch; 0: one per row group. Contexts of at most twelve steps are
-// not cut (one sequence of 600 tokens, with the merge's launch: 20.3 us whole, 23.5 cut; of
-// 900 tokens 26.2 and 23.5), and a line of 2^31 steps is not formed.
+// not cut, and a line of 2^31 steps is not formed. Whole / cut, with the merge's launch, us, at 500, 800 and
+// 1,200 tokens, 32 and 8 heads of 128: one sequence with 8 drafted 20 / 25, 23 / 25, 29 / 25 (fp8
+// 18 / 18, 24 / 22, 32 / 23), with 128 29 / 30, 36 / 32, 45 / 35; eight with 16 22 / 30, 26 / 31, 33 / 35; 14
+// and 2 heads of 64, one with 8: 21 / 25, 20 / 25, 23 / 25.
 static int tree_sharing(int batch, int Hkv, int G, int max_query_len, int max_seq) {
   const int64_t steps = (static_cast<int64_t>(max_seq) + 63) / 64;
   const int64_t groups = (static_cast<int64_t>(max_query_len) * G + kTreeRows - 1) / kTreeRows;

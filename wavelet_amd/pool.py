@@ -25,8 +25,9 @@ from .step import StepState
 
 
 # Device memory a pool sized from the engine's knobs leaves unclaimed beyond
-# ``non_kv_bytes``: the decode split-K workspace, sampler outputs and the
-# allocator's rounding.
+# ``non_kv_bytes``: the decode split-K workspace, a tree step's partials (68 MB at
+# head_dim 128, 35 at 64, per call in flight), sampler outputs and the allocator's
+# rounding.
 DEFAULT_RESERVE_BYTES = 512 << 20
 
 
