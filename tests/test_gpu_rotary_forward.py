@@ -70,3 +70,16 @@ def test_out_takes_no_tangents(cuda):
         with pytest.raises(ValueError, match="out and gradients"):
             apply_rotary(fwd.make_dual(q, tq), k, pos, freq, out=(q, k))
     assert torch.equal(q, before)
+
+
+def test_gradient_of_a_tangent(cuda):
+    """Reverse over forward: q = w x along v has the tangent R (w v), whose product with c has the gradient
+    v R^T c in w. float32: a few roundings of values below 2^6."""
+    x, _, v, _, pos, freq = _case(cuda)
+    w, c = torch.randn_like(x).requires_grad_(), torch.randn_like(x)
+    for k in (None, torch.randn_like(x)):
+        with fwd.dual_level():
+            y, _ = apply_rotary(w * fwd.make_dual(x, v), k, pos, freq)
+            (g,) = torch.autograd.grad((fwd.unpack_dual(y).tangent * c).sum(), w)
+        want = v * apply_rotary(c, None, pos, freq, inverse=True)[0]
+        torch.testing.assert_close(g, want, rtol=0, atol=2.0 ** 6 * 2.0 ** -21)

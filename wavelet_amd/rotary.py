@@ -159,9 +159,8 @@ class _Rotary(torch.autograd.Function):
         lone = gk if gq is None else None  # k's alone
         if gq is not None or gk is not None:
             interleaved, scale, inverse = ctx.how
-            turn = _Rotary.apply if torch.is_grad_enabled() or _dual(gq, gk) else _launch_back
-            gq, gk = turn(gq if lone is None else lone, gk if lone is None else None, *ctx.saved_tensors, interleaved,
-                          scale, not inverse)
+            gq, gk = _turned(gq if lone is None else lone, gk if lone is None else None, *ctx.saved_tensors, interleaved,
+                             scale, not inverse)
         if lone is not None:
             gq, gk = None, gq
         return gq, gk, None, None, None, None, None
@@ -173,11 +172,16 @@ class _Rotary(torch.autograd.Function):
             tq = some.new_zeros((some.shape[0], ctx.heads[0], some.shape[2]))
         if tk is None and k_heads is not None:
             tk = some.new_zeros((some.shape[0], k_heads, some.shape[2]))
-        return _launch(tq, tk, *ctx.saved_tensors, *ctx.how, None)
+        return _turned(tq, tk, *ctx.saved_tensors, *ctx.how)
 
 
-def _launch_back(*args):
-    return _launch(*args, None)
+def _differentiable(q, k) -> bool:
+    """Whether autograd has to know of their rotation."""
+    return torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) or _dual(q, k)
+
+
+def _turned(q, k, *how):
+    return _Rotary.apply(q, k, *how) if _differentiable(q, k) else _launch(q, k, *how, None)
 
 
 def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, *,
@@ -211,21 +215,19 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not 0 < 2 * inv_freq.shape[0] <= d:
         raise ValueError(f"inv_freq must be float64 [R / 2] with R <= {d} (got {inv_freq.dtype} {tuple(inv_freq.shape)})")
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
-    grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) or _dual(q, k)
-    if out is None and grad:
-        return _Rotary.apply(q, k, positions, inv_freq, bool(interleaved), float(scale), bool(inverse))
-    if out is not None:
-        if len(out) != 2 or (out[1] is None) != (k is None):
-            raise ValueError("out must hold the results' two tensors (None for no k)")
-        written = [o for o in out if o is not None]
-        if grad or torch.is_grad_enabled() and any(o.requires_grad for o in written) or _dual(*written):
-            raise ValueError("out and gradients do not go together: detach q, k and out, or leave out")
-        for name, o, x in (("q", out[0], q), ("k", out[1], k)):
-            if o is not None and (o.dtype != x.dtype or o.shape != x.shape or o.device != dev or o.stride(2) != 1
-                                  or (o.shape[0] > 1 and o.stride(0) == 0) or (o.shape[1] > 1 and o.stride(1) == 0)):
-                raise ValueError(f"out for {name} must be {x.dtype} {tuple(x.shape)} on {dev} with its last dim contiguous "
-                                 "and no row twice")
-    result = _launch(q, k, positions, inv_freq, bool(interleaved), float(scale), bool(inverse), out)
-    if out is not None:
-        torch.autograd.graph.increment_version(written)  # what autograd saved of them is stale
+    how = (positions, inv_freq, bool(interleaved), float(scale), bool(inverse))
+    if out is None:
+        return _turned(q, k, *how)
+    if len(out) != 2 or (out[1] is None) != (k is None):
+        raise ValueError("out must hold the results' two tensors (None for no k)")
+    written = [o for o in out if o is not None]
+    if _differentiable(q, k) or torch.is_grad_enabled() and any(o.requires_grad for o in written) or _dual(*written):
+        raise ValueError("out and gradients do not go together: detach q, k and out, or leave out")
+    for name, o, x in (("q", out[0], q), ("k", out[1], k)):
+        if o is not None and (o.dtype != x.dtype or o.shape != x.shape or o.device != dev or o.stride(2) != 1
+                              or (o.shape[0] > 1 and o.stride(0) == 0) or (o.shape[1] > 1 and o.stride(1) == 0)):
+            raise ValueError(f"out for {name} must be {x.dtype} {tuple(x.shape)} on {dev} with its last dim contiguous "
+                             "and no row twice")
+    result = _launch(q, k, *how, out)
+    torch.autograd.graph.increment_version(written)  # what autograd saved of them is stale
     return result
