@@ -518,8 +518,8 @@ int wkv_accept_tree(const int64_t *draft_tokens, const int32_t *parents, const i
                     int64_t *next_tokens, int32_t *seq_lens_out, void *stream);
 
 /* The same, and pending [B] (NULL = none), the token that each sequence goes on
- * with: next_tokens[b] where the sequence accepted anything, else left as it is (a
- * sequence that a step refuses or leaves out keeps the token sampled before). */
+ * with: next_tokens[b] where the sequence accepted anything, else left as it is (so
+ * not next_tokens itself; a sequence that a step refuses or leaves out keeps the token sampled before). */
 int wkv_accept_tree_pending(const int64_t *draft_tokens, const int32_t *parents, const int64_t *target_tokens,
                             int64_t num_tokens, const int32_t *cu_seqlens_q, const int32_t *seq_lens,
                             const int32_t *context_lens, int32_t batch, int32_t max_depth, int32_t *accepted,

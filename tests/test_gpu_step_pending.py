@@ -109,3 +109,11 @@ def test_refused_and_paused_sequences_go_on(cuda, captured):
         assert texts[b] == model.text(first[b], len(texts[b]))
         assert state.next_tokens[b] == model.text(first[b], len(texts[b]) + 1)[-1]
         assert int(state.seq_lens[b]) == (14, 30, 31)[b] + len(texts[b])
+
+
+def test_pending_is_no_other_result(cuda):
+    z, i = torch.zeros(3, dtype=torch.int64, device=cuda), torch.zeros(2, dtype=torch.int32, device=cuda)
+    cu = torch.tensor([0, 1, 3], dtype=torch.int32, device=cuda)
+    got = accept_tree(z, z.int() - 1, z, cu, i, i, 4)
+    with pytest.raises(ValueError, match="pending"):
+        accept_tree(z, z.int() - 1, z, cu, i, i, 4, pending=got.next_tokens, out=got)

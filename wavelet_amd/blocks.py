@@ -43,7 +43,7 @@ class Loan:
 
     seq_ids: list
     blocks: list[int]  # in the order in which they are to be taken
-    copies: list[tuple]  # (sequence, place in its table, shared block, its own in the place of it)
+    copies: list[tuple] = field(default_factory=list)  # (sequence, place in its table, shared block, its own there)
     settled: bool = False
 
 

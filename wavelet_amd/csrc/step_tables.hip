@@ -335,6 +335,7 @@ extern "C" int wkv_accept_tree_pending(const int64_t *draft_tokens, const int32_
   WKV_CHECK_ARG(((draft_tokens && parents && target_tokens) || num_tokens == 0) && cu_seqlens_q && seq_lens &&
                     context_lens && accepted && path && next_tokens && seq_lens_out,
                 "an input or output is NULL");
+  WKV_CHECK_ARG(pending != next_tokens, "pending must not be next_tokens");
   accept_tree_kernel<<<static_cast<unsigned>((batch + 3) / 4), 256, 0, static_cast<hipStream_t>(stream)>>>(
       draft_tokens, parents, target_tokens, static_cast<int>(num_tokens), cu_seqlens_q, seq_lens, context_lens, batch,
       max_depth, accepted, path, next_tokens, seq_lens_out, pending);

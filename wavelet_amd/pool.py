@@ -209,7 +209,8 @@ class KVPool:
             torch.cuda.synchronize(self.device)
 
     def cancel(self, state: StepState) -> None:
-        """Take a loan back without its steps (``BlockManager.cancel``): the sequences are as before it."""
+        """Take a loan back without its steps (``BlockManager.cancel``): the sequences' tables and lengths are as
+        before it, and what its steps wrote behind the lengths counts for nothing."""
         self._wait()
         self.blocks.cancel(state.loan)
 
