@@ -4,7 +4,6 @@ Tokens past the limit are attended by no row; the others, context and drafted, a
 table without blocks past the limit, a multiple of the block size here.
 """
 
-import numpy as np
 import pytest
 
 from kvcase import bits_of, check_attention

@@ -1,6 +1,5 @@
 """Rows of sequences that a step refused: zeros, however the attention is launched."""
 
-import numpy as np
 import pytest
 import torch
 
