@@ -475,6 +475,71 @@ int wkv_rotary(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_strid
                const int64_t *positions, const double *inv_freq, int32_t rotary_dim, int32_t interleaved,
                int32_t inverse, float scale, int64_t num_tokens, void *stream);
 
+/* A rotation of heads. The angle of pair i at token t is positions[a, t] * inv_freq[i],
+ * a = axes[i]: positions are num_axes rows axis_stride elements apart (time, height and
+ * width of images and video, say), axes (int32, device memory) gives every pair its
+ * own; NULL: all are axis 0's. A pair whose axis is not in [0, num_axes) is turned by 0. The
+ * other fields as for wkv_rotary. */
+typedef struct {
+  const int64_t *positions; /* [num_axes, num_tokens] */
+  int64_t axis_stride;
+  const int32_t *axes;      /* [rotary_dim / 2], or NULL */
+  const double *inv_freq;   /* [rotary_dim / 2] */
+  int32_t num_axes;
+  int32_t rotary_dim;
+  int32_t interleaved;
+  int32_t inverse;
+  float scale;
+  int32_t reserved;         /* 0 */
+} wkv_rotary_t;
+
+/* A norm of every head by its root mean square, with weights for queries and keys:
+ * n = x (mean(x^2) + eps)^-1/2 (w + weight_offset). weight_dtype 0 (fp32) or the heads' own.
+ * NULL weights are ones (without the offset). */
+typedef struct {
+  const void *q_weight;      /* [head_dim], or [heads, head_dim] */
+  const void *k_weight;
+  int64_t q_weight_stride_h; /* 0: one for all heads */
+  int64_t k_weight_stride_h;
+  int32_t weight_dtype;
+  float weight_offset;
+  float eps;                 /* at least FLT_MIN */
+  int32_t reserved;          /* 0 */
+} wkv_head_norm_t;
+
+/* wkv_rotary with the rotation's axes. */
+int wkv_rotary_axes(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_stride_h, void *q_out,
+                    int64_t qo_stride_t, int64_t qo_stride_h, int32_t num_q_heads, const void *k, int64_t k_stride_t,
+                    int64_t k_stride_h, void *k_out, int64_t ko_stride_t, int64_t ko_stride_h, int32_t num_k_heads,
+                    int32_t head_dim, const wkv_rotary_t *rotary, int64_t num_tokens, void *stream);
+
+/* Every head normed, then turned (rotary NULL: only normed), in one pass. q, k and their outputs as for
+ * wkv_rotary. Computed in float32 and rounded once; a head whose squares
+ * pass float32's range comes out as zeros. Replaces the engine's norms of queries and keys and its
+ * rotary embedding (inside llm.generate, engine.py:887). */
+int wkv_norm_rotary(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_stride_h, void *q_out,
+                    int64_t qo_stride_t, int64_t qo_stride_h, int32_t num_q_heads, const void *k, int64_t k_stride_t,
+                    int64_t k_stride_h, void *k_out, int64_t ko_stride_t, int64_t ko_stride_h, int32_t num_k_heads,
+                    int32_t head_dim, const wkv_head_norm_t *norm, const wkv_rotary_t *rotary, int64_t num_tokens,
+                    void *stream);
+
+/* Its gradients: from the inputs q, k, and the gradients q_grad, k_grad of the
+ * outputs, dq and dk (NULL: not computed; else they do not overlap the inputs) and the weights' dq_weight, dk_weight (NULL: not
+ * computed; contiguous, [head_dim], or [heads, head_dim] where the weight has a head stride, of weight_dtype).
+ * A kind of heads without a gradient is given as 0 heads. Summed in float32, in an order that depends on the sizes alone.
+ * workspace: wkv_norm_rotary_workspace_size() bytes, 16-byte aligned, for a weight's gradient (else it may be NULL);
+ * rotary_dim 0 without a rotation; weight_each_head: that weight's gradient is asked for and is [heads, head_dim]. */
+int64_t wkv_norm_rotary_workspace_size(int64_t num_tokens, int32_t num_q_heads, int32_t num_k_heads, int32_t head_dim,
+                                       int32_t rotary_dim, int32_t q_weight_each_head, int32_t k_weight_each_head);
+
+int wkv_norm_rotary_backward(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *q_grad,
+                             int64_t qg_stride_t, int64_t qg_stride_h, void *dq, int64_t dq_stride_t,
+                             int64_t dq_stride_h, int32_t num_q_heads, const void *k, int64_t k_stride_t,
+                             int64_t k_stride_h, const void *k_grad, int64_t kg_stride_t, int64_t kg_stride_h,
+                             void *dk, int64_t dk_stride_t, int64_t dk_stride_h, int32_t num_k_heads, int32_t head_dim,
+                             const wkv_head_norm_t *norm, const wkv_rotary_t *rotary, void *dq_weight, void *dk_weight,
+                             int64_t num_tokens, void *workspace, int64_t workspace_bytes, void *stream);
+
 /* Attention of drafted tokens over the paged cache: wkv_prefill_gqa with a mask
  * in the place of the causal one. Row j of sequence b's n_b = cu_seqlens_q[b+1] -
  * cu_seqlens_q[b] new tokens attends to the seq_lens[b] - n_b cached tokens

@@ -23,7 +23,10 @@ Public surface (a drop-in for the KV path of the reference's inference engine):
   ``KVPool.lend`` / ``settle`` / ``cancel`` -- the blocks and lengths of such steps,
   lent to the device and taken back (``StepState``);
 * ``apply_rotary`` / ``rotary_frequencies`` -- rotary positions of queries and
-  keys, with gradients;
+  keys, with gradients; ``rotary_axes`` -- the pairs of a head dealt out to
+  positions of several axes;
+* ``norm_rotary`` -- every query and key head normed, and turned in the same
+  pass, with gradients;
 * ``sample`` -- the token sampler after decode (temperature, min_p, top_k,
   top_p, repetition penalty; processed logprobs and the sampling mask).
 
@@ -38,8 +41,9 @@ from .attention import (decode_order, decode_plan, grouped_decode_order, paged_d
                         paged_decode_mla, paged_tree_gqa, prefill_gqa)
 from .blocks import BlockManager
 from .cache import MLALatentCache, PagedKVCache, validate_group_prefix, validate_tables
+from .norm_rotary import norm_rotary
 from .pool import KVPool
-from .rotary import apply_rotary, rotary_frequencies
+from .rotary import apply_rotary, rotary_axes, rotary_frequencies
 from .sampler import sample
 from .step import Accepted, StepMaps, StepState, accept_tree, extend_tables
 
@@ -57,11 +61,13 @@ __all__ = [
     "grouped_decode_order",
     "decode_plan",
     "extend_tables",
+    "norm_rotary",
     "paged_decode_gqa",
     "paged_decode_gqa_grouped",
     "paged_decode_mla",
     "paged_tree_gqa",
     "prefill_gqa",
+    "rotary_axes",
     "rotary_frequencies",
     "sample",
     "validate_group_prefix",

@@ -51,6 +51,34 @@ class WkvMlaCache(ctypes.Structure):
     ]
 
 
+class WkvRotary(ctypes.Structure):
+    _fields_ = [
+        ("positions", c_void_p),
+        ("axis_stride", c_int64),
+        ("axes", c_void_p),
+        ("inv_freq", c_void_p),
+        ("num_axes", c_int32),
+        ("rotary_dim", c_int32),
+        ("interleaved", c_int32),
+        ("inverse", c_int32),
+        ("scale", c_float),
+        ("reserved", c_int32),
+    ]
+
+
+class WkvHeadNorm(ctypes.Structure):
+    _fields_ = [
+        ("q_weight", c_void_p),
+        ("k_weight", c_void_p),
+        ("q_weight_stride_h", c_int64),
+        ("k_weight_stride_h", c_int64),
+        ("weight_dtype", c_int32),
+        ("weight_offset", c_float),
+        ("eps", c_float),
+        ("reserved", c_int32),
+    ]
+
+
 _I64P = POINTER(c_int64)
 _SIGNATURES = {
     "wkv_append": (c_int, [POINTER(WkvCache), c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
@@ -91,6 +119,17 @@ _SIGNATURES = {
     "wkv_rotary": (c_int, [c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_void_p, c_int64,
                            c_int64, c_void_p, c_int64, c_int64, c_int32, c_int32, c_void_p, c_void_p, c_int32, c_int32,
                            c_int32, c_float, c_int64, c_void_p]),
+    "wkv_rotary_axes": (c_int, [c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_void_p,
+                                c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_int32, POINTER(WkvRotary),
+                                c_int64, c_void_p]),
+    "wkv_norm_rotary": (c_int, [c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_void_p,
+                                c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_int32, POINTER(WkvHeadNorm),
+                                POINTER(WkvRotary), c_int64, c_void_p]),
+    "wkv_norm_rotary_workspace_size": (c_int64, [c_int64, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
+    "wkv_norm_rotary_backward": (c_int, [c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
+                                         c_int64, c_int64, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64,
+                                         c_int64, c_void_p, c_int64, c_int64, c_int32, c_int32, POINTER(WkvHeadNorm),
+                                         POINTER(WkvRotary), c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
     "wkv_tree_workspace_size": (c_int64, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
     "wkv_tree_gqa": (c_int, [POINTER(WkvCache), c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
                              c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_void_p,

@@ -34,6 +34,9 @@ struct RotaryRows {
 struct RotaryArgs {
   RotaryRows q, k;
   const int64_t *pos;
+  int64_t axis_stride;  // between the axes' positions
+  const int32_t *axes;  // of every pair (nullptr: all of axis 0)
+  int num_axes;
   const double *inv_freq;
   int64_t tokens;
   int Hq, H;      // query heads; query and key heads
@@ -64,8 +67,12 @@ __global__ __launch_bounds__(64 * kRotaryWaves) void rotary_kernel(RotaryArgs a)
   if (t >= a.tokens) return;  // a whole wave; nothing below waits for another
   const int h0 = blockIdx.y * a.per;
   const int heads = a.H - h0 < a.per ? a.H - h0 : a.per;
-  const double p = static_cast<double>(a.pos[t]);
+  double p = a.axes == nullptr ? static_cast<double>(a.pos[t]) : 0.;
   for (int i = lane; i < a.half; i += 64) {
+    if (a.axes != nullptr) {  // uniform
+      const int ax = a.axes[i];
+      p = static_cast<unsigned>(ax) < static_cast<unsigned>(a.num_axes) ? static_cast<double>(a.pos[ax * a.axis_stride + t]) : 0.;
+    }
     const double x = p * a.inv_freq[i] * 0.15915494309189533577;  // 1 / 2 pi: the angle in turns
     float s, c;
     sincospif(2.f * static_cast<float>(x - rint(x)), &s, &c);
@@ -179,12 +186,15 @@ static void launch_rotary(const RotaryArgs &a, int v, bool far, dim3 grid, hipSt
 
 using namespace wkv;
 
-extern "C" int wkv_rotary(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_stride_h, void *q_out,
-                          int64_t qo_stride_t, int64_t qo_stride_h, int32_t num_q_heads, const void *k,
-                          int64_t k_stride_t, int64_t k_stride_h, void *k_out, int64_t ko_stride_t,
-                          int64_t ko_stride_h, int32_t num_k_heads, int32_t head_dim, const int64_t *positions,
-                          const double *inv_freq, int32_t rotary_dim, int32_t interleaved, int32_t inverse, float scale,
-                          int64_t num_tokens, void *stream) {
+static int rotary_call(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_stride_h, void *q_out,
+                       int64_t qo_stride_t, int64_t qo_stride_h, int32_t num_q_heads, const void *k,
+                       int64_t k_stride_t, int64_t k_stride_h, void *k_out, int64_t ko_stride_t, int64_t ko_stride_h,
+                       int32_t num_k_heads, int32_t head_dim, const wkv_rotary_t &rotary, int64_t num_tokens,
+                       void *stream) {
+  const int64_t *positions = rotary.positions;
+  const double *inv_freq = rotary.inv_freq;
+  const int32_t rotary_dim = rotary.rotary_dim;
+  const float scale = rotary.scale;
   WKV_CHECK_ARG(dtype >= 0 && dtype <= 2, "dtype must be 0 (fp32), 1 (bf16) or 2 (fp16) (got %d)", dtype);
   WKV_CHECK_ARG(num_tokens >= 0 && num_tokens <= INT32_MAX, "num_tokens must be in [0, 2^31) (got %lld)",
                 (long long)num_tokens);
@@ -214,6 +224,9 @@ extern "C" int wkv_rotary(int32_t dtype, const void *q, int64_t q_stride_t, int6
   a.q = RotaryRows{q, q_out, q_stride_t, q_stride_h, qo_stride_t, qo_stride_h};
   a.k = RotaryRows{k, k_out, k_stride_t, k_stride_h, ko_stride_t, ko_stride_h};
   a.pos = positions;
+  a.axis_stride = rotary.axis_stride;
+  a.axes = rotary.axes;
+  a.num_axes = rotary.num_axes;
   a.inv_freq = inv_freq;
   a.tokens = num_tokens;
   a.Hq = num_q_heads;
@@ -221,8 +234,8 @@ extern "C" int wkv_rotary(int32_t dtype, const void *q, int64_t q_stride_t, int6
   a.D = head_dim;
   a.half = rotary_dim / 2;
   a.scale = scale;
-  a.sign = inverse ? -1.f : 1.f;
-  const bool inter = interleaved != 0;
+  a.sign = rotary.inverse ? -1.f : 1.f;
+  const bool inter = rotary.interleaved != 0;
   const RotaryRows rows[2] = {num_q_heads ? a.q : a.k, num_k_heads ? a.k : a.q};
   const int v = rotary_width(esz, head_dim, a.half, inter, rows, 2);
   a.turned = a.half / v;
@@ -252,4 +265,28 @@ extern "C" int wkv_rotary(int32_t dtype, const void *q, int64_t q_stride_t, int6
   }
   WKV_CHECK_LAUNCH("rotary");
   return WKV_OK;
+}
+
+extern "C" int wkv_rotary(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_stride_h, void *q_out,
+                          int64_t qo_stride_t, int64_t qo_stride_h, int32_t num_q_heads, const void *k,
+                          int64_t k_stride_t, int64_t k_stride_h, void *k_out, int64_t ko_stride_t,
+                          int64_t ko_stride_h, int32_t num_k_heads, int32_t head_dim, const int64_t *positions,
+                          const double *inv_freq, int32_t rotary_dim, int32_t interleaved, int32_t inverse, float scale,
+                          int64_t num_tokens, void *stream) {
+  const wkv_rotary_t rotary{positions, 0, nullptr, inv_freq, 1, rotary_dim, interleaved, inverse, scale, 0};
+  return rotary_call(dtype, q, q_stride_t, q_stride_h, q_out, qo_stride_t, qo_stride_h, num_q_heads, k, k_stride_t,
+                     k_stride_h, k_out, ko_stride_t, ko_stride_h, num_k_heads, head_dim, rotary, num_tokens, stream);
+}
+
+extern "C" int wkv_rotary_axes(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_stride_h, void *q_out,
+                               int64_t qo_stride_t, int64_t qo_stride_h, int32_t num_q_heads, const void *k,
+                               int64_t k_stride_t, int64_t k_stride_h, void *k_out, int64_t ko_stride_t,
+                               int64_t ko_stride_h, int32_t num_k_heads, int32_t head_dim, const wkv_rotary_t *rotary,
+                               int64_t num_tokens, void *stream) {
+  WKV_CHECK_ARG(rotary != nullptr, "rotary must be given");
+  WKV_CHECK_ARG(rotary->num_axes >= 1 && rotary->axis_stride >= 0 && reinterpret_cast<uintptr_t>(rotary->axes) % 4 == 0,
+                "num_axes must be positive, axis_stride non-negative, axes int32");
+  WKV_CHECK_ARG(rotary->reserved == 0, "rotary descriptor field `reserved` must be 0 (got %d)", rotary->reserved);
+  return rotary_call(dtype, q, q_stride_t, q_stride_h, q_out, qo_stride_t, qo_stride_h, num_q_heads, k, k_stride_t,
+                     k_stride_h, k_out, ko_stride_t, ko_stride_h, num_k_heads, head_dim, *rotary, num_tokens, stream);
 }

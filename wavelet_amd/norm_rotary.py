@@ -1,0 +1,182 @@
+"""Norms of queries and keys for each head, with the rotary positions in the same pass.
+
+Models that norm their heads (a root mean square over each, with weights for queries and keys) do so between
+the projections and the rotary embedding of every layer; the engine runs both inside ``llm.generate``
+(wavelet/inference/engine.py:887). ``norm_rotary`` reads a head once for the two, in prompts, single tokens
+and under autograd for training, with the weights' gradients.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .cache import _on, _stream
+from .rotary import _DTYPES, _dual, check_rotation, rotation
+
+
+def check_weight(w, name: str, heads: int, x: torch.Tensor):
+    """A head norm's weight (None: ones) for ``heads`` heads of ``x``'s type and size, its last dim contiguous."""
+    if w is None:
+        return None
+    d = x.shape[-1]
+    if not isinstance(w, torch.Tensor) or w.device != x.device or w.dtype not in (torch.float32, x.dtype):
+        raise ValueError(f"{name} must be a float32 or {x.dtype} tensor on {x.device}")
+    if tuple(w.shape) not in ((d,), (heads, d)):
+        raise ValueError(f"{name} must be [{d}] or [{heads}, {d}] (got {list(w.shape)})")
+    return w if w.stride(-1) == 1 else w.contiguous()
+
+
+def _same_type(q_weight, k_weight):
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise ValueError(f"q_weight and k_weight must have one type (got {q_weight.dtype} and {k_weight.dtype})")
+
+
+def head_norm(q_weight, k_weight, eps: float, offset: float) -> _lib.WkvHeadNorm:
+    """The library's description of a norm (wkv_head_norm_t) from checked weights, which have to outlive it."""
+    def of(w):
+        return (None, 0) if w is None else (w.data_ptr(), w.stride(0) if w.dim() == 2 else 0)
+
+    some = k_weight if q_weight is None else q_weight
+    (qw, qs), (kw, ks) = of(q_weight), of(k_weight)
+    return _lib.WkvHeadNorm(q_weight=qw, k_weight=kw, q_weight_stride_h=qs, k_weight_stride_h=ks,
+                            weight_dtype=0 if some is None else _DTYPES[some.dtype], weight_offset=offset, eps=eps,
+                            reserved=0)
+
+
+def _rows(x: torch.Tensor | None, *others):
+    """Pointers and strides of a kind of heads: of x and of what goes with it (None: not there)."""
+    out = []
+    for t in (x, *others):
+        out += (None, 0, 0) if t is None else (t.data_ptr(), *t.stride()[:2])
+    return (*out, 0 if x is None else x.shape[1])
+
+
+def _packed(x):
+    return x if x is None or x.stride(-1) == 1 else x.contiguous()
+
+
+def _forward(q, k, q_weight, k_weight, rotary, interleaved, scale, eps, offset, out):
+    """One launch over checked tensors; rotary: (positions, inv_freq, axes), or None: only normed."""
+    qi, ki = _packed(q), _packed(k)
+    if out is None:
+        out = tuple(x if x is None else torch.empty_like(x, memory_format=torch.contiguous_format) for x in (qi, ki))
+    dev = q.device
+    norm = head_norm(q_weight, k_weight, eps, offset)
+    how = None if rotary is None else ctypes.byref(rotation(*rotary, interleaved, scale))
+    with _on(dev):
+        rc = _lib.load().wkv_norm_rotary(_DTYPES[q.dtype], *_rows(qi, out[0]), *_rows(ki, out[1]), q.shape[2],
+                                         ctypes.byref(norm), how, q.shape[0], _stream(dev))
+    _lib.check(rc, "norm_rotary")
+    return out
+
+
+def _backward(q, k, gq, gk, q_weight, k_weight, rotary, interleaved, scale, eps, offset, need):
+    """The gradients (dq, dk, dq_weight, dk_weight) that ``need`` asks for; gq or gk None: zero."""
+    if gq is None:
+        q = None
+    if gk is None:
+        k = None
+    some = k if q is None else q
+    dev, (tokens, _, d) = some.device, some.shape
+    q, k, gq, gk = (_packed(x) for x in (q, k, gq, gk))
+    dq, dk = (torch.empty_like(x, memory_format=torch.contiguous_format) if x is not None and n else None
+              for x, n in zip((q, k), need))
+    wants = [w if x is not None and n else None for x, w, n in zip((q, k), (q_weight, k_weight), need[2:])]
+    dqw, dkw = (w if w is None else torch.empty_like(w, memory_format=torch.contiguous_format) if x.shape[1]
+                else torch.zeros_like(w) for x, w in zip((q, k), wants))
+    wants = [w if w is not None and x.shape[1] else None for x, w in zip((q, k), wants)]  # (no head, no sum)
+    each = [int(w is not None and w.dim() == 2) for w in wants]
+    norm = head_norm(q_weight, k_weight, eps, offset)
+    how = None if rotary is None else ctypes.byref(rotation(*rotary, interleaved, scale))
+    lib = _lib.load()
+    ws, need_bytes = None, 0
+    if any(w is not None for w in wants):
+        need_bytes = lib.wkv_norm_rotary_workspace_size(tokens, 0 if q is None else q.shape[1],
+                                                        0 if k is None else k.shape[1], d,
+                                                        0 if rotary is None else 2 * rotary[1].shape[0], *each)
+        ws = torch.empty(need_bytes, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        rc = lib.wkv_norm_rotary_backward(
+            _DTYPES[some.dtype], *_rows(q, gq, dq), *_rows(k, gk, dk), d, ctypes.byref(norm), how,
+            *(None if w is None else dw.data_ptr() for w, dw in zip(wants, (dqw, dkw))), tokens,
+            None if ws is None else ws.data_ptr(), need_bytes, _stream(dev))
+    _lib.check(rc, "norm_rotary backward")
+    return dq, dk, dqw, dkw
+
+
+class _NormRotary(torch.autograd.Function):
+    """The inputs are kept, not the normed heads: the backward launch norms them again."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, rotary, interleaved, scale, eps, offset):
+        ctx.save_for_backward(q, k, q_weight, k_weight, *(rotary or ()))
+        ctx.how = (interleaved, scale, eps, offset)
+        ctx.set_materialize_grads(False)
+        return _forward(q, k, q_weight, k_weight, rotary, interleaved, scale, eps, offset, None)
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        if torch.is_grad_enabled():  # (create_graph: the launch's results would count as constants)
+            raise NotImplementedError("norm_rotary is differentiable once: its gradients have no create_graph")
+        q, k, q_weight, k_weight, *rotary = ctx.saved_tensors
+        need = ctx.needs_input_grad[:4]
+        gq, gk = (g if need[i] or need[i + 2] else None for i, g in enumerate((gq, gk)))
+        if gq is None and gk is None:
+            return (None,) * 9
+        grads = _backward(q, k, gq, gk, q_weight, k_weight, tuple(rotary) or None, *ctx.how, need)
+        return (*grads, None, None, None, None, None)
+
+
+def norm_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor | None = None,
+                inv_freq: torch.Tensor | None = None, *, q_weight: torch.Tensor | None = None,
+                k_weight: torch.Tensor | None = None, eps: float = 1e-6, weight_offset: float = 0.0,
+                axes: torch.Tensor | None = None, interleaved: bool = False, scale: float = 1.0,
+                out: tuple[torch.Tensor, torch.Tensor | None] | None = None):
+    """``q [T, Hq, D]`` and ``k [T, Hk, D]`` (or None) with every head normed and turned -> new tensors ``(q, k)``.
+
+    The norm: ``x / sqrt(mean(x ** 2) + eps) * (weight + weight_offset)`` over each head, weights ``[D]`` for all
+    heads or ``[H, D]``, of the heads' type or float32 (None: ones). The rotation: ``apply_rotary``'s, from
+    ``positions``, ``inv_freq``, ``axes``, ``interleaved`` and ``scale`` (``positions`` and ``inv_freq`` None: the heads
+    are only normed). bf16, fp16 or fp32, ``D`` even and at most 512, strided rows read in place; all of it is computed in float32
+    and rounded once. ``out``: the two results' tensors; ``out=(q, k)`` works in place, other tensors share no memory with
+    the inputs. Differentiable once, in ``q``, ``k`` and the weights (not with ``out``,
+    ``create_graph`` or forward mode).
+    """
+    if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype not in _DTYPES:
+        raise ValueError("q must be a bfloat16, float16 or float32 [T, Hq, D] tensor")
+    dev = q.device
+    if dev.type != "cuda":
+        raise ValueError(f"q is on {dev}: norm_rotary runs on the GPU")
+    tokens, hq, d = q.shape
+    if k is not None and (not isinstance(k, torch.Tensor) or k.dim() != 3 or k.dtype != q.dtype or k.device != dev
+                          or k.shape[0] != tokens or k.shape[2] != d):
+        raise ValueError(f"k must be {q.dtype} [{tokens}, Hk, {d}] on {dev}")
+    q_weight = check_weight(q_weight, "q_weight", hq, q)
+    if k is None and k_weight is not None:
+        raise ValueError("k_weight without k")
+    k_weight = check_weight(k_weight, "k_weight", 0 if k is None else k.shape[1], q)
+    _same_type(q_weight, k_weight)
+    if (positions is None) != (inv_freq is None) or (inv_freq is None and axes is not None):
+        raise ValueError("positions and inv_freq go together (both None: the heads are only normed)")
+    rotary = None if inv_freq is None else check_rotation(positions, inv_freq, axes, tokens, d, dev)
+    how = (rotary, bool(interleaved), float(scale), float(eps), float(weight_offset))
+    inputs = [x for x in (q, k, q_weight, k_weight) if x is not None]
+    differentiable = torch.is_grad_enabled() and any(x.requires_grad for x in inputs) or _dual(*inputs)
+    if out is None:
+        return (_NormRotary.apply if differentiable else lambda *a: _forward(*a, None))(q, k, q_weight, k_weight, *how)
+    if len(out) != 2 or (out[1] is None) != (k is None):
+        raise ValueError("out must hold the results' two tensors (None for no k)")
+    written = [o for o in out if o is not None]
+    if differentiable or torch.is_grad_enabled() and any(o.requires_grad for o in written) or _dual(*written):
+        raise ValueError("out and gradients do not go together: detach q, k, the weights and out, or leave out")
+    for name, o, x in (("q", out[0], q), ("k", out[1], k)):
+        if o is not None and (o.dtype != x.dtype or o.shape != x.shape or o.device != dev or o.stride(2) != 1
+                              or (o.shape[0] > 1 and o.stride(0) == 0) or (o.shape[1] > 1 and o.stride(1) == 0)):
+            raise ValueError(f"out for {name} must be {x.dtype} {tuple(x.shape)} on {dev} with its last dim contiguous "
+                             "and no row twice")
+    result = _forward(q, k, q_weight, k_weight, *how, tuple(out))
+    torch.autograd.graph.increment_version(written)  # what autograd saved of them is stale
+    return result

@@ -5,11 +5,13 @@ layer (inside ``llm.generate``, wavelet/inference/engine.py:887; the reference p
 wavelet/inference/deepseek_v4.py:15-126). ``rotary_frequencies`` gives a model's angle per position
 for each pair of dims, with the scalings for long contexts in use; ``apply_rotary`` turns ``q`` and
 ``k`` in one launch, for prompts, single tokens and drafted trees (any positions), and under autograd
-for training.
+for training. Positions may have several axes (time, height and width of images and video):
+``rotary_axes`` deals the pairs out to them.
 """
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -111,8 +113,59 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: dict 
     return torch.tensor(freq, dtype=torch.float64, device=dev), scale
 
 
-def _launch(q, k, positions, inv_freq, interleaved: bool, scale: float, inverse: bool, out):
-    """One launch over checked tensors (k may be None)."""
+def rotary_axes(sections, *, interleaved: bool = False, device: torch.device | str | None = None) -> torch.Tensor:
+    """The axis of every pair (int32 ``[sum(sections)]`` on ``device``, default: the current GPU) where axis ``a``
+    of the positions turns ``sections[a]`` pairs of a head.
+
+    The axes' pairs follow each other (a model config's ``mrope_section``), or are dealt out in turn if
+    ``interleaved`` (``mrope_interleaved``): axis ``a > 0`` gets pairs ``a``, ``a + n``, ... of ``n`` axes, as many as its
+    section says, and axis 0 the others.
+    """
+    sections = [int(s) for s in sections]
+    if not sections or min(sections) < 0 or sum(sections) == 0:
+        raise ValueError(f"sections must be non-negative counts of pairs, one an axis (got {sections})")
+    n, half = len(sections), sum(sections)
+    axes = [a for a, s in enumerate(sections) for _ in range(s)]
+    if interleaved:
+        axes = [0] * half
+        for a, s in enumerate(sections[1:], 1):
+            if s > 0 and a + n * (s - 1) >= half:
+                raise ValueError(f"sections {sections} cannot take turns over {half} pairs")
+            axes[a:a + n * s:n] = [a] * s
+    dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+    return torch.tensor(axes, dtype=torch.int32, device=dev)
+
+
+def check_rotation(positions, inv_freq, axes, tokens: int, d: int, dev: torch.device):
+    """A call's positions, frequencies and axes (None: one), checked and contiguous."""
+    _require_cuda(positions, "positions", dev)
+    if axes is None:
+        if positions.dtype != torch.int64 or tuple(positions.shape) != (tokens,):
+            raise ValueError(f"positions must be int64 [{tokens}] (got {positions.dtype} {tuple(positions.shape)})")
+    elif positions.dtype != torch.int64 or positions.dim() != 2 or positions.shape[0] < 1 or positions.shape[1] != tokens:
+        raise ValueError(f"positions must be int64 [axes, {tokens}] (got {positions.dtype} {tuple(positions.shape)})")
+    _require_cuda(inv_freq, "inv_freq", dev)
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not 0 < 2 * inv_freq.shape[0] <= d:
+        raise ValueError(f"inv_freq must be float64 [R / 2] with R <= {d} (got {inv_freq.dtype} {tuple(inv_freq.shape)})")
+    if axes is not None:
+        _require_cuda(axes, "axes", dev)
+        if axes.dtype != torch.int32 or axes.shape != inv_freq.shape:
+            raise ValueError(f"axes must be int32 {list(inv_freq.shape)}, one a pair (got {axes.dtype} {tuple(axes.shape)})")
+        axes = axes.contiguous()
+    return positions.contiguous(), inv_freq.contiguous(), axes
+
+
+def rotation(positions, inv_freq, axes, interleaved: bool, scale: float, inverse: bool = False) -> _lib.WkvRotary:
+    """The library's description of a rotation (wkv_rotary_t) from checked tensors, which have to outlive it."""
+    return _lib.WkvRotary(
+        positions=positions.data_ptr(), axis_stride=positions.stride(0) if positions.dim() == 2 else 0,
+        axes=None if axes is None else axes.data_ptr(), inv_freq=inv_freq.data_ptr(),
+        num_axes=positions.shape[0] if positions.dim() == 2 else 1, rotary_dim=2 * inv_freq.shape[0],
+        interleaved=interleaved, inverse=inverse, scale=scale, reserved=0)
+
+
+def _launch(q, k, positions, inv_freq, axes, interleaved: bool, scale: float, inverse: bool, out):
+    """One launch over checked tensors (k and axes may be None)."""
     qi = q if q.stride(2) == 1 else q.contiguous()
     qo = torch.empty_like(qi, memory_format=torch.contiguous_format) if out is None else out[0]
     tokens, hq, d = qi.shape
@@ -126,10 +179,14 @@ def _launch(q, k, positions, inv_freq, interleaved: bool, scale: float, inverse:
         ko = torch.empty_like(ki, memory_format=torch.contiguous_format) if out is None else out[1]
         tail = (ki.data_ptr(), *ki.stride()[:2], ko.data_ptr(), *ko.stride()[:2], ki.shape[1])
     dev = q.device
+    rows = (_DTYPES[q.dtype], qi.data_ptr(), st, sh, qo.data_ptr(), ot, oh, hq, *tail, d)
     with _on(dev):
-        rc = _lib.load().wkv_rotary(
-            _DTYPES[q.dtype], qi.data_ptr(), st, sh, qo.data_ptr(), ot, oh, hq, *tail, d, positions.data_ptr(),
-            inv_freq.data_ptr(), 2 * inv_freq.shape[0], interleaved, inverse, scale, tokens, _stream(dev))
+        if axes is None:
+            rc = _lib.load().wkv_rotary(*rows, positions.data_ptr(), inv_freq.data_ptr(), 2 * inv_freq.shape[0],
+                                        interleaved, inverse, scale, tokens, _stream(dev))
+        else:
+            how = rotation(positions, inv_freq, axes, interleaved, scale, inverse)
+            rc = _lib.load().wkv_rotary_axes(*rows, ctypes.byref(how), tokens, _stream(dev))
     _lib.check(rc, "apply_rotary")
     return qo, ko
 
@@ -145,13 +202,13 @@ class _Rotary(torch.autograd.Function):
     with the angles negated (and differentiable again), a tangent's the launch itself."""
 
     @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, interleaved, scale, inverse):
-        ctx.save_for_backward(positions, inv_freq)
-        ctx.save_for_forward(positions, inv_freq)
+    def forward(ctx, q, k, positions, inv_freq, axes, interleaved, scale, inverse):
+        ctx.save_for_backward(positions, inv_freq, axes)
+        ctx.save_for_forward(positions, inv_freq, axes)
         ctx.how = (interleaved, scale, inverse)
         ctx.heads = (q.shape[1], None if k is None else k.shape[1])
         ctx.set_materialize_grads(False)
-        return _launch(q, k, positions, inv_freq, interleaved, scale, inverse, None)
+        return _launch(q, k, positions, inv_freq, axes, interleaved, scale, inverse, None)
 
     @staticmethod
     def backward(ctx, gq, gk):
@@ -163,7 +220,7 @@ class _Rotary(torch.autograd.Function):
                              scale, not inverse)
         if lone is not None:
             gq, gk = None, gq
-        return gq, gk, None, None, None, None, None
+        return gq, gk, None, None, None, None, None, None
 
     @staticmethod
     def jvp(ctx, tq, tk, *_):
@@ -185,7 +242,7 @@ def _turned(q, k, *how):
 
 
 def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, *,
-                 interleaved: bool = False, scale: float = 1.0, inverse: bool = False,
+                 axes: torch.Tensor | None = None, interleaved: bool = False, scale: float = 1.0, inverse: bool = False,
                  out: tuple[torch.Tensor, torch.Tensor | None] | None = None):
     """``q [T, Hq, D]`` and ``k [T, Hk, D]`` (or None) with their heads turned by ``positions [T]`` int64 -> new
     tensors ``(q, k)``.
@@ -195,7 +252,9 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     of a head is turned by ``positions[t] * inv_freq[i]`` and multiplied by ``scale``. A pair is dims ``(i,
     i + R / 2)``, or ``(2 i, 2 i + 1)`` if ``interleaved``; dims from ``R`` on stay as they are. Positions
     may be any, in any order (a drafted tree's depths; far ones keep their exact angle). ``inverse``
-    turns back (the transpose, also by ``scale``). ``out``: the two results' tensors; ``out=(q, k)`` works in
+    turns back (the transpose, also by ``scale``). With ``axes`` (int32 ``[R / 2]``, from ``rotary_axes``) the
+    positions are int64 ``[A, T]`` and pair ``i`` is turned by those of axis ``axes[i]`` (a pair of an axis outside
+    ``[0, A)`` by none). ``out``: the two results' tensors; ``out=(q, k)`` works in
     place, other tensors share no memory with ``q`` and ``k``. Differentiable in ``q`` and ``k``, forward
     mode too (not with ``out``). For an MLA layer, ``q_pe`` and ``k_pe[:, None]``.
     """
@@ -208,14 +267,7 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     if k is not None and (not isinstance(k, torch.Tensor) or k.dim() != 3 or k.dtype != q.dtype or k.device != dev
                           or k.shape[0] != tokens or k.shape[2] != d):
         raise ValueError(f"k must be {q.dtype} [{tokens}, Hk, {d}] on {dev}")
-    _require_cuda(positions, "positions", dev)
-    if positions.dtype != torch.int64 or tuple(positions.shape) != (tokens,):
-        raise ValueError(f"positions must be int64 [{tokens}] (got {positions.dtype} {tuple(positions.shape)})")
-    _require_cuda(inv_freq, "inv_freq", dev)
-    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not 0 < 2 * inv_freq.shape[0] <= d:
-        raise ValueError(f"inv_freq must be float64 [R / 2] with R <= {d} (got {inv_freq.dtype} {tuple(inv_freq.shape)})")
-    positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
-    how = (positions, inv_freq, bool(interleaved), float(scale), bool(inverse))
+    how = (*check_rotation(positions, inv_freq, axes, tokens, d, dev), bool(interleaved), float(scale), bool(inverse))
     if out is None:
         return _turned(q, k, *how)
     if len(out) != 2 or (out[1] is None) != (k is None):
