@@ -540,6 +540,28 @@ int wkv_norm_rotary_backward(int32_t dtype, const void *q, int64_t q_stride_t, i
                              const wkv_head_norm_t *norm, const wkv_rotary_t *rotary, void *dq_weight, void *dk_weight,
                              int64_t num_tokens, void *workspace, int64_t workspace_bytes, void *stream);
 
+/* The append with the norm and the rotation on the way, in one launch: the queries normed and turned into
+ * q_out (or in place; num_q_heads may be 0), the keys normed and turned into the cache, the values into the cache. The cache then holds
+ * what wkv_norm_rotary (or wkv_rotary_axes) followed by wkv_append or wkv_append_fp8 leaves in it, keys rounded to bf16 before
+ * they are coded in fp8; key and value themselves are not changed. norm or rotary may be NULL, not both. key, value and
+ * slot_mapping as for wkv_append; a slot appears once in a call. q and its result bf16 [num_tokens, num_q_heads,
+ * head_dim], strides in elements; every token's queries are computed, also those of slot -1. Replaces the
+ * engine's norms, rotary embedding and reshape_and_cache of a layer (inside llm.generate, engine.py:887). */
+int wkv_rotary_append(const wkv_cache_t *cache, const void *key, int64_t key_stride_t, int64_t key_stride_h,
+                      const void *value, int64_t value_stride_t, int64_t value_stride_h, const int64_t *slot_mapping,
+                      const void *q, int64_t q_stride_t, int64_t q_stride_h, void *q_out, int64_t qo_stride_t,
+                      int64_t qo_stride_h, int32_t num_q_heads, const wkv_head_norm_t *norm,
+                      const wkv_rotary_t *rotary, int64_t num_tokens, void *stream);
+
+/* The same for a latent cache: latent[slot[t]] = concat(kv_c[t] normed (kv_norm's k_weight [kv_lora_rank], eps and
+ * offset; NULL: as it is), k_pe[t] turned), and the queries' q_pe [num_tokens, num_heads, rope_dim] turned into q_out. kv_c, k_pe and
+ * slot_mapping as for wkv_mla_append. Replaces the engine's norm of the compressed entries,
+ * its rotary embedding (wavelet/inference/deepseek_v4.py:15-66) and concat_and_cache_mla. */
+int wkv_mla_rotary_append(const wkv_mla_cache_t *cache, const void *kv_c, int64_t kv_c_stride, const void *k_pe,
+                          int64_t k_pe_stride, const int64_t *slot_mapping, const void *q_pe, int64_t q_stride_t,
+                          int64_t q_stride_h, void *q_out, int64_t qo_stride_t, int64_t qo_stride_h, int32_t num_heads,
+                          const wkv_head_norm_t *kv_norm, const wkv_rotary_t *rotary, int64_t num_tokens, void *stream);
+
 /* Attention of drafted tokens over the paged cache: wkv_prefill_gqa with a mask
  * in the place of the causal one. Row j of sequence b's n_b = cu_seqlens_q[b+1] -
  * cu_seqlens_q[b] new tokens attends to the seq_lens[b] - n_b cached tokens

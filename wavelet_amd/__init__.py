@@ -27,6 +27,8 @@ Public surface (a drop-in for the KV path of the reference's inference engine):
   positions of several axes;
 * ``norm_rotary`` -- every query and key head normed, and turned in the same
   pass, with gradients;
+* ``rotary_append`` / ``mla_rotary_append`` -- the append with the norm and the
+  rotation on the way, queries included, one launch a layer;
 * ``sample`` -- the token sampler after decode (temperature, min_p, top_k,
   top_p, repetition penalty; processed logprobs and the sampling mask).
 
@@ -44,6 +46,7 @@ from .cache import MLALatentCache, PagedKVCache, validate_group_prefix, validate
 from .norm_rotary import norm_rotary
 from .pool import KVPool
 from .rotary import apply_rotary, rotary_axes, rotary_frequencies
+from .rotary_append import mla_rotary_append, rotary_append
 from .sampler import sample
 from .step import Accepted, StepMaps, StepState, accept_tree, extend_tables
 
@@ -61,12 +64,14 @@ __all__ = [
     "grouped_decode_order",
     "decode_plan",
     "extend_tables",
+    "mla_rotary_append",
     "norm_rotary",
     "paged_decode_gqa",
     "paged_decode_gqa_grouped",
     "paged_decode_mla",
     "paged_tree_gqa",
     "prefill_gqa",
+    "rotary_append",
     "rotary_axes",
     "rotary_frequencies",
     "sample",

@@ -130,6 +130,12 @@ _SIGNATURES = {
                                          c_int64, c_int64, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64,
                                          c_int64, c_void_p, c_int64, c_int64, c_int32, c_int32, POINTER(WkvHeadNorm),
                                          POINTER(WkvRotary), c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
+    "wkv_rotary_append": (c_int, [POINTER(WkvCache), c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
+                                  c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32,
+                                  POINTER(WkvHeadNorm), POINTER(WkvRotary), c_int64, c_void_p]),
+    "wkv_mla_rotary_append": (c_int, [POINTER(WkvMlaCache), c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+                                      c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, POINTER(WkvHeadNorm),
+                                      POINTER(WkvRotary), c_int64, c_void_p]),
     "wkv_tree_workspace_size": (c_int64, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
     "wkv_tree_gqa": (c_int, [POINTER(WkvCache), c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
                              c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_void_p,

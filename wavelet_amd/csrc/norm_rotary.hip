@@ -37,91 +37,22 @@ __global__ __launch_bounds__(kNormThreads) void norm_rotary_kernel(NormRotaryArg
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tile;
   const int nt = a.tokens - t0 < a.tile ? static_cast<int>(a.tokens - t0) : a.tile;
   const FastDiv heads = blockIdx.y + 1 == gridDim.y ? a.last : a.per;
-  const int h0 = blockIdx.y * a.per.d;
-  for (int i = threadIdx.x; i < nt * a.a.half.d; i += kNormThreads) {
-    const int t = i / a.a.half;
-    turn[i] = angle_at(a.a, t0 + t, i - t * a.a.half.d);
-  }
+  tile_angles(a.a, t0, nt, kNormThreads, turn);
   __syncthreads();
-  const int lanes = 1 << a.r.log_lanes, group = threadIdx.x >> a.r.log_lanes, u0 = threadIdx.x & (lanes - 1);
-  const int groups = kNormThreads >> a.r.log_lanes, rows = nt * heads.d;
-  const float inv_d = 1.f / static_cast<float>(a.r.D);
-  constexpr int N = U == 1 ? 2 : 1;  // rows of a group in flight
-  for (int r0 = 0; r0 < rows; r0 += groups * N) {
-    Vec x0[N][U], x1[N][U];
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int r = r0 + groups * k + group;
-      const int t = r / heads, h = h0 + r - t * heads.d;
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int u = u0 + lanes * j;
-        if (r < rows && u < a.r.units) {
-          int e0, e1;
-          unit_runs<V, INTER>(a.r, u, e0, e1);
-          const HeadRows &s = h < a.Hq ? a.q : a.k;
-          const T *x = static_cast<const T *>(s.x) + (t0 + t) * s.xt + (h < a.Hq ? h : h - a.Hq) * s.xh;
-          const Vec *p0 = reinterpret_cast<const Vec *>(x + e0), *p1 = reinterpret_cast<const Vec *>(x + e1);
-          x0[k][j] = FAR ? __builtin_nontemporal_load(p0) : *p0;
-          x1[k][j] = FAR ? __builtin_nontemporal_load(p1) : *p1;
-        } else {
-          x0[k][j] = Vec{};
-          x1[k][j] = Vec{};
-        }
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int r = r0 + groups * k + group;
-      const int t = r / heads, h = h0 + r - t * heads.d;
-      float f0[U][V], f1[U][V], ss = 0.f;
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        widen<V, T>(x0[k][j], f0[j]);
-        widen<V, T>(x1[k][j], f1[j]);
-#pragma unroll
-        for (int v = 0; v < V; ++v) ss = __builtin_fmaf(f0[j][v], f0[j][v], __builtin_fmaf(f1[j][v], f1[j][v], ss));
-      }
-      ss = group_sum(ss, a.r.log_lanes);
-      const float inv = rsqrtf(__builtin_fmaf(ss, inv_d, a.n.eps));
-      if (r >= rows) continue;
-      const HeadRows &s = h < a.Hq ? a.q : a.k;
-      const int hr = h < a.Hq ? h : h - a.Hq;
-      T *y = static_cast<T *>(s.y) + (t0 + t) * s.yt + hr * s.yh;
-      const void *w = h < a.Hq ? a.n.qw : a.n.kw;
-      const int64_t wh = hr * (h < a.Hq ? a.n.qws : a.n.kws);
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int u = u0 + lanes * j;
-        if (u >= a.r.units) continue;
-        int e0, e1;
-        unit_runs<V, INTER>(a.r, u, e0, e1);
-        float w0[V], w1[V];
-        load_weights<T, V>(a.n, w, wh + e0, w0);
-        load_weights<T, V>(a.n, w, wh + e1, w1);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          f0[j][v] *= inv * w0[v];
-          f1[j][v] *= inv * w1[v];
-        }
-        turn_unit<V, INTER>(turn + t * a.a.half.d, a.r.half, e0, e1, f0[j], f1[j]);
-        Vec o0, o1;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          o0[v] = static_cast<T>(f0[j][v]);
-          o1[v] = static_cast<T>(f1[j][v]);
-        }
-        Vec *p0 = reinterpret_cast<Vec *>(y + e0), *p1 = reinterpret_cast<Vec *>(y + e1);
-        if (FAR) {
-          __builtin_nontemporal_store(o0, p0);
-          __builtin_nontemporal_store(o1, p1);
-        } else {
-          *p0 = o0;
-          *p1 = o1;
-        }
-      }
-    }
-  }
+  norm_turn_rows<T, V, INTER, U, U == 1 ? 2 : 1, FAR>(
+      a.r, a.n, a.Hq, turn, nt, heads, blockIdx.y * a.per.d, kNormThreads,
+      [&](int t, int h) {
+        const HeadRows &s = h < a.Hq ? a.q : a.k;
+        return static_cast<const T *>(s.x) + (t0 + t) * s.xt + (h < a.Hq ? h : h - a.Hq) * s.xh;
+      },
+      [&](int t, int h, int e, Vec v) {
+        const HeadRows &s = h < a.Hq ? a.q : a.k;
+        Vec *y = reinterpret_cast<Vec *>(static_cast<T *>(s.y) + (t0 + t) * s.yt + (h < a.Hq ? h : h - a.Hq) * s.yh + e);
+        if (FAR)
+          __builtin_nontemporal_store(v, y);
+        else
+          *y = v;
+      });
 }
 
 // ---------------------------------------------------------------------------
@@ -172,10 +103,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_rotary_grad_kernel(NormGrad
     const int64_t t0 = tile * a.tile;
     const int nt = a.tokens - t0 < a.tile ? static_cast<int>(a.tokens - t0) : a.tile;
     __syncthreads();
-    for (int i = threadIdx.x; i < nt * a.a.half.d; i += kNormThreads) {
-      const int t = i / a.a.half;
-      turn[i] = angle_at(a.a, t0 + t, i - t * a.a.half.d);
-    }
+    tile_angles(a.a, t0, nt, kNormThreads, turn);
     __syncthreads();
     const int rows = nt * heads.d;
     for (int r0 = 0; r0 < rows; r0 += groups * N) {

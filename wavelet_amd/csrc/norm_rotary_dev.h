@@ -44,7 +44,7 @@ __device__ __forceinline__ float2 angle_at(const Angles &a, int64_t t, int i) {
 struct HeadNorm {
   const void *qw, *kw;  // nullptr: ones
   int64_t qws, kws;     // between heads
-  int wide;             // float32 weights
+  int on, wide;         // whether there is a norm; float32 weights
   float offset, eps;
 };
 
@@ -148,6 +148,92 @@ __device__ __forceinline__ void turn_unit(const float2 *turn, int half, int e0, 
   }
 }
 
+// A tile's angles, by the whole workgroup of `threads`; a barrier follows before they are read.
+__device__ __forceinline__ void tile_angles(const Angles &a, int64_t t0, int nt, int threads, float2 *turn) {
+  for (int i = threadIdx.x; i < nt * a.half.d; i += threads) {
+    const int t = i / a.half;
+    turn[i] = angle_at(a, t0 + t, i - t * a.half.d);
+  }
+}
+
+// Rows of a tile of nt tokens, heads h0 .. h0 + heads.d - 1 of each, by a workgroup
+// of `threads`: normed (if norm.on), turned by turn[], stored. N rows of a group of lanes in
+// flight. src(t, h): where a row lies (nullptr: skipped); dst(t, h, e, v): stores its elements from e on.
+template <class T, int V, bool INTER, int U, int N, bool FAR, class Src, class Dst>
+__device__ __forceinline__ void norm_turn_rows(const RowUnits &ru, const HeadNorm &norm, int Hq, const float2 *turn,
+                                               int nt, const FastDiv &heads, int h0, int threads, Src src, Dst dst) {
+  typedef typename VecOf<T, V>::type Vec;
+  const int lanes = 1 << ru.log_lanes, group = threadIdx.x >> ru.log_lanes, u0 = threadIdx.x & (lanes - 1);
+  const int groups = threads >> ru.log_lanes, rows = nt * heads.d;
+  const float inv_d = 1.f / static_cast<float>(ru.D);
+  for (int r0 = 0; r0 < rows; r0 += groups * N) {
+    Vec x0[N][U], x1[N][U];
+    const T *x[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int r = r0 + groups * k + group;
+      const int t = r / heads, h = h0 + r - t * heads.d;
+      x[k] = r < rows ? src(t, h) : nullptr;
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int u = u0 + lanes * j;
+        if (x[k] != nullptr && u < ru.units) {
+          int e0, e1;
+          unit_runs<V, INTER>(ru, u, e0, e1);
+          const Vec *p0 = reinterpret_cast<const Vec *>(x[k] + e0), *p1 = reinterpret_cast<const Vec *>(x[k] + e1);
+          x0[k][j] = FAR ? __builtin_nontemporal_load(p0) : *p0;
+          x1[k][j] = FAR ? __builtin_nontemporal_load(p1) : *p1;
+        } else {
+          x0[k][j] = Vec{};
+          x1[k][j] = Vec{};
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int r = r0 + groups * k + group;
+      const int t = r / heads, h = h0 + r - t * heads.d;
+      float f0[U][V], f1[U][V], ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        widen<V, T>(x0[k][j], f0[j]);
+        widen<V, T>(x1[k][j], f1[j]);
+#pragma unroll
+        for (int v = 0; v < V; ++v) ss = __builtin_fmaf(f0[j][v], f0[j][v], __builtin_fmaf(f1[j][v], f1[j][v], ss));
+      }
+      ss = group_sum(ss, ru.log_lanes);
+      const float inv = norm.on ? rsqrtf(__builtin_fmaf(ss, inv_d, norm.eps)) : 1.f;
+      if (x[k] == nullptr) continue;
+      const void *w = h < Hq ? norm.qw : norm.kw;
+      const int64_t wh = h < Hq ? h * norm.qws : (h - Hq) * norm.kws;
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int u = u0 + lanes * j;
+        if (u >= ru.units) continue;
+        int e0, e1;
+        unit_runs<V, INTER>(ru, u, e0, e1);
+        float w0[V], w1[V];
+        load_weights<T, V>(norm, w, wh + e0, w0);
+        load_weights<T, V>(norm, w, wh + e1, w1);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          f0[j][v] *= inv * w0[v];
+          f1[j][v] *= inv * w1[v];
+        }
+        turn_unit<V, INTER>(turn + t * ru.half, ru.half, e0, e1, f0[j], f1[j]);
+        Vec o0, o1;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          o0[v] = static_cast<T>(f0[j][v]);
+          o1[v] = static_cast<T>(f1[j][v]);
+        }
+        dst(t, h, e0, o0);
+        dst(t, h, e1, o1);
+      }
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Host: the checks of a call's rotation and norm, and what the kernels take of them.
 inline int check_rotary(const wkv_rotary_t *r, int head_dim, int64_t num_tokens) {
@@ -184,7 +270,7 @@ inline int check_head_norm(const wkv_head_norm_t *n, int dtype) {
 
 inline HeadNorm head_norm(const wkv_head_norm_t *n) {
   if (n == nullptr) return HeadNorm{};
-  return HeadNorm{n->q_weight, n->k_weight, n->q_weight_stride_h, n->k_weight_stride_h, n->weight_dtype == 0,
+  return HeadNorm{n->q_weight, n->k_weight, n->q_weight_stride_h, n->k_weight_stride_h, 1, n->weight_dtype == 0,
                   n->weight_offset, n->eps};
 }
 
