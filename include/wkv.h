@@ -528,9 +528,9 @@ int wkv_norm_rotary(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_
  * computed; contiguous, [head_dim], or [heads, head_dim] where the weight has a head stride, of weight_dtype).
  * A kind of heads without a gradient is given as 0 heads. Summed in float32, in an order that depends on the sizes alone.
  * workspace: wkv_norm_rotary_workspace_size() bytes, 16-byte aligned, for a weight's gradient (else it may be NULL);
- * rotary_dim 0 without a rotation; weight_each_head: that weight's gradient is asked for and is [heads, head_dim]. */
+ * weight_each_head: that weight is [heads, head_dim]. */
 int64_t wkv_norm_rotary_workspace_size(int64_t num_tokens, int32_t num_q_heads, int32_t num_k_heads, int32_t head_dim,
-                                       int32_t rotary_dim, int32_t q_weight_each_head, int32_t k_weight_each_head);
+                                       int32_t q_weight_each_head, int32_t k_weight_each_head);
 
 int wkv_norm_rotary_backward(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *q_grad,
                              int64_t qg_stride_t, int64_t qg_stride_h, void *dq, int64_t dq_stride_t,

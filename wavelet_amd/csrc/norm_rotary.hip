@@ -1,9 +1,7 @@
 // Norms of queries and keys for each head with the rotary positions in the same
 // pass, forward and backward (gfx950). The mathematics: norm_rotary_dev.h.
 //
-// Forward: a workgroup takes a tile of tokens and some or all of their heads. It
-// forms the tile's angles once, in LDS, and walks the tile's rows, a few in flight
-// for each group of lanes.
+// Forward: a wave takes a few tokens and some or all of their queries or keys.
 //
 // Backward, from the inputs and the outputs' gradient g: with z = R^T g, m = z (w + offset), r the
 // reciprocal root mean square,
@@ -17,42 +15,34 @@
 
 namespace wkv {
 
-constexpr int kNormThreads = 256;
+constexpr int kNormThreads = 256, kNormWaves = kNormThreads / 64;
 
 struct NormRotaryArgs {
-  HeadRows q, k;
+  Kind q, k;
   HeadNorm n;
   Angles a;
   RowUnits r;
   int64_t tokens;
-  int Hq, H;  // query heads; query and key heads
-  int tile;   // tokens of a workgroup
-  FastDiv per, last;  // heads of a workgroup; of the last along the grid's y
+  int q_wgs;  // workgroups that take queries; keys behind them
 };
 
-template <class T, int V, bool INTER, int U, bool FAR>
+template <class T, int V, bool INTER, int U, bool FAR, bool EACH, int LL>
 __global__ __launch_bounds__(kNormThreads) void norm_rotary_kernel(NormRotaryArgs a) {
-  typedef typename VecOf<T, V>::type Vec;
-  extern __shared__ float2 turn[];
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tile;
-  const int nt = a.tokens - t0 < a.tile ? static_cast<int>(a.tokens - t0) : a.tile;
-  const FastDiv heads = blockIdx.y + 1 == gridDim.y ? a.last : a.per;
-  tile_angles(a.a, t0, nt, kNormThreads, turn);
-  __syncthreads();
-  norm_turn_rows<T, V, INTER, U, U == 1 ? 2 : 1, FAR>(
-      a.r, a.n, a.Hq, turn, nt, heads, blockIdx.y * a.per.d, kNormThreads,
-      [&](int t, int h) {
-        const HeadRows &s = h < a.Hq ? a.q : a.k;
-        return static_cast<const T *>(s.x) + (t0 + t) * s.xt + (h < a.Hq ? h : h - a.Hq) * s.xh;
-      },
-      [&](int t, int h, int e, Vec v) {
-        const HeadRows &s = h < a.Hq ? a.q : a.k;
-        Vec *y = reinterpret_cast<Vec *>(static_cast<T *>(s.y) + (t0 + t) * s.yt + (h < a.Hq ? h : h - a.Hq) * s.yh + e);
-        if (FAR)
-          __builtin_nontemporal_store(v, y);
-        else
-          *y = v;
-      });
+  extern __shared__ float2 turns[];
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const bool is_q = static_cast<int>(blockIdx.x) < a.q_wgs;
+  const Kind &k = is_q ? a.q : a.k;
+  const WaveTile w = wave_tile(k, a.r, a.tokens, is_q ? blockIdx.x : blockIdx.x - a.q_wgs, wave);
+  if (w.tokens == 0) return;  // a whole wave; nothing below waits for another
+  float2 *turn = turns + (wave << k.log_tg) * a.r.half;
+  const void *weight = k.w;
+  if (EACH && weight != nullptr) weight = static_cast<const char *>(weight) + w.h0 * k.ws * (a.n.wide ? 4 : sizeof(T));
+  const int64_t t = w.t0 + w.t;
+  const HeadsOf<T> of{static_cast<const T *>(k.s.x) + t * k.s.xt + w.h0 * k.s.xh, k.s.xh,
+                      static_cast<T *>(k.s.y) + t * k.s.yt + w.h0 * k.s.yh, k.s.yh, 0, weight, k.ws};
+  norm_turn_heads<T, V, INTER, U, 1, FAR, false, EACH, LL>(
+      a.r, a.n, turn + w.t * a.r.half, w.there, w.group, (64 >> a.r.log_lanes) >> k.log_tg, w.heads, of,
+      [&] { wave_angles(a.a, w.t0, w.tokens, turn); });
 }
 
 // ---------------------------------------------------------------------------
@@ -63,203 +53,220 @@ struct GradRows {
   int64_t xt, xh, gt, gh, dt, dh;
 };
 
-// A workgroup's share: `heads` heads of one kind from one on, every gridth tile.
+// A kind's workgroups: `wgs` along the tokens for each of its ranges of heads. One weight for all heads: one
+// range, every wave's groups take tokens and walk all heads. Each head its own: a range of as many heads as a wave has groups,
+// and every group keeps to one.
+struct GradKind {
+  GradRows s;
+  const void *w;
+  int64_t ws;
+  int heads, each, ranges, wgs;
+  int log_tg;
+  int64_t first;  // of its sums in the workspace, in rows of D
+};
+
 struct NormGradArgs {
-  GradRows q, k;
+  GradKind q, k;
   HeadNorm n;
   Angles a;  // sign: the transpose's
   RowUnits r;
-  int64_t tokens, tiles;
-  int tile;
-  int q_ranges, k_ranges;  // ranges of heads: one of all, or each head's own
-  int q_wgs, k_wgs;        // workgroups of a range
-  FastDiv q_per, k_per;    // heads of a range
-  float *partial;          // [ranges' workgroups, D]; nullptr: no weight's gradient
+  int64_t tokens;
+  float *partial;  // [wgs][1 or heads][D] of queries, then keys; nullptr: no weight's gradient
 };
 
 template <class T, int V, bool INTER, int U, bool FAR, bool DW>
 __global__ __launch_bounds__(kNormThreads) void norm_rotary_grad_kernel(NormGradArgs a) {
   typedef typename VecOf<T, V>::type Vec;
-  extern __shared__ float2 turn[];
-  const int nq = a.q_ranges * a.q_wgs;
+  extern __shared__ float2 turns[];
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int nq = a.q.ranges * a.q.wgs;
   const bool is_q = static_cast<int>(blockIdx.x) < nq;
+  const GradKind &k = is_q ? a.q : a.k;
   const int b = is_q ? blockIdx.x : blockIdx.x - nq;
-  const int wgs = is_q ? a.q_wgs : a.k_wgs;
-  const FastDiv heads = is_q ? a.q_per : a.k_per;
-  const int range = b / wgs, h0 = range * heads.d;
-  const GradRows s = is_q ? a.q : a.k;
-  const void *w = is_q ? a.n.qw : a.n.kw;
-  const int64_t ws = is_q ? a.n.qws : a.n.kws;
-  const int lanes = 1 << a.r.log_lanes, group = threadIdx.x >> a.r.log_lanes, u0 = threadIdx.x & (lanes - 1);
-  const int groups = kNormThreads >> a.r.log_lanes;
+  const int range = b / k.wgs, wg = b - range * k.wgs;
+  const int lanes = 1 << a.r.log_lanes, u0 = threadIdx.x & (lanes - 1), g = (threadIdx.x & 63) >> a.r.log_lanes;
+  const int groups = 64 >> a.r.log_lanes, tg = 1 << k.log_tg, step = groups >> k.log_tg;
+  const int h0 = range * (k.each ? groups : k.heads), heads = k.each ? (k.heads - h0 < groups ? k.heads - h0 : groups) : k.heads;
+  const int t = g & (tg - 1), first = g >> k.log_tg;
+  float2 *turn = turns + (wave << k.log_tg) * a.r.half;
   const float inv_d = 1.f / static_cast<float>(a.r.D);
-  float acc0[U][V], acc1[U][V];
+  const bool all = 2 * a.r.half == a.r.D;
+  int e0[U], e1[U];
+  bool mine[U];
+  float w0[U][V], w1[U][V], acc0[U][V], acc1[U][V];
 #pragma unroll
-  for (int j = 0; j < U; ++j)
+  for (int j = 0; j < U; ++j) {
+    const int u = u0 + lanes * j;
+    mine[j] = u < a.r.units;
+    e0[j] = e1[j] = 0;
+    if (mine[j]) unit_runs<V, INTER>(a.r, u, e0[j], e1[j]);
+    const int64_t wh = k.each && first < heads ? (h0 + first) * k.ws : 0;
+    load_weights<T, V>(a.n, k.w, wh + e0[j], w0[j]);
+    load_weights<T, V>(a.n, k.w, wh + e1[j], w1[j]);
 #pragma unroll
     for (int v = 0; v < V; ++v) acc0[j][v] = acc1[j][v] = 0.f;
-  constexpr int N = U == 1 ? 2 : 1;
-  for (int64_t tile = b - range * wgs; tile < a.tiles; tile += wgs) {  // uniform
-    const int64_t t0 = tile * a.tile;
-    const int nt = a.tokens - t0 < a.tile ? static_cast<int>(a.tokens - t0) : a.tile;
-    __syncthreads();
-    tile_angles(a.a, t0, nt, kNormThreads, turn);
-    __syncthreads();
-    const int rows = nt * heads.d;
-    for (int r0 = 0; r0 < rows; r0 += groups * N) {
-      Vec x0[N][U], x1[N][U], g0[N][U], g1[N][U];
+  }
+  // A round is a block of the wave's tokens and `step` heads; the next one's loads are in flight over it.
+  const int64_t blocks = ((a.tokens - 1) >> k.log_tg) + 1, stride = static_cast<int64_t>(k.wgs) * kNormWaves;
+  Vec nx0[U], nx1[U], ng0[U], ng1[U];
+  auto load = [&](int64_t block, int hb) __attribute__((always_inline)) {
+    const int64_t tt = (block << k.log_tg) + t;
+    const int h = hb + first;
+    const T *x = static_cast<const T *>(k.s.x) + tt * k.s.xt + (h0 + h) * k.s.xh;
+    const T *gr = static_cast<const T *>(k.s.g) + tt * k.s.gt + (h0 + h) * k.s.gh;
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const int r = r0 + groups * k + group;
-        const int t = r / heads, h = h0 + r - t * heads.d;
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-          const int u = u0 + lanes * j;
-          if (r < rows && u < a.r.units) {
-            int e0, e1;
-            unit_runs<V, INTER>(a.r, u, e0, e1);
-            const T *x = static_cast<const T *>(s.x) + (t0 + t) * s.xt + h * s.xh;
-            const T *g = static_cast<const T *>(s.g) + (t0 + t) * s.gt + h * s.gh;
-            const Vec *px0 = reinterpret_cast<const Vec *>(x + e0), *px1 = reinterpret_cast<const Vec *>(x + e1);
-            const Vec *pg0 = reinterpret_cast<const Vec *>(g + e0), *pg1 = reinterpret_cast<const Vec *>(g + e1);
-            x0[k][j] = FAR ? __builtin_nontemporal_load(px0) : *px0;
-            x1[k][j] = FAR ? __builtin_nontemporal_load(px1) : *px1;
-            g0[k][j] = FAR ? __builtin_nontemporal_load(pg0) : *pg0;
-            g1[k][j] = FAR ? __builtin_nontemporal_load(pg1) : *pg1;
-          } else {
-            x0[k][j] = x1[k][j] = g0[k][j] = g1[k][j] = Vec{};
-          }
-        }
+    for (int j = 0; j < U; ++j) {
+      nx0[j] = nx1[j] = ng0[j] = ng1[j] = Vec{};
+      if (mine[j] && tt < a.tokens && h < heads) {
+        const Vec *px0 = reinterpret_cast<const Vec *>(x + e0[j]), *px1 = reinterpret_cast<const Vec *>(x + e1[j]);
+        const Vec *pg0 = reinterpret_cast<const Vec *>(gr + e0[j]), *pg1 = reinterpret_cast<const Vec *>(gr + e1[j]);
+        nx0[j] = FAR ? __builtin_nontemporal_load(px0) : *px0;
+        nx1[j] = FAR ? __builtin_nontemporal_load(px1) : *px1;
+        ng0[j] = FAR ? __builtin_nontemporal_load(pg0) : *pg0;
+        ng1[j] = FAR ? __builtin_nontemporal_load(pg1) : *pg1;
       }
+    }
+  };
+  UnitTurn<V> turned[U];
+  int64_t block = static_cast<int64_t>(wg) * kNormWaves + wave;
+  int hb = 0;
+  if (block < blocks) load(block, 0);
+  while (block < blocks) {  // uniform
+    Vec x0[U], x1[U], g0[U], g1[U];
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const int r = r0 + groups * k + group;
-        const int t = r / heads, h = h0 + r - t * heads.d;
-        float f0[U][V], f1[U][V], z0[U][V], z1[U][V], m0[U][V], m1[U][V], ss = 0.f, sm = 0.f;
+    for (int j = 0; j < U; ++j) {
+      x0[j] = nx0[j];
+      x1[j] = nx1[j];
+      g0[j] = ng0[j];
+      g1[j] = ng1[j];
+    }
+    const int64_t this_block = block;
+    const int this_h = hb;
+    hb += step;
+    if (hb >= heads) {
+      hb = 0;
+      block += stride;
+    }
+    if (block < blocks) load(block, hb);
+    if (this_h == 0) {
+      const int64_t t0 = this_block << k.log_tg;
+      const int nt = a.tokens - t0 < tg ? static_cast<int>(a.tokens - t0) : tg;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the block before has been read
+      __builtin_amdgcn_wave_barrier();
+      wave_angles(a.a, t0, nt, turn);
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-          const int u = u0 + lanes * j;
-          int e0 = 0, e1 = 0;
-          if (r < rows && u < a.r.units) unit_runs<V, INTER>(a.r, u, e0, e1);
-          widen<V, T>(x0[k][j], f0[j]);
-          widen<V, T>(x1[k][j], f1[j]);
-          widen<V, T>(g0[k][j], z0[j]);
-          widen<V, T>(g1[k][j], z1[j]);
-          // (a lane without a unit holds zeros, and turns them by some token's angles)
-          turn_unit<V, INTER>(turn + (r < rows ? t * a.a.half.d : 0), a.r.half, e0, e1, z0[j], z1[j]);
-          float w0[V], w1[V];
-          const int64_t wh = r < rows ? h * ws : 0;
-          load_weights<T, V>(a.n, w, wh + e0, w0);
-          load_weights<T, V>(a.n, w, wh + e1, w1);
+      for (int j = 0; j < U; ++j)
+        unit_turn<V, INTER>(turn + (t < nt ? t : 0) * a.r.half, a.r.half, all, e0[j], e1[j], turned[j]);
+    }
+    float f0[U][V], f1[U][V], z0[U][V], z1[U][V], ss = 0.f, sm = 0.f;
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            m0[j][v] = z0[j][v] * w0[v];
-            m1[j][v] = z1[j][v] * w1[v];
-            ss = __builtin_fmaf(f0[j][v], f0[j][v], __builtin_fmaf(f1[j][v], f1[j][v], ss));
-            sm = __builtin_fmaf(m0[j][v], f0[j][v], __builtin_fmaf(m1[j][v], f1[j][v], sm));
-          }
-        }
-        ss = group_sum(ss, a.r.log_lanes);
-        sm = group_sum(sm, a.r.log_lanes);
-        const float inv = rsqrtf(__builtin_fmaf(ss, inv_d, a.n.eps));
-        const float back = sm * inv_d * inv * inv;
+    for (int j = 0; j < U; ++j) {
+      widen<V, T>(x0[j], f0[j]);
+      widen<V, T>(x1[j], f1[j]);
+      widen<V, T>(g0[j], z0[j]);
+      widen<V, T>(g1[j], z1[j]);
+      unit_back<V, INTER>(turned[j], all, z0[j], z1[j]);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        ss = __builtin_fmaf(f0[j][v], f0[j][v], __builtin_fmaf(f1[j][v], f1[j][v], ss));
+        sm = __builtin_fmaf(z0[j][v] * w0[j][v], f0[j][v], __builtin_fmaf(z1[j][v] * w1[j][v], f1[j][v], sm));
+      }
+    }
+    ss = group_sum(ss, a.r.log_lanes);
+    sm = group_sum(sm, a.r.log_lanes);
+    const float inv = __builtin_amdgcn_rsqf(__builtin_fmaf(ss, inv_d, a.n.eps));
+    const float back = sm * inv_d * inv * inv;
+    const int64_t tt = (this_block << k.log_tg) + t;
+    const int h = this_h + first;
+    const bool store = k.s.dx != nullptr && tt < a.tokens && h < heads;
+    T *y = static_cast<T *>(k.s.dx) + tt * k.s.dt + (h0 + h) * k.s.dh;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      Vec o0, o1;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
         if (DW) {
-#pragma unroll
-          for (int j = 0; j < U; ++j)
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-              acc0[j][v] = __builtin_fmaf(z0[j][v], f0[j][v] * inv, acc0[j][v]);
-              acc1[j][v] = __builtin_fmaf(z1[j][v], f1[j][v] * inv, acc1[j][v]);
-            }
+          acc0[j][v] = __builtin_fmaf(z0[j][v], f0[j][v] * inv, acc0[j][v]);
+          acc1[j][v] = __builtin_fmaf(z1[j][v], f1[j][v] * inv, acc1[j][v]);
         }
-        if (r >= rows || s.dx == nullptr) continue;
-        T *y = static_cast<T *>(s.dx) + (t0 + t) * s.dt + h * s.dh;
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-          const int u = u0 + lanes * j;
-          if (u >= a.r.units) continue;
-          int e0, e1;
-          unit_runs<V, INTER>(a.r, u, e0, e1);
-          Vec o0, o1;
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            o0[v] = static_cast<T>(inv * __builtin_fmaf(-back, f0[j][v], m0[j][v]));
-            o1[v] = static_cast<T>(inv * __builtin_fmaf(-back, f1[j][v], m1[j][v]));
-          }
-          Vec *p0 = reinterpret_cast<Vec *>(y + e0), *p1 = reinterpret_cast<Vec *>(y + e1);
-          if (FAR) {
-            __builtin_nontemporal_store(o0, p0);
-            __builtin_nontemporal_store(o1, p1);
-          } else {
-            *p0 = o0;
-            *p1 = o1;
-          }
+        o0[v] = static_cast<T>(inv * __builtin_fmaf(-back, f0[j][v], z0[j][v] * w0[j][v]));
+        o1[v] = static_cast<T>(inv * __builtin_fmaf(-back, f1[j][v], z1[j][v] * w1[j][v]));
+      }
+      if (store && mine[j]) {
+        Vec *p0 = reinterpret_cast<Vec *>(y + e0[j]), *p1 = reinterpret_cast<Vec *>(y + e1[j]);
+        if (FAR) {
+          __builtin_nontemporal_store(o0, p0);
+          __builtin_nontemporal_store(o1, p1);
+        } else {
+          *p0 = o0;
+          *p1 = o1;
         }
       }
     }
   }
   if (!DW) return;
-  // The groups' sums: of a wave's groups by butterflies, of the waves through LDS.
-  float *sums = reinterpret_cast<float *>(turn);  // [waves, D]
+  // The sums: of a wave's groups by butterflies (one weight for all heads), of the waves through LDS.
+  float *sums = reinterpret_cast<float *>(turns);  // [waves][rows][D]
+  const int rows = k.each ? groups : 1;
   __syncthreads();
-  const int wave = threadIdx.x >> 6;
 #pragma unroll
   for (int j = 0; j < U; ++j) {
-    const int u = u0 + lanes * j;
-    int e0 = 0, e1 = 0;
-    if (u < a.r.units) unit_runs<V, INTER>(a.r, u, e0, e1);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       float s0 = acc0[j][v], s1 = acc1[j][v];
-      for (int o = lanes; o < 64; o *= 2) {  // uniform
-        s0 += __shfl_xor(s0, o, 64);
-        s1 += __shfl_xor(s1, o, 64);
-      }
-      if (u < a.r.units && (threadIdx.x & 63) < lanes) {
-        sums[wave * a.r.D + e0 + v] = s0;
-        sums[wave * a.r.D + e1 + v] = s1;
+      if (!k.each)
+        for (int o = lanes; o < 64; o *= 2) {  // uniform
+          s0 += __shfl_xor(s0, o, 64);
+          s1 += __shfl_xor(s1, o, 64);
+        }
+      if (mine[j] && g < rows) {
+        sums[(wave * rows + g) * a.r.D + e0[j] + v] = s0;
+        sums[(wave * rows + g) * a.r.D + e1[j] + v] = s1;
       }
     }
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < a.r.D; d += kNormThreads) {
-    float s0 = 0.f;
+  const int n = k.each ? heads : 1;  // a group's number is its head's, one token a wave
+  float *out = a.partial + (k.first + static_cast<int64_t>(wg) * (k.each ? k.heads : 1) + (k.each ? h0 : 0)) * a.r.D;
+  for (int d = threadIdx.x; d < n * a.r.D; d += kNormThreads) {
+    float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < kNormThreads / 64; ++i) s0 += sums[i * a.r.D + d];
-    a.partial[static_cast<int64_t>(blockIdx.x) * a.r.D + d] = s0;
+    for (int i = 0; i < kNormWaves; ++i) s += sums[i * rows * a.r.D + d];
+    out[d] = s;
   }
 }
 
 // The weights' gradients from the workgroups' sums: a workgroup adds up 64
-// elements of one range, a sixteenth of the sums each wave.
+// elements of one head's row, a sixteenth of the sums each wave.
 constexpr int kSumWaves = 16;
 struct WeightGrads {
   const float *partial;
   void *dq, *dk;  // nullptr: not asked for
-  int q_ranges, q_wgs, k_wgs, D;
+  int q_rows, k_rows, q_wgs, k_wgs, D;
   int dtype;  // of the gradients: 0 fp32, 1 bf16, 2 fp16
 };
 
 __global__ __launch_bounds__(64 * kSumWaves) void norm_weight_grad_kernel(WeightGrads a) {
   __shared__ float sums[kSumWaves][64];
-  const bool is_q = static_cast<int>(blockIdx.x) < a.q_ranges;
-  const int range = is_q ? blockIdx.x : blockIdx.x - a.q_ranges;
+  const bool is_q = static_cast<int>(blockIdx.x) < a.q_rows;
+  const int row = is_q ? blockIdx.x : blockIdx.x - a.q_rows;
   void *out = is_q ? a.dq : a.dk;
   if (out == nullptr) return;  // uniform
   const int n = is_q ? a.q_wgs : a.k_wgs;
-  const int64_t first = is_q ? static_cast<int64_t>(range) * n : static_cast<int64_t>(a.q_ranges) * a.q_wgs + static_cast<int64_t>(range) * n;
+  const int64_t rows = is_q ? a.q_rows : a.k_rows;
+  const float *p = a.partial + ((is_q ? 0 : static_cast<int64_t>(a.q_rows) * a.q_wgs) + row) * a.D;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, d = blockIdx.y * 64 + lane;
   float s = 0.f;
   if (d < a.D) {
 #pragma unroll 8
-    for (int i = wave; i < n; i += kSumWaves) s += a.partial[(first + i) * a.D + d];
+    for (int i = wave; i < n; i += kSumWaves) s += p[i * rows * a.D + d];
   }
   sums[wave][lane] = s;
   __syncthreads();
   if (wave != 0 || d >= a.D) return;
 #pragma unroll
   for (int i = 1; i < kSumWaves; ++i) s += sums[i][lane];
-  const int64_t at = static_cast<int64_t>(range) * a.D + d;
+  const int64_t at = static_cast<int64_t>(row) * a.D + d;
   if (a.dtype == 0)
     static_cast<float *>(out)[at] = s;
   else if (a.dtype == 1)
@@ -270,21 +277,22 @@ __global__ __launch_bounds__(64 * kSumWaves) void norm_weight_grad_kernel(Weight
 
 // ---------------------------------------------------------------------------
 // Host.
-// The forward launch.
-template <class T, int V, bool INTER>
-static void launch_norm(const NormRotaryArgs &a, bool far, dim3 grid, size_t lds, hipStream_t s) {
-  constexpr bool WIDE = V * sizeof(T) == 16;
+// The forward launch. Heads of 64 and 128 in 16-byte accesses have their lanes as a constant (16,384 tokens of 40 heads of
+// 128, bf16: 65.1 us, 67.2 without).
+template <class T, int V, bool INTER, bool EACH>
+static void launch_norm(const NormRotaryArgs &a, bool far, unsigned grid, size_t lds, hipStream_t s) {
   if (a.r.units > 64) {
-    if constexpr (V <= 2) norm_rotary_kernel<T, V, INTER, 4, false><<<grid, kNormThreads, lds, s>>>(a);
+    if constexpr (V <= 2) norm_rotary_kernel<T, V, INTER, 4, false, EACH, -1><<<grid, kNormThreads, lds, s>>>(a);
     return;
   }
-  if constexpr (WIDE) {
-    if (far) {
-      norm_rotary_kernel<T, V, INTER, 1, true><<<grid, kNormThreads, lds, s>>>(a);
-      return;
-    }
+  if constexpr (V * sizeof(T) == 16 && !EACH) {
+    constexpr int L64 = sizeof(T) == 2 ? 2 : 3, L128 = L64 + 1;
+    if (a.r.log_lanes == L128 && far) return norm_rotary_kernel<T, V, INTER, 1, true, EACH, L128><<<grid, kNormThreads, lds, s>>>(a);
+    if (a.r.log_lanes == L128) return norm_rotary_kernel<T, V, INTER, 1, false, EACH, L128><<<grid, kNormThreads, lds, s>>>(a);
+    if (a.r.log_lanes == L64 && far) return norm_rotary_kernel<T, V, INTER, 1, true, EACH, L64><<<grid, kNormThreads, lds, s>>>(a);
+    if (a.r.log_lanes == L64) return norm_rotary_kernel<T, V, INTER, 1, false, EACH, L64><<<grid, kNormThreads, lds, s>>>(a);
   }
-  norm_rotary_kernel<T, V, INTER, 1, false><<<grid, kNormThreads, lds, s>>>(a);
+  norm_rotary_kernel<T, V, INTER, 1, false, EACH, -1><<<grid, kNormThreads, lds, s>>>(a);
 }
 
 template <class T, int V, bool INTER>
@@ -353,12 +361,6 @@ bool rows_ok(const void *x, int64_t st, int64_t sh, int esz) {
   return x != nullptr && reinterpret_cast<uintptr_t>(x) % esz == 0 && st >= 0 && sh >= 0;
 }
 
-// Tokens whose angles take 8 KB.
-int tile_tokens(int half) {
-  const int t = half > 0 ? 1024 / half : 16;
-  return t < 1 ? 1 : t > 16 ? 16 : t;
-}
-
 }  // namespace
 
 extern "C" int wkv_norm_rotary(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_stride_h, void *q_out,
@@ -377,13 +379,9 @@ extern "C" int wkv_norm_rotary(int32_t dtype, const void *q, int64_t q_stride_t,
   const int half = rotary != nullptr ? rotary->rotary_dim / 2 : 0;
   const bool inter = rotary != nullptr && rotary->interleaved != 0;
   NormRotaryArgs a{};
-  a.q = HeadRows{q, q_out, q_stride_t, q_stride_h, qo_stride_t, qo_stride_h};
-  a.k = HeadRows{k, k_out, k_stride_t, k_stride_h, ko_stride_t, ko_stride_h};
   a.n = head_norm(norm);
   a.a = angles(rotary);
   a.tokens = num_tokens;
-  a.Hq = num_q_heads;
-  a.H = H;
   Widths w(esz, head_dim, half, inter);
   const int wsz = norm->weight_dtype == 0 ? 4 : 2;
   if (num_q_heads > 0) {
@@ -397,22 +395,24 @@ extern "C" int wkv_norm_rotary(int32_t dtype, const void *q, int64_t q_stride_t,
     w.weights(norm->k_weight, norm->k_weight_stride_h, wsz);
   }
   a.r = row_units(head_dim, half, w.v);
-  // With too few tokens for the chip, smaller tiles, then their heads over more workgroups.
-  a.tile = tile_tokens(half);
-  while (a.tile > 1 && (num_tokens + a.tile - 1) / a.tile < 1024) a.tile /= 2;
-  const int64_t tiles = (num_tokens + a.tile - 1) / a.tile;
-  const int groups = kNormThreads >> a.r.log_lanes;
-  const int64_t want = (1024 + tiles - 1) / tiles, most = (H + groups - 1) / groups;
-  const int split = static_cast<int>(want < most ? want : most);
-  a.per = fast_div((H + split - 1) / split);
-  const int ny = (H + a.per.d - 1) / a.per.d;
-  a.last = fast_div(H - (ny - 1) * a.per.d);
+  const KindGrid gq(num_tokens, num_q_heads, a.r.log_lanes, false), gk(num_tokens, num_k_heads, a.r.log_lanes, false);
+  a.q = Kind{HeadRows{q, q_out, q_stride_t, q_stride_h, qo_stride_t, qo_stride_h}, norm->q_weight,
+             norm->q_weight_stride_h, num_q_heads, gq.log_tg, gq.per, fast_div(gq.splits)};
+  a.k = Kind{HeadRows{k, k_out, k_stride_t, k_stride_h, ko_stride_t, ko_stride_h}, norm->k_weight,
+             norm->k_weight_stride_h, num_k_heads, gk.log_tg, gk.per, fast_div(gk.splits)};
+  WKV_CHECK_ARG(gq.wgs + gk.wgs <= INT32_MAX, "too many tokens and heads for one launch");
+  a.q_wgs = static_cast<int>(gq.wgs);
+  const bool each = (norm->q_weight != nullptr && norm->q_weight_stride_h != 0) ||
+                    (norm->k_weight != nullptr && norm->k_weight_stride_h != 0);
   const bool far = num_tokens * H * head_dim * esz >= (64 << 20);
-  const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(ny));
-  const size_t lds = static_cast<size_t>(a.tile) * half * sizeof(float2);
+  const unsigned grid = static_cast<unsigned>(gq.wgs + gk.wgs);
+  const int log_tg = gq.log_tg > gk.log_tg ? gq.log_tg : gk.log_tg;
+  const size_t lds = (static_cast<size_t>(kNormWaves) << log_tg) * half * sizeof(float2);
   auto s = static_cast<hipStream_t>(stream);
   with_types(dtype, w.v, inter, [&](auto zero, auto v, auto in) {
-    launch_norm<decltype(zero), decltype(v)::value, decltype(in)::value>(a, far, grid, lds, s);
+    using T = decltype(zero);
+    if (each) launch_norm<T, decltype(v)::value, decltype(in)::value, true>(a, far, grid, lds, s);
+    else launch_norm<T, decltype(v)::value, decltype(in)::value, false>(a, far, grid, lds, s);
   });
   WKV_CHECK_LAUNCH("norm_rotary");
   return WKV_OK;
@@ -420,39 +420,31 @@ extern "C" int wkv_norm_rotary(int32_t dtype, const void *q, int64_t q_stride_t,
 
 namespace {
 
-// Workgroups of the backward launch along the tokens, for each kind of heads.
+// A kind's workgroups of the backward launch along the tokens, and its rows of sums.
 struct GradGrid {
-  int tile, q_ranges, k_ranges, q_wgs, k_wgs;
-  int64_t tiles;
-  GradGrid(int64_t tokens, int Hq, int Hk, int half, bool q_each, bool k_each) {
-    tile = tile_tokens(half);
-    while (tile > 1 && (tokens + tile - 1) / tile < 512) tile /= 2;
-    tiles = (tokens + tile - 1) / tile;
-    q_ranges = Hq == 0 ? 0 : q_each ? Hq : 1;
-    k_ranges = Hk == 0 ? 0 : k_each ? Hk : 1;
-    const int64_t total = 1024, H = Hq + Hk > 0 ? Hq + Hk : 1;
-    auto wgs = [&](int heads, int ranges) -> int {
-      if (ranges == 0) return 0;
-      int64_t n = (total * heads + H * ranges - 1) / (H * ranges);
-      n = n < 1 ? 1 : n;
-      return static_cast<int>(n < tiles ? n : tiles);
-    };
-    q_wgs = wgs(Hq, q_ranges);
-    k_wgs = wgs(Hk, k_ranges);
+  int wgs, rows;
+  GradGrid(int64_t tokens, int heads, int all_heads, int D, bool each) {
+    rows = each ? heads : 1;
+    // 768 workgroups (three waves a SIMD) shared by heads; where each head has sums of its own, by ranges of 1,024 elements
+    const int64_t share = each ? 1024 / ((static_cast<int64_t>(heads) * D + 1023) / 1024 + 1) : 768ll * heads / (all_heads > 0 ? all_heads : 1);
+    const int64_t most = (tokens + kNormWaves - 1) / kNormWaves, n = share < 1 ? 1 : share;
+    wgs = heads == 0 ? 0 : static_cast<int>(n < most ? n : most);
   }
-  int64_t count() const { return static_cast<int64_t>(q_ranges) * q_wgs + static_cast<int64_t>(k_ranges) * k_wgs; }
+  int64_t floats(int D) const { return static_cast<int64_t>(wgs) * rows * D; }
 };
 
 }  // namespace
 
 extern "C" int64_t wkv_norm_rotary_workspace_size(int64_t num_tokens, int32_t num_q_heads, int32_t num_k_heads,
-                                                  int32_t head_dim, int32_t rotary_dim, int32_t q_weight_each_head,
+                                                  int32_t head_dim, int32_t q_weight_each_head,
                                                   int32_t k_weight_each_head) {
   if (num_tokens < 0 || num_tokens > INT32_MAX || num_q_heads < 0 || num_k_heads < 0 || num_q_heads > 65535 ||
-      num_k_heads > 65535 || head_dim <= 0 || head_dim > WKV_ROTARY_MAX_DIM || rotary_dim < 0 || rotary_dim > head_dim)
+      num_k_heads > 65535 || head_dim <= 0 || head_dim > WKV_ROTARY_MAX_DIM)
     return -1;
-  const GradGrid g(num_tokens, num_q_heads, num_k_heads, rotary_dim / 2, q_weight_each_head != 0, k_weight_each_head != 0);
-  return g.count() * head_dim * static_cast<int64_t>(sizeof(float));
+  const int all = num_q_heads + num_k_heads;
+  return (GradGrid(num_tokens, num_q_heads, all, head_dim, q_weight_each_head != 0).floats(head_dim) +
+          GradGrid(num_tokens, num_k_heads, all, head_dim, k_weight_each_head != 0).floats(head_dim)) *
+         static_cast<int64_t>(sizeof(float));
 }
 
 extern "C" int wkv_norm_rotary_backward(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_stride_h,
@@ -482,55 +474,60 @@ extern "C" int wkv_norm_rotary_backward(int32_t dtype, const void *q, int64_t q_
   const bool dw = dq_weight != nullptr || dk_weight != nullptr;
   const int half = rotary != nullptr ? rotary->rotary_dim / 2 : 0;
   const bool inter = rotary != nullptr && rotary->interleaved != 0;
-  const GradGrid g(num_tokens, num_q_heads, num_k_heads, half, dq_weight != nullptr && norm->q_weight_stride_h != 0,
-                   dk_weight != nullptr && norm->k_weight_stride_h != 0);
+  const bool q_each = norm->q_weight != nullptr && norm->q_weight_stride_h != 0;
+  const bool k_each = norm->k_weight != nullptr && norm->k_weight_stride_h != 0;
+  const int H = num_q_heads + num_k_heads;
+  const GradGrid gq(num_tokens, num_q_heads, H, head_dim, q_each), gk(num_tokens, num_k_heads, H, head_dim, k_each);
+  const int64_t need = (gq.floats(head_dim) + gk.floats(head_dim)) * static_cast<int64_t>(sizeof(float));
   if (dw)
-    WKV_CHECK_ARG(g.count() == 0 || (workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 &&
-                      workspace_bytes >= g.count() * head_dim * static_cast<int64_t>(sizeof(float))),
+    WKV_CHECK_ARG(need == 0 || (workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= need),
                   "workspace must hold wkv_norm_rotary_workspace_size() bytes, 16-byte aligned");
   auto s = static_cast<hipStream_t>(stream);
   if (num_tokens > 0) {
     NormGradArgs a{};
-    a.q = GradRows{q, q_grad, dq, q_stride_t, q_stride_h, qg_stride_t, qg_stride_h, dq_stride_t, dq_stride_h};
-    a.k = GradRows{k, k_grad, dk, k_stride_t, k_stride_h, kg_stride_t, kg_stride_h, dk_stride_t, dk_stride_h};
+    const GradRows rq{q, q_grad, dq, q_stride_t, q_stride_h, qg_stride_t, qg_stride_h, dq_stride_t, dq_stride_h};
+    const GradRows rk{k, k_grad, dk, k_stride_t, k_stride_h, kg_stride_t, kg_stride_h, dk_stride_t, dk_stride_h};
     a.n = head_norm(norm);
     a.a = angles(rotary);
     a.a.sign = -a.a.sign;
     a.tokens = num_tokens;
-    a.tiles = g.tiles;
-    a.tile = g.tile;
-    a.q_ranges = g.q_ranges;
-    a.k_ranges = g.k_ranges;
-    a.q_wgs = g.q_wgs;
-    a.k_wgs = g.k_wgs;
-    a.q_per = fast_div(g.q_ranges > 0 ? num_q_heads / g.q_ranges : 1);
-    a.k_per = fast_div(g.k_ranges > 0 ? num_k_heads / g.k_ranges : 1);
     a.partial = dw ? static_cast<float *>(workspace) : nullptr;
     Widths w(esz, head_dim, half, inter);
-    auto kind = [&](int heads, const GradRows &r, const void *weight, int64_t ws) {
+    auto fit = [&](int heads, const GradRows &r, const void *weight, int64_t ws) {
       if (heads == 0) return;
       w.rows(r.x, r.xt, r.xh);
       w.rows(r.g, r.gt, r.gh);
       if (r.dx != nullptr) w.rows(r.dx, r.dt, r.dh);
       w.weights(weight, ws, wsz);
     };
-    kind(num_q_heads, a.q, norm->q_weight, norm->q_weight_stride_h);
-    kind(num_k_heads, a.k, norm->k_weight, norm->k_weight_stride_h);
+    fit(num_q_heads, rq, norm->q_weight, norm->q_weight_stride_h);
+    fit(num_k_heads, rk, norm->k_weight, norm->k_weight_stride_h);
     a.r = row_units(head_dim, half, w.v);
-    const bool far = num_tokens * (num_q_heads + num_k_heads) * head_dim * esz >= (64 << 20);
-    const size_t turns = static_cast<size_t>(g.tile) * half * sizeof(float2);
-    const size_t sums = static_cast<size_t>(kNormThreads / 64) * head_dim * sizeof(float);
+    const int groups = 64 >> a.r.log_lanes;
+    auto kind = [&](const GradRows &r, const void *weight, int64_t ws, int heads, bool each, const GradGrid &g, int64_t first) {
+      int log_tg = 0;
+      if (!each)
+        while ((2 << log_tg) <= groups && (num_tokens >> (log_tg + 1)) >= 2 * static_cast<int64_t>(g.wgs) * kNormWaves) ++log_tg;
+      return GradKind{r, weight, ws, heads, each, heads == 0 ? 0 : each ? (heads + groups - 1) / groups : 1, g.wgs, log_tg, first};
+    };
+    a.q = kind(rq, norm->q_weight, norm->q_weight_stride_h, num_q_heads, q_each, gq, 0);
+    a.k = kind(rk, norm->k_weight, norm->k_weight_stride_h, num_k_heads, k_each, gk, static_cast<int64_t>(gq.wgs) * gq.rows);
+    const int64_t grid = static_cast<int64_t>(a.q.ranges) * a.q.wgs + static_cast<int64_t>(a.k.ranges) * a.k.wgs;
+    WKV_CHECK_ARG(grid <= INT32_MAX, "too many tokens and heads for one launch");
+    const bool far = num_tokens * H * head_dim * esz >= (64 << 20);
+    const int log_tg = a.q.log_tg > a.k.log_tg ? a.q.log_tg : a.k.log_tg;
+    const size_t turns = (static_cast<size_t>(kNormWaves) << log_tg) * half * sizeof(float2);
+    const size_t sums = static_cast<size_t>(kNormWaves) * (q_each || k_each ? groups : 1) * head_dim * sizeof(float);
     const size_t lds = turns > sums ? turns : sums;
     with_types(dtype, w.v, inter, [&](auto zero, auto v, auto in) {
-      launch_norm_grad<decltype(zero), decltype(v)::value, decltype(in)::value>(
-          a, far, static_cast<unsigned>(g.count()), lds, s);
+      launch_norm_grad<decltype(zero), decltype(v)::value, decltype(in)::value>(a, far, static_cast<unsigned>(grid), lds, s);
     });
     WKV_CHECK_LAUNCH("norm_rotary_backward");
   }
   if (dw) {
-    WeightGrads a{static_cast<const float *>(workspace), dq_weight, dk_weight, g.q_ranges,
-                  num_tokens > 0 ? g.q_wgs : 0, num_tokens > 0 ? g.k_wgs : 0, head_dim, norm->weight_dtype};
-    const dim3 grid(static_cast<unsigned>(g.q_ranges + g.k_ranges), static_cast<unsigned>((head_dim + 63) / 64));
+    WeightGrads a{static_cast<const float *>(workspace), dq_weight, dk_weight, num_q_heads > 0 ? gq.rows : 0,
+                  num_k_heads > 0 ? gk.rows : 0, gq.wgs, gk.wgs, head_dim, norm->weight_dtype};
+    const dim3 grid(static_cast<unsigned>(a.q_rows + a.k_rows), static_cast<unsigned>((head_dim + 63) / 64));
     norm_weight_grad_kernel<<<grid, 64 * kSumWaves, 0, s>>>(a);
     WKV_CHECK_LAUNCH("norm_weight_grad");
   }

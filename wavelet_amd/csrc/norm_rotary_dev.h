@@ -11,10 +11,15 @@
 // that holds its units, 64 at most: a unit is V pairs in two runs of V elements,
 // (V u, V u + half) or with adjacent pairs (V u, V (u + units)), so that a lane
 // moves 16 bytes at a time and both elements of a pair meet in one lane. The
-// sum of squares is a butterfly over the group.
+// sum of squares is a butterfly over the group. The groups of a wave take a few tokens and
+// walk their heads: a lane's token and unit stay the same, so that its
+// angles and weights are formed once, as the products that y is linear in x by,
+//   y_a = (x_a r) (w_a c) - (x_b r) (w_b s),  y_b = (x_b r) (w_b c) + (x_a r) (w_a s),
+// and a row costs some 7 instructions a value.
 #pragma once
 
 #include <cmath>
+#include <type_traits>
 
 #include "wkv_common.h"
 
@@ -30,12 +35,16 @@ struct Angles {
   float scale, sign;
 };
 
-// Cosine and sine of pair i at token t, times the scale. A pair of an axis that is not there stays.
-__device__ __forceinline__ float2 angle_at(const Angles &a, int64_t t, int i) {
-  const int ax = a.axes != nullptr ? a.axes[i] : 0;
-  double p = 0.;
-  if (static_cast<unsigned>(ax) < static_cast<unsigned>(a.num_axes)) p = static_cast<double>(a.pos[ax * a.axis_stride + t]);
-  const double x = p * a.inv_freq[i] * 0.15915494309189533577;  // 1 / 2 pi: the angle in turns
+// The position of pair i at token t. A pair of an axis that is not there stays (0).
+__device__ __forceinline__ int64_t position_at(const Angles &a, int64_t t, int i) {
+  if (a.axes == nullptr) return a.pos[t];  // uniform
+  const int ax = a.axes[i];
+  return static_cast<unsigned>(ax) < static_cast<unsigned>(a.num_axes) ? a.pos[ax * a.axis_stride + t] : 0;
+}
+
+// Cosine and sine of a position's angle, times the scale.
+__device__ __forceinline__ float2 angle_of(const Angles &a, int64_t pos, double freq) {
+  const double x = static_cast<double>(pos) * freq * 0.15915494309189533577;  // 1 / 2 pi: the angle in turns
   float s, c;
   sincospif(2.f * static_cast<float>(x - rint(x)), &s, &c);
   return make_float2(c * a.scale, s * a.scale * a.sign);
@@ -77,8 +86,10 @@ __device__ __forceinline__ void unit_runs(const RowUnits &a, int u, int &e0, int
   }
 }
 
-// The sum over a group of 2^log_lanes lanes, the same in each.
+// The sum over a group of 2^log_lanes lanes, the same in each. LL: log_lanes as a constant (-1: it is none).
+template <int LL = -1>
 __device__ __forceinline__ float group_sum(float v, int log_lanes) {
+  if (LL >= 0) log_lanes = LL;
   if (log_lanes > 0) v += lane_xor<1>(v);
   if (log_lanes > 1) v += lane_xor<2>(v);
   if (log_lanes > 2) v += lane_xor<4>(v);
@@ -122,77 +133,278 @@ __device__ __forceinline__ void load_weights(const HeadNorm &n, const void *w, i
   }
 }
 
-// A pair turned by (cos, sin).
-__device__ __forceinline__ void turn_pair(float2 cs, float &a, float &b) {
-  const float x = a, y = b;
-  a = __builtin_fmaf(x, cs.x, -(y * cs.y));
-  b = __builtin_fmaf(y, cs.x, x * cs.y);
-}
-
-// A unit's pairs turned: runs fa from element e0 on and fb from e1 on, turn[]
-// the angles of the row's token.
+// Pair p of a unit, as its elements of the runs x0 and x1.
 template <int V, bool INTER>
-__device__ __forceinline__ void turn_unit(const float2 *turn, int half, int e0, int e1, float *fa, float *fb) {
-  if (INTER && V > 1) {
+__device__ __forceinline__ float &pair_a(int p, float *x0, float *x1) {
+  return INTER && V > 1 ? (p < V / 2 ? x0[2 * p] : x1[2 * p - V]) : x0[p];
+}
+template <int V, bool INTER>
+__device__ __forceinline__ float &pair_b(int p, float *x0, float *x1) {
+  return INTER && V > 1 ? (p < V / 2 ? x0[2 * p + 1] : x1[2 * p - V + 1]) : x1[p];
+}
+
+// A unit's cosines and sines; pairs that are not turned: (1, 0), and their bits of `live` are clear.
+template <int V>
+struct UnitTurn {
+  float c[V], s[V];
+  uint32_t live;
+};
+
+template <int V, bool INTER>
+__device__ __forceinline__ void unit_turn(const float2 *turn, int half, bool all, int e0, int e1, UnitTurn<V> &t) {
+  auto pair = [&](int p) { return INTER && V > 1 ? (p < V / 2 ? e0 / 2 + p : e1 / 2 + p - V / 2) : INTER ? e0 / 2 : e0 + p; };
+  t.live = (1u << V) - 1u;
+  if (all) {  // uniform
 #pragma unroll
-    for (int v = 0; v < V; v += 2) {
-      if ((e0 + v) / 2 < half) turn_pair(turn[(e0 + v) / 2], fa[v], fa[v + 1]);
-      if ((e1 + v) / 2 < half) turn_pair(turn[(e1 + v) / 2], fb[v], fb[v + 1]);
+    for (int p = 0; p < V; ++p) {
+      const float2 cs = turn[pair(p)];
+      t.c[p] = cs.x;
+      t.s[p] = cs.y;
     }
-  } else {
-    const int p = INTER ? e0 / 2 : e0;
-    if (p < half) {
+    return;
+  }
 #pragma unroll
-      for (int v = 0; v < V; ++v) turn_pair(turn[p + v], fa[v], fb[v]);
-    }
+  for (int p = 0; p < V; ++p) {
+    const int i = pair(p);
+    const float2 cs = half > 0 ? turn[i < half ? i : half - 1] : make_float2(1.f, 0.f);
+    t.c[p] = i < half ? cs.x : 1.f;
+    t.s[p] = i < half ? cs.y : 0.f;
+    if (i >= half) t.live &= ~(1u << p);
   }
 }
 
-// A tile's angles, by the whole workgroup of `threads`; a barrier follows before they are read.
-__device__ __forceinline__ void tile_angles(const Angles &a, int64_t t0, int nt, int threads, float2 *turn) {
-  for (int i = threadIdx.x; i < nt * a.half.d; i += threads) {
-    const int t = i / a.half;
-    turn[i] = angle_at(a, t0 + t, i - t * a.half.d);
+// The products of a unit's weights, cosines and sines.
+template <int V>
+struct UnitCoef {
+  float ac[V], bs[V], bc[V], as[V];
+};
+
+template <int V, bool INTER>
+__device__ __forceinline__ void unit_coef(const UnitTurn<V> &t, float *w0, float *w1, UnitCoef<V> &k) {
+#pragma unroll
+  for (int p = 0; p < V; ++p) {
+    const float a = pair_a<V, INTER>(p, w0, w1), b = pair_b<V, INTER>(p, w0, w1);
+    k.ac[p] = a * t.c[p];
+    k.bs[p] = b * t.s[p];
+    k.bc[p] = b * t.c[p];
+    k.as[p] = a * t.s[p];
   }
 }
 
-// Rows of a tile of nt tokens, heads h0 .. h0 + heads.d - 1 of each, by a workgroup
-// of `threads`: normed (if norm.on), turned by turn[], stored. N rows of a group of lanes in
-// flight. src(t, h): where a row lies (nullptr: skipped); dst(t, h, e, v): stores its elements from e on.
-template <class T, int V, bool INTER, int U, int N, bool FAR, class Src, class Dst>
-__device__ __forceinline__ void norm_turn_rows(const RowUnits &ru, const HeadNorm &norm, int Hq, const float2 *turn,
-                                               int nt, const FastDiv &heads, int h0, int threads, Src src, Dst dst) {
+// A unit of x times inv, normed and turned in place. all: every pair is turned (else an infinity's pair would
+// take it in as a NaN).
+template <int V, bool INTER>
+__device__ __forceinline__ void unit_apply(const UnitCoef<V> &k, uint32_t live, bool all, float inv, float *x0, float *x1) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    x0[v] *= inv;
+    x1[v] *= inv;
+  }
+  auto turn = [&](auto whole) __attribute__((always_inline)) {
+#pragma unroll
+    for (int p = 0; p < V; ++p) {
+      float &a = pair_a<V, INTER>(p, x0, x1), &b = pair_b<V, INTER>(p, x0, x1);
+      float t = b * k.bs[p], u = a * k.as[p];
+      if (!decltype(whole)::value && !(live >> p & 1)) t = u = 0.f;
+      a = __builtin_fmaf(a, k.ac[p], -t);
+      b = __builtin_fmaf(b, k.bc[p], u);
+    }
+  };
+  if (all)
+    turn(std::true_type{});
+  else
+    turn(std::false_type{});
+}
+
+// unit_turn, unit_coef and unit_apply of one row, pair by pair: the same values from fewer registers.
+template <int V, bool INTER>
+__device__ __forceinline__ void unit_once(const float2 *turn, int half, bool all, int e0, int e1, const float *w0, const float *w1,
+                                          float inv, float *x0, float *x1) {
+  auto pair = [&](int p) { return INTER && V > 1 ? (p < V / 2 ? e0 / 2 + p : e1 / 2 + p - V / 2) : INTER ? e0 / 2 : e0 + p; };
+#pragma unroll
+  for (int p = 0; p < V; ++p) {
+    const int i = pair(p);
+    float2 cs = make_float2(1.f, 0.f);
+    if (half > 0) cs = turn[all || i < half ? i : 0];
+    const bool live = all || i < half;
+    if (!live) cs = make_float2(1.f, 0.f);
+    float &a = pair_a<V, INTER>(p, x0, x1), &b = pair_b<V, INTER>(p, x0, x1);
+    const float wa = pair_a<V, INTER>(p, const_cast<float *>(w0), const_cast<float *>(w1));
+    const float wb = pair_b<V, INTER>(p, const_cast<float *>(w0), const_cast<float *>(w1));
+    const float xa = a * inv, xb = b * inv;
+    float t = xb * (wb * cs.y), u = xa * (wa * cs.y);
+    if (!live) t = u = 0.f;
+    a = __builtin_fmaf(xa, wa * cs.x, -t);
+    b = __builtin_fmaf(xb, wb * cs.x, u);
+  }
+}
+
+// A unit turned alone, without weights (a gradient's, by the transpose's angles).
+template <int V, bool INTER>
+__device__ __forceinline__ void unit_back(const UnitTurn<V> &t, bool all, float *x0, float *x1) {
+  auto turn = [&](auto whole) __attribute__((always_inline)) {
+#pragma unroll
+    for (int p = 0; p < V; ++p) {
+      float &a = pair_a<V, INTER>(p, x0, x1), &b = pair_b<V, INTER>(p, x0, x1);
+      float u = b * t.s[p], v = a * t.s[p];
+      if (!decltype(whole)::value && !(t.live >> p & 1)) u = v = 0.f;
+      a = __builtin_fmaf(a, t.c[p], -u);
+      b = __builtin_fmaf(b, t.c[p], v);
+    }
+  };
+  if (all)
+    turn(std::true_type{});
+  else
+    turn(std::false_type{});
+}
+
+// The angles of tokens t0 .. t0 + nt - 1, thread `tid` of `threads`, while there are as many B at a time: their positions and frequencies
+// are all requested before the first is used.
+template <int B>
+__device__ __forceinline__ void angles_of(const Angles &a, int64_t t0, int nt, int tid, int threads, float2 *turn) {
+  const int n = nt * a.half.d;
+  int i = tid;
+  if constexpr (B > 1) {
+    for (; i - tid + B * threads <= n; i += B * threads) {  // uniform
+      int64_t pos[B];
+      double freq[B];
+#pragma unroll
+      for (int k = 0; k < B; ++k) {
+        const int t = (i + threads * k) / a.half, p = i + threads * k - t * a.half.d;
+        pos[k] = position_at(a, t0 + t, p);
+        freq[k] = a.inv_freq[p];
+      }
+#pragma unroll
+      for (int k = 0; k < B; ++k) turn[i + threads * k] = angle_of(a, pos[k], freq[k]);
+    }
+  }
+  for (; i < n; i += threads) {
+    const int t = i / a.half, p = i - t * a.half.d;
+    turn[i] = angle_of(a, position_at(a, t0 + t, p), a.inv_freq[p]);
+  }
+}
+
+// The same by one wave, for its own reads.
+template <int B = 1>
+__device__ __forceinline__ void wave_angles(const Angles &a, int64_t t0, int nt, float2 *turn) {
+  angles_of<B>(a, t0, nt, threadIdx.x & 63, 64, turn);
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// A kind of heads of one token, as a lane sees them.
+template <class T>
+struct HeadsOf {
+  const T *x;      // head 0 (of those that the wave takes)
+  int64_t xh;      // elements between heads
+  T *y;
+  int64_t yh;
+  int piece;       // 0: y is a row; else element e is at (e / 8) piece + e % 8 (a cache's keys)
+  const void *w;   // the weights of head 0 (nullptr: ones)
+  int64_t ws;      // between heads; not 0: each head has its own
+};
+
+// A kind of heads in a launch.
+struct Kind {
+  HeadRows s;
+  const void *w;
+  int64_t ws;
+  int heads;
+  int log_tg, per;  // KindGrid
+  FastDiv splits;
+};
+
+// Which tokens and heads wave `wave` of workgroup wg of a kind takes, and where its lane stands.
+struct WaveTile {
+  int64_t t0;        // the wave's first token
+  int tokens;        // of it; 0: none
+  int h0, heads;     // its heads
+  int t, group;      // the lane's token of them, its group's number among the token's
+  bool there;        // there is such a token
+};
+
+__device__ __forceinline__ WaveTile wave_tile(const Kind &k, const RowUnits &r, int64_t tokens, int wg, int wave) {
+  WaveTile w;
+  const int x = wg / k.splits, split = wg - x * k.splits.d, tg = 1 << k.log_tg;
+  w.t0 = (static_cast<int64_t>(x) * 4 + wave) << k.log_tg;
+  w.tokens = w.t0 >= tokens ? 0 : tokens - w.t0 < tg ? static_cast<int>(tokens - w.t0) : tg;
+  w.h0 = split * k.per;
+  w.heads = k.heads - w.h0 < k.per ? k.heads - w.h0 : k.per;
+  const int g = (threadIdx.x & 63) >> r.log_lanes;
+  w.t = g & (tg - 1);
+  w.group = g >> k.log_tg;
+  w.there = w.t < w.tokens;
+  if (!w.there) w.t = 0;
+  return w;
+}
+
+// The heads first, first + step, .. below `heads` of the lane's token (there: it has one), normed (if norm.on) and turned by
+// turn[], N rows at a time, the next N in flight meanwhile; ready(): called once the first are, before turn[] is read.
+// EACH: each head's own weights.
+template <class T, int V, bool INTER, int U, int N, bool FAR, bool NEAR_STORE, bool EACH, int LL, class Ready>
+__device__ __forceinline__ void norm_turn_heads(const RowUnits &ru, const HeadNorm &norm, const float2 *turn, bool there,
+                                                int first, int step, int heads, const HeadsOf<T> &of, Ready ready) {
   typedef typename VecOf<T, V>::type Vec;
-  const int lanes = 1 << ru.log_lanes, group = threadIdx.x >> ru.log_lanes, u0 = threadIdx.x & (lanes - 1);
-  const int groups = threads >> ru.log_lanes, rows = nt * heads.d;
+  const int lanes = 1 << (LL >= 0 ? LL : ru.log_lanes), u0 = threadIdx.x & (lanes - 1);
   const float inv_d = 1.f / static_cast<float>(ru.D);
-  for (int r0 = 0; r0 < rows; r0 += groups * N) {
-    Vec x0[N][U], x1[N][U];
-    const T *x[N];
+  const bool all = 2 * ru.half == ru.D;
+  int e0[U], e1[U];
+  bool mine[U];
+#pragma unroll
+  for (int j = 0; j < U; ++j) {
+    const int u = u0 + lanes * j;
+    mine[j] = there && u < ru.units;
+    e0[j] = e1[j] = 0;
+    if (u < ru.units) unit_runs<V, INTER>(ru, u, e0[j], e1[j]);
+  }
+  Vec n0[N][U], n1[N][U];
+  auto load = [&](int h0) __attribute__((always_inline)) {
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const int r = r0 + groups * k + group;
-      const int t = r / heads, h = h0 + r - t * heads.d;
-      x[k] = r < rows ? src(t, h) : nullptr;
+      const int h = h0 + step * k;
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const int u = u0 + lanes * j;
-        if (x[k] != nullptr && u < ru.units) {
-          int e0, e1;
-          unit_runs<V, INTER>(ru, u, e0, e1);
-          const Vec *p0 = reinterpret_cast<const Vec *>(x[k] + e0), *p1 = reinterpret_cast<const Vec *>(x[k] + e1);
-          x0[k][j] = FAR ? __builtin_nontemporal_load(p0) : *p0;
-          x1[k][j] = FAR ? __builtin_nontemporal_load(p1) : *p1;
-        } else {
-          x0[k][j] = Vec{};
-          x1[k][j] = Vec{};
+        n0[k][j] = n1[k][j] = Vec{};
+        if (mine[j] && h < heads) {
+          const Vec *p0 = reinterpret_cast<const Vec *>(of.x + h * of.xh + e0[j]);
+          const Vec *p1 = reinterpret_cast<const Vec *>(of.x + h * of.xh + e1[j]);
+          n0[k][j] = FAR ? __builtin_nontemporal_load(p0) : *p0;
+          n1[k][j] = FAR ? __builtin_nontemporal_load(p1) : *p1;
         }
       }
     }
+  };
+  load(first);
+  float w0[U][V], w1[U][V];
+  if (!EACH) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      load_weights<T, V>(norm, of.w, e0[j], w0[j]);
+      load_weights<T, V>(norm, of.w, e1[j], w1[j]);
+    }
+  }
+  ready();
+  UnitTurn<V> t[U];
+  UnitCoef<V> coef[U];
+#pragma unroll
+  for (int j = 0; j < U; ++j) {
+    unit_turn<V, INTER>(turn, ru.half, all, e0[j], e1[j], t[j]);
+    if (!EACH) unit_coef<V, INTER>(t[j], w0[j], w1[j], coef[j]);
+  }
+  for (int hb = 0; hb < heads; hb += step * N) {  // uniform; the lane's rows are hb + first, + step, ..
+    Vec x0[N][U], x1[N][U];
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        x0[k][j] = n0[k][j];
+        x1[k][j] = n1[k][j];
+      }
+    if (hb + step * N < heads) load(hb + step * N + first);
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const int r = r0 + groups * k + group;
-      const int t = r / heads, h = h0 + r - t * heads.d;
+      const int h = hb + first + step * k;
       float f0[U][V], f1[U][V], ss = 0.f;
 #pragma unroll
       for (int j = 0; j < U; ++j) {
@@ -201,34 +413,35 @@ __device__ __forceinline__ void norm_turn_rows(const RowUnits &ru, const HeadNor
 #pragma unroll
         for (int v = 0; v < V; ++v) ss = __builtin_fmaf(f0[j][v], f0[j][v], __builtin_fmaf(f1[j][v], f1[j][v], ss));
       }
-      ss = group_sum(ss, ru.log_lanes);
-      const float inv = norm.on ? rsqrtf(__builtin_fmaf(ss, inv_d, norm.eps)) : 1.f;
-      if (x[k] == nullptr) continue;
-      const void *w = h < Hq ? norm.qw : norm.kw;
-      const int64_t wh = h < Hq ? h * norm.qws : (h - Hq) * norm.kws;
+      ss = group_sum<LL>(ss, ru.log_lanes);
+      const float inv = norm.on ? __builtin_amdgcn_rsqf(__builtin_fmaf(ss, inv_d, norm.eps)) : 1.f;
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const int u = u0 + lanes * j;
-        if (u >= ru.units) continue;
-        int e0, e1;
-        unit_runs<V, INTER>(ru, u, e0, e1);
-        float w0[V], w1[V];
-        load_weights<T, V>(norm, w, wh + e0, w0);
-        load_weights<T, V>(norm, w, wh + e1, w1);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          f0[j][v] *= inv * w0[v];
-          f1[j][v] *= inv * w1[v];
+        if (EACH) {
+          const int64_t wh = h < heads ? h * of.ws : 0;
+          load_weights<T, V>(norm, of.w, wh + e0[j], w0[j]);
+          load_weights<T, V>(norm, of.w, wh + e1[j], w1[j]);
+          unit_coef<V, INTER>(t[j], w0[j], w1[j], coef[j]);
         }
-        turn_unit<V, INTER>(turn + t * ru.half, ru.half, e0, e1, f0[j], f1[j]);
-        Vec o0, o1;
+        unit_apply<V, INTER>(coef[j], t[j].live, all, inv, f0[j], f1[j]);
+        if (mine[j] && h < heads) {
+          Vec o0, o1;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          o0[v] = static_cast<T>(f0[j][v]);
-          o1[v] = static_cast<T>(f1[j][v]);
+          for (int v = 0; v < V; ++v) {
+            o0[v] = static_cast<T>(f0[j][v]);
+            o1[v] = static_cast<T>(f1[j][v]);
+          }
+          T *y = of.y + h * of.yh;
+          const int i0 = of.piece == 0 ? e0[j] : (e0[j] >> 3) * of.piece + (e0[j] & 7);
+          const int i1 = of.piece == 0 ? e1[j] : (e1[j] >> 3) * of.piece + (e1[j] & 7);
+          if (FAR && !NEAR_STORE) {
+            __builtin_nontemporal_store(o0, reinterpret_cast<Vec *>(y + i0));
+            __builtin_nontemporal_store(o1, reinterpret_cast<Vec *>(y + i1));
+          } else {
+            *reinterpret_cast<Vec *>(y + i0) = o0;
+            *reinterpret_cast<Vec *>(y + i1) = o1;
+          }
         }
-        dst(t, h, e0, o0);
-        dst(t, h, e1, o1);
       }
     }
   }
@@ -285,6 +498,26 @@ inline RowUnits row_units(int D, int half, int v) {
   while (r.log_lanes < 6 && (1 << r.log_lanes) < r.units) ++r.log_lanes;
   return r;
 }
+
+// Waves over the tokens and heads of a kind, four a workgroup: a token a wave (its heads lie together; by_token: as many as
+// the wave's groups, whose stores of one head then lie together in a cache), and with too few tokens for the chip the heads
+// dealt over more waves, down to a round of the wave's groups.
+struct KindGrid {
+  int log_tg = 0, per = 1, splits = 1;
+  int64_t waves = 0, wgs = 0;
+  KindGrid(int64_t tokens, int heads, int log_lanes, bool by_token) {
+    if (tokens <= 0 || heads <= 0) return;
+    const int log_groups = 6 - log_lanes;
+    while (by_token && log_tg < log_groups && (tokens >> (log_tg + 1)) * heads >= 4096) ++log_tg;
+    waves = ((tokens - 1) >> log_tg) + 1;
+    const int step = (1 << log_groups) >> log_tg, rounds = (heads + step - 1) / step;
+    const int64_t want = (4096 + waves - 1) / waves;
+    const int n = static_cast<int>(want < rounds ? want : rounds);
+    per = (rounds + n - 1) / n * step;
+    splits = (heads + per - 1) / per;
+    wgs = (waves + 3) / 4 * splits;
+  }
+};
 
 // The elements of an access: 16 bytes of them, else two, else one, as the layout and every operand allow.
 struct Widths {

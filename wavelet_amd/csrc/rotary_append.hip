@@ -2,10 +2,9 @@
 // positions on the way, and the queries to the attention, in one launch (gfx950).
 // The mathematics of heads: norm_rotary_dev.h; the fp8 rule: kv_append_dev.h.
 //
-// The workgroups of a launch have one of two roles. Rows: a tile of tokens, its angles in
-// LDS, and the heads that are stored as rows: queries, the keys of a bf16 cache, whose
-// 16-byte runs are the cache's own pieces, and the shared key of a latent
-// cache. The rest: values (bf16: a window of 64 tokens of one head, transposed through LDS; few
+// The workgroups of a launch have one of three roles. Queries, and the shared key of a latent cache: rows to rows.
+// Keys of a bf16 cache: a wave's tokens follow each other, so that the
+// 16-byte pieces that it stores of a head lie together in the cache. The rest: values (bf16: a window of 64 tokens of one head, transposed through LDS; few
 // tokens: an element at a time), keys and values (fp8, run by run, because a block's scale follows from all of
 // its new keys: a wave norms and turns 16 of them into LDS and codes them from there),
 // or a latent cache's compressed entries, normed.
@@ -18,66 +17,70 @@ namespace wkv {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 
+// A cache's slots as blocks and offsets.
+struct Slots {
+  const int64_t *of;  // each token's
+  int64_t count;      // slots of the cache
+  FastDiv block;
+  // Whether there is such a slot. Caches of 2^31 slots and more divide in 64 bits.
+  __device__ __forceinline__ bool at(int64_t token, int64_t &blk, int &off) const {
+    const int64_t slot = of[token];
+    const bool there = slot >= 0 && slot < count;
+    if (count <= INT32_MAX) {  // uniform
+      const int s = there ? static_cast<int>(slot) : 0, b = s / block;
+      blk = b;
+      off = s - b * block.d;
+    } else {
+      blk = there ? slot / block.d : 0;
+      off = there ? static_cast<int>(slot - blk * block.d) : 0;
+    }
+    return there;
+  }
+};
+
 struct AppendArgs {
-  HeadRows q;  // y: the queries' result
+  Kind q, k;       // q.s.y: the queries' result; k.s.x: the keys
+  int k_wgs, v_wgs;  // workgroups of keys, and of values; queries behind them
   const uint16_t *key, *val;
   int64_t kst, ksh, vst, vsh;
-  const int64_t *slots;
+  Slots slots;
   HeadNorm n;
   Angles a;
   RowUnits r;
   int64_t tokens;
-  int Hq, Hk;
+  int Hk;
   void *kc, *vc;
   float *ks, *vs;
   int BS;
-  int64_t NB;
-  int rows;           // heads of the rows role: queries, and a bf16 cache's keys
-  int tile;           // its tokens of a workgroup
-  FastDiv per, last;  // its heads of a workgroup; of a token's last one
-  FastDiv splits;     // its workgroups of a tile
-  int64_t row_wgs;    // all of them
-  int window;         // tokens of a workgroup of the other role
+  int window;  // tokens of a workgroup of the last role
 };
 
-__device__ __forceinline__ bool block_of(int64_t slot, int BS, int64_t NB, int64_t &blk, int &off) {
-  blk = slot / BS;
-  off = static_cast<int>(slot - blk * BS);
-  return slot >= 0 && blk < NB;
-}
-
-template <int V, bool INTER, bool PAGED_K>
-__device__ __forceinline__ void rows_role(const AppendArgs &a, int64_t wg, float2 *turn) {
-  typedef typename VecOf<__bf16, V>::type Vec;
-  const int64_t tile = wg / a.splits.d;
-  const int split = static_cast<int>(wg - tile * a.splits.d);
-  const int64_t t0 = tile * a.tile;
-  const int nt = a.tokens - t0 < a.tile ? static_cast<int>(a.tokens - t0) : a.tile;
-  tile_angles(a.a, t0, nt, kThreads, turn);
-  __syncthreads();
-  norm_turn_rows<__bf16, V, INTER, 1, 2, false>(
-      a.r, a.n, a.Hq, turn, nt, split + 1 == a.splits.d ? a.last : a.per, split * a.per.d, kThreads,
-      [&](int t, int h) {
-        if (PAGED_K && h >= a.Hq) {
-          int64_t blk;
-          int off;
-          if (!block_of(a.slots[t0 + t], a.BS, a.NB, blk, off)) return static_cast<const __bf16 *>(nullptr);
-          return reinterpret_cast<const __bf16 *>(a.key) + (t0 + t) * a.kst + (h - a.Hq) * a.ksh;
-        }
-        return static_cast<const __bf16 *>(a.q.x) + (t0 + t) * a.q.xt + h * a.q.xh;
-      },
-      [&](int t, int h, int e, Vec v) {
-        __bf16 *y;
-        if (PAGED_K && h >= a.Hq) {
-          int64_t blk;
-          int off;
-          block_of(a.slots[t0 + t], a.BS, a.NB, blk, off);
-          y = static_cast<__bf16 *>(a.kc) + (((blk * a.Hk + h - a.Hq) * (a.r.D / 8) + (e >> 3)) * a.BS + off) * 8 + (e & 7);
-        } else {
-          y = static_cast<__bf16 *>(a.q.y) + (t0 + t) * a.q.yt + h * a.q.yh + e;
-        }
-        *reinterpret_cast<Vec *>(y) = v;
-      });
+// Queries to rows (K false), or keys to a bf16 cache.
+template <int V, bool INTER, bool EACH, bool K, int LL, bool FAR>
+__device__ __forceinline__ void heads_role(const AppendArgs &a, const Kind &k, int wg, float2 *turns) {
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const WaveTile w = wave_tile(k, a.r, a.tokens, wg, wave);
+  if (w.tokens == 0) return;  // a whole wave; nothing below waits for another
+  float2 *turn = turns + (wave << k.log_tg) * a.r.half;
+  const void *weight = k.w;
+  if (EACH && weight != nullptr) weight = static_cast<const char *>(weight) + w.h0 * k.ws * (a.n.wide ? 4 : 2);
+  const int64_t t = w.t0 + w.t;
+  HeadsOf<__bf16> of{static_cast<const __bf16 *>(k.s.x) + t * k.s.xt + w.h0 * k.s.xh, k.s.xh, nullptr, 0, 0, weight, k.ws};
+  bool there = w.there;
+  if (K) {
+    int64_t blk;
+    int off;
+    there = a.slots.at(t, blk, off) && there;
+    of.yh = static_cast<int64_t>(a.r.D) * a.BS;
+    of.y = static_cast<__bf16 *>(a.kc) + (blk * a.Hk + w.h0) * of.yh + off * 8;  // (not used where there is no such block)
+    of.piece = a.BS * 8;
+  } else {
+    of.y = static_cast<__bf16 *>(k.s.y) + t * k.s.yt + w.h0 * k.s.yh;
+    of.yh = k.s.yh;
+  }
+  norm_turn_heads<__bf16, V, INTER, 1, 1, FAR, K, EACH, LL>(
+      a.r, a.n, turn + w.t * a.r.half, there, w.group, (64 >> a.r.log_lanes) >> k.log_tg, w.heads, of,
+      [&] { wave_angles<K ? 2 : 1>(a.a, w.t0, w.tokens, turn); });
 }
 
 // ---------------------------------------------------------------------------
@@ -86,11 +89,11 @@ constexpr int kValueWindow = 64;
 constexpr int64_t kValueWindowTokens = 256;  // below this the values go element by element, over more workgroups
 
 template <int D>
-__device__ __forceinline__ void values_role(const AppendArgs &a, int64_t wg, uint8_t *lds) {
+__device__ __forceinline__ void values_role(const AppendArgs &a, int wg, uint8_t *lds) {
   constexpr int C = D / 8;
   uint16_t *vc = static_cast<uint16_t *>(a.vc);
   if (a.window == 1) {  // an item a thread: 8 elements of a token's head
-    const int64_t i = wg * kThreads + threadIdx.x;
+    const int64_t i = static_cast<int64_t>(wg) * kThreads + threadIdx.x;
     if (i >= a.tokens * a.Hk * C) return;
     const int c = static_cast<int>(i % C);
     const int64_t th = i / C;
@@ -98,7 +101,7 @@ __device__ __forceinline__ void values_role(const AppendArgs &a, int64_t wg, uin
     const int64_t t = th / a.Hk;
     int64_t blk;
     int off;
-    if (!block_of(a.slots[t], a.BS, a.NB, blk, off)) return;
+    if (!a.slots.at(t, blk, off)) return;
     const u32x4 v = *reinterpret_cast<const u32x4 *>(a.val + t * a.vst + h * a.vsh + c * 8);
     uint16_t *y = vc + ((blk * a.Hk + h) * D + c * 8) * a.BS + off;
 #pragma unroll
@@ -109,9 +112,10 @@ __device__ __forceinline__ void values_role(const AppendArgs &a, int64_t wg, uin
   // start 8-aligned in a block is stored 16 bytes of a d row at a time, another token by token.
   constexpr int RP = D * 2 + 8;  // pitch of a token's row in LDS
   constexpr int NG = kValueWindow / 8;
-  int64_t *gslot = reinterpret_cast<int64_t *>(lds + kValueWindow * RP);
-  const int64_t w = wg / a.Hk, t0 = w * kValueWindow;
-  const int h = static_cast<int>(wg - w * a.Hk), tid = threadIdx.x;
+  int64_t *place = reinterpret_cast<int64_t *>(lds + kValueWindow * RP);  // of a token's first value in the cache, -1: none
+  int *whole = reinterpret_cast<int *>(place + kValueWindow);             // groups that are one run
+  const int w = wg / a.Hk, h = wg - w * a.Hk, tid = threadIdx.x;
+  const int64_t t0 = static_cast<int64_t>(w) * kValueWindow;
 #pragma unroll
   for (int k = 0; k < kValueWindow * C / kThreads; ++k) {
     const int t = tid / C + k * (kThreads / C), c = tid % C;
@@ -122,27 +126,25 @@ __device__ __forceinline__ void values_role(const AppendArgs &a, int64_t wg, uin
       for (int j = 0; j < 4; ++j) l[j] = v[j];
     }
   }
-  if (tid < NG) {
-    const int64_t ta = t0 + 8 * tid;
-    int64_t first = -1;
-    if (ta + 7 < a.tokens) {
-      int64_t s[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] = a.slots[ta + j];
-      bool run = s[0] >= 0 && s[0] / a.BS < a.NB && (s[0] % a.BS) % 8 == 0;
-#pragma unroll
-      for (int j = 1; j < 8; ++j) run = run && s[j] == s[0] + j;
-      if (run) first = s[0];
+  if (tid < kValueWindow) {  // wave 0
+    int64_t blk = 0, slot = -1;
+    int off = 0;
+    bool there = false;
+    if (t0 + tid < a.tokens) {
+      slot = a.slots.of[t0 + tid];
+      there = a.slots.at(t0 + tid, blk, off);
     }
-    gslot[tid] = first;
+    place[tid] = there ? (blk * a.Hk + h) * D * a.BS + off : -1;
+    const int64_t first = __shfl(slot, tid & ~7, 64);
+    const uint64_t runs = __ballot(there && first % 8 == 0 && slot == first + (tid & 7));  // (blocks are multiples of 16)
+    if ((tid & 7) == 0) whole[tid / 8] = ((runs >> tid) & 0xffu) == 0xffu;
   }
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < NG * D / kThreads; ++k) {
     const int i = tid + kThreads * k;
     const int g = 2 * (i / (2 * D)) + (i & 1), d = (i >> 1) % D;
-    const int64_t first = gslot[g];
-    if (first >= 0) {
+    if (whole[g]) {
       uint32_t o[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -150,16 +152,11 @@ __device__ __forceinline__ void values_role(const AppendArgs &a, int64_t wg, uin
         const uint32_t hi = *reinterpret_cast<const uint16_t *>(lds + (8 * g + 2 * j + 1) * RP + 2 * d);
         o[j] = lo | (hi << 16);
       }
-      const int64_t blk = first / a.BS;
-      *reinterpret_cast<u32x4 *>(vc + ((blk * a.Hk + h) * D + d) * a.BS + (first - blk * a.BS)) = u32x4{o[0], o[1], o[2], o[3]};
+      *reinterpret_cast<u32x4 *>(vc + place[8 * g] + static_cast<int64_t>(d) * a.BS) = u32x4{o[0], o[1], o[2], o[3]};
     } else {
       for (int j = 0; j < 8; ++j) {
         const int t = 8 * g + j;
-        if (t0 + t >= a.tokens) break;
-        int64_t blk;
-        int off;
-        if (!block_of(a.slots[t0 + t], a.BS, a.NB, blk, off)) continue;
-        vc[((blk * a.Hk + h) * D + d) * a.BS + off] = *reinterpret_cast<const uint16_t *>(lds + t * RP + 2 * d);
+        if (place[t] >= 0) vc[place[t] + static_cast<int64_t>(d) * a.BS] = *reinterpret_cast<const uint16_t *>(lds + t * RP + 2 * d);
       }
     }
   }
@@ -169,160 +166,231 @@ __device__ __forceinline__ void values_role(const AppendArgs &a, int64_t wg, uin
 // fp8 keys and values.
 constexpr int kPiece = 16;  // tokens of a run taken at a time
 
-template <int D>
-constexpr int kKeyPitch = D + 8;  // of a key in LDS, in elements
-
-// Piece p0 of a run (tokens t + p0 ..): its n keys of head h normed and turned into the wave's rows of LDS.
-template <int D, int V, bool INTER>
-__device__ __forceinline__ void stage_keys(const AppendArgs &a, const float2 *turn, int64_t t, int n, int h,
-                                           uint16_t *rows) {
-  typedef typename VecOf<__bf16, V>::type Vec;
-  const int lane = threadIdx.x & 63, lanes = 1 << a.r.log_lanes, group = lane >> a.r.log_lanes, u = lane & (lanes - 1);
-  const int groups = 64 >> a.r.log_lanes;
-  int e0 = 0, e1 = 0;
-  if (u < a.r.units) unit_runs<V, INTER>(a.r, u, e0, e1);
-  float w0[V], w1[V];
-  load_weights<__bf16, V>(a.n, a.n.kw, h * a.n.kws + e0, w0);
-  load_weights<__bf16, V>(a.n, a.n.kw, h * a.n.kws + e1, w1);
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the rows of the piece before have been read
-  __builtin_amdgcn_wave_barrier();
-  for (int i0 = 0; i0 < n; i0 += groups) {  // uniform
-    const int i = i0 + group;
-    const bool in = i < n && u < a.r.units;
-    float f0[V], f1[V], ss = 0.f;
-    Vec x0 = Vec{}, x1 = Vec{};
-    if (in) {
-      const __bf16 *x = reinterpret_cast<const __bf16 *>(a.key) + (t + i) * a.kst + h * a.ksh;
-      x0 = *reinterpret_cast<const Vec *>(x + e0);
-      x1 = *reinterpret_cast<const Vec *>(x + e1);
-    }
-    widen<V, __bf16>(x0, f0);
-    widen<V, __bf16>(x1, f1);
+// Codes of bf16 bits times inv, by the hardware's conversion; a NaN, which that codes with a sign of its own, as 0x7f and the
+// NaN's sign.
+struct Coder {
+  float inv;
+  bool any_nan;
+  __device__ __forceinline__ u32x2 eight(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) const {
+    u32x2 c = e4m3_pack8(w0, w1, w2, w3, inv);
+    if (any_nan) {  // uniform
+      const uint32_t w[4] = {w0, w1, w2, w3};
 #pragma unroll
-    for (int v = 0; v < V; ++v) ss = __builtin_fmaf(f0[v], f0[v], __builtin_fmaf(f1[v], f1[v], ss));
-    ss = group_sum(ss, a.r.log_lanes);
-    if (!in) continue;
-    const float inv = a.n.on ? rsqrtf(__builtin_fmaf(ss, 1.f / static_cast<float>(D), a.n.eps)) : 1.f;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      f0[v] *= inv * w0[v];
-      f1[v] *= inv * w1[v];
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t b = (w[i >> 1] >> (16 * (i & 1))) & 0xffffu, at = 8 * (i & 3);
+        if ((b & 0x7fffu) > 0x7f80u) c[i >> 2] = (c[i >> 2] & ~(0xffu << at)) | ((0x7fu | (b >> 8 & 0x80u)) << at);
+      }
     }
-    turn_unit<V, INTER>(turn + i * a.r.half, a.r.half, e0, e1, f0, f1);
-    Vec o0, o1;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      o0[v] = static_cast<__bf16>(f0[v]);
-      o1[v] = static_cast<__bf16>(f1[v]);
-    }
-    *reinterpret_cast<Vec *>(rows + i * kKeyPitch<D> + e0) = o0;
-    *reinterpret_cast<Vec *>(rows + i * kKeyPitch<D> + e1) = o1;
+    return c;
   }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
+  __device__ __forceinline__ uint32_t one(uint32_t bits) const { return eight(bits, 0u, 0u, 0u)[0] & 0xffu; }
+};
+
+// The largest magnitude of bf16 pairs, as bits: the two halves side by side; a NaN's are above infinity's.
+struct Largest {
+  typedef __attribute__((__vector_size__(4))) uint16_t u16x2;
+  u16x2 top = {0, 0};
+  __device__ __forceinline__ void pair(uint32_t w) {
+    const u16x2 x = __builtin_bit_cast(u16x2, w & 0x7fff7fffu);
+    top = __builtin_elementwise_max(top, x);
+  }
+  __device__ __forceinline__ uint32_t of_lane() const { return max(static_cast<uint32_t>(top[0]), static_cast<uint32_t>(top[1])); }
+};
+
+// 1 / s of a run's scale, a power of two in [2^-42, 2^120].
+__device__ __forceinline__ float pow2_inverse(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
+
+__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
+  return wave_reduce(v, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
 }
 
-// A run of r tokens from t on (block blk, the first at offset `first`): the wave's head h, as
-// fp8_append_run_kv appends it, its keys from LDS. Every wave of the workgroup calls it (the
-// pieces' angles are the workgroup's); active: the wave has a head.
-template <int D, int V, bool INTER>
-__device__ __forceinline__ void append_run(const AppendArgs &a, float2 *turn, uint16_t *rows, int64_t t, int r,
-                                           int64_t blk, int first, int h, bool active) {
-  constexpr int NC = D / 64, RV = D / 64;
-  uint8_t *kc = static_cast<uint8_t *>(a.kc), *vc = static_cast<uint8_t *>(a.vc);
-  const int lane = threadIdx.x & 63, m = lane & 15, H = a.Hk, BS = a.BS;
-  const int64_t si = blk * H + h;
-  float sk_old = 0.f, sv_old = 0.f;
-  if (active && first != 0) {
-    sk_old = a.ks[si];
-    sv_old = a.vs[si];
+// A pair's larger magnitude where a NaN counts as none.
+__device__ __forceinline__ uint32_t without_nan(uint32_t w) {
+  const uint32_t lo = w & 0x7fffu, hi = (w >> 16) & 0x7fffu;
+  return max(lo > 0x7f80u ? 0u : lo, hi > 0x7f80u ? 0u : hi);
+}
+
+// A run's scale: its own, or where it does not begin the block the block's, grown if it is smaller, what the block
+// held before coded again. The wave stores it.
+template <int D, bool IS_V>
+__device__ __forceinline__ float run_scale(uint8_t *codes, float *scales, int64_t blk, int h, int H, int BS, int first,
+                                           float old, float amax) {
+  float s = pow2_scale(amax);
+  if (first != 0) {
+    if (s > old)
+      fp8_reencode_block<D, IS_V, true>(codes, blk, h, H, BS, first, old / s);
+    else
+      s = old;
   }
-  u32x4 kw[NC][2];
+  if ((threadIdx.x & 63) == 0) scales[blk * H + h] = s;
+  return s;
+}
+
+// The keys of head h of a run (r tokens from t on in block blk, the first at offset `first`), by a wave: as many tokens as it has
+// groups side by side, the codes stored from where the heads were normed and turned, 8 bytes a lane's run. Every wave of the workgroup calls it
+// (a piece's angles are the workgroup's); active: the wave has a head. More than 16 tokens are normed and turned
+// twice, for the scale and for the codes.
+template <int D, int V, bool INTER, int LL>
+__device__ __forceinline__ void append_keys(const AppendArgs &a, float2 *turn, int64_t t, int r, int64_t blk, int first,
+                                            int h, bool active) {
+  typedef typename VecOf<__bf16, V>::type Vec;
+  constexpr int G = 64 >> LL, P = kPiece / G, W = V == 8 ? 4 : 1;
+  static_assert(P * G == kPiece && (V == 8 || V == 1), "rows of a piece");
+  uint8_t *kc = static_cast<uint8_t *>(a.kc);
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // (nothing that depends on it is held across the runs: registers)
+  const int group = lane >> LL, u = lane & ((1 << LL) - 1), H = a.Hk, BS = a.BS;
+  const bool all = 2 * a.r.half == D;
+  int e0, e1;
+  unit_runs<V, INTER>(a.r, u, e0, e1);
+  float old = 0.f, w0[V], w1[V];
+  if (active) {
+    if (first != 0) old = a.ks[blk * H + h];
+    load_weights<__bf16, V>(a.n, a.n.kw, h * a.n.kws + e0, w0);
+    load_weights<__bf16, V>(a.n, a.n.kw, h * a.n.kws + e1, w1);
+  }
+  uint32_t k0[P][W], k1[P][W];
+  int off[P];
+  auto load = [&](int p0) __attribute__((always_inline)) {
+    const int n = r - p0 < kPiece ? r - p0 : kPiece;
+    Vec x0[P], x1[P];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const int i = p * G + group;
+      x0[p] = x1[p] = Vec{};
+      off[p] = -1;
+      if (active && i < n) {
+        const __bf16 *x = reinterpret_cast<const __bf16 *>(a.key) + (t + p0 + i) * a.kst + h * a.ksh;
+        x0[p] = *reinterpret_cast<const Vec *>(x + e0);
+        x1[p] = *reinterpret_cast<const Vec *>(x + e1);
+        off[p] = static_cast<int>(a.slots.of[t + p0 + i] - blk * BS);
+      }
+    }
+    __syncthreads();  // the angles before have been read
+    angles_of<4>(a.a, t + p0, n, threadIdx.x, kThreads, turn);
+    __syncthreads();
+    if (!active) return;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      if (p * G >= n) {  // uniform
+#pragma unroll
+        for (int i = 0; i < W; ++i) k0[p][i] = k1[p][i] = 0u;
+        continue;
+      }
+      float f0[V], f1[V], ss = 0.f;
+      widen<V, __bf16>(x0[p], f0);
+      widen<V, __bf16>(x1[p], f1);
+#pragma unroll
+      for (int v = 0; v < V; ++v) ss = __builtin_fmaf(f0[v], f0[v], __builtin_fmaf(f1[v], f1[v], ss));
+      ss = group_sum<LL>(ss, LL);
+      const float inv = a.n.on ? __builtin_amdgcn_rsqf(__builtin_fmaf(ss, 1.f / static_cast<float>(D), a.n.eps)) : 1.f;
+      unit_once<V, INTER>(turn + (off[p] >= 0 ? p * G + group : 0) * a.r.half, a.r.half, all, e0, e1, w0, w1, inv, f0, f1);
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        k0[p][i] = V == 8 ? pack_bf16x2(f0[2 * i % V], f0[(2 * i + 1) % V]) : pack_bf16x2(f0[0], 0.f);
+        k1[p][i] = V == 8 ? pack_bf16x2(f1[2 * i % V], f1[(2 * i + 1) % V]) : pack_bf16x2(f1[0], 0.f);
+      }
+      __builtin_amdgcn_sched_barrier(0);  // (a round's registers are free before the next one's are taken)
+    }
+  };
+  Largest top;
+  uint32_t finite = 0u;  // the largest without NaNs
+  for (int p0 = 0; p0 < r; p0 += kPiece) {  // uniform
+    load(p0);
+    if (!active) continue;
+    uint32_t here = 0u;
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        k0[p][i] = off[p] >= 0 ? k0[p][i] : 0u;
+        k1[p][i] = off[p] >= 0 ? k1[p][i] : 0u;
+        top.pair(k0[p][i]);
+        top.pair(k1[p][i]);
+      }
+    if (__any(top.of_lane() > 0x7f80u)) {
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int i = 0; i < W; ++i) here = max(here, max(without_nan(k0[p][i]), without_nan(k1[p][i])));
+    } else {
+      here = top.of_lane();
+    }
+    finite = max(finite, here);
+  }
+  float s = 0.f;
+  const uint32_t most = wave_max_bits(finite);
+  if (active) s = run_scale<D, false>(kc, a.ks, blk, h, H, BS, first, old, __uint_as_float(most << 16));
+  const Coder code{pow2_inverse(s), static_cast<bool>(__any(top.of_lane() > 0x7f80u))};  
+  for (int p0 = 0; p0 < r; p0 += kPiece) {
+    if (r > kPiece) load(p0);
+    if (!active) continue;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      uint8_t *y0 = kc + fp8_k_index<D>(blk, h, H, BS, off[p], e0), *y1 = kc + fp8_k_index<D>(blk, h, H, BS, off[p], e1);
+      if constexpr (V == 8) {
+        const u32x2 c0 = code.eight(k0[p][0], k0[p][1], k0[p][2], k0[p][3]);
+        const u32x2 c1 = code.eight(k1[p][0], k1[p][1], k1[p][2], k1[p][3]);
+        if (off[p] >= 0) {
+          *reinterpret_cast<u32x2 *>(y0) = c0;
+          *reinterpret_cast<u32x2 *>(y1) = c1;
+        }
+      } else if (off[p] >= 0) {
+        *y0 = static_cast<uint8_t>(code.one(k0[p][0] & 0xffffu));
+        *y1 = static_cast<uint8_t>(code.one(k1[p][0] & 0xffffu));
+      }
+    }
+  }
+}
+
+// The values of head h of a run, by a wave: every lane has D / 64 of the d rows, and a byte of each for a token.
+template <int D>
+__device__ __forceinline__ void append_values(const AppendArgs &a, int64_t t, int r, int64_t blk, int first, int h) {
+  constexpr int RV = D / 64;
+  uint8_t *vc = static_cast<uint8_t *>(a.vc);
+  const int lane = threadIdx.x & 63, m = lane & 15, H = a.Hk, BS = a.BS;
+  const float old = first != 0 ? a.vs[blk * H + h] : 0.f;
   uint32_t vw[kPiece];
   int off = 0;  // offset in the block of the piece's token m
   auto load = [&](int p0) __attribute__((always_inline)) {
     const int n = r - p0 < kPiece ? r - p0 : kPiece, last = n - 1;
-    __syncthreads();  // the angles before have been read
-    tile_angles(a.a, t + p0, n, kThreads, turn);
-    __syncthreads();
-    if (!active) return;
+    if (n == 1) {  // uniform (a token a sequence)
+      const uint16_t *p = a.val + (t + p0) * a.vst + h * a.vsh + RV * lane;
+      vw[0] = RV == 2 ? *reinterpret_cast<const uint32_t *>(p) : *p;
 #pragma unroll
-    for (int i = 0; i < kPiece; ++i) {
-      const uint16_t *p = a.val + (t + p0 + (i < last ? i : last)) * a.vst + h * a.vsh + RV * lane;
-      if constexpr (RV == 2)
-        vw[i] = *reinterpret_cast<const uint32_t *>(p);
-      else
-        vw[i] = *p;
-    }
-    const int mm = m < last ? m : last;
-    off = static_cast<int>(a.slots[t + p0 + mm] - blk * BS);
-    stage_keys<D, V, INTER>(a, turn, t + p0, n, h, rows);
+      for (int i = 1; i < kPiece; ++i) vw[i] = vw[0];
+    } else {
 #pragma unroll
-    for (int j = 0; j < NC; ++j) {
-      const uint16_t *p = rows + mm * kKeyPitch<D> + 16 * ((lane >> 4) + 4 * j);
-      kw[j][0] = *reinterpret_cast<const u32x4 *>(p);
-      kw[j][1] = *reinterpret_cast<const u32x4 *>(p + 8);
-    }
-  };
-  uint32_t ka = 0u, va = 0u;  // largest magnitude bits, as bf16; a NaN counts as none, and is remembered
-  bool nan = false;
-  auto mag = [&](uint32_t x, uint32_t w) __attribute__((always_inline)) {
-    const uint32_t lo = w & 0x7fffu, hi = (w >> 16) & 0x7fffu;
-    nan = nan || lo > 0x7f80u || hi > 0x7f80u;
-    return max(x, max(lo > 0x7f80u ? 0u : lo, hi > 0x7f80u ? 0u : hi));
-  };
-  for (int p0 = 0; p0 < r; p0 += kPiece) {  // uniform
-    load(p0);
-    if (!active) continue;
-#pragma unroll
-    for (int j = 0; j < NC; ++j)
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) ka = mag(ka, kw[j][q][e]);
-#pragma unroll
-    for (int i = 0; i < kPiece; ++i) va = mag(va, vw[i]);
-  }
-  ka = wave_reduce(ka, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
-  va = wave_reduce(va, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
-  const bool any_nan = __any(nan);
-  float sk = pow2_scale(__uint_as_float(ka << 16)), sv = pow2_scale(__uint_as_float(va << 16));
-  if (active && first != 0) {
-    if (sk > sk_old)
-      fp8_reencode_block<D, false>(kc, blk, h, H, BS, first, sk_old / sk);
-    else
-      sk = sk_old;
-    if (sv > sv_old)
-      fp8_reencode_block<D, true>(vc, blk, h, H, BS, first, sv_old / sv);
-    else
-      sv = sv_old;
-  }
-  const float ik = 1.0f / sk, iv = 1.0f / sv;  // exact: powers of two
-  auto q = [](uint32_t bits, float inv) {
-    float v = __uint_as_float(bits << 16) * inv;
-    v = (v != v) ? v : fminf(fmaxf(v, -448.0f), 448.0f);
-    return e4m3_encode(v);
-  };
-  auto pack8 = [&](uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, float inv) __attribute__((always_inline)) {
-    if (!any_nan) return e4m3_pack8(w0, w1, w2, w3, inv);  // uniform
-    u32x2 o;
-    o[0] = q(w0 & 0xffffu, inv) | (q(w0 >> 16, inv) << 8) | (q(w1 & 0xffffu, inv) << 16) | (q(w1 >> 16, inv) << 24);
-    o[1] = q(w2 & 0xffffu, inv) | (q(w2 >> 16, inv) << 8) | (q(w3 & 0xffffu, inv) << 16) | (q(w3 >> 16, inv) << 24);
-    return o;
-  };
-  for (int p0 = 0; p0 < r; p0 += kPiece) {
-    if (r > kPiece) load(p0);
-    if (!active) continue;
-    const int n = r - p0 < kPiece ? r - p0 : kPiece;
-    if (m < n) {
-#pragma unroll
-      for (int j = 0; j < NC; ++j) {
-        const u32x2 x = pack8(kw[j][0][0], kw[j][0][1], kw[j][0][2], kw[j][0][3], ik);
-        const u32x2 y = pack8(kw[j][1][0], kw[j][1][1], kw[j][1][2], kw[j][1][3], ik);
-        *reinterpret_cast<u32x4 *>(kc + fp8_k_index<D>(blk, h, H, BS, off, 16 * ((lane >> 4) + 4 * j))) =
-            u32x4{x[0], x[1], y[0], y[1]};
+      for (int i = 0; i < kPiece; ++i) {
+        const uint16_t *p = a.val + (t + p0 + (i < last ? i : last)) * a.vst + h * a.vsh + RV * lane;
+        if constexpr (RV == 2)
+          vw[i] = *reinterpret_cast<const uint32_t *>(p);
+        else
+          vw[i] = *p;
       }
     }
+    off = static_cast<int>(a.slots.of[t + p0 + (m < last ? m : last)] - blk * BS);
+  };
+  Largest top;
+  uint32_t finite = 0u;
+  for (int p0 = 0; p0 < r; p0 += kPiece) {  // uniform
+    load(p0);
+    uint32_t here = 0u;
+#pragma unroll
+    for (int i = 0; i < kPiece; ++i) top.pair(vw[i]);
+    if (__any(top.of_lane() > 0x7f80u)) {
+#pragma unroll
+      for (int i = 0; i < kPiece; ++i) here = max(here, without_nan(vw[i]));
+    } else {
+      here = top.of_lane();
+    }
+    finite = max(finite, here);
+  }
+  const float s = run_scale<D, true>(vc, a.vs, blk, h, H, BS, first, old, __uint_as_float(wave_max_bits(finite) << 16));
+  const Coder code{pow2_inverse(s), static_cast<bool>(__any(top.of_lane() > 0x7f80u))};
+  for (int p0 = 0; p0 < r; p0 += kPiece) {
+    if (r > kPiece) load(p0);
+    const int n = r - p0 < kPiece ? r - p0 : kPiece;
     // consecutive offsets from a 16-aligned one on: a d row's 16 tokens in one store
     const int off0 = __builtin_amdgcn_readfirstlane(off);
     const bool whole = n == kPiece && off0 % kPiece == 0 && __all(off == off0 + m);
@@ -330,8 +398,8 @@ __device__ __forceinline__ void append_run(const AppendArgs &a, float2 *turn, ui
     for (int rr = 0; rr < RV; ++rr) {
       uint8_t *row = vc + fp8_v_index<D>(blk, h, H, BS, 0, RV * lane + rr);
       auto pair = [&](int i) { return ((vw[i] >> (16 * rr)) & 0xffffu) | (((vw[i + 1] >> (16 * rr)) & 0xffffu) << 16); };
-      const u32x2 c0 = pack8(pair(0), pair(2), pair(4), pair(6), iv);
-      const u32x2 c1 = pack8(pair(8), pair(10), pair(12), pair(14), iv);
+      const u32x2 c0 = code.eight(pair(0), pair(2), pair(4), pair(6));
+      const u32x2 c1 = code.eight(pair(8), pair(10), pair(12), pair(14));
       if (whole) {
         *reinterpret_cast<u32x4 *>(row + off0) = u32x4{c0[0], c0[1], c1[0], c1[1]};
       } else {
@@ -341,32 +409,28 @@ __device__ __forceinline__ void append_run(const AppendArgs &a, float2 *turn, ui
       }
     }
   }
-  if (active && lane == 0) {
-    a.ks[si] = sk;
-    a.vs[si] = sv;
-  }
 }
 
-// A window's runs, four heads a workgroup, one a wave.
-template <int D, int V, bool INTER>
-__device__ __forceinline__ void fp8_role(const AppendArgs &a, int64_t wg, float2 *turn, uint16_t *all_rows) {
+// The runs that begin in a window of the call's tokens, four heads a workgroup, one a wave: f(t, r, blk, first, h, active). The
+// same in every wave.
+template <class F>
+__device__ __forceinline__ void window_runs(const AppendArgs &a, int wg, F f) {
   const int chunks = (a.Hk + kWaves - 1) / kWaves;
-  const int64_t w = wg / chunks, t0 = w * a.window;
+  const int w = wg / chunks;
+  const int64_t t0 = static_cast<int64_t>(w) * a.window;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  const int h = static_cast<int>(wg - w * chunks) * kWaves + wave;
-  const bool active = h < a.Hk;
-  uint16_t *rows = all_rows + wave * kPiece * kKeyPitch<D>;
+  const int h = (wg - w * chunks) * kWaves + wave;
   // lane l: token t0 - 1 + l, its block (-1: none); the window and, behind it, up to 63 - window tokens
   auto block_at = [&](int64_t tok) {
     int64_t blk;
     int off;
-    return tok >= 0 && tok < a.tokens && block_of(a.slots[tok], a.BS, a.NB, blk, off) ? static_cast<int>(blk) : -1;
+    return tok >= 0 && tok < a.tokens && a.slots.at(tok, blk, off) ? static_cast<int>(blk) : -1;
   };
   const int mine = block_at(t0 - 1 + lane);
   const int before = __shfl_up(mine, 1, 64);
   const uint64_t cont = __ballot(lane > 0 && mine >= 0 && mine == before);
   uint64_t starts = __ballot(lane > 0 && lane <= a.window && mine >= 0 && mine != before);
-  while (starts != 0) {  // uniform, and the same in every wave
+  while (starts != 0) {  // uniform
     const int i = __builtin_ctzll(starts);
     starts &= starts - 1;
     const int blk = __builtin_amdgcn_readlane(mine, i);
@@ -381,83 +445,90 @@ __device__ __forceinline__ void fp8_role(const AppendArgs &a, int64_t wg, float2
       }
     }
     const int64_t t = t0 - 1 + i;
-    const int first = static_cast<int>(a.slots[t] - static_cast<int64_t>(blk) * a.BS);
-    append_run<D, V, INTER>(a, turn, rows, t, r, blk, first, h, active);
+    f(t, r, static_cast<int64_t>(blk), static_cast<int>(a.slots.of[t] - static_cast<int64_t>(blk) * a.BS), h, h < a.Hk);
   }
 }
 
-template <int D, int V, bool INTER, bool FP8>
-__global__ __launch_bounds__(kThreads) void rotary_append_kernel(AppendArgs a) {
+template <int D, int V, bool INTER, bool FP8, bool EACH, bool FAR>
+__global__ __launch_bounds__(kThreads, FP8 ? 4 : 1) void rotary_append_kernel(AppendArgs a) {
+  constexpr int UNITS = D / (2 * V), LL = UNITS == 64 ? 6 : UNITS == 32 ? 5 : UNITS == 8 ? 3 : 2;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  const int64_t wg = blockIdx.x;
-  if (wg < a.row_wgs)
-    rows_role<V, INTER, !FP8>(a, wg, reinterpret_cast<float2 *>(lds));
-  else if (FP8)
-    fp8_role<D, V, INTER>(a, wg - a.row_wgs, reinterpret_cast<float2 *>(lds + kWaves * kPiece * kKeyPitch<D> * 2),
-                          reinterpret_cast<uint16_t *>(lds));
-  else
-    values_role<D>(a, wg - a.row_wgs, lds);
+  const int wg = blockIdx.x;
+  float2 *turn = reinterpret_cast<float2 *>(lds);
+  if (wg < a.k_wgs) {
+    if constexpr (FP8)
+      window_runs(a, wg, [&](int64_t t, int r, int64_t blk, int first, int h, bool active) {
+        append_keys<D, V, INTER, LL>(a, turn, t, r, blk, first, h, active);
+      });
+    else
+      heads_role<V, INTER, EACH, true, LL, FAR>(a, a.k, wg, turn);
+  } else if (wg < a.k_wgs + a.v_wgs) {
+    if constexpr (FP8)
+      window_runs(a, wg - a.k_wgs, [&](int64_t t, int r, int64_t blk, int first, int h, bool active) {
+        if (active) append_values<D>(a, t, r, blk, first, h);
+      });
+    else
+      values_role<D>(a, wg - a.k_wgs, lds);
+  } else {
+    heads_role<V, INTER, EACH, false, LL, FAR>(a, a.q, wg - a.k_wgs - a.v_wgs, turn);
+  }
 }
 
 // ---------------------------------------------------------------------------
 // The latent cache: rows of rope_dim (every query head's, and the shared key as one more), and the compressed
 // entries, a wave each.
 struct LatentArgs {
-  HeadRows q;
-  const __bf16 *kvc, *kpe;
-  int64_t kvc_st, kpe_st;
-  const int64_t *slots;
+  Kind q, k;  // queries; the shared key, one head
+  int q_wgs, k_wgs;
+  const __bf16 *kvc;
+  int64_t kvc_st;
+  Slots slots;
   HeadNorm n;  // of the entries: kw
   Angles a;
   RowUnits r;
   int64_t tokens;
-  int heads, rank;
+  int rank;
   __bf16 *latent;
-  int BS;
-  int64_t NB;
-  int tile;
-  FastDiv per, last, splits;
-  int64_t row_wgs;
 };
 
-template <int V, bool INTER>
+template <int V, bool INTER, int LL, bool FAR>
 __global__ __launch_bounds__(kThreads) void mla_rotary_append_kernel(LatentArgs a) {
-  typedef typename VecOf<__bf16, V>::type Vec;
-  extern __shared__ float2 turn[];
+  extern __shared__ float2 turns[];
   const int width = a.rank + a.r.D;
-  const int64_t wg = blockIdx.x;
-  if (wg < a.row_wgs) {
-    const int64_t tile = wg / a.splits.d, t0 = tile * a.tile;
-    const int split = static_cast<int>(wg - tile * a.splits.d);
-    const int nt = a.tokens - t0 < a.tile ? static_cast<int>(a.tokens - t0) : a.tile;
-    tile_angles(a.a, t0, nt, kThreads, turn);
-    __syncthreads();
+  const int wg = blockIdx.x;
+  if (wg < a.q_wgs + a.k_wgs) {
+    const bool is_q = wg < a.q_wgs;
+    const Kind &k = is_q ? a.q : a.k;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    const WaveTile w = wave_tile(k, a.r, a.tokens, is_q ? wg : wg - a.q_wgs, wave);
+    if (w.tokens == 0) return;  // a whole wave; nothing below waits for another
+    float2 *turn = turns + (wave << k.log_tg) * a.r.half;
+    const int64_t t = w.t0 + w.t;
+    HeadsOf<__bf16> of{static_cast<const __bf16 *>(k.s.x) + t * k.s.xt + w.h0 * k.s.xh, k.s.xh, nullptr, k.s.yh, 0, nullptr, 0};
+    bool there = w.there;
+    if (is_q) {
+      of.y = static_cast<__bf16 *>(k.s.y) + t * k.s.yt + w.h0 * k.s.yh;
+    } else {
+      int64_t blk;
+      int off;
+      there = a.slots.at(t, blk, off) && there;
+      of.y = a.latent + (blk * a.slots.block.d + off) * width + a.rank;
+    }
     const HeadNorm none{};
-    norm_turn_rows<__bf16, V, INTER, 1, 2, false>(
-        a.r, none, a.heads, turn, nt, split + 1 == a.splits.d ? a.last : a.per, split * a.per.d, kThreads,
-        [&](int t, int h) {
-          if (h < a.heads) return static_cast<const __bf16 *>(a.q.x) + (t0 + t) * a.q.xt + h * a.q.xh;
-          int64_t blk;
-          int off;
-          if (!block_of(a.slots[t0 + t], a.BS, a.NB, blk, off)) return static_cast<const __bf16 *>(nullptr);
-          return a.kpe + (t0 + t) * a.kpe_st;
-        },
-        [&](int t, int h, int e, Vec v) {
-          __bf16 *y = h < a.heads ? static_cast<__bf16 *>(a.q.y) + (t0 + t) * a.q.yt + h * a.q.yh + e
-                                  : a.latent + a.slots[t0 + t] * width + a.rank + e;
-          *reinterpret_cast<Vec *>(y) = v;
-        });
+    norm_turn_heads<__bf16, V, INTER, 1, 1, FAR, false, false, LL>(
+        a.r, none, turn + w.t * a.r.half, there, w.group, (64 >> a.r.log_lanes) >> k.log_tg, w.heads, of,
+        [&] { wave_angles(a.a, w.t0, w.tokens, turn); });
     return;
   }
   const int lane = threadIdx.x & 63;
-  const int64_t t = (wg - a.row_wgs) * kWaves + (threadIdx.x >> 6);
+  const int64_t t = static_cast<int64_t>(wg - a.q_wgs - a.k_wgs) * kWaves + (threadIdx.x >> 6);
   if (t >= a.tokens) return;  // a whole wave; nothing below waits for another
   int64_t blk;
   int off;
-  if (!block_of(a.slots[t], a.BS, a.NB, blk, off)) return;
+  if (!a.slots.at(t, blk, off)) return;
   typedef typename VecOf<__bf16, 8>::type Vec8;
   const __bf16 *x = a.kvc + t * a.kvc_st;
-  __bf16 *y = a.latent + a.slots[t] * width;
+  __bf16 *y = a.latent + (blk * a.slots.block.d + off) * width;
   float f[8], ss = 0.f, inv = 1.f;
   if (a.n.on) {
     for (int e = 8 * lane; e < a.rank; e += 512) {
@@ -465,7 +536,7 @@ __global__ __launch_bounds__(kThreads) void mla_rotary_append_kernel(LatentArgs 
 #pragma unroll
       for (int v = 0; v < 8; ++v) ss = __builtin_fmaf(f[v], f[v], ss);
     }
-    inv = rsqrtf(__builtin_fmaf(wave_sum(ss), 1.f / static_cast<float>(a.rank), a.n.eps));
+    inv = __builtin_amdgcn_rsqf(__builtin_fmaf(wave_sum(ss), 1.f / static_cast<float>(a.rank), a.n.eps));
   }
   for (int e = 8 * lane; e < a.rank; e += 512) {
     float w[8];
@@ -490,26 +561,6 @@ int check_rows16(const void *p, int64_t st, int64_t sh, const char *name) {
                 name, (long long)st, (long long)sh);
   return WKV_OK;
 }
-
-// The rows role's grid: tiles of tokens, and with too few of them for the chip, their heads over more workgroups.
-struct RowGrid {
-  int tile, per, splits, last;
-  int64_t wgs;
-  RowGrid(int64_t tokens, int heads, int half, int log_lanes) {
-    tile = half > 0 && 1024 / half < 16 ? 1024 / half : 16;
-    while (tile > 1 && (tokens + tile - 1) / tile < 1024) tile /= 2;
-    const int64_t tiles = (tokens + tile - 1) / tile;
-    const int groups = kThreads >> log_lanes;
-    const int64_t want = (1024 + tiles - 1) / tiles, most = (heads + groups - 1) / groups;
-    int n = static_cast<int>(want < most ? want : most);
-    if (n < 1) n = 1;
-    per = (heads + n - 1) / n;
-    if (per < 1) per = 1;
-    splits = heads > 0 ? (heads + per - 1) / per : 1;
-    last = heads - (splits - 1) * per;
-    wgs = heads > 0 ? tiles * splits : 0;
-  }
-};
 
 }  // namespace
 
@@ -553,40 +604,38 @@ extern "C" int wkv_rotary_append(const wkv_cache_t *cache, const void *key, int6
   }
   if (w.v < 8) w.v = 1;
   AppendArgs a{};
-  a.q = HeadRows{q, q_out, q_stride_t, q_stride_h, qo_stride_t, qo_stride_h};
   a.key = static_cast<const uint16_t *>(key);
   a.val = static_cast<const uint16_t *>(value);
   a.kst = key_stride_t;
   a.ksh = key_stride_h;
   a.vst = value_stride_t;
   a.vsh = value_stride_h;
-  a.slots = slot_mapping;
+  a.slots = Slots{slot_mapping, cache->num_blocks * cache->block_size, fast_div(cache->block_size)};
   a.n = head_norm(norm);
   a.a = angles(rotary);
   a.r = row_units(D, half, w.v);
   a.tokens = num_tokens;
-  a.Hq = num_q_heads;
   a.Hk = Hk;
   a.kc = cache->k;
   a.vc = cache->v;
   a.ks = cache->k_scale;
   a.vs = cache->v_scale;
   a.BS = cache->block_size;
-  a.NB = cache->num_blocks;
-  a.rows = num_q_heads + (fp8 ? 0 : Hk);
-  const RowGrid g(num_tokens, a.rows, half, a.r.log_lanes);
-  a.tile = g.tile;
-  a.per = fast_div(g.per);
-  a.last = fast_div(g.last > 0 ? g.last : 1);
-  a.splits = fast_div(g.splits);
-  a.row_wgs = g.wgs;
-  size_t lds = static_cast<size_t>(g.tile) * half * sizeof(float2);
+  const KindGrid gq(num_tokens, num_q_heads, a.r.log_lanes, false), gk(num_tokens, fp8 ? 0 : Hk, a.r.log_lanes, true);
+  int64_t k_wgs = gk.wgs;
+  a.q = Kind{HeadRows{q, q_out, q_stride_t, q_stride_h, qo_stride_t, qo_stride_h}, a.n.qw, a.n.qws, num_q_heads, gq.log_tg,
+             gq.per, fast_div(gq.splits)};
+  a.k = Kind{HeadRows{key, nullptr, key_stride_t, key_stride_h, 0, 0}, a.n.kw, a.n.kws, Hk, gk.log_tg, gk.per,
+             fast_div(gk.splits)};
+  const bool each = (a.n.qw != nullptr && a.n.qws != 0) || (a.n.kw != nullptr && a.n.kws != 0);
+  size_t lds = (static_cast<size_t>(kWaves) << (gq.log_tg > gk.log_tg ? gq.log_tg : gk.log_tg)) * half * sizeof(float2);
   int64_t rest;
   if (fp8) {
     // a window of 16 tokens for prompts, of one where there is a token a sequence
     a.window = num_tokens >= 4096 ? 16 : num_tokens >= 1024 ? 4 : 1;
     rest = (num_tokens + a.window - 1) / a.window * ((Hk + kWaves - 1) / kWaves);
-    const size_t need = kWaves * kPiece * (D + 8) * 2 + static_cast<size_t>(kPiece) * half * sizeof(float2);
+    k_wgs = rest;
+    const size_t need = static_cast<size_t>(kPiece) * half * sizeof(float2);
     lds = lds > need ? lds : need;
   } else if (num_tokens < kValueWindowTokens) {
     a.window = 1;
@@ -594,17 +643,28 @@ extern "C" int wkv_rotary_append(const wkv_cache_t *cache, const void *key, int6
   } else {
     a.window = kValueWindow;
     rest = (num_tokens + kValueWindow - 1) / kValueWindow * Hk;
-    const size_t need = kValueWindow * (D * 2 + 8) + kValueWindow / 8 * sizeof(int64_t);
+    const size_t need = kValueWindow * (D * 2 + 8) + kValueWindow * sizeof(int64_t) + kValueWindow / 8 * sizeof(int);
     lds = lds > need ? lds : need;
   }
-  WKV_CHECK_ARG(a.row_wgs + rest <= INT32_MAX, "too many tokens and heads for one launch");
-  const unsigned grid = static_cast<unsigned>(a.row_wgs + rest);
+  WKV_CHECK_ARG(gq.wgs + k_wgs + rest <= INT32_MAX, "too many tokens and heads for one launch");
+  a.k_wgs = static_cast<int>(k_wgs);
+  a.v_wgs = static_cast<int>(rest);
+  const unsigned grid = static_cast<unsigned>(gq.wgs + k_wgs + rest);
+  // Rows far larger than the caches go past them (8 prompts of 2,048 tokens, 32/8 heads of 128: 82.3 us, 88.7 near); the cache's
+  // keys and values stay, for the attention.
+  const bool far = num_tokens * (num_q_heads + Hk) * D * 2 >= (64 << 20);
   auto s = static_cast<hipStream_t>(stream);
   auto launch = [&](auto d, auto v, auto in) {
     constexpr int DD = decltype(d)::value, VV = decltype(v)::value;
     constexpr bool IN = decltype(in)::value;
-    if (fp8) rotary_append_kernel<DD, VV, IN, true><<<grid, kThreads, lds, s>>>(a);
-    else rotary_append_kernel<DD, VV, IN, false><<<grid, kThreads, lds, s>>>(a);
+    if constexpr (VV == 8) {
+      if (far && fp8 && !each) return rotary_append_kernel<DD, VV, IN, true, false, true><<<grid, kThreads, lds, s>>>(a);
+      if (far && !each) return rotary_append_kernel<DD, VV, IN, false, false, true><<<grid, kThreads, lds, s>>>(a);
+    }
+    if (fp8 && each) return rotary_append_kernel<DD, VV, IN, true, true, false><<<grid, kThreads, lds, s>>>(a);
+    if (fp8) return rotary_append_kernel<DD, VV, IN, true, false, false><<<grid, kThreads, lds, s>>>(a);
+    if (each) return rotary_append_kernel<DD, VV, IN, false, true, false><<<grid, kThreads, lds, s>>>(a);
+    rotary_append_kernel<DD, VV, IN, false, false, false><<<grid, kThreads, lds, s>>>(a);
   };
   auto layout = [&](auto d, auto v) {
     if (inter) launch(d, v, std::true_type{}); else launch(d, v, std::false_type{});
@@ -652,38 +712,39 @@ extern "C" int wkv_mla_rotary_append(const wkv_mla_cache_t *cache, const void *k
     w.rows(q_out, qo_stride_t, qo_stride_h);
   }
   LatentArgs a{};
-  a.q = HeadRows{q_pe, q_out, q_stride_t, q_stride_h, qo_stride_t, qo_stride_h};
   a.kvc = static_cast<const __bf16 *>(kv_c);
-  a.kpe = static_cast<const __bf16 *>(k_pe);
   a.kvc_st = kv_c_stride;
-  a.kpe_st = k_pe_stride;
-  a.slots = slot_mapping;
+  a.slots = Slots{slot_mapping, cache->num_blocks * cache->block_size, fast_div(cache->block_size)};
   a.n = head_norm(kv_norm);
   a.a = angles(rotary);
   a.r = row_units(D, half, w.v);
   if (a.r.units > 64)
     return fail(WKV_ERR_UNSUPPORTED, "rope_dim %d with rotary_dim %d and rows of this alignment not supported", D, rotary->rotary_dim);
   a.tokens = num_tokens;
-  a.heads = num_heads;
   a.rank = cache->kv_lora_rank;
   a.latent = static_cast<__bf16 *>(cache->latent);
-  a.BS = cache->block_size;
-  a.NB = cache->num_blocks;
-  const RowGrid g(num_tokens, num_heads + 1, half, a.r.log_lanes);
-  a.tile = g.tile;
-  a.per = fast_div(g.per);
-  a.last = fast_div(g.last);
-  a.splits = fast_div(g.splits);
-  a.row_wgs = g.wgs;
+  const KindGrid gq(num_tokens, num_heads, a.r.log_lanes, false), gk(num_tokens, 1, a.r.log_lanes, true);
+  a.q = Kind{HeadRows{q_pe, q_out, q_stride_t, q_stride_h, qo_stride_t, qo_stride_h}, nullptr, 0, num_heads, gq.log_tg, gq.per,
+             fast_div(gq.splits)};
+  a.k = Kind{HeadRows{k_pe, nullptr, k_pe_stride, 0, 0, 0}, nullptr, 0, 1, gk.log_tg, gk.per, fast_div(gk.splits)};
   const int64_t rest = (num_tokens + kWaves - 1) / kWaves;
-  WKV_CHECK_ARG(a.row_wgs + rest <= INT32_MAX, "too many tokens and heads for one launch");
-  const unsigned grid = static_cast<unsigned>(a.row_wgs + rest);
-  const size_t lds = static_cast<size_t>(g.tile) * half * sizeof(float2);
+  WKV_CHECK_ARG(gq.wgs + gk.wgs + rest <= INT32_MAX, "too many tokens and heads for one launch");
+  a.q_wgs = static_cast<int>(gq.wgs);
+  a.k_wgs = static_cast<int>(gk.wgs);
+  const unsigned grid = static_cast<unsigned>(gq.wgs + gk.wgs + rest);
+  const size_t lds = (static_cast<size_t>(kWaves) << (gq.log_tg > gk.log_tg ? gq.log_tg : gk.log_tg)) * half * sizeof(float2);
   auto s = static_cast<hipStream_t>(stream);
   auto layout = [&](auto v) {
     constexpr int VV = decltype(v)::value;
-    if (inter) mla_rotary_append_kernel<VV, true><<<grid, kThreads, lds, s>>>(a);
-    else mla_rotary_append_kernel<VV, false><<<grid, kThreads, lds, s>>>(a);
+    if constexpr (VV == 8) {  // rows of 64: their lanes as a constant
+      const bool far = num_tokens * num_heads * D * 2 >= (64 << 20);
+      if (a.r.log_lanes == 2 && inter && far) return mla_rotary_append_kernel<VV, true, 2, true><<<grid, kThreads, lds, s>>>(a);
+      if (a.r.log_lanes == 2 && inter) return mla_rotary_append_kernel<VV, true, 2, false><<<grid, kThreads, lds, s>>>(a);
+      if (a.r.log_lanes == 2 && far) return mla_rotary_append_kernel<VV, false, 2, true><<<grid, kThreads, lds, s>>>(a);
+      if (a.r.log_lanes == 2) return mla_rotary_append_kernel<VV, false, 2, false><<<grid, kThreads, lds, s>>>(a);
+    }
+    if (inter) mla_rotary_append_kernel<VV, true, -1, false><<<grid, kThreads, lds, s>>>(a);
+    else mla_rotary_append_kernel<VV, false, -1, false><<<grid, kThreads, lds, s>>>(a);
   };
   if (w.v == 8) layout(std::integral_constant<int, 8>{});
   else if (w.v == 2) layout(std::integral_constant<int, 2>{});

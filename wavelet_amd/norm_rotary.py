@@ -88,15 +88,14 @@ def _backward(q, k, gq, gk, q_weight, k_weight, rotary, interleaved, scale, eps,
     dqw, dkw = (w if w is None else torch.empty_like(w, memory_format=torch.contiguous_format) if x.shape[1]
                 else torch.zeros_like(w) for x, w in zip((q, k), wants))
     wants = [w if w is not None and x.shape[1] else None for x, w in zip((q, k), wants)]  # (no head, no sum)
-    each = [int(w is not None and w.dim() == 2) for w in wants]
+    each = [int(x is not None and w is not None and w.dim() == 2) for x, w in zip((q, k), (q_weight, k_weight))]
     norm = head_norm(q_weight, k_weight, eps, offset)
     how = None if rotary is None else ctypes.byref(rotation(*rotary, interleaved, scale))
     lib = _lib.load()
     ws, need_bytes = None, 0
     if any(w is not None for w in wants):
         need_bytes = lib.wkv_norm_rotary_workspace_size(tokens, 0 if q is None else q.shape[1],
-                                                        0 if k is None else k.shape[1], d,
-                                                        0 if rotary is None else 2 * rotary[1].shape[0], *each)
+                                                        0 if k is None else k.shape[1], d, *each)
         ws = torch.empty(need_bytes, dtype=torch.uint8, device=dev)
     with _on(dev):
         rc = lib.wkv_norm_rotary_backward(
