@@ -65,8 +65,12 @@ def _token_rows(x: torch.Tensor, name: str, shape: tuple[int, ...], device: torc
     _require_cuda(x, name, device)
     if x.dtype != torch.bfloat16 or tuple(x.shape[1:]) != shape:
         raise ValueError(f"{name} must be bfloat16 [T, {', '.join(map(str, shape))}] (got {x.dtype} {tuple(x.shape)})")
-    if x.stride(-1) != 1 or any(s % 8 for s in x.stride()[:-1]) or x.data_ptr() % 16:
-        x = x.contiguous()
+    *strides, last = x.stride()
+    if last != 1 or x.data_ptr() % 16:
+        return x.contiguous()
+    for s in strides:
+        if s % 8:
+            return x.contiguous()
     return x
 
 

@@ -501,7 +501,9 @@ inline RowUnits row_units(int D, int half, int v) {
 
 // Waves over the tokens and heads of a kind, four a workgroup: a token a wave (its heads lie together; by_token: as many as
 // the wave's groups, whose stores of one head then lie together in a cache), and with too few tokens for the chip the heads
-// dealt over more waves, down to a round of the wave's groups.
+// dealt over more waves, down to a round of the wave's groups below 4,096 waves (four a SIMD), to two
+// rounds below 16,384 (4,696 tokens of 128 heads of 64: 38.2 us, 45.4 a wave a token; 8,191 of 16 heads of 128, two rounds,
+// lose 1 us in halves).
 struct KindGrid {
   int log_tg = 0, per = 1, splits = 1;
   int64_t waves = 0, wgs = 0;
@@ -511,8 +513,11 @@ struct KindGrid {
     while (by_token && log_tg < log_groups && (tokens >> (log_tg + 1)) * heads >= 4096) ++log_tg;
     waves = ((tokens - 1) >> log_tg) + 1;
     const int step = (1 << log_groups) >> log_tg, rounds = (heads + step - 1) / step;
-    const int64_t want = (4096 + waves - 1) / waves;
-    const int n = static_cast<int>(want < rounds ? want : rounds);
+    auto share = [&](int64_t want, int most) {
+      const int64_t n = (want + waves - 1) / waves;
+      return static_cast<int>(n < most ? n : most);
+    };
+    const int few = share(4096, rounds), many = by_token ? 1 : share(16384, rounds / 2), n = few > many ? few : many;
     per = (rounds + n - 1) / n * step;
     splits = (heads + per - 1) / per;
     wgs = (waves + 3) / 4 * splits;

@@ -479,7 +479,7 @@ __global__ __launch_bounds__(kThreads, FP8 ? 4 : 1) void rotary_append_kernel(Ap
 // entries, a wave each.
 struct LatentArgs {
   Kind q, k;  // queries; the shared key, one head
-  int q_wgs, k_wgs;
+  int entry_wgs, k_wgs;  // workgroups of entries, and of shared keys; queries behind them
   const __bf16 *kvc;
   int64_t kvc_st;
   Slots slots;
@@ -491,16 +491,16 @@ struct LatentArgs {
   __bf16 *latent;
 };
 
-template <int V, bool INTER, int LL, bool FAR>
+template <int V, bool INTER, int LL>
 __global__ __launch_bounds__(kThreads) void mla_rotary_append_kernel(LatentArgs a) {
   extern __shared__ float2 turns[];
   const int width = a.rank + a.r.D;
-  const int wg = blockIdx.x;
-  if (wg < a.q_wgs + a.k_wgs) {
-    const bool is_q = wg < a.q_wgs;
+  const int wg = static_cast<int>(blockIdx.x) - a.entry_wgs;
+  if (wg >= 0) {
+    const bool is_q = wg >= a.k_wgs;
     const Kind &k = is_q ? a.q : a.k;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-    const WaveTile w = wave_tile(k, a.r, a.tokens, is_q ? wg : wg - a.q_wgs, wave);
+    const WaveTile w = wave_tile(k, a.r, a.tokens, is_q ? wg - a.k_wgs : wg, wave);
     if (w.tokens == 0) return;  // a whole wave; nothing below waits for another
     float2 *turn = turns + (wave << k.log_tg) * a.r.half;
     const int64_t t = w.t0 + w.t;
@@ -515,13 +515,13 @@ __global__ __launch_bounds__(kThreads) void mla_rotary_append_kernel(LatentArgs 
       of.y = a.latent + (blk * a.slots.block.d + off) * width + a.rank;
     }
     const HeadNorm none{};
-    norm_turn_heads<__bf16, V, INTER, 1, 1, FAR, false, false, LL>(
+    norm_turn_heads<__bf16, V, INTER, 1, 1, false, false, false, LL>(
         a.r, none, turn + w.t * a.r.half, there, w.group, (64 >> a.r.log_lanes) >> k.log_tg, w.heads, of,
         [&] { wave_angles(a.a, w.t0, w.tokens, turn); });
     return;
   }
   const int lane = threadIdx.x & 63;
-  const int64_t t = static_cast<int64_t>(wg - a.q_wgs - a.k_wgs) * kWaves + (threadIdx.x >> 6);
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kWaves + (threadIdx.x >> 6);
   if (t >= a.tokens) return;  // a whole wave; nothing below waits for another
   int64_t blk;
   int off;
@@ -729,7 +729,7 @@ extern "C" int wkv_mla_rotary_append(const wkv_mla_cache_t *cache, const void *k
   a.k = Kind{HeadRows{k_pe, nullptr, k_pe_stride, 0, 0, 0}, nullptr, 0, 1, gk.log_tg, gk.per, fast_div(gk.splits)};
   const int64_t rest = (num_tokens + kWaves - 1) / kWaves;
   WKV_CHECK_ARG(gq.wgs + gk.wgs + rest <= INT32_MAX, "too many tokens and heads for one launch");
-  a.q_wgs = static_cast<int>(gq.wgs);
+  a.entry_wgs = static_cast<int>(rest);
   a.k_wgs = static_cast<int>(gk.wgs);
   const unsigned grid = static_cast<unsigned>(gq.wgs + gk.wgs + rest);
   const size_t lds = (static_cast<size_t>(kWaves) << (gq.log_tg > gk.log_tg ? gq.log_tg : gk.log_tg)) * half * sizeof(float2);
@@ -737,14 +737,11 @@ extern "C" int wkv_mla_rotary_append(const wkv_mla_cache_t *cache, const void *k
   auto layout = [&](auto v) {
     constexpr int VV = decltype(v)::value;
     if constexpr (VV == 8) {  // rows of 64: their lanes as a constant
-      const bool far = num_tokens * num_heads * D * 2 >= (64 << 20);
-      if (a.r.log_lanes == 2 && inter && far) return mla_rotary_append_kernel<VV, true, 2, true><<<grid, kThreads, lds, s>>>(a);
-      if (a.r.log_lanes == 2 && inter) return mla_rotary_append_kernel<VV, true, 2, false><<<grid, kThreads, lds, s>>>(a);
-      if (a.r.log_lanes == 2 && far) return mla_rotary_append_kernel<VV, false, 2, true><<<grid, kThreads, lds, s>>>(a);
-      if (a.r.log_lanes == 2) return mla_rotary_append_kernel<VV, false, 2, false><<<grid, kThreads, lds, s>>>(a);
+      if (a.r.log_lanes == 2 && inter) return mla_rotary_append_kernel<VV, true, 2><<<grid, kThreads, lds, s>>>(a);
+      if (a.r.log_lanes == 2) return mla_rotary_append_kernel<VV, false, 2><<<grid, kThreads, lds, s>>>(a);
     }
-    if (inter) mla_rotary_append_kernel<VV, true, -1, false><<<grid, kThreads, lds, s>>>(a);
-    else mla_rotary_append_kernel<VV, false, -1, false><<<grid, kThreads, lds, s>>>(a);
+    if (inter) mla_rotary_append_kernel<VV, true, -1><<<grid, kThreads, lds, s>>>(a);
+    else mla_rotary_append_kernel<VV, false, -1><<<grid, kThreads, lds, s>>>(a);
   };
   if (w.v == 8) layout(std::integral_constant<int, 8>{});
   else if (w.v == 2) layout(std::integral_constant<int, 2>{});

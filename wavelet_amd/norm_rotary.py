@@ -8,8 +8,6 @@ and under autograd for training, with the weights' gradients.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
@@ -21,29 +19,31 @@ def check_weight(w, name: str, heads: int, x: torch.Tensor):
     """A head norm's weight (None: ones) for ``heads`` heads of ``x``'s type and size, its last dim contiguous."""
     if w is None:
         return None
-    d = x.shape[-1]
-    if not isinstance(w, torch.Tensor) or w.device != x.device or w.dtype not in (torch.float32, x.dtype):
+    if not isinstance(w, torch.Tensor) or w.device != x.device or (w.dtype is not x.dtype and w.dtype is not torch.float32):
         raise ValueError(f"{name} must be a float32 or {x.dtype} tensor on {x.device}")
-    if tuple(w.shape) not in ((d,), (heads, d)):
-        raise ValueError(f"{name} must be [{d}] or [{heads}, {d}] (got {list(w.shape)})")
+    shape, d = w.shape, x.shape[-1]
+    if shape != (d,) and shape != (heads, d):
+        raise ValueError(f"{name} must be [{d}] or [{heads}, {d}] (got {list(shape)})")
     return w if w.stride(-1) == 1 else w.contiguous()
-
-
-def _same_type(q_weight, k_weight):
-    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
-        raise ValueError(f"q_weight and k_weight must have one type (got {q_weight.dtype} and {k_weight.dtype})")
 
 
 def head_norm(q_weight, k_weight, eps: float, offset: float) -> _lib.WkvHeadNorm:
     """The library's description of a norm (wkv_head_norm_t) from checked weights, which have to outlive it."""
-    def of(w):
-        return (None, 0) if w is None else (w.data_ptr(), w.stride(0) if w.dim() == 2 else 0)
-
-    some = k_weight if q_weight is None else q_weight
-    (qw, qs), (kw, ks) = of(q_weight), of(k_weight)
-    return _lib.WkvHeadNorm(q_weight=qw, k_weight=kw, q_weight_stride_h=qs, k_weight_stride_h=ks,
-                            weight_dtype=0 if some is None else _DTYPES[some.dtype], weight_offset=offset, eps=eps,
-                            reserved=0)
+    qw = kw = None
+    qs = ks = dtype = 0
+    if q_weight is not None:
+        qw, dtype = q_weight.data_ptr(), _DTYPES[q_weight.dtype]
+        if q_weight.dim() == 2:
+            qs = q_weight.stride(0)
+    if k_weight is not None:
+        kw = k_weight.data_ptr()
+        if q_weight is None:
+            dtype = _DTYPES[k_weight.dtype]
+        elif k_weight.dtype is not q_weight.dtype:
+            raise ValueError(f"q_weight and k_weight must have one type (got {q_weight.dtype} and {k_weight.dtype})")
+        if k_weight.dim() == 2:
+            ks = k_weight.stride(0)
+    return _lib.WkvHeadNorm(qw, kw, qs, ks, dtype, offset, eps, 0)
 
 
 def _rows(x: torch.Tensor | None, *others):
@@ -60,16 +60,31 @@ def _packed(x):
 
 def _forward(q, k, q_weight, k_weight, rotary, interleaved, scale, eps, offset, out):
     """One launch over checked tensors; rotary: (positions, inv_freq, axes), or None: only normed."""
-    qi, ki = _packed(q), _packed(k)
-    if out is None:
-        out = tuple(x if x is None else torch.empty_like(x, memory_format=torch.contiguous_format) for x in (qi, ki))
+    tokens, hq, d = q.shape
     dev = q.device
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    if k is not None and k.stride(2) != 1:
+        k = k.contiguous()
+    if out is None:
+        out = (torch.empty_like(q, memory_format=torch.contiguous_format),
+               None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format))
     norm = head_norm(q_weight, k_weight, eps, offset)
-    how = None if rotary is None else ctypes.byref(rotation(*rotary, interleaved, scale))
+    how = None if rotary is None else rotation(*rotary, interleaved, scale)  # (a struct goes by reference)
+    qo, ko = out
+    st, sh, _ = q.stride()
+    ot, oh, _ = qo.stride()
+    if k is None:
+        tail = (None, 0, 0, None, 0, 0, 0)
+    else:
+        kst, ksh, _ = k.stride()
+        kot, koh, _ = ko.stride()
+        tail = (k.data_ptr(), kst, ksh, ko.data_ptr(), kot, koh, k.shape[1])
     with _on(dev):
-        rc = _lib.load().wkv_norm_rotary(_DTYPES[q.dtype], *_rows(qi, out[0]), *_rows(ki, out[1]), q.shape[2],
-                                         ctypes.byref(norm), how, q.shape[0], _stream(dev))
-    _lib.check(rc, "norm_rotary")
+        rc = _lib.load().wkv_norm_rotary(_DTYPES[q.dtype], q.data_ptr(), st, sh, qo.data_ptr(), ot, oh, hq, *tail, d, norm,
+                                         how, tokens, _stream(dev))
+    if rc:
+        _lib.check(rc, "norm_rotary")
     return out
 
 
@@ -90,7 +105,7 @@ def _backward(q, k, gq, gk, q_weight, k_weight, rotary, interleaved, scale, eps,
     wants = [w if w is not None and x.shape[1] else None for x, w in zip((q, k), wants)]  # (no head, no sum)
     each = [int(x is not None and w is not None and w.dim() == 2) for x, w in zip((q, k), (q_weight, k_weight))]
     norm = head_norm(q_weight, k_weight, eps, offset)
-    how = None if rotary is None else ctypes.byref(rotation(*rotary, interleaved, scale))
+    how = None if rotary is None else rotation(*rotary, interleaved, scale)
     lib = _lib.load()
     ws, need_bytes = None, 0
     if any(w is not None for w in wants):
@@ -99,7 +114,7 @@ def _backward(q, k, gq, gk, q_weight, k_weight, rotary, interleaved, scale, eps,
         ws = torch.empty(need_bytes, dtype=torch.uint8, device=dev)
     with _on(dev):
         rc = lib.wkv_norm_rotary_backward(
-            _DTYPES[some.dtype], *_rows(q, gq, dq), *_rows(k, gk, dk), d, ctypes.byref(norm), how,
+            _DTYPES[some.dtype], *_rows(q, gq, dq), *_rows(k, gk, dk), d, norm, how,
             *(None if w is None else dw.data_ptr() for w, dw in zip(wants, (dqw, dkw))), tokens,
             None if ws is None else ws.data_ptr(), need_bytes, _stream(dev))
     _lib.check(rc, "norm_rotary backward")
@@ -157,15 +172,17 @@ def norm_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
     if k is None and k_weight is not None:
         raise ValueError("k_weight without k")
     k_weight = check_weight(k_weight, "k_weight", 0 if k is None else k.shape[1], q)
-    _same_type(q_weight, k_weight)
     if (positions is None) != (inv_freq is None) or (inv_freq is None and axes is not None):
         raise ValueError("positions and inv_freq go together (both None: the heads are only normed)")
     rotary = None if inv_freq is None else check_rotation(positions, inv_freq, axes, tokens, d, dev)
     how = (rotary, bool(interleaved), float(scale), float(eps), float(weight_offset))
-    inputs = [x for x in (q, k, q_weight, k_weight) if x is not None]
-    differentiable = torch.is_grad_enabled() and any(x.requires_grad for x in inputs) or _dual(*inputs)
+    differentiable = _dual(q, k, q_weight, k_weight) or torch.is_grad_enabled() and (
+        q.requires_grad or k is not None and k.requires_grad or q_weight is not None and q_weight.requires_grad
+        or k_weight is not None and k_weight.requires_grad)
     if out is None:
-        return (_NormRotary.apply if differentiable else lambda *a: _forward(*a, None))(q, k, q_weight, k_weight, *how)
+        if differentiable:
+            return _NormRotary.apply(q, k, q_weight, k_weight, *how)
+        return _forward(q, k, q_weight, k_weight, *how, None)
     if len(out) != 2 or (out[1] is None) != (k is None):
         raise ValueError("out must hold the results' two tensors (None for no k)")
     written = [o for o in out if o is not None]

@@ -139,17 +139,18 @@ def rotary_axes(sections, *, interleaved: bool = False, device: torch.device | s
 def check_rotation(positions, inv_freq, axes, tokens: int, d: int, dev: torch.device):
     """A call's positions, frequencies and axes (None: one), checked and contiguous."""
     _require_cuda(positions, "positions", dev)
+    shape = positions.shape
     if axes is None:
-        if positions.dtype != torch.int64 or tuple(positions.shape) != (tokens,):
-            raise ValueError(f"positions must be int64 [{tokens}] (got {positions.dtype} {tuple(positions.shape)})")
-    elif positions.dtype != torch.int64 or positions.dim() != 2 or positions.shape[0] < 1 or positions.shape[1] != tokens:
-        raise ValueError(f"positions must be int64 [axes, {tokens}] (got {positions.dtype} {tuple(positions.shape)})")
+        if positions.dtype is not torch.int64 or len(shape) != 1 or shape[0] != tokens:
+            raise ValueError(f"positions must be int64 [{tokens}] (got {positions.dtype} {tuple(shape)})")
+    elif positions.dtype is not torch.int64 or len(shape) != 2 or shape[0] < 1 or shape[1] != tokens:
+        raise ValueError(f"positions must be int64 [axes, {tokens}] (got {positions.dtype} {tuple(shape)})")
     _require_cuda(inv_freq, "inv_freq", dev)
-    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not 0 < 2 * inv_freq.shape[0] <= d:
+    if inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 or not 0 < 2 * inv_freq.shape[0] <= d:
         raise ValueError(f"inv_freq must be float64 [R / 2] with R <= {d} (got {inv_freq.dtype} {tuple(inv_freq.shape)})")
     if axes is not None:
         _require_cuda(axes, "axes", dev)
-        if axes.dtype != torch.int32 or axes.shape != inv_freq.shape:
+        if axes.dtype is not torch.int32 or axes.shape != inv_freq.shape:
             raise ValueError(f"axes must be int32 {list(inv_freq.shape)}, one a pair (got {axes.dtype} {tuple(axes.shape)})")
         axes = axes.contiguous()
     return positions.contiguous(), inv_freq.contiguous(), axes
@@ -157,11 +158,11 @@ def check_rotation(positions, inv_freq, axes, tokens: int, d: int, dev: torch.de
 
 def rotation(positions, inv_freq, axes, interleaved: bool, scale: float, inverse: bool = False) -> _lib.WkvRotary:
     """The library's description of a rotation (wkv_rotary_t) from checked tensors, which have to outlive it."""
-    return _lib.WkvRotary(
-        positions=positions.data_ptr(), axis_stride=positions.stride(0) if positions.dim() == 2 else 0,
-        axes=None if axes is None else axes.data_ptr(), inv_freq=inv_freq.data_ptr(),
-        num_axes=positions.shape[0] if positions.dim() == 2 else 1, rotary_dim=2 * inv_freq.shape[0],
-        interleaved=interleaved, inverse=inverse, scale=scale, reserved=0)
+    r = 2 * inv_freq.shape[0]
+    if axes is None:
+        return _lib.WkvRotary(positions.data_ptr(), 0, None, inv_freq.data_ptr(), 1, r, interleaved, inverse, scale, 0)
+    return _lib.WkvRotary(positions.data_ptr(), positions.stride(0), axes.data_ptr(), inv_freq.data_ptr(),
+                          positions.shape[0], r, interleaved, inverse, scale, 0)
 
 
 def _launch(q, k, positions, inv_freq, axes, interleaved: bool, scale: float, inverse: bool, out):

@@ -9,21 +9,24 @@ queries for the attention and the cache; ``mla_rotary_append`` is the same for a
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
 from .cache import MLALatentCache, PagedKVCache, _on, _require_cuda, _slots, _stream, _token_rows
-from .norm_rotary import _same_type, check_weight, head_norm
+from .norm_rotary import check_weight, head_norm
 from .rotary import _dual, check_rotation, rotation
 
 
 def _no_gradients(what: str, *tensors) -> None:
     """A cache keeps no graph: what goes into it cannot be differentiated."""
-    there = [t for t in tensors if t is not None]
-    if torch.is_grad_enabled() and any(t.requires_grad for t in there) or _dual(*there):
-        raise ValueError(f"{what} has no gradient: detach its inputs, or call it under torch.no_grad()")
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if grad and t is not None and t.requires_grad:
+            break
+    else:
+        if not _dual(*tensors):
+            return
+    raise ValueError(f"{what} has no gradient: detach its inputs, or call it under torch.no_grad()")
 
 
 def _result(x: torch.Tensor, out, name: str) -> torch.Tensor:
@@ -36,6 +39,15 @@ def _result(x: torch.Tensor, out, name: str) -> torch.Tensor:
         raise ValueError(f"out must be {x.dtype} {tuple(x.shape)} on {x.device} for {name}, with its last dim contiguous "
                          "and no row twice")
     return out
+
+
+def _rows(q, result) -> tuple:
+    """Pointers, strides and heads of the queries and their result (None: there are none)."""
+    if q is None:
+        return None, 0, 0, None, 0, 0, 0
+    st, sh, _ = q.stride()
+    ot, oh, _ = result.stride()
+    return q.data_ptr(), st, sh, result.data_ptr(), ot, oh, q.shape[1]
 
 
 def _queries(q, name: str, tokens: int, d: int, dev: torch.device) -> torch.Tensor:
@@ -65,7 +77,6 @@ def rotary_append(q: torch.Tensor | None, key: torch.Tensor, value: torch.Tensor
         raise ValueError("cache must be a PagedKVCache (mla_rotary_append appends to latent caches)")
     dev, d = cache.device, cache.head_dim
     shape = (cache.num_kv_heads, d)
-    _no_gradients("rotary_append", *(t for t in (q, key, value, q_weight, k_weight, out) if isinstance(t, torch.Tensor)))
     key = _token_rows(key, "key", shape, dev)
     value = _token_rows(value, "value", shape, dev)
     tokens = key.shape[0]
@@ -85,20 +96,20 @@ def rotary_append(q: torch.Tensor | None, key: torch.Tensor, value: torch.Tensor
     if eps is not None:
         q_weight = None if q is None else check_weight(q_weight, "q_weight", q.shape[1], q)
         k_weight = check_weight(k_weight, "k_weight", shape[0], key)
-        _same_type(q_weight, k_weight)
-        norm = ctypes.byref(head_norm(q_weight, k_weight, float(eps), float(weight_offset)))
+        norm = head_norm(q_weight, k_weight, float(eps), float(weight_offset))
     how = None
     if inv_freq is not None:
         positions, inv_freq, axes = check_rotation(positions, inv_freq, axes, tokens, d, dev)
-        how = ctypes.byref(rotation(positions, inv_freq, axes, bool(interleaved), float(scale)))
+        how = rotation(positions, inv_freq, axes, bool(interleaved), float(scale))
     result = None if q is None else _result(q, out, "q")
-    rows = (None, 0, 0, None, 0, 0, 0) if q is None else (
-        q.data_ptr(), *q.stride()[:2], result.data_ptr(), *result.stride()[:2], q.shape[1])
+    _no_gradients("rotary_append", q, key, value, q_weight, k_weight, out)
+    kst, ksh, _ = key.stride()
+    vst, vsh, _ = value.stride()
     with _on(dev):
-        rc = _lib.load().wkv_rotary_append(
-            ctypes.byref(cache.descriptor()), key.data_ptr(), *key.stride()[:2], value.data_ptr(), *value.stride()[:2],
-            slots.data_ptr(), *rows, norm, how, tokens, _stream(dev))
-    _lib.check(rc, "rotary_append")
+        rc = _lib.load().wkv_rotary_append(cache.descriptor(), key.data_ptr(), kst, ksh, value.data_ptr(), vst, vsh,
+                                           slots.data_ptr(), *_rows(q, result), norm, how, tokens, _stream(dev))
+    if rc:
+        _lib.check(rc, "rotary_append")
     if out is not None:
         torch.autograd.graph.increment_version([out])
     return result
@@ -119,7 +130,6 @@ def mla_rotary_append(q_pe: torch.Tensor | None, kv_c: torch.Tensor, k_pe: torch
     if not isinstance(cache, MLALatentCache):
         raise ValueError("cache must be an MLALatentCache (rotary_append appends to key and value caches)")
     dev = cache.device
-    _no_gradients("mla_rotary_append", *(t for t in (q_pe, kv_c, k_pe, kv_weight, out) if isinstance(t, torch.Tensor)))
     kv_c = _token_rows(kv_c, "kv_c", (cache.kv_lora_rank,), dev)
     k_pe = _token_rows(k_pe, "k_pe", (cache.rope_dim,), dev)
     tokens = kv_c.shape[0]
@@ -132,7 +142,7 @@ def mla_rotary_append(q_pe: torch.Tensor | None, kv_c: torch.Tensor, k_pe: torch
     else:
         q_pe = _queries(q_pe, "q_pe", tokens, cache.rope_dim, dev)
     positions, inv_freq, axes = check_rotation(positions, inv_freq, axes, tokens, cache.rope_dim, dev)
-    how = ctypes.byref(rotation(positions, inv_freq, axes, bool(interleaved), float(scale)))
+    how = rotation(positions, inv_freq, axes, bool(interleaved), float(scale))
     norm = None
     if eps is None:
         if kv_weight is not None or weight_offset != 0.0:
@@ -144,15 +154,15 @@ def mla_rotary_append(q_pe: torch.Tensor | None, kv_c: torch.Tensor, k_pe: torch
                 raise ValueError(f"kv_weight must be [{cache.kv_lora_rank}]")
             if kv_weight.data_ptr() % 16:
                 kv_weight = kv_weight.clone()
-        norm = ctypes.byref(head_norm(None, kv_weight, float(eps), float(weight_offset)))
+        norm = head_norm(None, kv_weight, float(eps), float(weight_offset))
     result = None if q_pe is None else _result(q_pe, out, "q_pe")
-    rows = (None, 0, 0, None, 0, 0, 0) if q_pe is None else (
-        q_pe.data_ptr(), *q_pe.stride()[:2], result.data_ptr(), *result.stride()[:2], q_pe.shape[1])
+    _no_gradients("mla_rotary_append", q_pe, kv_c, k_pe, kv_weight, out)
     with _on(dev):
-        rc = _lib.load().wkv_mla_rotary_append(
-            ctypes.byref(cache.descriptor()), kv_c.data_ptr(), kv_c.stride(0), k_pe.data_ptr(), k_pe.stride(0),
-            slots.data_ptr(), *rows, norm, how, tokens, _stream(dev))
-    _lib.check(rc, "mla_rotary_append")
+        rc = _lib.load().wkv_mla_rotary_append(cache.descriptor(), kv_c.data_ptr(), kv_c.stride(0), k_pe.data_ptr(),
+                                               k_pe.stride(0), slots.data_ptr(), *_rows(q_pe, result), norm, how, tokens,
+                                               _stream(dev))
+    if rc:
+        _lib.check(rc, "mla_rotary_append")
     if out is not None:
         torch.autograd.graph.increment_version([out])
     return result
