@@ -214,7 +214,8 @@ def test_rows_that_are_not_aligned(cuda, shift):
 
 @pytest.mark.parametrize("kv", ["bf16", "fp8_e4m3"])
 def test_prompt_and_decode_as_they_are_used(cuda, kv):
-    """A prompt and then tokens one by one: rotary_append and the attentions against norm_rotary and theirs."""
+    """A prompt and then tokens one by one: rotary_append and the attentions against norm_rotary and theirs. (A decode
+    step's two results are apart as test_gpu_step_heads.py derives.)"""
     hq, hk, d, block, new = 8, 2, 128, 16, [37, 5]
     g = torch.Generator(device=cuda).manual_seed(9)
     freq, scale = rotary_frequencies(d, 1e6, device=cuda)
@@ -250,7 +251,7 @@ def test_prompt_and_decode_as_they_are_used(cuda, kv):
         one = paged_decode_gqa(q1, a, table, lens, d ** -0.5, max_seq_len=64)
         two = paged_decode_gqa(q2, b, table, lens, d ** -0.5, max_seq_len=64, new_key=k2, new_value=value,
                                slot_mapping=slots)
-        torch.testing.assert_close(one.float(), two.float(), rtol=2.0 ** -7, atol=2.0 ** -9)
+        torch.testing.assert_close(one.float(), two.float(), rtol=2.0 ** -7, atol=5 * 2.0 ** -8)
         for x, y in zip(_held(a), _held(b)):
             np.testing.assert_array_equal(x, y)
 

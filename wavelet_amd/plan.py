@@ -17,13 +17,15 @@ build a new plan after ``wake_up``.
 from __future__ import annotations
 
 import ctypes
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import torch
 
 from . import _lib
 from .attention import _workspace, decode_plan
 from .cache import KV_DTYPES, PagedKVCache, _on, _require_cuda, _stream, check_tables
+from .norm_rotary import check_weight, head_norm
+from .rotary import check_rotation, rotation
 from .step import MAX_DEPTH, MAX_NODES, Accepted, StepState, accept_tree, new_step_maps
 
 
@@ -40,6 +42,69 @@ def _plan_slots(slot_mapping: torch.Tensor, device: torch.device, n: int | None)
     if n is not None and slot_mapping.numel() != n:
         raise ValueError(f"slot_mapping must hold one slot per sequence ({n}), got {slot_mapping.numel()}")
     return slot_mapping
+
+
+@dataclass
+class Heads:
+    """What a plan does to its layers' queries and keys on their way to the cache and the attention.
+
+    The norm where ``eps`` is given (``q_weight[l]`` and ``k_weight[l]`` for layer ``l``; None: ones), the rotation
+    where ``inv_freq`` is, as ``rotary_append`` takes them; for an MLA plan ``k_weight[l]`` is the weight of the compressed entries.
+    ``positions`` ``[T]`` (``[A, T]`` with ``axes``) are refilled in place between steps, like the plan's other
+    buffers (``TreeStep`` has its own).
+    """
+
+    positions: torch.Tensor | None = None
+    inv_freq: torch.Tensor | None = None
+    axes: torch.Tensor | None = None
+    scale: float = 1.0
+    interleaved: bool = False
+    q_weight: list | None = None
+    k_weight: list | None = None
+    eps: float | None = None
+    weight_offset: float = 0.0
+
+    def rotation(self, tokens: int, d: int, device: torch.device):
+        """The library's rotation over the plan's own tensors (None without one)."""
+        if self.inv_freq is None:
+            if self.positions is not None or self.axes is not None:
+                raise ValueError("positions and axes go with inv_freq")
+            return None
+        if self.positions is None:
+            raise ValueError("inv_freq needs positions")
+        checked = check_rotation(self.positions, self.inv_freq, self.axes, tokens, d, device)
+        if any(a is not b for a, b in zip(checked, (self.positions, self.inv_freq, self.axes))):
+            raise ValueError("a plan needs contiguous positions, inv_freq and axes: it reads the tensors handed to it on every step")
+        return rotation(*checked, bool(self.interleaved), float(self.scale))
+
+    def norm(self, layer: int, layers: int, q: torch.Tensor | None, k: torch.Tensor):
+        """The library's norm of one layer (None without one)."""
+        if self.eps is None:
+            if self.q_weight is not None or self.k_weight is not None or self.weight_offset != 0.0:
+                raise ValueError("the norm's weights need its eps")
+            return None
+        of = []
+        for name, weights, x in (("q_weight", self.q_weight, q), ("k_weight", self.k_weight, k)):
+            if weights is not None and (x is None or len(weights) != layers):
+                raise ValueError(f"{name} must have one weight per layer ({layers})")
+            w = None if weights is None else weights[layer]
+            if check_weight(w, f"layer {layer}: {name}", 0 if x is None else x.shape[1], k if x is None else x) is not w:
+                raise ValueError(f"layer {layer}: {name} must have its last dim contiguous")
+            of.append(w)
+        return head_norm(*of, float(self.eps), float(self.weight_offset))
+
+    def check(self) -> None:
+        if self.eps is None and self.inv_freq is None:
+            raise ValueError("heads need a norm (eps) or a rotation (inv_freq)")
+
+
+def _rows(*tensors) -> tuple:
+    return tuple(x for t in tensors for x in (t.data_ptr(), t.stride(0), t.stride(1)))
+
+
+def _append_heads(cache, key, value, slots: int, q, norm, how, tokens: int) -> tuple:
+    """wkv_rotary_append's arguments but the stream: the queries in place, key and value as they are."""
+    return (ctypes.byref(cache.descriptor()), *_rows(key, value), slots, *_rows(q, q), q.shape[1], norm, how, tokens)
 
 
 class _Live:
@@ -102,13 +167,16 @@ class DecodeStep:
     computes it from the block manager's reference counts once per step). The
     group-aware decode sets its own: each group's prompt cached, the members' own
     tokens streamed.
+
+    With ``heads`` the queries and keys come as the projections leave them: a layer's append norms and turns
+    them (``wkv_rotary_append``: ``q[l]`` in place, ``key[l]`` left as it is), then the attention runs without an append.
     """
 
     def __init__(self, caches: list[PagedKVCache], q: list[torch.Tensor], key: list[torch.Tensor],
                  value: list[torch.Tensor], out: list[torch.Tensor], block_table: torch.Tensor,
                  seq_lens: torch.Tensor, slot_mapping: torch.Tensor, scale: float, max_seq_len: int,
                  partition_size: int = 0, *, group_size: int = 0, prefix_lens: torch.Tensor | None = None,
-                 max_prefix_len: int = 0, order_by_length: bool | None = None) -> None:
+                 max_prefix_len: int = 0, order_by_length: bool | None = None, heads: Heads | None = None) -> None:
         if not caches:
             raise ValueError("no layers")
         dev = caches[0].device
@@ -145,6 +213,9 @@ class DecodeStep:
         self.order = torch.arange(batch, dtype=torch.int32, device=dev)
         order_ptr = self.order.data_ptr() if self.ordered else None
         self.calls: list[_LayerCall] = []
+        self.heads = heads
+        if heads is not None:
+            heads.check()
         for layer, cache in enumerate(caches):
             qq, kk, vv, oo = q[layer], key[layer], value[layer], out[layer]
             for name, t, shape in (("q", qq, (batch, hq, cache.head_dim)), ("out", oo, (batch, hq, cache.head_dim)),
@@ -156,6 +227,11 @@ class DecodeStep:
             append_args = (ctypes.byref(cache.descriptor()), kk.data_ptr(), kk.stride(0), kk.stride(1),
                            vv.data_ptr(), vv.stride(0), vv.stride(1), slot_mapping.data_ptr(), slot_mapping.numel(),
                            self.stream)
+            if heads is not None:
+                fn = lib.wkv_rotary_append
+                append_args = (*_append_heads(cache, kk, vv, slot_mapping.data_ptr(), qq,
+                                              heads.norm(layer, len(caches), qq, kk),
+                                              heads.rotation(batch, cache.head_dim, dev), batch), self.stream)
             tail = (qq.data_ptr(), qq.stride(0), qq.stride(1), oo.data_ptr(), hq,
                     self.block_table.data_ptr(), self.block_table.stride(0), self.block_table.shape[1],
                     self.seq_lens.data_ptr(), batch, int(max_seq_len), ctypes.c_float(scale),
@@ -210,7 +286,11 @@ class DecodeStep:
             _lib.check(rc, f"decode layer {layer}")
 
     def step_layer(self, layer: int, shared_blocks: bool | None = None) -> None:
-        """Append + attention of one layer in a single launch (plus the partition merge)."""
+        """Append + attention of one layer in a single launch (plus the partition merge); with ``heads`` in two."""
+        if self.heads is not None:
+            self.append(layer)
+            self.attend(layer, shared_blocks)
+            return
         self._live.check(layer)
         c = self.calls[layer]
         fn = self.lib.wkv_paged_decode_gqa_grouped if self.grouped else self.lib.wkv_append_paged_decode_gqa
@@ -249,7 +329,8 @@ class GraphDecodeStep:
     default). Every call on a GPU shares that GPU's scratch: two plans' replays must
     not overlap (one stream, or ordered). Geometries whose partials exceed the scratch
     (``wkv_decode_workspace_size`` > ``WKV_NOALLOC_SCRATCH_BYTES``) are refused. The
-    group-aware decode is not captured here.
+    group-aware decode is not captured here. A plan with ``heads`` is captured with its queries and keys normed and
+    turned in place before the fused append (so ``key`` is refilled for every replay, as ``q`` is).
     """
 
     def __init__(self, step: DecodeStep, *, shared_blocks: bool | None = None) -> None:
@@ -301,6 +382,13 @@ class GraphDecodeStep:
             if step.ordered:
                 _lib.check(lib.wkv_decode_order(sl.data_ptr(), batch, step.order.data_ptr(), cur), "decode order")
             for layer, args in enumerate(calls(cur)):
+                if step.heads is not None:
+                    qq, kk, h = q[layer], key[layer], step.heads
+                    rows = (1, *_rows(qq, qq), qq.shape[1], *_rows(kk, kk), kk.shape[1], qq.shape[2])
+                    how = h.rotation(batch, qq.shape[2], dev)
+                    norm = h.norm(layer, len(caches), qq, kk)
+                    _lib.check(lib.wkv_rotary_axes(*rows, how, batch, cur) if norm is None
+                               else lib.wkv_norm_rotary(*rows, norm, how, batch, cur), f"heads of layer {layer}")
                 _lib.check(fn(*args), f"allocation-free append+decode layer {layer}")
         torch.cuda.current_stream(dev).wait_stream(capture)
 
@@ -312,13 +400,19 @@ class GraphDecodeStep:
 
 class MLADecodeStep:
     """Pre-validated MLA decode for every layer: append one latent entry per
-    sequence, then weight-absorbed attention over the latent cache."""
+    sequence, then weight-absorbed attention over the latent cache. With ``heads`` the
+    append norms the entries (where its ``eps`` is given) and turns ``k_pe``, and ``q_pe`` in place
+    (``wkv_mla_rotary_append``); the attention then runs without an append."""
 
     def __init__(self, caches, q_nope: list[torch.Tensor], q_pe: list[torch.Tensor], kv_c: list[torch.Tensor],
                  k_pe: list[torch.Tensor], out: list[torch.Tensor], block_table: torch.Tensor, seq_lens: torch.Tensor,
-                 slot_mapping: torch.Tensor, scale: float, max_seq_len: int, partition_size: int = 0) -> None:
+                 slot_mapping: torch.Tensor, scale: float, max_seq_len: int, partition_size: int = 0, *,
+                 heads: Heads | None = None) -> None:
         if not caches:
             raise ValueError("no layers")
+        if heads is not None and heads.inv_freq is None:
+            raise ValueError("heads of an MLA plan need a rotation")
+        self.heads = heads
         c0 = caches[0]
         dev = c0.device
         self.block_table, self.seq_lens = check_tables(block_table, seq_lens, dev, c0.block_size, strict=True)
@@ -327,9 +421,9 @@ class MLADecodeStep:
         if not len(q_nope) == len(q_pe) == len(kv_c) == len(k_pe) == len(out) == len(caches):
             raise ValueError("q_nope, q_pe, kv_c, k_pe and out need one tensor per layer")
         self._live = _Live(caches)
-        heads = q_nope[0].shape[1]
+        heads_n = q_nope[0].shape[1]
         lib = _lib.load()
-        need = lib.wkv_mla_workspace_size(batch, heads, c0.kv_lora_rank, max_seq_len, int(partition_size))
+        need = lib.wkv_mla_workspace_size(batch, heads_n, c0.kv_lora_rank, max_seq_len, int(partition_size))
         if need < 0:
             raise ValueError("invalid MLA decode geometry")
         self.workspace = _workspace(dev, need)
@@ -338,9 +432,9 @@ class MLADecodeStep:
         self.calls = []
         for layer, cache in enumerate(caches):
             qn, qp, kc, kp, oo = q_nope[layer], q_pe[layer], kv_c[layer], k_pe[layer], out[layer]
-            for name, t, shape in (("q_nope", qn, (batch, heads, cache.kv_lora_rank)),
-                                   ("q_pe", qp, (batch, heads, cache.rope_dim)),
-                                   ("out", oo, (batch, heads, cache.kv_lora_rank)),
+            for name, t, shape in (("q_nope", qn, (batch, heads_n, cache.kv_lora_rank)),
+                                   ("q_pe", qp, (batch, heads_n, cache.rope_dim)),
+                                   ("out", oo, (batch, heads_n, cache.kv_lora_rank)),
                                    ("kv_c", kc, (slot_mapping.numel(), cache.kv_lora_rank)),
                                    ("k_pe", kp, (slot_mapping.numel(), cache.rope_dim))):
                 if t.dtype != torch.bfloat16 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != dev:
@@ -349,18 +443,22 @@ class MLADecodeStep:
             append_args = (desc, kc.data_ptr(), kc.stride(0), kp.data_ptr(), kp.stride(0), slot_mapping.data_ptr(),
                            slot_mapping.numel(), self.stream)
             decode_args = (desc, qn.data_ptr(), qn.stride(0), qn.stride(1), qp.data_ptr(), qp.stride(0), qp.stride(1),
-                           oo.data_ptr(), heads, self.block_table.data_ptr(), self.block_table.stride(0),
+                           oo.data_ptr(), heads_n, self.block_table.data_ptr(), self.block_table.stride(0),
                            self.block_table.shape[1], self.seq_lens.data_ptr(), batch, int(max_seq_len),
                            ctypes.c_float(scale), int(partition_size), self.workspace.data_ptr(),
                            self.workspace.numel(), self.stream)
             fused_args = (desc, kc.data_ptr(), kc.stride(0), kp.data_ptr(), kp.stride(0), slot_mapping.data_ptr(),
                           *decode_args[1:])
+            if heads is not None:
+                append_args = (*append_args[:6], *_rows(qp, qp), heads_n, heads.norm(layer, len(caches), None, kc),
+                               heads.rotation(batch, cache.rope_dim, dev), batch, self.stream)
             self.calls.append((append_args, decode_args, fused_args))
         self._keep = (caches, q_nope, q_pe, kv_c, k_pe, out, slot_mapping)
 
     def append(self, layer: int) -> None:
         self._live.check(layer)
-        rc = self.lib.wkv_mla_append(*self.calls[layer][0])
+        fn = self.lib.wkv_mla_append if self.heads is None else self.lib.wkv_mla_rotary_append
+        rc = fn(*self.calls[layer][0])
         if rc:
             _lib.check(rc, f"mla append layer {layer}")
 
@@ -371,7 +469,11 @@ class MLADecodeStep:
             _lib.check(rc, f"mla decode layer {layer}")
 
     def step_layer(self, layer: int) -> None:
-        """Latent append + attention of one layer in a single launch (plus the partition merge)."""
+        """Latent append + attention of one layer in a single launch (plus the partition merge); with ``heads`` in two."""
+        if self.heads is not None:
+            self.append(layer)
+            self.attend(layer)
+            return
         self._live.check(layer)
         rc = self.lib.wkv_append_paged_decode_mla(*self.calls[layer][2])
         if rc:
@@ -389,13 +491,14 @@ class PrefillStep:
     ``q[l]`` ``[T, Hq, D]``, ``key[l]`` / ``value[l]`` ``[T, Hkv, D]`` and
     ``out[l]`` are layer ``l``'s buffers; ``cu_seqlens_q [B+1]`` int32 splits
     the ``T`` rows by sequence and ``slot_mapping [T]`` places them. ``max_query_len`` and
-    ``max_seq_len`` are upper bounds of the lengths in the buffers, as for ``prefill_gqa``.
+    ``max_seq_len`` are upper bounds of the lengths in the buffers, as for ``prefill_gqa``. With ``heads`` the
+    queries and keys come as the projections leave them, as for ``DecodeStep``.
     """
 
     def __init__(self, caches: list[PagedKVCache], q: list[torch.Tensor], key: list[torch.Tensor],
                  value: list[torch.Tensor], out: list[torch.Tensor], block_table: torch.Tensor,
                  seq_lens: torch.Tensor, cu_seqlens_q: torch.Tensor, slot_mapping: torch.Tensor, scale: float,
-                 max_query_len: int, max_seq_len: int) -> None:
+                 max_query_len: int, max_seq_len: int, *, heads: Heads | None = None) -> None:
         if not caches:
             raise ValueError("no layers")
         dev = caches[0].device
@@ -411,6 +514,9 @@ class PrefillStep:
             raise ValueError("q, key, value and out need one tensor per layer")
         self._live = _Live(caches)
         T = slot_mapping.numel()
+        self.heads = heads
+        if heads is not None:
+            heads.check()
         self.lib = lib = _lib.load()
         self.stream = torch.cuda.current_stream(dev).cuda_stream
         need = max(lib.wkv_prefill_workspace_size(
@@ -436,8 +542,13 @@ class PrefillStep:
                     self.block_table.stride(0), self.block_table.shape[1], batch, int(max_query_len),
                     int(max_seq_len), ctypes.c_float(scale), *split, self.stream)
             fn = lib.wkv_append_fp8 if cache.kv_dtype == "fp8_e4m3" else lib.wkv_append
-            self.calls.append((fn, (desc, *kv, T, self.stream), (desc, *kv, T, *tail),
-                               (desc, None, 0, 0, None, 0, 0, None, 0, *tail)))
+            append_args = (desc, *kv, T, self.stream)
+            if heads is not None:
+                fn = lib.wkv_rotary_append
+                append_args = (*_append_heads(cache, kk, vv, slot_mapping.data_ptr(), qq,
+                                              heads.norm(layer, len(caches), qq, kk),
+                                              heads.rotation(T, cache.head_dim, dev), T), self.stream)
+            self.calls.append((fn, append_args, (desc, *kv, T, *tail), (desc, None, 0, 0, None, 0, 0, None, 0, *tail)))
         self._keep = (caches, q, key, value, out, cu_seqlens_q, slot_mapping)
 
     def append(self, layer: int) -> None:
@@ -455,6 +566,10 @@ class PrefillStep:
 
     def step_layer(self, layer: int) -> None:
         """Append + causal attention of one layer (two launches: the append, then the attention)."""
+        if self.heads is not None:
+            self.append(layer)
+            self.attend(layer)
+            return
         self._live.check(layer)
         rc = self.lib.wkv_prefill_gqa_shared(*self.calls[layer][2])
         if rc:
@@ -474,7 +589,8 @@ class TreeStep:
     layer once its ``q[l]`` ``[T, Hq, D]``, ``key[l]`` / ``value[l]`` ``[T, Hkv, D]`` are there: queries and keys
     are turned in place by their positions (``inv_freq`` from ``rotary_frequencies``; None: they come
     turned), keys and values appended, and ``out[l]`` is their attention over context and tree
-    (``paged_tree_gqa``) --, then ``finish()`` once ``target_tokens`` holds what was sampled after every
+    (``paged_tree_gqa``; with ``heads``, whose positions are the step's, queries and keys are normed and turned
+    by the append itself, ``q[l]`` in place, ``key[l]`` left as it is) --, then ``finish()`` once ``target_tokens`` holds what was sampled after every
     node: the path that agrees is accepted (``accept_tree``), its keys and values move together in every layer's
     cache (``compact``) and ``state.seq_lens`` moves on. ``maps`` and ``accepted`` are the step's results;
     ``state.next_tokens`` are the next step's first nodes: what was sampled after the accepted path, and what
@@ -494,7 +610,8 @@ class TreeStep:
                  value: list[torch.Tensor], out: list[torch.Tensor], state: StepState, new_lens: torch.Tensor,
                  parents: torch.Tensor, draft_tokens: torch.Tensor, target_tokens: torch.Tensor, scale: float,
                  max_nodes: int, max_seq_len: int, max_depth: int, *, inv_freq: torch.Tensor | None = None,
-                 rotary_scale: float = 1.0, interleaved: bool = False, shared_blocks: bool | None = None) -> None:
+                 rotary_scale: float = 1.0, interleaved: bool = False, shared_blocks: bool | None = None,
+                 heads: Heads | None = None) -> None:
         if not caches:
             raise ValueError("no layers")
         if not len(q) == len(key) == len(value) == len(out) == len(caches):
@@ -518,6 +635,10 @@ class TreeStep:
         if inv_freq is not None and (inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.device != dev
                                      or not inv_freq.is_contiguous()):
             raise ValueError(f"inv_freq must be a contiguous float64 vector on {dev}")
+        if heads is not None:
+            heads.check()
+            if inv_freq is not None or heads.positions is not None or heads.axes is not None:
+                raise ValueError("heads bring their own inv_freq, and no positions or axes: they are the step's")
         pending = state.next_tokens
         if pending is not None and (pending.dtype != torch.int64 or tuple(pending.shape) != (batch,)
                                     or not pending.is_contiguous() or pending.device != dev):
@@ -555,13 +676,20 @@ class TreeStep:
                 turned = (x for t in (qq, kk) for x in (t.data_ptr(), t.stride(0), t.stride(1)) * 2 + (t.shape[1],))
                 rotary = (1, *turned, d, m.positions.data_ptr(), inv_freq.data_ptr(), 2 * inv_freq.shape[0], int(interleaved), 0,
                           ctypes.c_float(rotary_scale), T)
-            attend = (ctypes.byref(cache.descriptor(shared_blocks)), kk.data_ptr(), kk.stride(0), kk.stride(1),
-                      vv.data_ptr(), vv.stride(0), vv.stride(1), m.slot_mapping.data_ptr(), T, qq.data_ptr(),
+            new = (kk.data_ptr(), kk.stride(0), kk.stride(1), vv.data_ptr(), vv.stride(0), vv.stride(1),
+                   m.slot_mapping.data_ptr(), T)
+            if heads is not None:
+                how = None if heads.inv_freq is None else replace(heads, positions=m.positions).rotation(T, d, dev)
+                rotary = _append_heads(cache, kk, vv, m.slot_mapping.data_ptr(), qq, heads.norm(layer, len(caches), qq, kk),
+                                       how, T)
+                new = (None, 0, 0, None, 0, 0, None, 0)
+            attend = (ctypes.byref(cache.descriptor(shared_blocks)), *new, qq.data_ptr(),
                       qq.stride(0), qq.stride(1), oo.data_ptr(), oo.stride(0), oo.stride(1), hq,
                       m.cu_seqlens_q.data_ptr(), m.context_lens.data_ptr(), bt.data_ptr(), bt.stride(0), bt.shape[1],
                       batch, min(max_nodes, T), longest, m.tree_mask.data_ptr(), m.tree_mask.shape[1],
                       ctypes.c_float(scale), self.workspace.data_ptr() if need > 0 else None, need, None)
             self.calls.append((rotary, attend))
+        self.heads = heads
         self._keep = (q, key, value, out, inv_freq)
 
     def begin(self) -> None:
@@ -576,7 +704,7 @@ class TreeStep:
         with _on(self.device):
             stream = _stream(self.device)
             if rotary is not None:
-                rc = self.lib.wkv_rotary(*rotary, stream)
+                rc = (self.lib.wkv_rotary if self.heads is None else self.lib.wkv_rotary_append)(*rotary, stream)
                 if rc:
                     _lib.check(rc, f"rotary layer {layer}")
             rc = self.lib.wkv_tree_gqa(*attend, stream)
