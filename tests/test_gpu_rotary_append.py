@@ -1,5 +1,6 @@
 """The append with norm and rotation on the way: the queries and keys against the float64 oracle (bounds:
-headcase.py), the cache bit for bit against the oracle's append of the keys that norm_rotary rounds."""
+headcase.py), the cache bit for bit against the oracle's append of the keys that norm_rotary rounds (without a norm: that a
+bf16 cache holds, each at a slot of its own)."""
 
 import numpy as np
 import pytest
@@ -8,7 +9,7 @@ from headcase import U, check, check_forward, f64, size
 from kvcase import assert_guards, bits_of, guard_cache
 
 from oracle import heads, paged
-from wavelet_amd import (MLALatentCache, PagedKVCache, apply_rotary, mla_rotary_append, norm_rotary, paged_decode_gqa,
+from wavelet_amd import (MLALatentCache, PagedKVCache, mla_rotary_append, norm_rotary, paged_decode_gqa,
                          prefill_gqa, rotary_append, rotary_axes, rotary_frequencies)
 
 pytestmark = pytest.mark.gpu
@@ -70,7 +71,7 @@ def _run(cuda, q, key, value, c, slots, w, pos, freq, eps, **how):
     guards = guard_cache(c)
     norm = {} if eps is None else dict(q_weight=w[0], k_weight=w[1], eps=eps)
     if eps is None:
-        want_q, want_k = apply_rotary(q, key, pos, freq, **how)
+        want_q, want_k = _turned(cuda, q, key, value, pos, freq, how)
     else:
         want_q, want_k = norm_rotary(q, key, pos, freq, **norm, **how)
     want = _expected(c, want_k, value, slots)
@@ -83,6 +84,19 @@ def _run(cuda, q, key, value, c, slots, w, pos, freq, eps, **how):
     for a, b in zip((q, key, value), before):
         assert torch.equal(a, b)
     return got
+
+
+def _turned(cuda, q, key, value, pos, freq, how):
+    """Queries and keys as they are turned without a norm, checked against the oracle."""
+    tokens, hk, d = key.shape
+    c = PagedKVCache(-(-tokens // 16), 16, hk, d, device=cuda)
+    got = rotary_append(q, key, value, c, torch.arange(tokens, device=cuda), pos, freq, **how)
+    k = c.k.permute(0, 3, 1, 2, 4).reshape(-1, hk, d)[:tokens].contiguous()
+    axes, inter, scale = how.get("axes"), how.get("interleaved", False), how.get("scale", 1.0)
+    angle = heads.phases(f64(pos), f64(freq), None if axes is None else axes.cpu().numpy())
+    for y, x in ((got, q), (k, key)):
+        check(y, heads.turn(f64(x), angle, inter, scale), 16 * U * size(f64(x), angle.shape[1], inter, scale), "turned")
+    return got, k
 
 
 SHAPES = [  # head layout, new tokens, contexts, block size

@@ -9,7 +9,7 @@ import pytest
 import torch
 from kvcase import bits_of
 
-from wavelet_amd import KVPool, MLALatentCache, PagedKVCache, apply_rotary, norm_rotary, rotary_axes, rotary_frequencies
+from wavelet_amd import KVPool, MLALatentCache, PagedKVCache, mla_rotary_append, norm_rotary, rotary_axes, rotary_frequencies
 from wavelet_amd.plan import DecodeStep, GraphDecodeStep, Heads, MLADecodeStep, PrefillStep, TreeStep
 
 pytestmark = pytest.mark.gpu
@@ -173,7 +173,10 @@ def test_latent_decode(cuda):
                 bufs[0][j][layer].normal_(generator=g)
                 bufs[1][j][layer].copy_(bufs[0][j][layer])
             qp, kc, kp = bufs[1][1][layer], bufs[1][2][layer], bufs[1][3][layer]
-            apply_rotary(qp, kp[:, None], pos, freq, interleaved=True, out=(qp, kp[:, None]))
+            # (turned without a norm: apply_rotary's angles are rounded otherwise)
+            alone = MLALatentCache(1, BS, device=cuda)
+            mla_rotary_append(qp, kc, kp, alone, torch.arange(3, device=cuda), pos, freq, interleaved=True, out=qp)
+            kp.copy_(alone.latent[0, :3, 512:])
             norm_rotary(kc[:, None], None, q_weight=weights[layer], eps=1e-6, out=(kc[:, None], None))
         for s in steps:
             s.run()

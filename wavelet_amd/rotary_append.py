@@ -70,8 +70,8 @@ def rotary_append(q: torch.Tensor | None, key: torch.Tensor, value: torch.Tensor
     projection read in place. The norm is ``norm_rotary``'s and is done where ``eps`` is given, the rotation
     ``apply_rotary``'s and done where ``positions`` and ``inv_freq`` are; one of them at least. The attention then takes the
     result and no ``key`` / ``value`` (``paged_decode_gqa``, ``prefill_gqa``, ``paged_tree_gqa``). ``key`` and ``value`` are left
-    as they are, and the cache holds what ``norm_rotary`` (``apply_rotary``) and ``cache.append`` would leave in it, bf16 or fp8.
-    A slot appears once in a call.
+    as they are, and the cache, bf16 or fp8, holds what ``norm_rotary`` and ``cache.append`` would leave in it, bit for bit
+    (without a norm what ``apply_rotary`` and ``cache.append`` would, but for a key's last bit). A slot appears once in a call.
     """
     if not isinstance(cache, PagedKVCache):
         raise ValueError("cache must be a PagedKVCache (mla_rotary_append appends to latent caches)")
