@@ -43,10 +43,10 @@ from .attention import (decode_order, decode_plan, grouped_decode_order, paged_d
                         paged_decode_mla, paged_tree_gqa, prefill_gqa)
 from .blocks import BlockManager
 from .cache import MLALatentCache, PagedKVCache, validate_group_prefix, validate_tables
-from .norm_rotary import norm_rotary
+from .heads import norm_rotary
 from .pool import KVPool
 from .rotary import apply_rotary, rotary_axes, rotary_frequencies
-from .rotary_append import mla_rotary_append, rotary_append
+from .head_append import mla_rotary_append, rotary_append
 from .sampler import sample
 from .step import Accepted, StepMaps, StepState, accept_tree, extend_tables
 

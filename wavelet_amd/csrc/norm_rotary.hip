@@ -400,7 +400,7 @@ extern "C" int wkv_norm_rotary(int32_t dtype, const void *q, int64_t q_stride_t,
              norm->q_weight_stride_h, num_q_heads, gq.log_tg, gq.per, fast_div(gq.splits)};
   a.k = Kind{HeadRows{k, k_out, k_stride_t, k_stride_h, ko_stride_t, ko_stride_h}, norm->k_weight,
              norm->k_weight_stride_h, num_k_heads, gk.log_tg, gk.per, fast_div(gk.splits)};
-  WKV_CHECK_ARG(gq.wgs + gk.wgs <= INT32_MAX, "too many tokens and heads for one launch");
+  WKV_CHECK_ARG(gq.wgs + gk.wgs <= kMaxWorkgroups, "too many tokens and heads for one launch");
   a.q_wgs = static_cast<int>(gq.wgs);
   const bool each = (norm->q_weight != nullptr && norm->q_weight_stride_h != 0) ||
                     (norm->k_weight != nullptr && norm->k_weight_stride_h != 0);
@@ -513,7 +513,7 @@ extern "C" int wkv_norm_rotary_backward(int32_t dtype, const void *q, int64_t q_
     a.q = kind(rq, norm->q_weight, norm->q_weight_stride_h, num_q_heads, q_each, gq, 0);
     a.k = kind(rk, norm->k_weight, norm->k_weight_stride_h, num_k_heads, k_each, gk, static_cast<int64_t>(gq.wgs) * gq.rows);
     const int64_t grid = static_cast<int64_t>(a.q.ranges) * a.q.wgs + static_cast<int64_t>(a.k.ranges) * a.k.wgs;
-    WKV_CHECK_ARG(grid <= INT32_MAX, "too many tokens and heads for one launch");
+    WKV_CHECK_ARG(grid <= kMaxWorkgroups, "too many tokens and heads for one launch");
     const bool far = num_tokens * H * head_dim * esz >= (64 << 20);
     const int log_tg = a.q.log_tg > a.k.log_tg ? a.q.log_tg : a.k.log_tg;
     const size_t turns = (static_cast<size_t>(kNormWaves) << log_tg) * half * sizeof(float2);

@@ -513,6 +513,9 @@ inline RowUnits row_units(int D, int half, int v) {
   return r;
 }
 
+// Workgroups of a launch: 2^32 work items.
+constexpr int64_t kMaxWorkgroups = (1 << 24) - 1;
+
 // Waves over the tokens and heads of a kind, four a workgroup: a token a wave (its heads lie together; by_token: as many as
 // the wave's groups, whose stores of one head then lie together in a cache), and with too few tokens for the chip the heads
 // dealt over more waves, down to a round of the wave's groups below 4,096 waves (four a SIMD), to two

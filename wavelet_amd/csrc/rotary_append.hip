@@ -646,7 +646,7 @@ extern "C" int wkv_rotary_append(const wkv_cache_t *cache, const void *key, int6
     const size_t need = kValueWindow * (D * 2 + 8) + kValueWindow * sizeof(int64_t) + kValueWindow / 8 * sizeof(int);
     lds = lds > need ? lds : need;
   }
-  WKV_CHECK_ARG(gq.wgs + k_wgs + rest <= INT32_MAX, "too many tokens and heads for one launch");
+  WKV_CHECK_ARG(gq.wgs + k_wgs + rest <= kMaxWorkgroups, "too many tokens and heads for one launch");
   a.k_wgs = static_cast<int>(k_wgs);
   a.v_wgs = static_cast<int>(rest);
   const unsigned grid = static_cast<unsigned>(gq.wgs + k_wgs + rest);
@@ -728,7 +728,7 @@ extern "C" int wkv_mla_rotary_append(const wkv_mla_cache_t *cache, const void *k
              fast_div(gq.splits)};
   a.k = Kind{HeadRows{k_pe, nullptr, k_pe_stride, 0, 0, 0}, nullptr, 0, 1, gk.log_tg, gk.per, fast_div(gk.splits)};
   const int64_t rest = (num_tokens + kWaves - 1) / kWaves;
-  WKV_CHECK_ARG(gq.wgs + gk.wgs + rest <= INT32_MAX, "too many tokens and heads for one launch");
+  WKV_CHECK_ARG(gq.wgs + gk.wgs + rest <= kMaxWorkgroups, "too many tokens and heads for one launch");
   a.entry_wgs = static_cast<int>(rest);
   a.k_wgs = static_cast<int>(gk.wgs);
   const unsigned grid = static_cast<unsigned>(gq.wgs + gk.wgs + rest);

@@ -13,7 +13,7 @@ import torch
 
 from . import _lib
 from .cache import MLALatentCache, PagedKVCache, _on, _require_cuda, _slots, _stream, _token_rows
-from .norm_rotary import check_weight, head_norm
+from .heads import check_weight, head_norm
 from .rotary import _dual, check_rotation, rotation
 
 
@@ -71,7 +71,8 @@ def rotary_append(q: torch.Tensor | None, key: torch.Tensor, value: torch.Tensor
     ``apply_rotary``'s and done where ``positions`` and ``inv_freq`` are; one of them at least. The attention then takes the
     result and no ``key`` / ``value`` (``paged_decode_gqa``, ``prefill_gqa``, ``paged_tree_gqa``). ``key`` and ``value`` are left
     as they are, and the cache, bf16 or fp8, holds what ``norm_rotary`` and ``cache.append`` would leave in it, bit for bit
-    (without a norm what ``apply_rotary`` and ``cache.append`` would, but for a key's last bit). A slot appears once in a call.
+    (without a norm what ``apply_rotary`` and ``cache.append`` would, but for a key's last bit). A slot appears once in a call, a
+    block of an fp8 cache in one run of it (as for ``cache.append``).
     """
     if not isinstance(cache, PagedKVCache):
         raise ValueError("cache must be a PagedKVCache (mla_rotary_append appends to latent caches)")

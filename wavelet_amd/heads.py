@@ -46,18 +46,6 @@ def head_norm(q_weight, k_weight, eps: float, offset: float) -> _lib.WkvHeadNorm
     return _lib.WkvHeadNorm(qw, kw, qs, ks, dtype, offset, eps, 0)
 
 
-def _rows(x: torch.Tensor | None, *others):
-    """Pointers and strides of a kind of heads: of x and of what goes with it (None: not there)."""
-    out = []
-    for t in (x, *others):
-        out += (None, 0, 0) if t is None else (t.data_ptr(), *t.stride()[:2])
-    return (*out, 0 if x is None else x.shape[1])
-
-
-def _packed(x):
-    return x if x is None or x.stride(-1) == 1 else x.contiguous()
-
-
 def _forward(q, k, q_weight, k_weight, rotary, interleaved, scale, eps, offset, out):
     """One launch over checked tensors; rotary: (positions, inv_freq, axes), or None: only normed."""
     tokens, hq, d = q.shape
@@ -88,6 +76,35 @@ def _forward(q, k, q_weight, k_weight, rotary, interleaved, scale, eps, offset, 
     return out
 
 
+def _grad_rows(x, g, want: bool):
+    """A kind's part of the backward call: its result (None: not wanted), and pointers, strides and heads (x None: none)."""
+    if x is None:
+        return None, (None, 0, 0, None, 0, 0, None, 0, 0, 0)
+    xt, xh, last = x.stride()
+    if last != 1:
+        x = x.contiguous()
+        xt, xh, _ = x.stride()
+    gt, gh, last = g.stride()
+    if last != 1:
+        g = g.contiguous()
+        gt, gh, _ = g.stride()
+    if not want:
+        return (None, x, g), (x.data_ptr(), xt, xh, g.data_ptr(), gt, gh, None, 0, 0, x.shape[1])
+    d = torch.empty_like(x, memory_format=torch.contiguous_format)
+    dt, dh, _ = d.stride()
+    return (d, x, g), (x.data_ptr(), xt, xh, g.data_ptr(), gt, gh, d.data_ptr(), dt, dh, x.shape[1])
+
+
+def _weight_grad(x, w, want: bool):
+    """A weight's gradient, empty, and its pointer (None: not wanted; no head, no sum)."""
+    if not want or x is None or w is None:
+        return None, None
+    if x.shape[1] == 0:
+        return torch.zeros_like(w), None
+    d = torch.empty_like(w, memory_format=torch.contiguous_format)
+    return d, d.data_ptr()
+
+
 def _backward(q, k, gq, gk, q_weight, k_weight, rotary, interleaved, scale, eps, offset, need):
     """The gradients (dq, dk, dq_weight, dk_weight) that ``need`` asks for; gq or gk None: zero."""
     if gq is None:
@@ -95,30 +112,28 @@ def _backward(q, k, gq, gk, q_weight, k_weight, rotary, interleaved, scale, eps,
     if gk is None:
         k = None
     some = k if q is None else q
-    dev, (tokens, _, d) = some.device, some.shape
-    q, k, gq, gk = (_packed(x) for x in (q, k, gq, gk))
-    dq, dk = (torch.empty_like(x, memory_format=torch.contiguous_format) if x is not None and n else None
-              for x, n in zip((q, k), need))
-    wants = [w if x is not None and n else None for x, w, n in zip((q, k), (q_weight, k_weight), need[2:])]
-    dqw, dkw = (w if w is None else torch.empty_like(w, memory_format=torch.contiguous_format) if x.shape[1]
-                else torch.zeros_like(w) for x, w in zip((q, k), wants))
-    wants = [w if w is not None and x.shape[1] else None for x, w in zip((q, k), wants)]  # (no head, no sum)
-    each = [int(x is not None and w is not None and w.dim() == 2) for x, w in zip((q, k), (q_weight, k_weight))]
+    dev = some.device
+    tokens, _, d = some.shape
+    keep_q, rows_q = _grad_rows(q, gq, need[0])  # (what was copied lives until the launch)
+    keep_k, rows_k = _grad_rows(k, gk, need[1])
+    dqw, dqw_ptr = _weight_grad(q, q_weight, need[2])
+    dkw, dkw_ptr = _weight_grad(k, k_weight, need[3])
     norm = head_norm(q_weight, k_weight, eps, offset)
     how = None if rotary is None else rotation(*rotary, interleaved, scale)
     lib = _lib.load()
-    ws, need_bytes = None, 0
-    if any(w is not None for w in wants):
-        need_bytes = lib.wkv_norm_rotary_workspace_size(tokens, 0 if q is None else q.shape[1],
-                                                        0 if k is None else k.shape[1], d, *each)
-        ws = torch.empty(need_bytes, dtype=torch.uint8, device=dev)
+    ws, size, ws_ptr = None, 0, None
+    if dqw_ptr is not None or dkw_ptr is not None:
+        size = lib.wkv_norm_rotary_workspace_size(tokens, rows_q[-1], rows_k[-1], d,
+                                                  q is not None and q_weight is not None and q_weight.dim() == 2,
+                                                  k is not None and k_weight is not None and k_weight.dim() == 2)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        ws_ptr = ws.data_ptr()
     with _on(dev):
-        rc = lib.wkv_norm_rotary_backward(
-            _DTYPES[some.dtype], *_rows(q, gq, dq), *_rows(k, gk, dk), d, norm, how,
-            *(None if w is None else dw.data_ptr() for w, dw in zip(wants, (dqw, dkw))), tokens,
-            None if ws is None else ws.data_ptr(), need_bytes, _stream(dev))
-    _lib.check(rc, "norm_rotary backward")
-    return dq, dk, dqw, dkw
+        rc = lib.wkv_norm_rotary_backward(_DTYPES[some.dtype], *rows_q, *rows_k, d, norm, how, dqw_ptr, dkw_ptr, tokens,
+                                          ws_ptr, size, _stream(dev))
+    if rc:
+        _lib.check(rc, "norm_rotary backward")
+    return None if q is None else keep_q[0], None if k is None else keep_k[0], dqw, dkw
 
 
 class _NormRotary(torch.autograd.Function):

@@ -24,7 +24,7 @@ import torch
 from . import _lib
 from .attention import _workspace, decode_plan
 from .cache import KV_DTYPES, PagedKVCache, _on, _require_cuda, _stream, check_tables
-from .norm_rotary import check_weight, head_norm
+from .heads import check_weight, head_norm
 from .rotary import check_rotation, rotation
 from .step import MAX_DEPTH, MAX_NODES, Accepted, StepState, accept_tree, new_step_maps
 

@@ -40,7 +40,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: dict 
     """``(inv_freq, scale)`` of a rotary embedding: float64 ``[rotary_dim / 2]`` on ``device`` (default: the
     current GPU), the angle that pair ``i`` gains per position, and the factor of the turned values.
 
-    Without ``scaling``: ``base ** (-2 i / rotary_dim)`` and 1. ``scaling`` is a model config's
+    Without ``scaling`` (and for ``"mrope"``, whose ``mrope_section`` is ``rotary_axes``'s):
+    ``base ** (-2 i / rotary_dim)`` and 1. ``scaling`` is a model config's
     ``rope_scaling`` dict, by its ``rope_type``:
 
     * ``"linear"``: positions divided by ``factor``;
@@ -107,8 +108,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: dict 
             scale = gain(float(scaling["mscale"])) / gain(float(scaling["mscale_all_dim"]))
         else:
             scale = gain(1.0)
-    elif kind not in ("default", "dynamic"):
-        raise NotImplementedError(f"rope scaling {kind!r} is not supported (linear, dynamic, llama3, yarn)")
+    elif kind not in ("default", "dynamic", "mrope"):
+        raise NotImplementedError(f"rope scaling {kind!r} is not supported (linear, dynamic, llama3, yarn, mrope)")
     dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     return torch.tensor(freq, dtype=torch.float64, device=dev), scale
 
