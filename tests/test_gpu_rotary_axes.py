@@ -63,6 +63,8 @@ def test_the_axes_of_pairs():
     assert rotary_axes((2, 3, 1), device="cpu").tolist() == [0, 0, 1, 1, 1, 2]
     assert rotary_axes((4, 2, 2), interleaved=True, device="cpu").tolist() == [0, 1, 2, 0, 1, 2, 0, 0]
     assert rotary_axes((4, 3, 1), interleaved=True, device="cpu").tolist() == [0, 1, 2, 0, 1, 0, 0, 1]
+    freq, scale = rotary_frequencies(16, 1e4, scaling=dict(type="mrope", mrope_section=[2, 3, 3]), device="cpu")
+    assert scale == 1.0 and torch.equal(freq, rotary_frequencies(16, 1e4, device="cpu")[0])
 
 
 def test_refusals(cuda):

@@ -42,10 +42,11 @@ __device__ __forceinline__ int64_t position_at(const Angles &a, int64_t t, int i
   return static_cast<unsigned>(ax) < static_cast<unsigned>(a.num_axes) ? a.pos[ax * a.axis_stride + t] : 0;
 }
 
-// Cosine and sine of a position's angle, times the scale: the angle in turns and its distance from the nearest quarter of one in
-// float64, then the Taylor series of that distance, at most pi / 4: to z^4 (sine) and z^5 (cosine) of its square z, whose
-// next terms are below 2^-28 of it and 2^-32. Off by at most 1.3 x 2^-24 (a float32 of half a turn alone by 1.6), 0.3 in the mean,
-// which decides how often a key's last bit, and its code, is the exact one's.
+// Cosine and sine of a position's angle, times the scale: the angle in turns and its distance from the
+// nearest quarter of one in float64, then the Taylor series of that distance, at most pi / 4: to z^4 (sine)
+// and z^5 (cosine) of its square z, whose next terms are below 2^-28 of it and 2^-32. Off by at most 1.3 x
+// 2^-24 (a float32 of half a turn alone by 1.6), 0.3 in the mean, which decides how often a key's last bit,
+// and its code, is the exact one's.
 __device__ __forceinline__ float2 angle_of(const Angles &a, int64_t pos, double freq) {
   const double x = static_cast<double>(pos) * freq * 0.15915494309189533577;  // 1 / 2 pi
   const double y = 4. * (x - rint(x)), n = rint(y);
@@ -272,8 +273,8 @@ __device__ __forceinline__ void unit_back(const UnitTurn<V> &t, bool all, float 
     turn(std::false_type{});
 }
 
-// The angles of tokens t0 .. t0 + nt - 1, thread `tid` of `threads`, while there are as many B at a time: their positions and frequencies
-// are all requested before the first is used.
+// The angles of tokens t0 .. t0 + nt - 1, thread `tid` of `threads`, while there are as many B at a time:
+// their positions and frequencies are all requested before the first is used.
 template <int B>
 __device__ __forceinline__ void angles_of(const Angles &a, int64_t t0, int nt, int tid, int threads, float2 *turn) {
   const int n = nt * a.half.d;
@@ -353,9 +354,9 @@ __device__ __forceinline__ WaveTile wave_tile(const Kind &k, const RowUnits &r, 
   return w;
 }
 
-// The heads first, first + step, .. below `heads` of the lane's token (there: it has one), normed (if norm.on) and turned by
-// turn[], N rows at a time, the next N in flight meanwhile; ready(): called once the first are, before turn[] is read.
-// EACH: each head's own weights.
+// The heads first, first + step, .. below `heads` of the lane's token (there: it has one), normed (if
+// norm.on) and turned by turn[], N rows at a time, the next N in flight meanwhile; ready(): called once the
+// first are, before turn[] is read. EACH: each head's own weights.
 template <class T, int V, bool INTER, int U, int N, bool FAR, bool NEAR_STORE, bool EACH, int LL, class Ready>
 __device__ __forceinline__ void norm_turn_heads(const RowUnits &ru, const HeadNorm &norm, const float2 *turn, bool there,
                                                 int first, int step, int heads, const HeadsOf<T> &of, Ready ready) {
@@ -516,11 +517,11 @@ inline RowUnits row_units(int D, int half, int v) {
 // Workgroups of a launch: 2^32 work items.
 constexpr int64_t kMaxWorkgroups = (1 << 24) - 1;
 
-// Waves over the tokens and heads of a kind, four a workgroup: a token a wave (its heads lie together; by_token: as many as
-// the wave's groups, whose stores of one head then lie together in a cache), and with too few tokens for the chip the heads
-// dealt over more waves, down to a round of the wave's groups below 4,096 waves (four a SIMD), to two
-// rounds below 16,384 (4,696 tokens of 128 heads of 64: 38.2 us, 45.4 a wave a token; 8,191 of 16 heads of 128, two rounds,
-// lose 1 us in halves).
+// Waves over the tokens and heads of a kind, four a workgroup: a token a wave (its heads lie together;
+// by_token: as many as the wave's groups, whose stores of one head then lie together in a cache), and with
+// too few tokens for the chip the heads dealt over more waves, down to a round of the wave's groups below
+// 4,096 waves (four a SIMD), to two rounds below 16,384 (4,696 tokens of 128 heads of 64: 38.2 us, 45.4 a
+// wave a token; 8,191 of 16 heads of 128, two rounds, lose 1 us in halves).
 struct KindGrid {
   int log_tg = 0, per = 1, splits = 1;
   int64_t waves = 0, wgs = 0;

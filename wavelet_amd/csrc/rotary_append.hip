@@ -2,12 +2,19 @@
 // positions on the way, and the queries to the attention, in one launch (gfx950).
 // The mathematics of heads: norm_rotary_dev.h; the fp8 rule: kv_append_dev.h.
 //
-// The workgroups of a launch have one of three roles. Queries, and the shared key of a latent cache: rows to rows.
-// Keys of a bf16 cache: a wave's tokens follow each other, so that the
-// 16-byte pieces that it stores of a head lie together in the cache. The rest: values (bf16: a window of 64 tokens of one head, transposed through LDS; few
-// tokens: an element at a time), keys and values (fp8, run by run, because a block's scale follows from all of
-// its new keys: a wave norms and turns 16 of them into LDS and codes them from there),
-// or a latent cache's compressed entries, normed.
+// The workgroups of a launch have one of three roles. Keys: of a bf16 cache as rows, several tokens a wave,
+// so that the 16-byte pieces that it stores of a head lie together in the cache; of an fp8 cache run by run,
+// because a block's scale follows from all of its new keys, coded from the registers in which they were
+// normed and turned. Values: in bf16 a window of 64 tokens of one head, transposed through LDS (few tokens:
+// an element at a time), in fp8 run by run. Queries: rows to rows. A latent cache has entries, a wave each,
+// in the place of values, and its shared key is a kind of one head.
+//
+// Prompts are bound by HBM: 8 of 2,048 tokens, 32/8 heads of 128, bf16: 79 us for 403 MB, 5.1 TB/s, as a
+// large copy (norm_rotary and append in turn: 65 + 34). Into fp8, 8,386 tokens of 28/4 heads take 37, of
+// which the queries alone are 27: a run's keys are a chain of round trips (slots, rows and positions, scale)
+// of 6.5 us in a wave, so the workgroups of keys and values come first and the queries' fill the chip beside
+// them (36.1 so, 41.1 behind them). Few tokens are bound by the launch and that chain (64 tokens bf16: 5.0
+// us; 5 tokens fp8: 6.3).
 #include <type_traits>
 
 #include "kv_append_dev.h"
@@ -39,7 +46,7 @@ struct Slots {
 };
 
 struct AppendArgs {
-  Kind q, k;       // q.s.y: the queries' result; k.s.x: the keys
+  Kind q, k;         // q.s.y: the queries' result; k.s.x: the keys
   int k_wgs, v_wgs;  // workgroups of keys, and of values; queries behind them
   const uint16_t *key, *val;
   int64_t kst, ksh, vst, vsh;
@@ -52,7 +59,7 @@ struct AppendArgs {
   void *kc, *vc;
   float *ks, *vs;
   int BS;
-  int window;  // tokens of a workgroup of the last role
+  int window;  // tokens of a workgroup of values (and of fp8 keys)
 };
 
 // Queries to rows (K false), or keys to a bf16 cache.
@@ -166,8 +173,8 @@ __device__ __forceinline__ void values_role(const AppendArgs &a, int wg, uint8_t
 // fp8 keys and values.
 constexpr int kPiece = 16;  // tokens of a run taken at a time
 
-// Codes of bf16 bits times inv, by the hardware's conversion; a NaN, which that codes with a sign of its own, as 0x7f and the
-// NaN's sign.
+// Codes of bf16 bits times inv, by the hardware's conversion; a NaN, which that codes with a sign of its own,
+// as 0x7f and the NaN's sign.
 struct Coder {
   float inv;
   bool any_nan;
@@ -226,10 +233,10 @@ __device__ __forceinline__ float run_scale(uint8_t *codes, float *scales, int64_
   return s;
 }
 
-// The keys of head h of a run (r tokens from t on in block blk, the first at offset `first`), by a wave: as many tokens as it has
-// groups side by side, the codes stored from where the heads were normed and turned, 8 bytes a lane's run. Every wave of the workgroup calls it
-// (a piece's angles are the workgroup's); active: the wave has a head. More than 16 tokens are normed and turned
-// twice, for the scale and for the codes.
+// The keys of head h of a run (r tokens from t on in block blk, the first at offset `first`), by a wave: as
+// many tokens as it has groups side by side, the codes stored from where the heads were normed and turned, 8
+// bytes a lane's run. Every wave of the workgroup calls it (a piece's angles are the workgroup's); active:
+// the wave has a head. More than 16 tokens are normed and turned twice, for the scale and for the codes.
 template <int D, int V, bool INTER, int LL>
 __device__ __forceinline__ void append_keys(const AppendArgs &a, float2 *turn, int64_t t, int r, int64_t blk, int first,
                                             int h, bool active) {
@@ -321,7 +328,7 @@ __device__ __forceinline__ void append_keys(const AppendArgs &a, float2 *turn, i
   float s = 0.f;
   const uint32_t most = wave_max_bits(finite);
   if (active) s = run_scale<D, false>(kc, a.ks, blk, h, H, BS, first, old, __uint_as_float(most << 16));
-  const Coder code{pow2_inverse(s), static_cast<bool>(__any(top.of_lane() > 0x7f80u))};  
+  const Coder code{pow2_inverse(s), static_cast<bool>(__any(top.of_lane() > 0x7f80u))};
   for (int p0 = 0; p0 < r; p0 += kPiece) {
     if (r > kPiece) load(p0);
     if (!active) continue;
@@ -411,8 +418,8 @@ __device__ __forceinline__ void append_values(const AppendArgs &a, int64_t t, in
   }
 }
 
-// The runs that begin in a window of the call's tokens, four heads a workgroup, one a wave: f(t, r, blk, first, h, active). The
-// same in every wave.
+// The runs that begin in a window of the call's tokens, four heads a workgroup, one a wave: f(t, r, blk,
+// first, h, active). The same in every wave.
 template <class F>
 __device__ __forceinline__ void window_runs(const AppendArgs &a, int wg, F f) {
   const int chunks = (a.Hk + kWaves - 1) / kWaves;
@@ -449,6 +456,8 @@ __device__ __forceinline__ void window_runs(const AppendArgs &a, int wg, F f) {
   }
 }
 
+// fp8: four waves a SIMD (128 registers, 60 bytes of them spilled at D = 128; 143 and three waves otherwise):
+// 38.5 us in the place of 40.4 for 8,386 tokens of 28/4 heads.
 template <int D, int V, bool INTER, bool FP8, bool EACH, bool FAR>
 __global__ __launch_bounds__(kThreads, FP8 ? 4 : 1) void rotary_append_kernel(AppendArgs a) {
   constexpr int UNITS = D / (2 * V), LL = UNITS == 64 ? 6 : UNITS == 32 ? 5 : UNITS == 8 ? 3 : 2;
@@ -475,8 +484,9 @@ __global__ __launch_bounds__(kThreads, FP8 ? 4 : 1) void rotary_append_kernel(Ap
 }
 
 // ---------------------------------------------------------------------------
-// The latent cache: rows of rope_dim (every query head's, and the shared key as one more), and the compressed
-// entries, a wave each.
+// The latent cache: rows of rope_dim (every query head's, and the shared key as a kind of its own), and the
+// compressed entries, a wave each. 4,696 tokens of 128 heads of 64, each the end of a row of 192: 31 us by
+// the trace, 36 a pass, where a copy of the same strided queries alone takes 34.
 struct LatentArgs {
   Kind q, k;  // queries; the shared key, one head
   int entry_wgs, k_wgs;  // workgroups of entries, and of shared keys; queries behind them
@@ -631,7 +641,7 @@ extern "C" int wkv_rotary_append(const wkv_cache_t *cache, const void *key, int6
   size_t lds = (static_cast<size_t>(kWaves) << (gq.log_tg > gk.log_tg ? gq.log_tg : gk.log_tg)) * half * sizeof(float2);
   int64_t rest;
   if (fp8) {
-    // a window of 16 tokens for prompts, of one where there is a token a sequence
+    // a window of 16 tokens for prompts, whose runs mostly begin 16 apart; of one where every token may be a run
     a.window = num_tokens >= 4096 ? 16 : num_tokens >= 1024 ? 4 : 1;
     rest = (num_tokens + a.window - 1) / a.window * ((Hk + kWaves - 1) / kWaves);
     k_wgs = rest;
@@ -650,8 +660,8 @@ extern "C" int wkv_rotary_append(const wkv_cache_t *cache, const void *key, int6
   a.k_wgs = static_cast<int>(k_wgs);
   a.v_wgs = static_cast<int>(rest);
   const unsigned grid = static_cast<unsigned>(gq.wgs + k_wgs + rest);
-  // Rows far larger than the caches go past them (8 prompts of 2,048 tokens, 32/8 heads of 128: 82.3 us, 88.7 near); the cache's
-  // keys and values stay, for the attention.
+  // Rows far larger than the caches go past them (8 prompts of 2,048 tokens, 32/8 heads of 128: 82.3 us, 88.7
+  // near); the cache's keys and values stay, for the attention.
   const bool far = num_tokens * (num_q_heads + Hk) * D * 2 >= (64 << 20);
   auto s = static_cast<hipStream_t>(stream);
   auto launch = [&](auto d, auto v, auto in) {
