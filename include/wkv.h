@@ -523,12 +523,12 @@ int wkv_norm_rotary(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_
                     int32_t head_dim, const wkv_head_norm_t *norm, const wkv_rotary_t *rotary, int64_t num_tokens,
                     void *stream);
 
-/* Its gradients: from the inputs q, k, and the gradients q_grad, k_grad of the
- * outputs, dq and dk (NULL: not computed; else they do not overlap the inputs) and the weights' dq_weight, dk_weight (NULL: not
- * computed; contiguous, [head_dim], or [heads, head_dim] where the weight has a head stride, of weight_dtype).
- * A kind of heads without a gradient is given as 0 heads. Summed in float32, in an order that depends on the sizes alone.
- * workspace: wkv_norm_rotary_workspace_size() bytes, 16-byte aligned, for a weight's gradient (else it may be NULL);
- * weight_each_head: that weight is [heads, head_dim]. */
+/* Its gradients: from the inputs q, k, and the gradients q_grad, k_grad of the outputs, dq and dk (NULL: not
+ * computed; else they do not overlap the inputs) and the weights' dq_weight, dk_weight (NULL: not computed;
+ * contiguous, [head_dim], or [heads, head_dim] where the weight has a head stride, of weight_dtype). A kind of
+ * heads without a gradient is given as 0 heads. Summed in float32, in an order that depends on the sizes alone.
+ * workspace: wkv_norm_rotary_workspace_size() bytes, 16-byte aligned, for a weight's gradient (else it may be
+ * NULL); weight_each_head: that weight is [heads, head_dim]. */
 int64_t wkv_norm_rotary_workspace_size(int64_t num_tokens, int32_t num_q_heads, int32_t num_k_heads, int32_t head_dim,
                                        int32_t q_weight_each_head, int32_t k_weight_each_head);
 
@@ -540,13 +540,15 @@ int wkv_norm_rotary_backward(int32_t dtype, const void *q, int64_t q_stride_t, i
                              const wkv_head_norm_t *norm, const wkv_rotary_t *rotary, void *dq_weight, void *dk_weight,
                              int64_t num_tokens, void *workspace, int64_t workspace_bytes, void *stream);
 
-/* The append with the norm and the rotation on the way, in one launch: the queries normed and turned into
- * q_out (or in place; num_q_heads may be 0), the keys normed and turned into the cache, the values into the cache. The cache then holds
- * what wkv_norm_rotary followed by wkv_append or wkv_append_fp8 leaves in it, bit for bit (without a norm: what wkv_rotary_axes and
- * they would, but for the last bit of a key), keys rounded to bf16 before they are coded in fp8; key and value themselves are not changed. norm or rotary may be NULL, not both. key, value and
- * slot_mapping as for wkv_append (wkv_append_fp8); a slot appears once in a call, and an fp8 cache's block in one run. q and its result bf16 [num_tokens, num_q_heads,
- * head_dim], strides in elements; every token's queries are computed, also those of slot -1. Replaces the
- * engine's norms, rotary embedding and reshape_and_cache of a layer (inside llm.generate, engine.py:887). */
+/* The append with the norm and the rotation on the way, in one launch: the queries normed and turned into q_out (or
+ * in place; num_q_heads may be 0), the keys normed and turned into the cache, the values into the cache. The cache
+ * then holds what wkv_norm_rotary followed by wkv_append or wkv_append_fp8 leaves in it, bit for bit where queries
+ * and weights are 16-byte aligned too (otherwise, and without a norm, where wkv_rotary_axes goes first, but for the
+ * last bit of a key), keys rounded to bf16 before they are coded in fp8; key and value themselves are not changed. norm or rotary may be NULL, not both. key, value and
+ * slot_mapping as for wkv_append (wkv_append_fp8); a slot appears once in a call, and an fp8 cache's block in one
+ * run. q and its result bf16 [num_tokens, num_q_heads, head_dim], strides in elements; every token's queries are
+ * computed, also those of slot -1. Replaces the engine's norms, rotary embedding and append of a layer (inside
+ * llm.generate, engine.py:887). */
 int wkv_rotary_append(const wkv_cache_t *cache, const void *key, int64_t key_stride_t, int64_t key_stride_h,
                       const void *value, int64_t value_stride_t, int64_t value_stride_h, const int64_t *slot_mapping,
                       const void *q, int64_t q_stride_t, int64_t q_stride_h, void *q_out, int64_t qo_stride_t,
@@ -554,9 +556,9 @@ int wkv_rotary_append(const wkv_cache_t *cache, const void *key, int64_t key_str
                       const wkv_rotary_t *rotary, int64_t num_tokens, void *stream);
 
 /* The same for a latent cache: latent[slot[t]] = concat(kv_c[t] normed (kv_norm's k_weight [kv_lora_rank], eps and
- * offset; NULL: as it is), k_pe[t] turned), and the queries' q_pe [num_tokens, num_heads, rope_dim] turned into q_out. kv_c, k_pe and
- * slot_mapping as for wkv_mla_append. Replaces the engine's norm of the compressed entries,
- * its rotary embedding (wavelet/inference/deepseek_v4.py:15-66) and concat_and_cache_mla. */
+ * offset; NULL: as it is), k_pe[t] turned), and the queries' q_pe [num_tokens, num_heads, rope_dim] turned into
+ * q_out. kv_c, k_pe and slot_mapping as for wkv_mla_append. Replaces the engine's norm of the compressed entries,
+ * its rotary embedding (wavelet/inference/deepseek_v4.py:15-66) and its latent append. */
 int wkv_mla_rotary_append(const wkv_mla_cache_t *cache, const void *kv_c, int64_t kv_c_stride, const void *k_pe,
                           int64_t k_pe_stride, const int64_t *slot_mapping, const void *q_pe, int64_t q_stride_t,
                           int64_t q_stride_h, void *q_out, int64_t qo_stride_t, int64_t qo_stride_h, int32_t num_heads,

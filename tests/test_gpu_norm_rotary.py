@@ -14,7 +14,8 @@ TYPES = [torch.bfloat16, torch.float16, torch.float32]
 # tokens, query heads, key heads, head dim, turned dims (0: none)
 SHAPES = [(1, 32, 8, 128, 128), (5, 14, 2, 64, 64), (37, 28, 4, 128, 64), (3, 1, 1, 64, 16), (130, 3, 1, 80, 20),
           (9, 2, 2, 128, 74), (2, 5, 3, 2, 2), (1030, 2, 1, 64, 32), (7, 1, 1, 512, 512), (6, 4, 1, 66, 34),
-          (5, 16, 16, 192, 64), (3, 2, 1, 510, 510), (4, 7, 3, 96, 0), (2, 3, 1, 256, 256)]
+          (5, 16, 16, 192, 64), (3, 2, 1, 510, 510), (4, 7, 3, 96, 0), (2, 3, 1, 256, 256), (3, 257, 129, 64, 64),
+          (5001, 33, 3, 64, 64)]
 
 
 def _case(cuda, tokens, hq, hk, d, r, dtype, weights, wide, seed=0):
@@ -295,3 +296,43 @@ def test_refusals(cuda):
         rotary_axes((10, 22), interleaved=True, device=cuda)
     with pytest.raises(ValueError):
         rotary_axes((), device=cuda)
+
+
+def test_two_streams_at_once(cuda):
+    """Forward and backward on two streams that nothing orders, over inputs of their own."""
+    cs = [_case(cuda, 700, 8, 4, 128, 128, torch.bfloat16, "dim", False, seed=i) for i in range(2)]
+
+    def run(c):
+        leaves = [x.detach().requires_grad_() for x in (c["q"], c["k"], c["qw"], c["kw"])]
+        q, k = norm_rotary(leaves[0], leaves[1], c["pos"], c["freq"], q_weight=leaves[2], k_weight=leaves[3])
+        return [q.detach(), k.detach(), *torch.autograd.grad([q, k], leaves, [c["gq"], c["gk"]])]
+
+    want = [run(c) for c in cs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cs]
+    got = [None, None]
+    for _ in range(3):
+        for i, (s, c) in enumerate(zip(streams, cs)):
+            with torch.cuda.stream(s):
+                got[i] = run(c)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+
+
+def test_more_than_2_31_elements(cuda):
+    """The last tokens of 2^20 + 5 tokens of 16 heads of 128."""
+    tokens = (1 << 20) + 5
+    freq = rotary_frequencies(128, 1e4, device=cuda)[0]
+    q = torch.empty((tokens, 16, 128), dtype=torch.bfloat16, device=cuda).normal_()
+    pos = torch.arange(tokens, device=cuda)
+    w = torch.ones(128, device=cuda)
+    got, _ = norm_rotary(q, None, pos, freq, q_weight=w)
+    check_forward(got[-7:], q[-7:], w, 1e-6, heads.phases(f64(pos[-7:]), f64(freq)), 0.0, False, 1.0)
+    check_forward(got[:3], q[:3], w, 1e-6, heads.phases(f64(pos[:3]), f64(freq)), 0.0, False, 1.0)
+    del got
+    leaf = q.detach().requires_grad_()
+    out, _ = norm_rotary(leaf, None, pos, freq, q_weight=w)
+    dq, = torch.autograd.grad(out, leaf, q)
+    check_backward(dq[-5:], None, q[-5:], q[-5:], w, 1e-6, heads.phases(f64(pos[-5:]), f64(freq)), 0.0, False, 1.0)

@@ -108,6 +108,7 @@ SHAPES = [  # head layout, new tokens, contexts, block size
     ((8, 1, 64), [700, 411, 300], [9, 0, 16], 32),
     ((3, 3, 64), [4096, 37], [0, 11], 16),
     ((2, 1, 128), [1100], [5], 48),
+    ((4, 8, 64), [8192, 9], [0, 5], 16),
 ]
 
 
@@ -213,17 +214,33 @@ def test_axes_norm_alone_no_queries_and_in_place(cuda):
             np.testing.assert_array_equal(x, z)
 
 
-@pytest.mark.parametrize("shift", [1, 4])
+def _moved(cuda, tensors, shift):
+    """The same rows at another alignment."""
+    out = [torch.empty(len(t), t.shape[1] * 64 + 9, device=cuda).bfloat16()[:, shift:shift + t.shape[1] * 64].view(t.shape)
+           for t in tensors]
+    for a, b in zip(out, tensors):
+        a.copy_(b)
+    return out
+
+
+@pytest.mark.parametrize("shift", [1, 3])
 def test_rows_that_are_not_aligned(cuda, shift):
     rng = np.random.default_rng(6)
     slots, blocks = _slots(rng, [30], [2], 16)
     q, key, value, w, pos, freq = _inputs(cuda, 30, 4, 2, 64, 64, "dim")
     for kv in ("bf16", "fp8_e4m3"):
-        moved = [torch.empty(30, t.shape[1] * 64 + 9, device=cuda).bfloat16()[:, shift:shift + t.shape[1] * 64].view(t.shape)
-                 for t in (q, key, value)]
-        for a, b in zip(moved, (q, key, value)):
-            a.copy_(b)
-        _run(cuda, *moved, _cache(cuda, blocks, 16, 2, 64, kv), slots, w, pos, freq, 1e-6)
+        _run(cuda, *_moved(cuda, (q, key, value), shift), _cache(cuda, blocks, 16, 2, 64, kv), slots, w, pos, freq, 1e-6)
+
+
+def test_rows_aligned_to_eight_bytes(cuda):
+    """norm_rotary takes them two elements at a time, rotary_append one: squares are added in another order."""
+    q, key, value, w, pos, freq = _inputs(cuda, 30, 4, 2, 64, 64, "dim")
+    c = PagedKVCache(2, 16, 2, 64, device=cuda)
+    got = rotary_append(*_moved(cuda, (q, key, value), 4), c, torch.arange(30, device=cuda), pos, freq, q_weight=w[0],
+                        k_weight=w[1], eps=1e-6)
+    angle = heads.phases(f64(pos), f64(freq))
+    check_forward(got, q, w[0], 1e-6, angle, 0.0, False, 1.0)
+    check_forward(c.k.permute(0, 3, 1, 2, 4).reshape(-1, 2, 64)[:30], key, w[1], 1e-6, angle, 0.0, False, 1.0)
 
 
 @pytest.mark.parametrize("kv", ["bf16", "fp8_e4m3"])
@@ -351,6 +368,49 @@ def test_graph_replays(cuda):
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1]) and torch.equal(lat.latent, other.latent)
         for a, b in zip(_held(cache), _held(start)):
             np.testing.assert_array_equal(a, b)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8_e4m3"])
+def test_caches_of_more_than_2_31_elements(cuda, kv):
+    """The last block of 1.1 million, beside the first one's, which stays; and the same of a latent cache."""
+    blocks = 1_100_000
+    c = PagedKVCache(blocks, 16, 1, 128, kv_dtype=kv, device=cuda)
+    small = PagedKVCache(1, 16, 1, 128, kv_dtype=kv, device=cuda)
+    for tokens in (5, 300):
+        q, key, value, w, pos, freq = _inputs(cuda, tokens, 2, 1, 128, 128, "dim")
+        slots = torch.full((tokens,), -1, device=cuda)
+        slots[:5] = torch.arange(5, device=cuda)
+        rotary_append(None, key, value, small, slots, pos, freq, k_weight=w[1], eps=1e-6)
+        slots[:5] += (blocks - 1) * 16
+        rotary_append(None, key, value, c, slots, pos, freq, k_weight=w[1], eps=1e-6)
+        assert torch.equal(c.k[-1], small.k[0]) and torch.equal(c.v[-1], small.v[0])
+        assert not c.k[0].any() and not c.v[0].any() and small.k[0].any()
+    del c
+    lat = MLALatentCache(240_000, 16, device=cuda)
+    one = MLALatentCache(1, 16, device=cuda)
+    kv_c, k_pe = torch.randn((3, 512), device=cuda).bfloat16(), torch.randn((3, 64), device=cuda).bfloat16()
+    at, freq = torch.arange(3, device=cuda), rotary_frequencies(64, 1e4, device=cuda)[0]
+    mla_rotary_append(None, kv_c, k_pe, one, at, at, freq, eps=1e-6)
+    mla_rotary_append(None, kv_c, k_pe, lat, at + (240_000 - 1) * 16, at, freq, eps=1e-6)
+    assert torch.equal(lat.latent[-1], one.latent[0]) and not lat.latent[0].any() and one.latent.any()
+
+
+def test_latent_prompt_of_many_heads(cuda):
+    """Heads of a token over several waves."""
+    tokens = 4200
+    g = torch.Generator(device=cuda).manual_seed(2)
+    q = torch.randn((tokens, 70, 64), generator=g, device=cuda).bfloat16()
+    kv = torch.randn((tokens, 576), generator=g, device=cuda).bfloat16()
+    pos = torch.arange(tokens, device=cuda)
+    freq = rotary_frequencies(64, 1e4, device=cuda)[0]
+    c = MLALatentCache(264, 16, device=cuda)
+    got = mla_rotary_append(q, kv[:, :512], kv[:, 512:], c, pos, pos, freq)
+    angle = heads.phases(f64(pos), f64(freq))
+    check(got, heads.turn(f64(q), angle), 16 * U * size(f64(q), 32, False, 1.0), "q_pe")
+    rows = c.latent.view(-1, 576)[:tokens]
+    assert torch.equal(rows[:, :512], kv[:, :512])
+    x = f64(kv[:, None, 512:])
+    check(rows[:, None, 512:], heads.turn(x, angle), 16 * U * size(x, 32, False, 1.0), "k_pe")
 
 
 def test_no_tokens(cuda):

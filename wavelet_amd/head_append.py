@@ -36,8 +36,8 @@ def _result(x: torch.Tensor, out, name: str) -> torch.Tensor:
     if (not isinstance(out, torch.Tensor) or out.dtype != x.dtype or out.shape != x.shape or out.device != x.device
             or out.stride(2) != 1 or (out.shape[0] > 1 and out.stride(0) == 0)
             or (out.shape[1] > 1 and out.stride(1) == 0)):
-        raise ValueError(f"out must be {x.dtype} {tuple(x.shape)} on {x.device} for {name}, with its last dim contiguous "
-                         "and no row twice")
+        raise ValueError(f"out must be {x.dtype} {tuple(x.shape)} on {x.device} for {name}, with its last dim "
+                         "contiguous and no row twice")
     return out
 
 
@@ -68,11 +68,12 @@ def rotary_append(q: torch.Tensor | None, key: torch.Tensor, value: torch.Tensor
 
     ``q [T, Hq, D]`` (None: keys and values only), ``key`` and ``value`` ``[T, Hkv, D]`` bf16, strided rows of a fused
     projection read in place. The norm is ``norm_rotary``'s and is done where ``eps`` is given, the rotation
-    ``apply_rotary``'s and done where ``positions`` and ``inv_freq`` are; one of them at least. The attention then takes the
-    result and no ``key`` / ``value`` (``paged_decode_gqa``, ``prefill_gqa``, ``paged_tree_gqa``). ``key`` and ``value`` are left
-    as they are, and the cache, bf16 or fp8, holds what ``norm_rotary`` and ``cache.append`` would leave in it, bit for bit
-    (without a norm what ``apply_rotary`` and ``cache.append`` would, but for a key's last bit). A slot appears once in a call, a
-    block of an fp8 cache in one run of it (as for ``cache.append``).
+    ``apply_rotary``'s and done where ``positions`` and ``inv_freq`` are; one of them at least. The attention then
+    takes the result and no ``key`` / ``value`` (``paged_decode_gqa``, ``prefill_gqa``, ``paged_tree_gqa``). ``key`` and
+    ``value`` are left as they are, and the cache, bf16 or fp8, holds what ``norm_rotary`` and ``cache.append`` would
+    leave in it (bit for bit where queries and weights are aligned to 16 bytes; otherwise, and where ``apply_rotary``
+    goes first, but for a key's last bit). A slot appears once in a call, a block of an fp8 cache in one run of it (as
+    for ``cache.append``).
     """
     if not isinstance(cache, PagedKVCache):
         raise ValueError("cache must be a PagedKVCache (mla_rotary_append appends to latent caches)")
@@ -122,8 +123,8 @@ def mla_rotary_append(q_pe: torch.Tensor | None, kv_c: torch.Tensor, k_pe: torch
                       axes: torch.Tensor | None = None, interleaved: bool = False, scale: float = 1.0,
                       out: torch.Tensor | None = None) -> torch.Tensor | None:
     """The queries' ``q_pe [T, H, rope_dim]`` (None: none) turned -> a new tensor (or ``out``), and into the latent
-    ``cache`` at ``slot_mapping`` (-1: skipped) the compressed entries ``kv_c [T, kv_lora_rank]``, normed where ``eps`` is given
-    (weight ``[kv_lora_rank]``, None: ones), and ``k_pe [T, rope_dim]`` turned.
+    ``cache`` at ``slot_mapping`` (-1: skipped) the compressed entries ``kv_c [T, kv_lora_rank]``, normed where ``eps``
+    is given (weight ``[kv_lora_rank]``, None: ones), and ``k_pe [T, rope_dim]`` turned.
 
     bf16; the rotation as for ``apply_rotary``, the norm as ``norm_rotary``'s over a whole entry. The attention
     (``paged_decode_mla``) then takes the result as its ``q_pe`` and no ``kv_c`` / ``k_pe``. A slot appears once in a call.

@@ -19,7 +19,8 @@ def check_weight(w, name: str, heads: int, x: torch.Tensor):
     """A head norm's weight (None: ones) for ``heads`` heads of ``x``'s type and size, its last dim contiguous."""
     if w is None:
         return None
-    if not isinstance(w, torch.Tensor) or w.device != x.device or (w.dtype is not x.dtype and w.dtype is not torch.float32):
+    if (not isinstance(w, torch.Tensor) or w.device != x.device
+            or (w.dtype is not x.dtype and w.dtype is not torch.float32)):
         raise ValueError(f"{name} must be a float32 or {x.dtype} tensor on {x.device}")
     shape, d = w.shape, x.shape[-1]
     if shape != (d,) and shape != (heads, d):
@@ -69,15 +70,15 @@ def _forward(q, k, q_weight, k_weight, rotary, interleaved, scale, eps, offset, 
         kot, koh, _ = ko.stride()
         tail = (k.data_ptr(), kst, ksh, ko.data_ptr(), kot, koh, k.shape[1])
     with _on(dev):
-        rc = _lib.load().wkv_norm_rotary(_DTYPES[q.dtype], q.data_ptr(), st, sh, qo.data_ptr(), ot, oh, hq, *tail, d, norm,
-                                         how, tokens, _stream(dev))
+        rc = _lib.load().wkv_norm_rotary(_DTYPES[q.dtype], q.data_ptr(), st, sh, qo.data_ptr(), ot, oh, hq, *tail, d,
+                                         norm, how, tokens, _stream(dev))
     if rc:
         _lib.check(rc, "norm_rotary")
     return out
 
 
 def _grad_rows(x, g, want: bool):
-    """A kind's part of the backward call: its result (None: not wanted), and pointers, strides and heads (x None: none)."""
+    """A kind's part of the backward call: its result (None: not wanted), and pointers, strides and heads."""
     if x is None:
         return None, (None, 0, 0, None, 0, 0, None, 0, 0, 0)
     xt, xh, last = x.stride()
@@ -169,9 +170,9 @@ def norm_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
     The norm: ``x / sqrt(mean(x ** 2) + eps) * (weight + weight_offset)`` over each head, weights ``[D]`` for all
     heads or ``[H, D]``, of the heads' type or float32 (None: ones). The rotation: ``apply_rotary``'s, from
     ``positions``, ``inv_freq``, ``axes``, ``interleaved`` and ``scale`` (``positions`` and ``inv_freq`` None: the heads
-    are only normed). bf16, fp16 or fp32, ``D`` even and at most 512, strided rows read in place; all of it is computed in float32
-    and rounded once. ``out``: the two results' tensors; ``out=(q, k)`` works in place, other tensors share no memory with
-    the inputs. Differentiable once, in ``q``, ``k`` and the weights (not with ``out``,
+    are only normed). bf16, fp16 or fp32, ``D`` even and at most 512, strided rows read in place; all of it is
+    computed in float32 and rounded once. ``out``: the two results' tensors; ``out=(q, k)`` works in place, other
+    tensors share no memory with the inputs. Differentiable once, in ``q``, ``k`` and the weights (not with ``out``,
     ``create_graph`` or forward mode).
     """
     if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype not in _DTYPES:

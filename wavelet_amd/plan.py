@@ -49,7 +49,8 @@ class Heads:
     """What a plan does to its layers' queries and keys on their way to the cache and the attention.
 
     The norm where ``eps`` is given (``q_weight[l]`` and ``k_weight[l]`` for layer ``l``; None: ones), the rotation
-    where ``inv_freq`` is, as ``rotary_append`` takes them; for an MLA plan ``k_weight[l]`` is the weight of the compressed entries.
+    where ``inv_freq`` is, as ``rotary_append`` takes them; for an MLA plan ``k_weight[l]`` is the weight of the
+    compressed entries.
     ``positions`` ``[T]`` (``[A, T]`` with ``axes``) are refilled in place between steps, like the plan's other
     buffers (``TreeStep`` has its own).
     """
@@ -74,7 +75,8 @@ class Heads:
             raise ValueError("inv_freq needs positions")
         checked = check_rotation(self.positions, self.inv_freq, self.axes, tokens, d, device)
         if any(a is not b for a, b in zip(checked, (self.positions, self.inv_freq, self.axes))):
-            raise ValueError("a plan needs contiguous positions, inv_freq and axes: it reads the tensors handed to it on every step")
+            raise ValueError("a plan needs contiguous positions, inv_freq and axes: it reads the tensors handed to it "
+                             "on every step")
         return rotation(*checked, bool(self.interleaved), float(self.scale))
 
     def norm(self, layer: int, layers: int, q: torch.Tensor | None, k: torch.Tensor):
@@ -590,8 +592,8 @@ class TreeStep:
     are turned in place by their positions (``inv_freq`` from ``rotary_frequencies``; None: they come
     turned), keys and values appended, and ``out[l]`` is their attention over context and tree
     (``paged_tree_gqa``; with ``heads``, whose positions are the step's, queries and keys are normed and turned
-    by the append itself, ``q[l]`` in place, ``key[l]`` left as it is) --, then ``finish()`` once ``target_tokens`` holds what was sampled after every
-    node: the path that agrees is accepted (``accept_tree``), its keys and values move together in every layer's
+    by the append itself, ``q[l]`` in place, ``key[l]`` left as it is) --, then ``finish()`` once ``target_tokens``
+    holds what was sampled after every node: the path that agrees is accepted (``accept_tree``), its keys and values move together in every layer's
     cache (``compact``) and ``state.seq_lens`` moves on. ``maps`` and ``accepted`` are the step's results;
     ``state.next_tokens`` are the next step's first nodes: what was sampled after the accepted path, and what
     it was for a sequence of which nothing was accepted (paused, ``new_lens`` 0, or refused).

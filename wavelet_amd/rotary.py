@@ -144,7 +144,7 @@ def check_rotation(positions, inv_freq, axes, tokens: int, d: int, dev: torch.de
     if axes is None:
         if positions.dtype is not torch.int64 or len(shape) != 1 or shape[0] != tokens:
             raise ValueError(f"positions must be int64 [{tokens}] (got {positions.dtype} {tuple(shape)})")
-    elif positions.dtype is not torch.int64 or len(shape) != 2 or shape[0] < 1 or shape[1] != tokens:
+    elif positions.dtype is not torch.int64 or len(shape) != 2 or not shape[0] or shape[1] != tokens:
         raise ValueError(f"positions must be int64 [axes, {tokens}] (got {positions.dtype} {tuple(shape)})")
     _require_cuda(inv_freq, "inv_freq", dev)
     if inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 or not 0 < 2 * inv_freq.shape[0] <= d:
