@@ -42,7 +42,8 @@ _HERE = contextlib.nullcontext()
 
 def _on(device: torch.device):
     """The device made current for a launch (a launch goes to the current one); nothing where it is already."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    index = device.index
+    if index is None or index == torch._C._cuda_getDevice():  # (current_device() looks at the start-up first)
         return _HERE
     return torch.cuda.device(device)
 
@@ -63,12 +64,12 @@ def _slots(slot_mapping: torch.Tensor, n: int, device: torch.device) -> torch.Te
 
 def _token_rows(x: torch.Tensor, name: str, shape: tuple[int, ...], device: torch.device) -> torch.Tensor:
     _require_cuda(x, name, device)
-    if x.dtype != torch.bfloat16 or tuple(x.shape[1:]) != shape:
+    if x.dtype is not torch.bfloat16 or x.shape[1:] != shape:
         raise ValueError(f"{name} must be bfloat16 [T, {', '.join(map(str, shape))}] (got {x.dtype} {tuple(x.shape)})")
-    *strides, last = x.stride()
-    if last != 1 or x.data_ptr() % 16:
+    strides = x.stride()
+    if strides[-1] != 1 or x.data_ptr() % 16:
         return x.contiguous()
-    for s in strides:
+    for s in strides[:-1]:
         if s % 8:
             return x.contiguous()
     return x

@@ -19,13 +19,15 @@ from .rotary import _dual, check_rotation, rotation
 
 def _no_gradients(what: str, *tensors) -> None:
     """A cache keeps no graph: what goes into it cannot be differentiated."""
-    grad = torch.is_grad_enabled()
-    for t in tensors:
-        if grad and t is not None and t.requires_grad:
-            break
-    else:
-        if not _dual(*tensors):
-            return
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                break
+        else:
+            if not _dual(*tensors):
+                return
+    elif not _dual(*tensors):
+        return
     raise ValueError(f"{what} has no gradient: detach its inputs, or call it under torch.no_grad()")
 
 
