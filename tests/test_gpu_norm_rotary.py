@@ -167,6 +167,24 @@ def test_expanded_gradients_and_heads(cuda):
     np.testing.assert_allclose(f64(dw), want_w, rtol=0, atol=1e-3)
 
 
+@pytest.mark.parametrize("hq", [1, 5, 40])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_expanded_weights(cuda, dtype, hq):
+    """One weight expanded over the heads, each of which has a gradient; their sum (a few u more, within the bound's
+    slack) is the one weight's. Also one head's with a head stride of zero."""
+    c = _case(cuda, 23, hq, 2, 64, 64, dtype, "dim", True)
+    one = [c[x].clone().requires_grad_() for x in ("qw", "kw")]
+    wide = one[0].expand(hq, 64) if hq > 1 else one[0].as_strided((1, 64), (0, 1)), one[1].expand(2, 64)
+    q, k = norm_rotary(c["q"], c["k"], c["pos"], c["freq"], q_weight=wide[0], k_weight=wide[1], eps=1e-5)
+    del_me = [torch.full((hq, 64), float("nan"), device=cuda) for _ in range(2)]  # (what a gradient's memory may hold)
+    del del_me
+    each = torch.autograd.grad([q, k], wide, [c["gq"], c["gk"]], retain_graph=True)
+    both = torch.autograd.grad([q, k], one, [c["gq"], c["gk"]])
+    for x, g, w, dw, dw1 in zip((c["q"], c["k"]), (c["gq"], c["gk"]), wide, each, both):
+        check_backward(None, dw, x, g, w, 1e-5, c["angle"], 0.0, False, 1.0)
+        check_backward(None, dw1, x, g, w[0], 1e-5, c["angle"], 0.0, False, 1.0)
+
+
 def test_only_some_gradients(cuda):
     c = _case(cuda, 10, 4, 2, 64, 64, torch.bfloat16, "dim", True)
     full = [x.detach().requires_grad_() for x in (c["q"], c["k"], c["qw"], c["kw"])]

@@ -97,13 +97,15 @@ def _grad_rows(x, g, want: bool):
 
 
 def _weight_grad(x, w, want: bool):
-    """A weight's gradient, empty, and its pointer (None: not wanted; no head, no sum)."""
+    """The weight that the launch takes, its gradient, empty, and that one's pointer (None: not wanted; no head, no sum)."""
     if not want or x is None or w is None:
-        return None, None
+        return w, None, None
     if x.shape[1] == 0:
-        return torch.zeros_like(w), None
+        return w, torch.zeros_like(w), None
+    if w.dim() == 2 and w.shape[0] > 1 and w.stride(0) == 0:
+        w = w.contiguous()  # (an expanded weight has a gradient for every head)
     d = torch.empty_like(w, memory_format=torch.contiguous_format)
-    return d, d.data_ptr()
+    return w, d, d.data_ptr()
 
 
 def _backward(q, k, gq, gk, q_weight, k_weight, rotary, interleaved, scale, eps, offset, need):
@@ -117,16 +119,15 @@ def _backward(q, k, gq, gk, q_weight, k_weight, rotary, interleaved, scale, eps,
     tokens, _, d = some.shape
     keep_q, rows_q = _grad_rows(q, gq, need[0])  # (what was copied lives until the launch)
     keep_k, rows_k = _grad_rows(k, gk, need[1])
-    dqw, dqw_ptr = _weight_grad(q, q_weight, need[2])
-    dkw, dkw_ptr = _weight_grad(k, k_weight, need[3])
+    q_weight, dqw, dqw_ptr = _weight_grad(q, q_weight, need[2])
+    k_weight, dkw, dkw_ptr = _weight_grad(k, k_weight, need[3])
     norm = head_norm(q_weight, k_weight, eps, offset)
     how = None if rotary is None else rotation(*rotary, interleaved, scale)
     lib = _lib.load()
     ws, size, ws_ptr = None, 0, None
     if dqw_ptr is not None or dkw_ptr is not None:
         size = lib.wkv_norm_rotary_workspace_size(tokens, rows_q[-1], rows_k[-1], d,
-                                                  q is not None and q_weight is not None and q_weight.dim() == 2,
-                                                  k is not None and k_weight is not None and k_weight.dim() == 2)
+                                                  norm.q_weight_stride_h != 0, norm.k_weight_stride_h != 0)
         ws = torch.empty(size, dtype=torch.uint8, device=dev)
         ws_ptr = ws.data_ptr()
     with _on(dev):
@@ -168,7 +169,7 @@ def norm_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
     """``q [T, Hq, D]`` and ``k [T, Hk, D]`` (or None) with every head normed and turned -> new tensors ``(q, k)``.
 
     The norm: ``x / sqrt(mean(x ** 2) + eps) * (weight + weight_offset)`` over each head, weights ``[D]`` for all
-    heads or ``[H, D]``, of the heads' type or float32 (None: ones). The rotation: ``apply_rotary``'s, from
+    heads or ``[H, D]``, of the heads' type or float32 (None: ones, without the offset). The rotation: ``apply_rotary``'s, from
     ``positions``, ``inv_freq``, ``axes``, ``interleaved`` and ``scale`` (``positions`` and ``inv_freq`` None: the heads
     are only normed). bf16, fp16 or fp32, ``D`` even and at most 512, strided rows read in place; all of it is
     computed in float32 and rounded once. ``out``: the two results' tensors; ``out=(q, k)`` works in place, other
