@@ -190,6 +190,27 @@ def test_latent_decode(cuda):
             assert torch.equal(bufs[0][4][layer], bufs[1][4][layer])
 
 
+def test_plans_keep_what_they_were_built_with(cuda):
+    """Fields of the heads that are set anew, and lists changed, after the plan was built."""
+    t = Two(cuda, "bf16", 2, 5)
+    table = torch.arange(4, dtype=torch.int32, device=cuda).view(2, 2)
+    lens, slots = torch.tensor([1, 1], dtype=torch.int32, device=cuda), torch.tensor([0, 32], device=cuda)
+    heads = Heads(t.pos, t.freq, q_weight=list(t.qw), k_weight=list(t.kw), eps=1e-6)
+    step = DecodeStep(t.pairs[0], t.q[0], t.k[0], t.v[0], t.out[0], table, lens, slots, D ** -0.5, 32, heads=heads)
+    heads.positions = heads.inv_freq = None
+    heads.q_weight[:] = heads.k_weight[:] = [None] * LAYERS
+    assert step.heads.positions is t.pos and step.heads.inv_freq is t.freq
+    assert all(a is b for a, b in zip(step.heads.q_weight + step.heads.k_weight, t.qw + t.kw))
+    other = DecodeStep(t.pairs[1], t.q[1], t.k[1], t.v[1], t.out[1], table, lens, slots, D ** -0.5, 32)
+    t.pos.copy_(torch.tensor([0, 7], device=cuda))
+    for run in (step.run, GraphDecodeStep(step).replay):
+        t.fill()
+        run()
+        other.run()
+        for layer in range(LAYERS):
+            _same(t.pairs[0][layer], t.pairs[1][layer])
+
+
 def test_refusals(cuda):
     t = Two(cuda, "bf16", 2, 1)
     table, lens = torch.zeros((2, 2), dtype=torch.int32, device=cuda), torch.ones(2, dtype=torch.int32, device=cuda)

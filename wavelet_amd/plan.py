@@ -95,9 +95,12 @@ class Heads:
             of.append(w)
         return head_norm(*of, float(self.eps), float(self.weight_offset))
 
-    def check(self) -> None:
+    def check(self) -> "Heads":
+        """What the plan keeps: the tensors as they are now (it reads them by address)."""
         if self.eps is None and self.inv_freq is None:
             raise ValueError("heads need a norm (eps) or a rotation (inv_freq)")
+        return replace(self, q_weight=None if self.q_weight is None else list(self.q_weight),
+                       k_weight=None if self.k_weight is None else list(self.k_weight))
 
 
 def _rows(*tensors) -> tuple:
@@ -215,9 +218,7 @@ class DecodeStep:
         self.order = torch.arange(batch, dtype=torch.int32, device=dev)
         order_ptr = self.order.data_ptr() if self.ordered else None
         self.calls: list[_LayerCall] = []
-        self.heads = heads
-        if heads is not None:
-            heads.check()
+        self.heads = heads = None if heads is None else heads.check()
         for layer, cache in enumerate(caches):
             qq, kk, vv, oo = q[layer], key[layer], value[layer], out[layer]
             for name, t, shape in (("q", qq, (batch, hq, cache.head_dim)), ("out", oo, (batch, hq, cache.head_dim)),
@@ -414,7 +415,7 @@ class MLADecodeStep:
             raise ValueError("no layers")
         if heads is not None and heads.inv_freq is None:
             raise ValueError("heads of an MLA plan need a rotation")
-        self.heads = heads
+        self.heads = heads = None if heads is None else heads.check()
         c0 = caches[0]
         dev = c0.device
         self.block_table, self.seq_lens = check_tables(block_table, seq_lens, dev, c0.block_size, strict=True)
@@ -516,9 +517,7 @@ class PrefillStep:
             raise ValueError("q, key, value and out need one tensor per layer")
         self._live = _Live(caches)
         T = slot_mapping.numel()
-        self.heads = heads
-        if heads is not None:
-            heads.check()
+        self.heads = heads = None if heads is None else heads.check()
         self.lib = lib = _lib.load()
         self.stream = torch.cuda.current_stream(dev).cuda_stream
         need = max(lib.wkv_prefill_workspace_size(
@@ -638,7 +637,7 @@ class TreeStep:
                                      or not inv_freq.is_contiguous()):
             raise ValueError(f"inv_freq must be a contiguous float64 vector on {dev}")
         if heads is not None:
-            heads.check()
+            heads = heads.check()
             if inv_freq is not None or heads.positions is not None or heads.axes is not None:
                 raise ValueError("heads bring their own inv_freq, and no positions or axes: they are the step's")
         pending = state.next_tokens
