@@ -232,6 +232,33 @@ def test_rows_that_are_not_aligned(cuda, shift):
         _run(cuda, *_moved(cuda, (q, key, value), shift), _cache(cuda, blocks, 16, 2, 64, kv), slots, w, pos, freq, 1e-6)
 
 
+@pytest.mark.parametrize("shift", [0, 1, 4])
+@pytest.mark.parametrize("kv", ["bf16", "fp8_e4m3"])
+def test_one_row_that_is_not_aligned(cuda, kv, shift):
+    """A token whose row of projections is of an odd length, or starts off a 16-byte boundary: contiguous all the same."""
+    q, key, value, w, pos, freq = _inputs(cuda, 1, 4, 2, 64, 64, "dim")
+    row = torch.zeros((1, shift + 8 * 64 + 3), dtype=torch.bfloat16, device=cuda)
+    parts = [row[:, shift + at:shift + at + n].view(1, -1, 64) for at, n in ((0, 256), (256, 128), (384, 128))]
+    for p, x in zip(parts, (q, key, value)):
+        p.copy_(x)
+    slot = torch.tensor([17], device=cuda)
+    got, want = (_cache(cuda, 3, 16, 2, 64, kv) for _ in range(2))
+    a = rotary_append(parts[0], parts[1], parts[2], got, slot, pos, freq, q_weight=w[0], k_weight=w[1], eps=1e-6)
+    b = rotary_append(q.contiguous(), key.contiguous(), value.contiguous(), want, slot, pos, freq, q_weight=w[0],
+                      k_weight=w[1], eps=1e-6)
+    check_forward(a, q, w[0], 1e-6, heads.phases(f64(pos), f64(freq)), 0.0, False, 1.0)
+    check_forward(b, q, w[0], 1e-6, heads.phases(f64(pos), f64(freq)), 0.0, False, 1.0)
+    np.testing.assert_array_equal(_held(got)[1], _held(want)[1])
+    if kv == "bf16":
+        check_forward(got.k[1, :, :, 1].reshape(1, 2, 64), key, w[1], 1e-6, heads.phases(f64(pos), f64(freq)), 0.0, False, 1.0)
+    # and appended alone
+    alone, packed = (_cache(cuda, 3, 16, 2, 64, kv) for _ in range(2))
+    alone.append(parts[1], parts[2], slot)
+    packed.append(key.contiguous(), value.contiguous(), slot)
+    for x, y in zip(_held(alone), _held(packed)):
+        np.testing.assert_array_equal(x, y)
+
+
 def test_rows_aligned_to_eight_bytes(cuda):
     """norm_rotary takes them two elements at a time, rotary_append one: squares are added in another order."""
     q, key, value, w, pos, freq = _inputs(cuda, 30, 4, 2, 64, 64, "dim")

@@ -67,12 +67,12 @@ def _token_rows(x: torch.Tensor, name: str, shape: tuple[int, ...], device: torc
     if x.dtype is not torch.bfloat16 or x.shape[1:] != shape:
         raise ValueError(f"{name} must be bfloat16 [T, {', '.join(map(str, shape))}] (got {x.dtype} {tuple(x.shape)})")
     strides = x.stride()
-    if strides[-1] != 1 or x.data_ptr() % 16:
-        return x.contiguous()
+    aligned = strides[-1] == 1 and x.data_ptr() % 16 == 0
     for s in strides[:-1]:
         if s % 8:
-            return x.contiguous()
-    return x
+            aligned = False
+    # (not contiguous(): a row counts as contiguous whatever its address and its strides)
+    return x if aligned else x.clone(memory_format=torch.contiguous_format)
 
 
 class PagedKVCache:
