@@ -65,8 +65,8 @@ def rotary_append(q: torch.Tensor | None, key: torch.Tensor, value: torch.Tensor
                   k_weight: torch.Tensor | None = None, eps: float | None = None, weight_offset: float = 0.0,
                   axes: torch.Tensor | None = None, interleaved: bool = False, scale: float = 1.0,
                   out: torch.Tensor | None = None) -> torch.Tensor | None:
-    """Queries normed and turned -> a new tensor (or ``out``; ``out=q`` works in place), keys normed and turned and
-    values into ``cache`` at ``slot_mapping`` (-1: skipped).
+    """Queries normed and turned -> a new tensor (or ``out``: ``q`` itself, or one that shares no memory with the inputs),
+    keys normed and turned and values into ``cache`` at ``slot_mapping`` (-1: skipped).
 
     ``q [T, Hq, D]`` (None: keys and values only), ``key`` and ``value`` ``[T, Hkv, D]`` bf16, strided rows of a fused
     projection read in place. The norm is ``norm_rotary``'s and is done where ``eps`` is given, the rotation
@@ -124,7 +124,7 @@ def mla_rotary_append(q_pe: torch.Tensor | None, kv_c: torch.Tensor, k_pe: torch
                       kv_weight: torch.Tensor | None = None, eps: float | None = None, weight_offset: float = 0.0,
                       axes: torch.Tensor | None = None, interleaved: bool = False, scale: float = 1.0,
                       out: torch.Tensor | None = None) -> torch.Tensor | None:
-    """The queries' ``q_pe [T, H, rope_dim]`` (None: none) turned -> a new tensor (or ``out``), and into the latent
+    """The queries' ``q_pe [T, H, rope_dim]`` (None: none) turned -> a new tensor (or ``out``, as for ``rotary_append``), and into the latent
     ``cache`` at ``slot_mapping`` (-1: skipped) the compressed entries ``kv_c [T, kv_lora_rank]``, normed where ``eps``
     is given (weight ``[kv_lora_rank]``, None: ones), and ``k_pe [T, rope_dim]`` turned.
 
