@@ -71,6 +71,22 @@ def test_backward(cuda, shape, dtype, inter):
         check_backward(dk, dkw, c["k"], c["gk"], c["kw"], 1e-5, c["angle"], offset, inter, scale)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1401, 66, 8, 64, 64), (3, 64, 1, 64, 64), (1, 33, 2, 128, 32), (1500, 8, 32, 128, 128),
+                                   (1100, 17, 2, 512, 64)])
+def test_backward_of_long_rows_of_heads(cuda, shape, dtype):
+    """Rows of 4,096 elements and more, with one weight, with each head's, and with one of each."""
+    c, each = (_case(cuda, *shape, dtype, w, True) for w in ("dim", "each"))
+    for qw, kw in ((c["qw"], c["kw"]), (each["qw"], each["kw"]), (c["qw"], each["kw"]), (each["qw"], None)):
+        leaves = [x.detach().requires_grad_() for x in (c["q"], c["k"])]
+        ws = [None if x is None else x.detach().requires_grad_() for x in (qw, kw)]
+        q, k = norm_rotary(*leaves, c["pos"], c["freq"], q_weight=ws[0], k_weight=ws[1], eps=1e-5)
+        dq, dk, dqw, dkw = (*torch.autograd.grad([q, k], leaves + [w for w in ws if w is not None], [c["gq"], c["gk"]]),
+                            None)[:4]
+        check_backward(dq, dqw, c["q"], c["gq"], qw, 1e-5, c["angle"], 0.0, False, 1.0)
+        check_backward(dk, dkw, c["k"], c["gk"], kw, 1e-5, c["angle"], 0.0, False, 1.0)
+
+
 def test_gradients_against_differences(cuda):
     """Derivatives along random directions, by central differences of the float64 oracle: off by h^2 / 6 of a third
     derivative (some 1e-9 here) and the kernel's own bound, a few u of sums of some 4,000 terms of either sign."""

@@ -10,8 +10,10 @@
 // reciprocal root mean square,
 //   dx = r (m - x r^2 mean(m x)),   dw = sum over rows of z x r.
 // A group of lanes keeps its elements of dw in registers over all the rows that it takes; workgroups leave
-// their sums in the workspace, and a second kernel adds them up, in an order that the sizes alone give. 8,191 tokens of 24 heads of 128, bf16: 36 us
-// (151 MB, 4.2 TB/s) and 4.
+// their sums in the workspace, and a second kernel adds them up, in an order that the sizes alone give. Bound by
+// HBM: 16,384 tokens of 40 heads of 128, bf16, 100 us with the sums (503 MB, 5.0 TB/s); 8,191 tokens of 24 heads 36
+// (151 MB, 4.2 TB/s) and 4 for the sums.
+#include <algorithm>
 #include <type_traits>
 
 #include "norm_rotary_dev.h"
@@ -56,14 +58,14 @@ struct GradRows {
   int64_t xt, xh, gt, gh, dt, dh;
 };
 
-// A kind's workgroups: `wgs` along the tokens for each of its ranges of heads. One weight for all heads: one
-// range, every wave's groups take tokens and walk all heads. Each head its own: a range of as many heads as a
-// wave has groups, and every group keeps to one.
+// A kind's workgroups: `wgs` along the tokens for each of its ranges of heads. split: a range is as many heads as
+// a wave has groups, and every group keeps to one (also where each head has a weight of its own); else it is
+// all heads, which every wave's groups walk for some tokens.
 struct GradKind {
   GradRows s;
   const void *w;
   int64_t ws;
-  int heads, each, ranges, wgs;
+  int heads, each, split, ranges, wgs;
   int log_tg;
   int64_t first;  // of its sums in the workspace, in rows of D
 };
@@ -74,10 +76,10 @@ struct NormGradArgs {
   Angles a;  // sign: the transpose's
   RowUnits r;
   int64_t tokens;
-  float *partial;  // [wgs][1 or heads][D] of queries, then keys; nullptr: no weight's gradient
+  float *partial;  // [wgs][heads][D], or [ranges][wgs][D], of queries, then keys; nullptr: no weight's gradient
 };
 
-template <class T, int V, bool INTER, int U, bool FAR, bool DW>
+template <class T, int V, bool INTER, int U, bool FAR, bool DW, int LL>
 __global__ __launch_bounds__(kNormThreads) void norm_rotary_grad_kernel(NormGradArgs a) {
   typedef typename VecOf<T, V>::type Vec;
   extern __shared__ float2 turns[];
@@ -87,10 +89,12 @@ __global__ __launch_bounds__(kNormThreads) void norm_rotary_grad_kernel(NormGrad
   const GradKind &k = is_q ? a.q : a.k;
   const int b = is_q ? blockIdx.x : blockIdx.x - nq;
   const int range = b / k.wgs, wg = b - range * k.wgs;
-  const int lanes = 1 << a.r.log_lanes, u0 = threadIdx.x & (lanes - 1), g = (threadIdx.x & 63) >> a.r.log_lanes;
-  const int groups = 64 >> a.r.log_lanes, tg = 1 << k.log_tg, step = groups >> k.log_tg;
-  const int h0 = range * (k.each ? groups : k.heads), heads = k.each ? (k.heads - h0 < groups ? k.heads - h0 : groups) : k.heads;
-  const int t = g & (tg - 1), first = g >> k.log_tg;
+  const int log_lanes = LL >= 0 ? LL : a.r.log_lanes;
+  const int lanes = 1 << log_lanes, u0 = threadIdx.x & (lanes - 1), g = (threadIdx.x & 63) >> log_lanes;
+  const int groups = 64 >> log_lanes, tg = 1 << k.log_tg, step = k.split ? groups : groups >> k.log_tg;
+  const int h0 = range * (k.split ? groups : k.heads), heads = k.split ? (k.heads - h0 < groups ? k.heads - h0 : groups) : k.heads;
+  const int t = k.split ? 0 : g & (tg - 1), first = k.split ? g : g >> k.log_tg;
+  const int rounds = k.split ? tg : (heads + step - 1) / step;
   float2 *turn = turns + (wave << k.log_tg) * a.r.half;
   const float inv_d = 1.f / static_cast<float>(a.r.D);
   const bool all = 2 * a.r.half == a.r.D;
@@ -109,12 +113,13 @@ __global__ __launch_bounds__(kNormThreads) void norm_rotary_grad_kernel(NormGrad
 #pragma unroll
     for (int v = 0; v < V; ++v) acc0[j][v] = acc1[j][v] = 0.f;
   }
-  // A round is a block of the wave's tokens and `step` heads; the next one's loads are in flight over it.
+  // A round is the wave's tokens of a block and `step` heads (split: one of the tokens and the range's heads); the
+  // next one's loads are in flight over it.
   const int64_t blocks = ((a.tokens - 1) >> k.log_tg) + 1, stride = static_cast<int64_t>(k.wgs) * kNormWaves;
   Vec nx0[U], nx1[U], ng0[U], ng1[U];
-  auto load = [&](int64_t block, int hb) __attribute__((always_inline)) {
-    const int64_t tt = (block << k.log_tg) + t;
-    const int h = hb + first;
+  auto load = [&](int64_t block, int round) __attribute__((always_inline)) {
+    const int64_t tt = (block << k.log_tg) + (k.split ? round : t);
+    const int h = (k.split ? 0 : round * step) + first;
     const T *x = static_cast<const T *>(k.s.x) + tt * k.s.xt + (h0 + h) * k.s.xh;
     const T *gr = static_cast<const T *>(k.s.g) + tt * k.s.gt + (h0 + h) * k.s.gh;
 #pragma unroll
@@ -132,7 +137,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_rotary_grad_kernel(NormGrad
   };
   UnitTurn<V> turned[U];
   int64_t block = static_cast<int64_t>(wg) * kNormWaves + wave;
-  int hb = 0;
+  int round = 0;
   if (block < blocks) load(block, 0);
   while (block < blocks) {  // uniform
     Vec x0[U], x1[U], g0[U], g1[U];
@@ -144,22 +149,24 @@ __global__ __launch_bounds__(kNormThreads) void norm_rotary_grad_kernel(NormGrad
       g1[j] = ng1[j];
     }
     const int64_t this_block = block;
-    const int this_h = hb;
-    hb += step;
-    if (hb >= heads) {
-      hb = 0;
+    const int this_round = round;
+    if (++round == rounds) {
+      round = 0;
       block += stride;
     }
-    if (block < blocks) load(block, hb);
-    if (this_h == 0) {
-      const int64_t t0 = this_block << k.log_tg;
-      const int nt = a.tokens - t0 < tg ? static_cast<int>(a.tokens - t0) : tg;
+    if (block < blocks) load(block, round);
+    const int64_t t0 = this_block << k.log_tg;
+    const int nt = a.tokens - t0 < tg ? static_cast<int>(a.tokens - t0) : tg;
+    const int mt = k.split ? this_round : t;  // the lane's token of the block
+    if (this_round == 0) {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the block before has been read
       __builtin_amdgcn_wave_barrier();
       wave_angles(a.a, t0, nt, turn);
+    }
+    if (this_round == 0 || k.split) {
 #pragma unroll
       for (int j = 0; j < U; ++j)
-        unit_turn<V, INTER>(turn + (t < nt ? t : 0) * a.r.half, a.r.half, all, e0[j], e1[j], turned[j]);
+        unit_turn<V, INTER>(turn + (mt < nt ? mt : 0) * a.r.half, a.r.half, all, e0[j], e1[j], turned[j]);
     }
     float f0[U][V], f1[U][V], z0[U][V], z1[U][V], ss = 0.f, sm = 0.f;
 #pragma unroll
@@ -175,12 +182,12 @@ __global__ __launch_bounds__(kNormThreads) void norm_rotary_grad_kernel(NormGrad
         sm = __builtin_fmaf(z0[j][v] * w0[j][v], f0[j][v], __builtin_fmaf(z1[j][v] * w1[j][v], f1[j][v], sm));
       }
     }
-    ss = group_sum(ss, a.r.log_lanes);
-    sm = group_sum(sm, a.r.log_lanes);
+    ss = group_sum<LL>(ss, log_lanes);
+    sm = group_sum<LL>(sm, log_lanes);
     const float inv = __builtin_amdgcn_rsqf(__builtin_fmaf(ss, inv_d, a.n.eps));
     const float back = sm * inv_d * inv * inv;
-    const int64_t tt = (this_block << k.log_tg) + t;
-    const int h = this_h + first;
+    const int64_t tt = t0 + mt;
+    const int h = (k.split ? 0 : this_round * step) + first;
     const bool store = k.s.dx != nullptr && tt < a.tokens && h < heads;
     T *y = static_cast<T *>(k.s.dx) + tt * k.s.dt + (h0 + h) * k.s.dh;
 #pragma unroll
@@ -230,7 +237,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_rotary_grad_kernel(NormGrad
   }
   __syncthreads();
   const int n = k.each ? heads : 1;  // a group's number is its head's, one token a wave
-  float *out = a.partial + (k.first + static_cast<int64_t>(wg) * (k.each ? k.heads : 1) + (k.each ? h0 : 0)) * a.r.D;
+  float *out = a.partial + (k.first + (k.each ? static_cast<int64_t>(wg) * k.heads + h0 : b)) * a.r.D;
   for (int d = threadIdx.x; d < n * a.r.D; d += kNormThreads) {
     float s = 0.f;
 #pragma unroll
@@ -279,15 +286,15 @@ __global__ __launch_bounds__(64 * kSumWaves) void norm_weight_grad_kernel(Weight
 }
 
 // ---------------------------------------------------------------------------
-// Host. The forward launch. Heads of 64 and 128 in 16-byte accesses have their lanes as a constant (16,384
-// tokens of 40 heads of 128, bf16: 65.1 us, 67.2 without).
+// Host. The launches. Heads of 64 and 128 in 16-byte accesses have their lanes as a constant (16,384 tokens of 40
+// heads of 128, bf16: 65.1 us forward, 67.2 without, and 67.2 and 74.5 with each head's weights; backward 119 and 122).
 template <class T, int V, bool INTER, bool EACH>
 static void launch_norm(const NormRotaryArgs &a, bool far, unsigned grid, size_t lds, hipStream_t s) {
   if (a.r.units > 64) {
     if constexpr (V <= 2) norm_rotary_kernel<T, V, INTER, 4, false, EACH, -1><<<grid, kNormThreads, lds, s>>>(a);
     return;
   }
-  if constexpr (V * sizeof(T) == 16 && !EACH) {
+  if constexpr (V * sizeof(T) == 16) {
     constexpr int L64 = sizeof(T) == 2 ? 2 : 3, L128 = L64 + 1;
     if (a.r.log_lanes == L128 && far) return norm_rotary_kernel<T, V, INTER, 1, true, EACH, L128><<<grid, kNormThreads, lds, s>>>(a);
     if (a.r.log_lanes == L128) return norm_rotary_kernel<T, V, INTER, 1, false, EACH, L128><<<grid, kNormThreads, lds, s>>>(a);
@@ -297,26 +304,21 @@ static void launch_norm(const NormRotaryArgs &a, bool far, unsigned grid, size_t
   norm_rotary_kernel<T, V, INTER, 1, false, EACH, -1><<<grid, kNormThreads, lds, s>>>(a);
 }
 
-template <class T, int V, bool INTER>
+template <class T, int V, bool INTER, bool DW>
 static void launch_norm_grad(const NormGradArgs &a, bool far, unsigned grid, size_t lds, hipStream_t s) {
-  constexpr bool WIDE = V * sizeof(T) == 16;
-  const bool dw = a.partial != nullptr;
   if (a.r.units > 64) {
-    if constexpr (V <= 2) {
-      if (dw) norm_rotary_grad_kernel<T, V, INTER, 4, false, true><<<grid, kNormThreads, lds, s>>>(a);
-      else norm_rotary_grad_kernel<T, V, INTER, 4, false, false><<<grid, kNormThreads, lds, s>>>(a);
-    }
+    if constexpr (V <= 2) norm_rotary_grad_kernel<T, V, INTER, 4, false, DW, -1><<<grid, kNormThreads, lds, s>>>(a);
     return;
   }
-  if constexpr (WIDE) {
-    if (far) {
-      if (dw) norm_rotary_grad_kernel<T, V, INTER, 1, true, true><<<grid, kNormThreads, lds, s>>>(a);
-      else norm_rotary_grad_kernel<T, V, INTER, 1, true, false><<<grid, kNormThreads, lds, s>>>(a);
-      return;
-    }
+  if constexpr (V * sizeof(T) == 16) {
+    constexpr int L64 = sizeof(T) == 2 ? 2 : 3, L128 = L64 + 1;
+    if (a.r.log_lanes == L128 && far) return norm_rotary_grad_kernel<T, V, INTER, 1, true, DW, L128><<<grid, kNormThreads, lds, s>>>(a);
+    if (a.r.log_lanes == L128) return norm_rotary_grad_kernel<T, V, INTER, 1, false, DW, L128><<<grid, kNormThreads, lds, s>>>(a);
+    if (a.r.log_lanes == L64 && far) return norm_rotary_grad_kernel<T, V, INTER, 1, true, DW, L64><<<grid, kNormThreads, lds, s>>>(a);
+    if (a.r.log_lanes == L64) return norm_rotary_grad_kernel<T, V, INTER, 1, false, DW, L64><<<grid, kNormThreads, lds, s>>>(a);
+    if (far) return norm_rotary_grad_kernel<T, V, INTER, 1, true, DW, -1><<<grid, kNormThreads, lds, s>>>(a);
   }
-  if (dw) norm_rotary_grad_kernel<T, V, INTER, 1, false, true><<<grid, kNormThreads, lds, s>>>(a);
-  else norm_rotary_grad_kernel<T, V, INTER, 1, false, false><<<grid, kNormThreads, lds, s>>>(a);
+  norm_rotary_grad_kernel<T, V, INTER, 1, false, DW, -1><<<grid, kNormThreads, lds, s>>>(a);
 }
 
 // f(element type's zero, width, layout) for the call's.
@@ -422,18 +424,24 @@ extern "C" int wkv_norm_rotary(int32_t dtype, const void *q, int64_t q_stride_t,
 
 namespace {
 
-// A kind's workgroups of the backward launch along the tokens, and its rows of sums.
-struct GradGrid {
-  int wgs, rows;
-  GradGrid(int64_t tokens, int heads, int all_heads, int D, bool each) {
-    rows = each ? heads : 1;
-    // 768 workgroups (the three waves a SIMD that its registers allow: 36 us; 512 or 1,024 workgroups 46)
-    // shared by heads; where each head has sums of its own, by ranges of 1,024 elements
-    const int64_t share = each ? 1024 / ((static_cast<int64_t>(heads) * D + 1023) / 1024 + 1) : 768ll * heads / (all_heads > 0 ? all_heads : 1);
-    const int64_t most = (tokens + kNormWaves - 1) / kNormWaves, n = share < 1 ? 1 : share;
-    wgs = heads == 0 ? 0 : static_cast<int>(n < most ? n : most);
+// Most workgroups of the backward launch: the three waves a SIMD that its registers allow (8,191 tokens of 24
+// heads of 128, bf16: 36 us; 512 or 1,024 workgroups 46).
+constexpr int64_t kGradWorkgroups = 768;
+
+// The most rows of sums that a kind's workgroups leave: one each, of their share of the workgroups, or, where
+// each head has sums of its own, one a head from every workgroup along the tokens, of which a range of heads (a
+// wave's: 1,024 elements at most) has its share.
+struct GradSums {
+  int64_t rows = 0;
+  GradSums(int64_t tokens, int heads, int all_heads, int D, bool each) {
+    if (tokens == 0 || heads == 0) return;
+    const int64_t ranges = (static_cast<int64_t>(heads) * D + 1023) / 1024;
+    rows = each ? std::min(share(kGradWorkgroups, ranges), most(tokens)) * heads
+                : std::min(share(kGradWorkgroups * heads, all_heads), most(tokens) * (long_row(heads, D) ? heads : 1));
   }
-  int64_t floats(int D) const { return static_cast<int64_t>(wgs) * rows * D; }
+  static int64_t share(int64_t of, int64_t among) { return std::max<int64_t>(of / among, 1); }
+  static bool long_row(int heads, int D) { return heads * D >= 4096; }  // (taken by ranges also with one weight)
+  static int64_t most(int64_t tokens) { return (tokens + kNormWaves - 1) / kNormWaves; }
 };
 
 }  // namespace
@@ -445,9 +453,9 @@ extern "C" int64_t wkv_norm_rotary_workspace_size(int64_t num_tokens, int32_t nu
       num_k_heads > 65535 || head_dim <= 0 || head_dim > WKV_ROTARY_MAX_DIM)
     return -1;
   const int all = num_q_heads + num_k_heads;
-  return (GradGrid(num_tokens, num_q_heads, all, head_dim, q_weight_each_head != 0).floats(head_dim) +
-          GradGrid(num_tokens, num_k_heads, all, head_dim, k_weight_each_head != 0).floats(head_dim)) *
-         static_cast<int64_t>(sizeof(float));
+  return (GradSums(num_tokens, num_q_heads, all, head_dim, q_weight_each_head != 0).rows +
+          GradSums(num_tokens, num_k_heads, all, head_dim, k_weight_each_head != 0).rows) *
+         head_dim * static_cast<int64_t>(sizeof(float));
 }
 
 extern "C" int wkv_norm_rotary_backward(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_stride_h,
@@ -480,8 +488,10 @@ extern "C" int wkv_norm_rotary_backward(int32_t dtype, const void *q, int64_t q_
   const bool q_each = norm->q_weight != nullptr && norm->q_weight_stride_h != 0;
   const bool k_each = norm->k_weight != nullptr && norm->k_weight_stride_h != 0;
   const int H = num_q_heads + num_k_heads;
-  const GradGrid gq(num_tokens, num_q_heads, H, head_dim, q_each), gk(num_tokens, num_k_heads, H, head_dim, k_each);
-  const int64_t need = (gq.floats(head_dim) + gk.floats(head_dim)) * static_cast<int64_t>(sizeof(float));
+  const GradSums sq(num_tokens, num_q_heads, H, head_dim, q_each), sk(num_tokens, num_k_heads, H, head_dim, k_each);
+  const int64_t need = (sq.rows + sk.rows) * head_dim * static_cast<int64_t>(sizeof(float));
+  WeightGrads sum{static_cast<const float *>(workspace), dq_weight, dk_weight, q_each ? num_q_heads : num_q_heads > 0,
+                  k_each ? num_k_heads : num_k_heads > 0, 0, 0, head_dim, norm->weight_dtype};
   if (dw)
     WKV_CHECK_ARG(need == 0 || (workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= need),
                   "workspace must hold wkv_norm_rotary_workspace_size() bytes, 16-byte aligned");
@@ -507,14 +517,36 @@ extern "C" int wkv_norm_rotary_backward(int32_t dtype, const void *q, int64_t q_
     fit(num_k_heads, rk, norm->k_weight, norm->k_weight_stride_h);
     a.r = row_units(head_dim, half, w.v);
     const int groups = 64 >> a.r.log_lanes;
-    auto kind = [&](const GradRows &r, const void *weight, int64_t ws, int heads, bool each, const GradGrid &g, int64_t first) {
-      int log_tg = 0;
-      if (!each)
-        while ((2 << log_tg) <= groups && (num_tokens >> (log_tg + 1)) >= 2 * static_cast<int64_t>(g.wgs) * kNormWaves) ++log_tg;
-      return GradKind{r, weight, ws, heads, each, heads == 0 ? 0 : each ? (heads + groups - 1) / groups : 1, g.wgs, log_tg, first};
+    // Long rows of heads go by ranges with one weight too (16,384 tokens of 40 heads of 128, bf16: 100 us, 110 where a
+    // wave walks a token's heads; fp32 172 and 200), but not short ones (8,191 of 24: 40 and 37.5) or where a token's
+    // angles, which each range forms, cost more (32 of 256: 92 and 83). The workgroups are dealt by what a
+    // token of a kind costs, in heads: a range costs a whole wave.
+    auto in_ranges = [&](int heads, bool each, const GradSums &most) {
+      return each || (GradSums::long_row(heads, head_dim) && half <= 64 && most.rows >= (heads + groups - 1) / groups);
     };
-    a.q = kind(rq, norm->q_weight, norm->q_weight_stride_h, num_q_heads, q_each, gq, 0);
-    a.k = kind(rk, norm->k_weight, norm->k_weight_stride_h, num_k_heads, k_each, gk, static_cast<int64_t>(gq.wgs) * gq.rows);
+    const bool q_split = in_ranges(num_q_heads, q_each, sq), k_split = in_ranges(num_k_heads, k_each, sk);
+    auto ranges = [&](int heads, bool split) { return heads == 0 ? 0 : split ? (heads + groups - 1) / groups : 1; };
+    const int64_t cost_q = q_split ? ranges(num_q_heads, true) * groups : num_q_heads;
+    const int64_t cost_k = k_split ? ranges(num_k_heads, true) * groups : num_k_heads;
+    auto kind = [&](const GradRows &r, const void *weight, int64_t ws, int heads, bool each, bool split, int64_t cost,
+                    const GradSums &most, int64_t first) {
+      GradKind k{r, weight, ws, heads, each, split, ranges(heads, split), 0, 0, first};
+      if (heads == 0) return k;
+      const int64_t wgs = std::min(GradSums::share(kGradWorkgroups * cost, (cost_q + cost_k) * k.ranges), GradSums::most(num_tokens));
+      k.wgs = static_cast<int>(std::min(wgs, most.rows / (each ? heads : k.ranges)));  // (what the workspace is for)
+      // Two tokens a block in ranges (16,384 tokens of 40 heads of 128, bf16: 98 us, 105 of one, 103 of four);
+      // else as many as give every group of lanes a head (8,192 of 16 + 16 heads of 256: one 83, two 99).
+      const int64_t waves = static_cast<int64_t>(k.wgs) * kNormWaves;
+      while (split ? k.log_tg < 1 && (num_tokens >> 1) >= waves
+                   : (heads << k.log_tg) <= groups && (2 << k.log_tg) <= groups && (num_tokens >> (k.log_tg + 1)) >= waves)
+        ++k.log_tg;
+      return k;
+    };
+    a.q = kind(rq, norm->q_weight, norm->q_weight_stride_h, num_q_heads, q_each, q_split, cost_q, sq, 0);
+    sum.q_wgs = a.q.wgs * (q_each ? 1 : a.q.ranges);
+    a.k = kind(rk, norm->k_weight, norm->k_weight_stride_h, num_k_heads, k_each, k_split, cost_k, sk,
+               static_cast<int64_t>(sum.q_wgs) * sum.q_rows);
+    sum.k_wgs = a.k.wgs * (k_each ? 1 : a.k.ranges);
     const int64_t grid = static_cast<int64_t>(a.q.ranges) * a.q.wgs + static_cast<int64_t>(a.k.ranges) * a.k.wgs;
     WKV_CHECK_ARG(grid <= kMaxWorkgroups, "too many tokens and heads for one launch");
     const bool far = num_tokens * H * head_dim * esz >= (64 << 20);
@@ -523,15 +555,15 @@ extern "C" int wkv_norm_rotary_backward(int32_t dtype, const void *q, int64_t q_
     const size_t sums = static_cast<size_t>(kNormWaves) * (q_each || k_each ? groups : 1) * head_dim * sizeof(float);
     const size_t lds = turns > sums ? turns : sums;
     with_types(dtype, w.v, inter, [&](auto zero, auto v, auto in) {
-      launch_norm_grad<decltype(zero), decltype(v)::value, decltype(in)::value>(a, far, static_cast<unsigned>(grid), lds, s);
+      using T = decltype(zero);
+      if (dw) launch_norm_grad<T, decltype(v)::value, decltype(in)::value, true>(a, far, static_cast<unsigned>(grid), lds, s);
+      else launch_norm_grad<T, decltype(v)::value, decltype(in)::value, false>(a, far, static_cast<unsigned>(grid), lds, s);
     });
     WKV_CHECK_LAUNCH("norm_rotary_backward");
   }
   if (dw) {
-    WeightGrads a{static_cast<const float *>(workspace), dq_weight, dk_weight, num_q_heads > 0 ? gq.rows : 0,
-                  num_k_heads > 0 ? gk.rows : 0, gq.wgs, gk.wgs, head_dim, norm->weight_dtype};
-    const dim3 grid(static_cast<unsigned>(a.q_rows + a.k_rows), static_cast<unsigned>((head_dim + 63) / 64));
-    norm_weight_grad_kernel<<<grid, 64 * kSumWaves, 0, s>>>(a);
+    const dim3 grid(static_cast<unsigned>(sum.q_rows + sum.k_rows), static_cast<unsigned>((head_dim + 63) / 64));
+    norm_weight_grad_kernel<<<grid, 64 * kSumWaves, 0, s>>>(sum);
     WKV_CHECK_LAUNCH("norm_weight_grad");
   }
   return WKV_OK;
