@@ -555,10 +555,11 @@ int wkv_rotary_append(const wkv_cache_t *cache, const void *key, int64_t key_str
                       int64_t qo_stride_h, int32_t num_q_heads, const wkv_head_norm_t *norm,
                       const wkv_rotary_t *rotary, int64_t num_tokens, void *stream);
 
-/* The same for a latent cache: latent[slot[t]] = concat(kv_c[t] normed (kv_norm's k_weight [kv_lora_rank], eps and
- * offset; NULL: as it is), k_pe[t] turned), and the queries' q_pe [num_tokens, num_heads, rope_dim] turned into
- * q_out. kv_c, k_pe and slot_mapping as for wkv_mla_append. Replaces the engine's norm of the compressed entries,
- * its rotary embedding (wavelet/inference/deepseek_v4.py:15-66) and its latent append. */
+/* The same for a latent cache: latent[slot[t]] = concat(kv_c[t] normed (kv_norm's k_weight [kv_lora_rank], 16-byte
+ * aligned, its head stride 0, eps and offset; NULL: as it is), k_pe[t] turned), and the queries' q_pe
+ * [num_tokens, num_heads, rope_dim] turned into q_out. kv_c, k_pe and slot_mapping as for wkv_mla_append. Replaces the
+ * engine's norm of the compressed entries, its rotary embedding (wavelet/inference/deepseek_v4.py:15-66) and its
+ * latent append. */
 int wkv_mla_rotary_append(const wkv_mla_cache_t *cache, const void *kv_c, int64_t kv_c_stride, const void *k_pe,
                           int64_t k_pe_stride, const int64_t *slot_mapping, const void *q_pe, int64_t q_stride_t,
                           int64_t q_stride_h, void *q_out, int64_t qo_stride_t, int64_t qo_stride_h, int32_t num_heads,

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from wavelet_amd import _lib
+from wavelet_amd.plan import Heads
 
 # fake device pointers: only where no GPU is visible, so that no call can reach a device
 pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="fake device pointers: host-only test")
@@ -150,3 +151,36 @@ def test_mla_rotary_append():
             assert call(norm=_norm(**{"q_weight": None, **bad})) == _lib.WKV_ERR_INVALID, bad
     # rows of 16-byte pieces only from rope_dim 136 on, where a lane would hold more than one unit
     assert call(cache=ctypes.byref(cache(rope_dim=256)), q=A + 2, rotary=_rotary(rotary_dim=256)) == _lib.WKV_ERR_UNSUPPORTED
+
+
+def test_mla_norm_weight_is_one_row():
+    """A weight for each head has no meaning for an entry: the kernel would take the first row for all."""
+    lib = _lib.load()
+    cache = _lib.WkvMlaCache(latent=A, num_blocks=4, block_size=64, kv_lora_rank=512, rope_dim=64)
+
+    def call(**norm):
+        return lib.wkv_mla_rotary_append(ctypes.byref(cache), A, 576, A, 576, A, A, 8192, 64, A, 8192, 64, 128,
+                                         _norm(q_weight=None, **norm), _rotary(rotary_dim=64), 0, None)
+
+    assert call() == _lib.WKV_OK
+    assert call(k_weight_stride_h=512) == _lib.WKV_ERR_INVALID
+    assert "one row" in _lib.last_error()
+
+
+def test_a_plan_s_entry_weights():
+    """What MLADecodeStep checks of a layer's norm when it is built (as mla_rotary_append does for a call)."""
+    entries = torch.zeros((3, 512), dtype=torch.bfloat16)
+    good = torch.ones(512, dtype=torch.bfloat16)
+    off = torch.ones(520, dtype=torch.bfloat16)[1:513]
+    norm = Heads(eps=1e-6, k_weight=[good]).entry_norm(0, 1, entries)
+    assert norm.k_weight == good.data_ptr() and norm.k_weight_stride_h == 0
+    assert Heads(eps=1e-6).entry_norm(0, 1, entries).k_weight is None
+    assert Heads(eps=1e-6, k_weight=[None, good]).entry_norm(0, 2, entries).k_weight is None
+    assert Heads().entry_norm(0, 1, entries) is None
+    for bad in (torch.ones((512, 512), dtype=torch.bfloat16), torch.ones((1, 512), dtype=torch.bfloat16), off, good[:64],
+                good.half()):
+        with pytest.raises(ValueError):
+            Heads(eps=1e-6, k_weight=[bad]).entry_norm(0, 1, entries)
+    for bad in (Heads(k_weight=[good]), Heads(eps=1e-6, k_weight=[good, good]), Heads(eps=1e-6, q_weight=[good])):
+        with pytest.raises(ValueError):
+            bad.entry_norm(0, 1, entries)

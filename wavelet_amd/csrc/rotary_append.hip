@@ -704,7 +704,8 @@ extern "C" int wkv_mla_rotary_append(const wkv_mla_cache_t *cache, const void *k
   if (kv_norm != nullptr) {
     if (const int rc = check_head_norm(kv_norm, 1)) return rc;
     WKV_CHECK_ARG(kv_norm->q_weight == nullptr, "kv_norm norms the compressed entries alone (k_weight)");
-    WKV_CHECK_ARG(kv_norm->k_weight == nullptr || aligned16(kv_norm->k_weight), "the norm's weight must be 16-byte aligned");
+    WKV_CHECK_ARG(kv_norm->k_weight == nullptr || (aligned16(kv_norm->k_weight) && kv_norm->k_weight_stride_h == 0),
+                  "the norm's weight must be one row of kv_lora_rank, 16-byte aligned");
   }
   if (num_tokens == 0) return WKV_OK;
   WKV_CHECK_ARG(slot_mapping != nullptr && reinterpret_cast<uintptr_t>(slot_mapping) % 8 == 0, "slot_mapping must be int64");

@@ -95,6 +95,13 @@ class Heads:
             of.append(w)
         return head_norm(*of, float(self.eps), float(self.weight_offset))
 
+    def entry_norm(self, layer: int, layers: int, entries: torch.Tensor):
+        """The library's norm of one layer's compressed entries (None without one): a weight for a whole entry."""
+        for w in self.k_weight or ():
+            if w is not None and (w.dim() != 1 or w.data_ptr() % 16):
+                raise ValueError(f"k_weight must be [{entries.shape[1]}] for each layer, aligned to 16 bytes")
+        return self.norm(layer, layers, None, entries)
+
     def check(self) -> "Heads":
         """What the plan keeps: the tensors as they are now (it reads them by address)."""
         if self.eps is None and self.inv_freq is None:
@@ -453,7 +460,7 @@ class MLADecodeStep:
             fused_args = (desc, kc.data_ptr(), kc.stride(0), kp.data_ptr(), kp.stride(0), slot_mapping.data_ptr(),
                           *decode_args[1:])
             if heads is not None:
-                append_args = (*append_args[:6], *_rows(qp, qp), heads_n, heads.norm(layer, len(caches), None, kc),
+                append_args = (*append_args[:6], *_rows(qp, qp), heads_n, heads.entry_norm(layer, len(caches), kc),
                                heads.rotation(batch, cache.rope_dim, dev), batch, self.stream)
             self.calls.append((append_args, decode_args, fused_args))
         self._keep = (caches, q_nope, q_pe, kv_c, k_pe, out, slot_mapping)
