@@ -542,13 +542,13 @@ int wkv_norm_rotary_backward(int32_t dtype, const void *q, int64_t q_stride_t, i
 
 /* The append with the norm and the rotation on the way, in one launch: the queries normed and turned into q_out (or
  * in place; num_q_heads may be 0), the keys normed and turned into the cache, the values into the cache. The cache
- * then holds what wkv_norm_rotary followed by wkv_append or wkv_append_fp8 leaves in it, bit for bit where queries
- * and weights are 16-byte aligned too (otherwise, and without a norm, where wkv_rotary_axes goes first, but for the
- * last bit of a key), keys rounded to bf16 before they are coded in fp8; key and value themselves are not changed. norm or rotary may be NULL, not both. key, value and
- * slot_mapping as for wkv_append (wkv_append_fp8); a slot appears once in a call, and an fp8 cache's block in one
- * run. q and its result bf16 [num_tokens, num_q_heads, head_dim], strides in elements; every token's queries are
- * computed, also those of slot -1. Replaces the engine's norms, rotary embedding and append of a layer (inside
- * llm.generate, engine.py:887). */
+ * then holds what wkv_norm_rotary of the same rows (its k_out's 16-byte aligned) followed by wkv_append or
+ * wkv_append_fp8 leaves in it, bit for bit (without a norm, where wkv_rotary_axes goes first, but for the last bit of
+ * a key), keys rounded to bf16 before they are coded in fp8; key and value themselves are not changed. norm or rotary
+ * may be NULL, not both. key, value and slot_mapping as for wkv_append (wkv_append_fp8); a slot appears once in a
+ * call, and an fp8 cache's block in one run. q and its result bf16 [num_tokens, num_q_heads, head_dim], strides in
+ * elements; every token's queries are computed, also those of slot -1. Replaces the engine's norms, rotary embedding
+ * and append of a layer (inside llm.generate, engine.py:887). */
 int wkv_rotary_append(const wkv_cache_t *cache, const void *key, int64_t key_stride_t, int64_t key_stride_h,
                       const void *value, int64_t value_stride_t, int64_t value_stride_h, const int64_t *slot_mapping,
                       const void *q, int64_t q_stride_t, int64_t q_stride_h, void *q_out, int64_t qo_stride_t,

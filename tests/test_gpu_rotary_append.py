@@ -271,6 +271,23 @@ def test_rows_aligned_to_eight_bytes(cuda):
 
 
 @pytest.mark.parametrize("kv", ["bf16", "fp8_e4m3"])
+@pytest.mark.parametrize("d,r,inter,shift", [(64, 20, False, 0), (128, 20, False, 0), (128, 92, False, 0), (64, 64, True, 4),
+                                             (64, 34, False, 0)])
+def test_squares_are_added_in_norm_rotary_s_order(cuda, d, r, inter, shift, kv):
+    """Pairs that are taken two or one at a time, from values of many sizes, whose sum depends on the order in its last bit
+    (and some 1 in 2^16 results with it: tens of these)."""
+    rng = np.random.default_rng(r)
+    slots, blocks = _slots(rng, [3000, 1096], [0, 5], 16)
+    q, key, value, w, pos, freq = _inputs(cuda, len(slots), 16, 8, d, r, "dim")
+    g = torch.Generator(device=cuda).manual_seed(1)
+    q, key = ((x * torch.exp(2 * torch.randn(x.shape, generator=g, device=cuda))).bfloat16() for x in (q, key))
+    if shift:  # (rows aligned to 8 bytes)
+        wide = torch.empty((len(slots), 16 * d + 12), device=cuda).bfloat16()[:, shift:shift + 16 * d].view(q.shape)
+        q = wide.copy_(q)
+    _run(cuda, q, key, value, _cache(cuda, blocks, 16, 8, d, kv), slots, w, pos, freq, 1e-6, interleaved=inter)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8_e4m3"])
 def test_prompt_and_decode_as_they_are_used(cuda, kv):
     """A prompt and then tokens one by one: rotary_append and the attentions against norm_rotary and theirs. (A decode
     step's two results are apart as test_gpu_step_heads.py derives.)"""

@@ -190,7 +190,7 @@ struct Coder {
     }
     return c;
   }
-  __device__ __forceinline__ uint32_t one(uint32_t bits) const { return eight(bits, 0u, 0u, 0u)[0] & 0xffu; }
+  __device__ __forceinline__ uint32_t two(uint32_t w) const { return eight(w, 0u, 0u, 0u)[0]; }  // (and those of zeros)
 };
 
 // The largest magnitude of bf16 pairs, as bits: the two halves side by side; a NaN's are above infinity's.
@@ -242,7 +242,7 @@ __device__ __forceinline__ void append_keys(const AppendArgs &a, float2 *turn, i
                                             int h, bool active) {
   typedef typename VecOf<__bf16, V>::type Vec;
   constexpr int G = 64 >> LL, P = kPiece / G, W = V == 8 ? 4 : 1;
-  static_assert(P * G == kPiece && (V == 8 || V == 1), "rows of a piece");
+  static_assert(P * G == kPiece && (V == 8 || V == 2 || V == 1), "rows of a piece");
   uint8_t *kc = static_cast<uint8_t *>(a.kc);
   int lane = threadIdx.x & 63;
   asm volatile("" : "+v"(lane));  // (nothing that depends on it is held across the runs: registers)
@@ -294,8 +294,8 @@ __device__ __forceinline__ void append_keys(const AppendArgs &a, float2 *turn, i
       unit_once<V, INTER>(turn + (off[p] >= 0 ? p * G + group : 0) * a.r.half, a.r.half, all, e0, e1, w0, w1, inv, f0, f1);
 #pragma unroll
       for (int i = 0; i < W; ++i) {
-        k0[p][i] = V == 8 ? pack_bf16x2(f0[2 * i % V], f0[(2 * i + 1) % V]) : pack_bf16x2(f0[0], 0.f);
-        k1[p][i] = V == 8 ? pack_bf16x2(f1[2 * i % V], f1[(2 * i + 1) % V]) : pack_bf16x2(f1[0], 0.f);
+        k0[p][i] = V > 1 ? pack_bf16x2(f0[2 * i % V], f0[(2 * i + 1) % V]) : pack_bf16x2(f0[0], 0.f);
+        k1[p][i] = V > 1 ? pack_bf16x2(f1[2 * i % V], f1[(2 * i + 1) % V]) : pack_bf16x2(f1[0], 0.f);
       }
       __builtin_amdgcn_sched_barrier(0);  // (a round's registers are free before the next one's are taken)
     }
@@ -343,8 +343,9 @@ __device__ __forceinline__ void append_keys(const AppendArgs &a, float2 *turn, i
           *reinterpret_cast<u32x2 *>(y1) = c1;
         }
       } else if (off[p] >= 0) {
-        *y0 = static_cast<uint8_t>(code.one(k0[p][0] & 0xffffu));
-        *y1 = static_cast<uint8_t>(code.one(k1[p][0] & 0xffffu));
+        typedef std::conditional_t<V == 2, uint16_t, uint8_t> Codes;
+        *reinterpret_cast<Codes *>(y0) = static_cast<Codes>(code.two(k0[p][0]));
+        *reinterpret_cast<Codes *>(y1) = static_cast<Codes>(code.two(k1[p][0]));
       }
     }
   }
@@ -460,7 +461,7 @@ __device__ __forceinline__ void window_runs(const AppendArgs &a, int wg, F f) {
 // 38.5 us in the place of 40.4 for 8,386 tokens of 28/4 heads.
 template <int D, int V, bool INTER, bool FP8, bool EACH, bool FAR>
 __global__ __launch_bounds__(kThreads, FP8 ? 4 : 1) void rotary_append_kernel(AppendArgs a) {
-  constexpr int UNITS = D / (2 * V), LL = UNITS == 64 ? 6 : UNITS == 32 ? 5 : UNITS == 8 ? 3 : 2;
+  constexpr int UNITS = D / (2 * V), LL = UNITS == 64 ? 6 : UNITS == 32 ? 5 : UNITS == 16 ? 4 : UNITS == 8 ? 3 : 2;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int wg = blockIdx.x;
   float2 *turn = reinterpret_cast<float2 *>(lds);
@@ -612,7 +613,6 @@ extern "C" int wkv_rotary_append(const wkv_cache_t *cache, const void *key, int6
     if (num_q_heads > 0) w.weights(norm->q_weight, norm->q_weight_stride_h, wsz);
     w.weights(norm->k_weight, norm->k_weight_stride_h, wsz);
   }
-  if (w.v < 8) w.v = 1;
   AppendArgs a{};
   a.key = static_cast<const uint16_t *>(key);
   a.val = static_cast<const uint16_t *>(value);
@@ -680,7 +680,9 @@ extern "C" int wkv_rotary_append(const wkv_cache_t *cache, const void *key, int6
     if (inter) launch(d, v, std::true_type{}); else launch(d, v, std::false_type{});
   };
   auto width = [&](auto d) {
-    if (w.v == 8) layout(d, std::integral_constant<int, 8>{}); else layout(d, std::integral_constant<int, 1>{});
+    if (w.v == 8) layout(d, std::integral_constant<int, 8>{});
+    else if (w.v == 2) layout(d, std::integral_constant<int, 2>{});
+    else layout(d, std::integral_constant<int, 1>{});
   };
   if (D == 128) width(std::integral_constant<int, 128>{}); else width(std::integral_constant<int, 64>{});
   WKV_CHECK_LAUNCH("rotary_append");

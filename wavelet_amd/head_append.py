@@ -73,8 +73,8 @@ def rotary_append(q: torch.Tensor | None, key: torch.Tensor, value: torch.Tensor
     ``apply_rotary``'s and done where ``positions`` and ``inv_freq`` are; one of them at least. The attention then
     takes the result and no ``key`` / ``value`` (``paged_decode_gqa``, ``prefill_gqa``, ``paged_tree_gqa``). ``key`` and
     ``value`` are left as they are, and the cache, bf16 or fp8, holds what ``norm_rotary`` and ``cache.append`` would
-    leave in it (bit for bit where queries and weights are aligned to 16 bytes; otherwise, and where ``apply_rotary``
-    goes first, but for a key's last bit). A slot appears once in a call, a block of an fp8 cache in one run of it (as
+    leave in it, bit for bit where the key's rows start on 16-byte boundaries (elsewhere they are copied, and then, as
+    where ``apply_rotary`` goes first, a key's last bit may differ). A slot appears once in a call, a block of an fp8 cache in one run of it (as
     for ``cache.append``).
     """
     if not isinstance(cache, PagedKVCache):
