@@ -104,6 +104,59 @@ def test_prompt_then_decode(cuda, kv, axes):
             assert torch.equal(t.out[0][layer], t.out[1][layer])
 
 
+def _decode_pair(cuda, kv, batch, make_heads, seed, per=2, start=0, **plan):
+    """Two decode plans over inputs that are the same (``per`` blocks a sequence, ``start`` tokens in each): their parts,
+    and a function that refills both."""
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    caches = [[PagedKVCache(per * batch, BS, HKV, D, kv_dtype=kv, device=cuda) for _ in range(LAYERS)] for _ in range(2)]
+    for a, b in zip(*caches):
+        x, y = (torch.randn((per * batch * BS, HKV, D), generator=g, device=cuda).bfloat16() for _ in range(2))
+        for c in (a, b):
+            c.append(x, y, torch.arange(per * batch * BS, device=cuda))
+    z = lambda h: [torch.zeros((batch, h, D), dtype=torch.bfloat16, device=cuda) for _ in range(LAYERS)]  # noqa: E731
+    bufs = [(z(HQ), z(HKV), z(HKV), z(HQ)) for _ in range(2)]
+    table = torch.randperm(per * batch, generator=g, device=cuda).int().view(batch, per)
+    lens, slots = (torch.full((batch,), n, dtype=dt, device=cuda) for n, dt in ((start, torch.int32), (0, torch.int64)))
+    pos3 = torch.zeros((3, batch), dtype=torch.int64, device=cuda)
+    steps = [DecodeStep(caches[i], *bufs[i], table, lens, slots, D ** -0.5, per * BS, heads=make_heads(i, pos3), **plan)
+             for i in range(2)]
+
+    def fill():
+        p = lens.long()
+        lens.add_(1)
+        slots.copy_(table[torch.arange(batch, device=cuda), p // BS].long() * BS + p % BS)
+        pos3.copy_(torch.randint(0, 1 << 17, pos3.shape, generator=g, device=cuda))
+        for layer in range(LAYERS):
+            for x, y in zip(bufs[0][:3], bufs[1][:3]):
+                x[layer].normal_(generator=g)
+                y[layer].copy_(x[layer])
+
+    return caches, bufs, steps, fill
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8_e4m3"])
+@pytest.mark.parametrize("axes", [False, True])
+@pytest.mark.parametrize("batch,per,start,part", [(256, 2, 0, 0), (3, 64, 1000, 128)])
+def test_turned_alone_and_captured(cuda, kv, axes, batch, per, start, part):
+    """Heads with a rotation and no norm: a captured plan leaves what the same plan leaves when it is run, also where a
+    context is shared out and merged."""
+    freq = rotary_frequencies(D, 1e4, device=cuda)[0]
+    of = rotary_axes((12, 10, 10), device=cuda) if axes else None
+    caches, bufs, steps, fill = _decode_pair(
+        cuda, kv, batch, lambda i, pos: Heads(pos if axes else pos[0], freq, of, scale=1.25), 21, per, start,
+        partition_size=part)
+    graph = GraphDecodeStep(steps[1])
+    for _ in range(5):
+        fill()
+        keys = [x.clone() for x in bufs[0][1]]
+        steps[0].run()
+        graph.replay()
+        for layer in range(LAYERS):
+            assert torch.equal(bufs[0][0][layer], bufs[1][0][layer]) and torch.equal(bufs[0][1][layer], keys[layer])
+            _same(caches[0][layer], caches[1][layer])
+            assert torch.equal(bufs[0][3][layer], bufs[1][3][layer])
+
+
 @pytest.mark.parametrize("kv", ["bf16", "fp8_e4m3"])
 def test_drafted_steps(cuda, kv):
     rows = 48
