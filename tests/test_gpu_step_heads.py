@@ -9,7 +9,8 @@ import pytest
 import torch
 from kvcase import bits_of
 
-from wavelet_amd import KVPool, MLALatentCache, PagedKVCache, mla_rotary_append, norm_rotary, rotary_axes, rotary_frequencies
+from wavelet_amd import (KVPool, MLALatentCache, PagedKVCache, mla_rotary_append, norm_rotary, rotary_append, rotary_axes,
+                         rotary_frequencies)
 from wavelet_amd.plan import DecodeStep, GraphDecodeStep, Heads, MLADecodeStep, PrefillStep, TreeStep
 
 pytestmark = pytest.mark.gpu
@@ -155,6 +156,136 @@ def test_turned_alone_and_captured(cuda, kv, axes, batch, per, start, part):
             assert torch.equal(bufs[0][0][layer], bufs[1][0][layer]) and torch.equal(bufs[0][1][layer], keys[layer])
             _same(caches[0][layer], caches[1][layer])
             assert torch.equal(bufs[0][3][layer], bufs[1][3][layer])
+
+
+KINDS = {  # what a plan's heads may be: (turned, several axes, normed, weights, offset)
+    "turned": (True, False, False, False, 0.0), "turned by axes": (True, True, False, False, 0.0),
+    "normed": (False, False, True, True, 0.0), "normed without weights": (False, False, True, False, 0.0),
+    "both, without weights": (True, False, True, False, 0.0), "both by axes": (True, True, True, True, 1.0),
+}
+
+
+class Kind:
+    """Heads of a kind, and the same by ``rotary_append`` alone."""
+
+    def __init__(self, cuda, kind, pos3, seed=0):
+        turned, axes, normed, weights, offset = KINDS[kind]
+        g = torch.Generator(device=cuda).manual_seed(seed)
+        how = {}
+        if turned:
+            how.update(positions=pos3 if axes else pos3[0], inv_freq=rotary_frequencies(48, 1e4, device=cuda)[0], scale=1.25,
+                       interleaved=True, axes=rotary_axes((10, 8, 6), device=cuda) if axes else None)
+        if normed:
+            how.update(eps=1e-5, weight_offset=offset)
+        self.how = how
+        self.w = [[1 + 0.2 * torch.randn(D, generator=g, device=cuda) for _ in range(LAYERS)] for _ in range(2)] if weights else None
+        self.heads = Heads(**how) if not weights else Heads(q_weight=self.w[0], k_weight=self.w[1], **how)
+
+    def append(self, layer, q, key, value, cache, slots):
+        w = {} if self.w is None else dict(q_weight=self.w[0][layer], k_weight=self.w[1][layer])
+        rotary_append(q, key, value, cache, slots, out=q, **w, **self.how)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8_e4m3"])
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("groups", [False, True])
+def test_kinds_of_heads_in_a_decode_step(cuda, kind, kv, groups):
+    """A plan, and but for groups a captured one, against rotary_append and the plan's attention alone; a normed plan's
+    captured attention takes the new token from its buffers (the tolerance above)."""
+    batch, made = 6, {}
+
+    def make(i, pos):
+        made["of"] = Kind(cuda, kind, pos)
+        return made["of"].heads if i == 0 else None
+
+    more = dict(group_size=3, prefix_lens=torch.tensor([32, 16], dtype=torch.int32, device=cuda), max_prefix_len=32) if groups else {}
+    caches, bufs, steps, fill = _decode_pair(cuda, kv, batch, make, 31, 8, 60, **more)
+    runs = [steps[0].run] if groups else [steps[0].run, GraphDecodeStep(steps[0]).replay]
+    for n in range(6):
+        fill()
+        keys = [x.clone() for x in bufs[0][1]]
+        captured = n % len(runs) == 1
+        runs[n % len(runs)]()
+        steps[1].prepare()
+        for layer in range(LAYERS):
+            q, k, v, out = (x[layer] for x in bufs[1])
+            made["of"].append(layer, q, k, v, caches[1][layer], steps[1].slot_mapping)
+            steps[1].attend(layer)
+            assert torch.equal(bufs[0][0][layer], q)
+            _same(caches[0][layer], caches[1][layer])
+            if captured and "eps" in made["of"].how:
+                torch.testing.assert_close(bufs[0][3][layer].float(), out.float(), rtol=2.0 ** -7, atol=5 * 2.0 ** -8)
+            else:
+                assert torch.equal(bufs[0][3][layer], out) and torch.equal(bufs[0][1][layer], keys[layer])
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8_e4m3"])
+@pytest.mark.parametrize("kind", KINDS)
+def test_kinds_of_heads_in_a_prompt(cuda, kind, kv):
+    lens = [37, 5, 20]
+    g = torch.Generator(device=cuda).manual_seed(41)
+    pairs = [[PagedKVCache(24, BS, HKV, D, kv_dtype=kv, device=cuda) for _ in range(LAYERS)] for _ in range(2)]
+    bufs = [[torch.randn((62, h, D), generator=g, device=cuda).bfloat16() for _ in range(LAYERS)] for h in (HQ, HKV, HKV, HQ)]
+    bufs = [[[x.clone() for x in of] for of in bufs] for _ in range(2)]
+    table = torch.randperm(24, generator=g, device=cuda).int().view(3, 8)
+    seq = torch.repeat_interleave(torch.arange(3, device=cuda), torch.tensor(lens, device=cuda))
+    pos = torch.cat([torch.arange(n, device=cuda) for n in lens])
+    slots = table[seq, pos // BS].long() * BS + pos % BS
+    seq_lens = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    cu = torch.tensor([0, 37, 42, 62], dtype=torch.int32, device=cuda)
+    of = Kind(cuda, kind, torch.stack([pos + 70000, pos // 2, pos % 5]))
+    steps = [PrefillStep(pairs[i], *bufs[i], table, seq_lens, cu, slots, D ** -0.5, 37, 128, heads=of.heads if i == 0 else None)
+             for i in range(2)]
+    steps[0].run()
+    for layer in range(LAYERS):
+        q, k, v, out = (x[layer] for x in bufs[1])
+        of.append(layer, q, k, v, pairs[1][layer], slots)
+        steps[1].attend(layer)
+        _same(pairs[0][layer], pairs[1][layer])
+        for a, b in zip(bufs[0], (q, k, v, out)):
+            assert torch.equal(a[layer], b)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8_e4m3"])
+@pytest.mark.parametrize("kind", [k for k in KINDS if "axes" not in k])
+def test_kinds_of_heads_in_a_drafted_step(cuda, kind, kv):
+    """Against the same step over heads that rotary_append has normed and turned into a cache of their own."""
+    rows, g = 24, torch.Generator(device=cuda).manual_seed(51)
+    x = [[torch.randn((rows, h, D), generator=g, device=cuda).bfloat16() for _ in range(LAYERS)] for h in (HQ, HKV, HKV, HQ)]
+    new = torch.tensor([9, 1], dtype=torch.int32, device=cuda)
+    parents = torch.full((rows,), -1, dtype=torch.int32, device=cuda)
+    parents[1:9] = torch.tensor([0, 0, 1, 2, 3, 3, 4, 0], device=cuda)
+    draft, target = (torch.randint(0, 2, (rows,), generator=g, device=cuda) for _ in range(2))
+    got = []
+    for i in range(2):
+        bufs = [[t.clone() for t in of] for of in x]
+        pool = KVPool(LAYERS, 24, BS, HKV, D, kv, device=cuda, max_model_len=96)
+        for j, n in enumerate((30, 4)):
+            pool.blocks.allocate(j, np.arange(n) + 1000 * j)
+        state = pool.lend([0, 1], 12)
+        kw = {}
+        if i == 0:
+            of = Kind(cuda, kind, torch.zeros((3, rows), dtype=torch.int64, device=cuda))
+            of.heads.positions = None  # (they are the step's)
+            kw["heads"] = of.heads
+        step = TreeStep(pool.layers, *bufs, state, new, parents, draft, target, D ** -0.5, 64, 96, 8, **kw)
+        step.begin()
+        if i == 1:
+            at = torch.arange(rows, device=cuda)
+            of = Kind(cuda, kind, torch.stack([step.maps.positions] * 3))
+            for layer in range(LAYERS):
+                c = PagedKVCache(-(-rows // BS), BS, HKV, D, device=cuda)
+                of.append(layer, bufs[0][layer], bufs[1][layer], bufs[2][layer], c, at)
+                bufs[1][layer].copy_(c.k.permute(0, 3, 1, 2, 4).reshape(-1, HKV, D)[:rows])
+        step.run()
+        step.finish()
+        got.append((pool, state, bufs, step))
+    a, b = got
+    for layer in range(LAYERS):
+        _same(a[0].layers[layer], b[0].layers[layer])
+        assert torch.equal(a[2][3][layer][:10], b[2][3][layer][:10]) and torch.equal(a[2][0][layer][:10], b[2][0][layer][:10])
+        assert torch.equal(a[2][1][layer], x[1][layer])
+    assert torch.equal(a[1].seq_lens, b[1].seq_lens) and torch.equal(a[3].accepted.path, b[3].accepted.path)
 
 
 @pytest.mark.parametrize("kv", ["bf16", "fp8_e4m3"])
