@@ -45,7 +45,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_rotary_kernel(NormRotaryArg
   const int64_t t = w.t0 + w.t;
   const HeadsOf<T> of{static_cast<const T *>(k.s.x) + t * k.s.xt + w.h0 * k.s.xh, k.s.xh,
                       static_cast<T *>(k.s.y) + t * k.s.yt + w.h0 * k.s.yh, k.s.yh, 0, weight, k.ws};
-  norm_turn_heads<T, V, INTER, U, 1, FAR, false, EACH, LL>(
+  norm_turn_heads<T, V, INTER, U, FAR, false, EACH, LL>(
       a.r, a.n, turn + w.t * a.r.half, w.there, w.group, (64 >> a.r.log_lanes) >> k.log_tg, w.heads, of,
       [&] { wave_angles(a.a, w.t0, w.tokens, turn); });
 }

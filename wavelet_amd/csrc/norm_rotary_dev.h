@@ -355,9 +355,9 @@ __device__ __forceinline__ WaveTile wave_tile(const Kind &k, const RowUnits &r, 
 }
 
 // The heads first, first + step, .. below `heads` of the lane's token (there: it has one), normed (if
-// norm.on) and turned by turn[], N rows at a time, the next N in flight meanwhile; ready(): called once the
-// first are, before turn[] is read. EACH: each head's own weights.
-template <class T, int V, bool INTER, int U, int N, bool FAR, bool NEAR_STORE, bool EACH, int LL, class Ready>
+// norm.on) and turned by turn[], the next one in flight meanwhile; ready(): called once the
+// first is, before turn[] is read. EACH: each head's own weights.
+template <class T, int V, bool INTER, int U, bool FAR, bool NEAR_STORE, bool EACH, int LL, class Ready>
 __device__ __forceinline__ void norm_turn_heads(const RowUnits &ru, const HeadNorm &norm, const float2 *turn, bool there,
                                                 int first, int step, int heads, const HeadsOf<T> &of, Ready ready) {
   typedef typename VecOf<T, V>::type Vec;
@@ -373,20 +373,16 @@ __device__ __forceinline__ void norm_turn_heads(const RowUnits &ru, const HeadNo
     e0[j] = e1[j] = 0;
     if (u < ru.units) unit_runs<V, INTER>(ru, u, e0[j], e1[j]);
   }
-  Vec n0[N][U], n1[N][U];
-  auto load = [&](int h0) __attribute__((always_inline)) {
+  Vec n0[U], n1[U];
+  auto load = [&](int h) __attribute__((always_inline)) {
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int h = h0 + step * k;
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        n0[k][j] = n1[k][j] = Vec{};
-        if (mine[j] && h < heads) {
-          const Vec *p0 = reinterpret_cast<const Vec *>(of.x + h * of.xh + e0[j]);
-          const Vec *p1 = reinterpret_cast<const Vec *>(of.x + h * of.xh + e1[j]);
-          n0[k][j] = FAR ? __builtin_nontemporal_load(p0) : *p0;
-          n1[k][j] = FAR ? __builtin_nontemporal_load(p1) : *p1;
-        }
+    for (int j = 0; j < U; ++j) {
+      n0[j] = n1[j] = Vec{};
+      if (mine[j] && h < heads) {
+        const Vec *p0 = reinterpret_cast<const Vec *>(of.x + h * of.xh + e0[j]);
+        const Vec *p1 = reinterpret_cast<const Vec *>(of.x + h * of.xh + e1[j]);
+        n0[j] = FAR ? __builtin_nontemporal_load(p0) : *p0;
+        n1[j] = FAR ? __builtin_nontemporal_load(p1) : *p1;
       }
     }
   };
@@ -407,55 +403,50 @@ __device__ __forceinline__ void norm_turn_heads(const RowUnits &ru, const HeadNo
     unit_turn<V, INTER>(turn, ru.half, all, e0[j], e1[j], t[j]);
     if (!EACH) unit_coef<V, INTER>(t[j], w0[j], w1[j], coef[j]);
   }
-  for (int hb = 0; hb < heads; hb += step * N) {  // uniform; the lane's rows are hb + first, + step, ..
-    Vec x0[N][U], x1[N][U];
+  for (int hb = 0; hb < heads; hb += step) {  // uniform; the lane's row is hb + first
+    Vec x0[U], x1[U];
 #pragma unroll
-    for (int k = 0; k < N; ++k)
+    for (int j = 0; j < U; ++j) {
+      x0[j] = n0[j];
+      x1[j] = n1[j];
+    }
+    if (hb + step < heads) load(hb + step + first);
+    const int h = hb + first;
+    float f0[U][V], f1[U][V], ss = 0.f;
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        x0[k][j] = n0[k][j];
-        x1[k][j] = n1[k][j];
+    for (int j = 0; j < U; ++j) {
+      widen<V, T>(x0[j], f0[j]);
+      widen<V, T>(x1[j], f1[j]);
+#pragma unroll
+      for (int v = 0; v < V; ++v) ss = __builtin_fmaf(f0[j][v], f0[j][v], __builtin_fmaf(f1[j][v], f1[j][v], ss));
+    }
+    ss = group_sum<LL>(ss, ru.log_lanes);
+    const float inv = norm.on ? __builtin_amdgcn_rsqf(__builtin_fmaf(ss, inv_d, norm.eps)) : 1.f;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      if (EACH) {
+        const int64_t wh = h < heads ? h * of.ws : 0;
+        load_weights<T, V>(norm, of.w, wh + e0[j], w0[j]);
+        load_weights<T, V>(norm, of.w, wh + e1[j], w1[j]);
+        unit_coef<V, INTER>(t[j], w0[j], w1[j], coef[j]);
       }
-    if (hb + step * N < heads) load(hb + step * N + first);
+      unit_apply<V, INTER>(coef[j], t[j].live, all, inv, f0[j], f1[j]);
+      if (mine[j] && h < heads) {
+        Vec o0, o1;
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int h = hb + first + step * k;
-      float f0[U][V], f1[U][V], ss = 0.f;
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        widen<V, T>(x0[k][j], f0[j]);
-        widen<V, T>(x1[k][j], f1[j]);
-#pragma unroll
-        for (int v = 0; v < V; ++v) ss = __builtin_fmaf(f0[j][v], f0[j][v], __builtin_fmaf(f1[j][v], f1[j][v], ss));
-      }
-      ss = group_sum<LL>(ss, ru.log_lanes);
-      const float inv = norm.on ? __builtin_amdgcn_rsqf(__builtin_fmaf(ss, inv_d, norm.eps)) : 1.f;
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        if (EACH) {
-          const int64_t wh = h < heads ? h * of.ws : 0;
-          load_weights<T, V>(norm, of.w, wh + e0[j], w0[j]);
-          load_weights<T, V>(norm, of.w, wh + e1[j], w1[j]);
-          unit_coef<V, INTER>(t[j], w0[j], w1[j], coef[j]);
+        for (int v = 0; v < V; ++v) {
+          o0[v] = static_cast<T>(f0[j][v]);
+          o1[v] = static_cast<T>(f1[j][v]);
         }
-        unit_apply<V, INTER>(coef[j], t[j].live, all, inv, f0[j], f1[j]);
-        if (mine[j] && h < heads) {
-          Vec o0, o1;
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            o0[v] = static_cast<T>(f0[j][v]);
-            o1[v] = static_cast<T>(f1[j][v]);
-          }
-          T *y = of.y + h * of.yh;
-          const int i0 = of.piece == 0 ? e0[j] : (e0[j] >> 3) * of.piece + (e0[j] & 7);
-          const int i1 = of.piece == 0 ? e1[j] : (e1[j] >> 3) * of.piece + (e1[j] & 7);
-          if (FAR && !NEAR_STORE) {
-            __builtin_nontemporal_store(o0, reinterpret_cast<Vec *>(y + i0));
-            __builtin_nontemporal_store(o1, reinterpret_cast<Vec *>(y + i1));
-          } else {
-            *reinterpret_cast<Vec *>(y + i0) = o0;
-            *reinterpret_cast<Vec *>(y + i1) = o1;
-          }
+        T *y = of.y + h * of.yh;
+        const int i0 = of.piece == 0 ? e0[j] : (e0[j] >> 3) * of.piece + (e0[j] & 7);
+        const int i1 = of.piece == 0 ? e1[j] : (e1[j] >> 3) * of.piece + (e1[j] & 7);
+        if (FAR && !NEAR_STORE) {
+          __builtin_nontemporal_store(o0, reinterpret_cast<Vec *>(y + i0));
+          __builtin_nontemporal_store(o1, reinterpret_cast<Vec *>(y + i1));
+        } else {
+          *reinterpret_cast<Vec *>(y + i0) = o0;
+          *reinterpret_cast<Vec *>(y + i1) = o1;
         }
       }
     }

@@ -85,7 +85,7 @@ __device__ __forceinline__ void heads_role(const AppendArgs &a, const Kind &k, i
     of.y = static_cast<__bf16 *>(k.s.y) + t * k.s.yt + w.h0 * k.s.yh;
     of.yh = k.s.yh;
   }
-  norm_turn_heads<__bf16, V, INTER, 1, 1, FAR, K, EACH, LL>(
+  norm_turn_heads<__bf16, V, INTER, 1, FAR, K, EACH, LL>(
       a.r, a.n, turn + w.t * a.r.half, there, w.group, (64 >> a.r.log_lanes) >> k.log_tg, w.heads, of,
       [&] { wave_angles<K ? 2 : 1>(a.a, w.t0, w.tokens, turn); });
 }
@@ -526,7 +526,7 @@ __global__ __launch_bounds__(kThreads) void mla_rotary_append_kernel(LatentArgs 
       of.y = a.latent + (blk * a.slots.block.d + off) * width + a.rank;
     }
     const HeadNorm none{};
-    norm_turn_heads<__bf16, V, INTER, 1, 1, false, false, false, LL>(
+    norm_turn_heads<__bf16, V, INTER, 1, false, false, false, LL>(
         a.r, none, turn + w.t * a.r.half, there, w.group, (64 >> a.r.log_lanes) >> k.log_tg, w.heads, of,
         [&] { wave_angles(a.a, w.t0, w.tokens, turn); });
     return;
