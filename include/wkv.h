@@ -523,6 +523,13 @@ int wkv_norm_rotary(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_
                     int32_t head_dim, const wkv_head_norm_t *norm, const wkv_rotary_t *rotary, int64_t num_tokens,
                     void *stream);
 
+/* wkv_rotary_axes with the angles of wkv_norm_rotary and wkv_rotary_append, which differ from wkv_rotary's in
+ * their last bit: a captured step turns its heads in place by it where the step itself calls wkv_rotary_append. */
+int wkv_turn_heads(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_stride_h, void *q_out,
+                   int64_t qo_stride_t, int64_t qo_stride_h, int32_t num_q_heads, const void *k, int64_t k_stride_t,
+                   int64_t k_stride_h, void *k_out, int64_t ko_stride_t, int64_t ko_stride_h, int32_t num_k_heads,
+                   int32_t head_dim, const wkv_rotary_t *rotary, int64_t num_tokens, void *stream);
+
 /* Its gradients: from the inputs q, k, and the gradients q_grad, k_grad of the outputs, dq and dk (NULL: not
  * computed; else they do not overlap the inputs) and the weights' dq_weight, dk_weight (NULL: not computed;
  * contiguous, [head_dim], or [heads, head_dim] where the weight has a head stride, of weight_dtype). A kind of
@@ -543,8 +550,8 @@ int wkv_norm_rotary_backward(int32_t dtype, const void *q, int64_t q_stride_t, i
 /* The append with the norm and the rotation on the way, in one launch: the queries normed and turned into q_out (or
  * in place; num_q_heads may be 0), the keys normed and turned into the cache, the values into the cache. The cache
  * then holds what wkv_norm_rotary of the same rows (its k_out's 16-byte aligned) followed by wkv_append or
- * wkv_append_fp8 leaves in it, bit for bit (without a norm, where wkv_rotary_axes goes first, but for the last bit of
- * a key), keys rounded to bf16 before they are coded in fp8; key and value themselves are not changed. norm or rotary
+ * wkv_append_fp8 leaves in it, bit for bit (without a norm, wkv_turn_heads; where wkv_rotary_axes goes first, but
+ * for the last bit of a key), keys rounded to bf16 before they are coded in fp8; key and value themselves are not changed. norm or rotary
  * may be NULL, not both. key, value and slot_mapping as for wkv_append (wkv_append_fp8); a slot appears once in a
  * call, and an fp8 cache's block in one run. q and its result bf16 [num_tokens, num_q_heads, head_dim], strides in
  * elements; every token's queries are computed, also those of slot -1. Replaces the engine's norms, rotary embedding

@@ -184,3 +184,19 @@ def test_a_plan_s_entry_weights():
     for bad in (Heads(k_weight=[good]), Heads(eps=1e-6, k_weight=[good, good]), Heads(eps=1e-6, q_weight=[good])):
         with pytest.raises(ValueError):
             bad.entry_norm(0, 1, entries)
+
+
+def test_turn_heads():
+    lib = _lib.load()
+
+    def call(**kw):
+        args = _rows_args(**kw)
+        del args[16]  # the norm
+        return lib.wkv_turn_heads(*args)
+
+    assert call(tokens=0) == _lib.WKV_OK and call(hq=0, hk=0) == _lib.WKV_OK
+    for bad in BAD_ROWS:
+        assert call(**bad) == _lib.WKV_ERR_INVALID, bad
+    for bad in BAD_ROTARY:
+        assert call(rotary=_rotary(**bad)) == _lib.WKV_ERR_INVALID, bad
+    assert call(rotary=None) == _lib.WKV_ERR_INVALID

@@ -139,8 +139,8 @@ def _decode_pair(cuda, kv, batch, make_heads, seed, per=2, start=0, **plan):
 @pytest.mark.parametrize("axes", [False, True])
 @pytest.mark.parametrize("batch,per,start,part", [(256, 2, 0, 0), (3, 64, 1000, 128)])
 def test_turned_alone_and_captured(cuda, kv, axes, batch, per, start, part):
-    """Heads with a rotation and no norm: a captured plan leaves what the same plan leaves when it is run, also where a
-    context is shared out and merged."""
+    """Heads with a rotation and no norm: a captured plan leaves the queries and the cache that the same plan leaves when it
+    is run, also where a context is shared out and merged; its attention takes the new token from its buffers."""
     freq = rotary_frequencies(D, 1e4, device=cuda)[0]
     of = rotary_axes((12, 10, 10), device=cuda) if axes else None
     caches, bufs, steps, fill = _decode_pair(
@@ -155,7 +155,7 @@ def test_turned_alone_and_captured(cuda, kv, axes, batch, per, start, part):
         for layer in range(LAYERS):
             assert torch.equal(bufs[0][0][layer], bufs[1][0][layer]) and torch.equal(bufs[0][1][layer], keys[layer])
             _same(caches[0][layer], caches[1][layer])
-            assert torch.equal(bufs[0][3][layer], bufs[1][3][layer])
+            torch.testing.assert_close(bufs[0][3][layer].float(), bufs[1][3][layer].float(), rtol=2.0 ** -7, atol=5 * 2.0 ** -8)
 
 
 KINDS = {  # what a plan's heads may be: (turned, several axes, normed, weights, offset)
@@ -190,8 +190,8 @@ class Kind:
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("groups", [False, True])
 def test_kinds_of_heads_in_a_decode_step(cuda, kind, kv, groups):
-    """A plan, and but for groups a captured one, against rotary_append and the plan's attention alone; a normed plan's
-    captured attention takes the new token from its buffers (the tolerance above)."""
+    """A plan, and but for groups a captured one, against rotary_append and the plan's attention alone; a captured plan's
+    attention takes the new token from its buffers (the tolerance above)."""
     batch, made = 6, {}
 
     def make(i, pos):
@@ -213,7 +213,7 @@ def test_kinds_of_heads_in_a_decode_step(cuda, kind, kv, groups):
             steps[1].attend(layer)
             assert torch.equal(bufs[0][0][layer], q)
             _same(caches[0][layer], caches[1][layer])
-            if captured and "eps" in made["of"].how:
+            if captured:
                 torch.testing.assert_close(bufs[0][3][layer].float(), out.float(), rtol=2.0 ** -7, atol=5 * 2.0 ** -8)
             else:
                 assert torch.equal(bufs[0][3][layer], out) and torch.equal(bufs[0][1][layer], keys[layer])

@@ -125,6 +125,9 @@ _SIGNATURES = {
     "wkv_norm_rotary": (c_int, [c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_void_p,
                                 c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_int32, POINTER(WkvHeadNorm),
                                 POINTER(WkvRotary), c_int64, c_void_p]),
+    "wkv_turn_heads": (c_int, [c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_void_p,
+                               c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_int32, POINTER(WkvRotary),
+                               c_int64, c_void_p]),
     "wkv_norm_rotary_workspace_size": (c_int64, [c_int64, c_int32, c_int32, c_int32, c_int32, c_int32]),
     "wkv_norm_rotary_backward": (c_int, [c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
                                          c_int64, c_int64, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64,

@@ -367,13 +367,12 @@ bool rows_ok(const void *x, int64_t st, int64_t sh, int esz) {
 
 }  // namespace
 
-extern "C" int wkv_norm_rotary(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_stride_h, void *q_out,
-                               int64_t qo_stride_t, int64_t qo_stride_h, int32_t num_q_heads, const void *k,
-                               int64_t k_stride_t, int64_t k_stride_h, void *k_out, int64_t ko_stride_t,
-                               int64_t ko_stride_h, int32_t num_k_heads, int32_t head_dim,
-                               const wkv_head_norm_t *norm, const wkv_rotary_t *rotary, int64_t num_tokens,
-                               void *stream) {
-  WKV_CHECK_ARG(norm != nullptr, "norm must be given (wkv_rotary_axes turns heads without one)");
+// norm or rotary may be NULL, not both.
+static int norm_rotary_call(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_stride_h, void *q_out,
+                            int64_t qo_stride_t, int64_t qo_stride_h, int32_t num_q_heads, const void *k,
+                            int64_t k_stride_t, int64_t k_stride_h, void *k_out, int64_t ko_stride_t,
+                            int64_t ko_stride_h, int32_t num_k_heads, int32_t head_dim, const wkv_head_norm_t *norm,
+                            const wkv_rotary_t *rotary, int64_t num_tokens, void *stream) {
   if (const int rc = check_norm_call(dtype, num_q_heads, num_k_heads, head_dim, norm, rotary, num_tokens)) return rc;
   const int H = num_q_heads + num_k_heads, esz = dtype == 0 ? 4 : 2;
   if (num_tokens == 0 || H == 0) return WKV_OK;
@@ -387,27 +386,26 @@ extern "C" int wkv_norm_rotary(int32_t dtype, const void *q, int64_t q_stride_t,
   a.a = angles(rotary);
   a.tokens = num_tokens;
   Widths w(esz, head_dim, half, inter);
-  const int wsz = norm->weight_dtype == 0 ? 4 : 2;
+  const int wsz = a.n.wide ? 4 : 2;
   if (num_q_heads > 0) {
     w.rows(q, q_stride_t, q_stride_h);
     w.rows(q_out, qo_stride_t, qo_stride_h);
-    w.weights(norm->q_weight, norm->q_weight_stride_h, wsz);
+    w.weights(a.n.qw, a.n.qws, wsz);
   }
   if (num_k_heads > 0) {
     w.rows(k, k_stride_t, k_stride_h);
     w.rows(k_out, ko_stride_t, ko_stride_h);
-    w.weights(norm->k_weight, norm->k_weight_stride_h, wsz);
+    w.weights(a.n.kw, a.n.kws, wsz);
   }
   a.r = row_units(head_dim, half, w.v);
   const KindGrid gq(num_tokens, num_q_heads, a.r.log_lanes, false), gk(num_tokens, num_k_heads, a.r.log_lanes, false);
-  a.q = Kind{HeadRows{q, q_out, q_stride_t, q_stride_h, qo_stride_t, qo_stride_h}, norm->q_weight,
-             norm->q_weight_stride_h, num_q_heads, gq.log_tg, gq.per, fast_div(gq.splits)};
-  a.k = Kind{HeadRows{k, k_out, k_stride_t, k_stride_h, ko_stride_t, ko_stride_h}, norm->k_weight,
-             norm->k_weight_stride_h, num_k_heads, gk.log_tg, gk.per, fast_div(gk.splits)};
+  a.q = Kind{HeadRows{q, q_out, q_stride_t, q_stride_h, qo_stride_t, qo_stride_h}, a.n.qw, a.n.qws, num_q_heads,
+             gq.log_tg, gq.per, fast_div(gq.splits)};
+  a.k = Kind{HeadRows{k, k_out, k_stride_t, k_stride_h, ko_stride_t, ko_stride_h}, a.n.kw, a.n.kws, num_k_heads,
+             gk.log_tg, gk.per, fast_div(gk.splits)};
   WKV_CHECK_ARG(gq.wgs + gk.wgs <= kMaxWorkgroups, "too many tokens and heads for one launch");
   a.q_wgs = static_cast<int>(gq.wgs);
-  const bool each = (norm->q_weight != nullptr && norm->q_weight_stride_h != 0) ||
-                    (norm->k_weight != nullptr && norm->k_weight_stride_h != 0);
+  const bool each = (a.n.qw != nullptr && a.n.qws != 0) || (a.n.kw != nullptr && a.n.kws != 0);
   const bool far = num_tokens * H * head_dim * esz >= (64 << 20);
   const unsigned grid = static_cast<unsigned>(gq.wgs + gk.wgs);
   const int log_tg = gq.log_tg > gk.log_tg ? gq.log_tg : gk.log_tg;
@@ -420,6 +418,29 @@ extern "C" int wkv_norm_rotary(int32_t dtype, const void *q, int64_t q_stride_t,
   });
   WKV_CHECK_LAUNCH("norm_rotary");
   return WKV_OK;
+}
+
+extern "C" int wkv_norm_rotary(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_stride_h, void *q_out,
+                               int64_t qo_stride_t, int64_t qo_stride_h, int32_t num_q_heads, const void *k,
+                               int64_t k_stride_t, int64_t k_stride_h, void *k_out, int64_t ko_stride_t,
+                               int64_t ko_stride_h, int32_t num_k_heads, int32_t head_dim,
+                               const wkv_head_norm_t *norm, const wkv_rotary_t *rotary, int64_t num_tokens,
+                               void *stream) {
+  WKV_CHECK_ARG(norm != nullptr, "norm must be given (wkv_rotary_axes turns heads without one)");
+  return norm_rotary_call(dtype, q, q_stride_t, q_stride_h, q_out, qo_stride_t, qo_stride_h, num_q_heads, k, k_stride_t,
+                          k_stride_h, k_out, ko_stride_t, ko_stride_h, num_k_heads, head_dim, norm, rotary, num_tokens,
+                          stream);
+}
+
+extern "C" int wkv_turn_heads(int32_t dtype, const void *q, int64_t q_stride_t, int64_t q_stride_h, void *q_out,
+                              int64_t qo_stride_t, int64_t qo_stride_h, int32_t num_q_heads, const void *k,
+                              int64_t k_stride_t, int64_t k_stride_h, void *k_out, int64_t ko_stride_t,
+                              int64_t ko_stride_h, int32_t num_k_heads, int32_t head_dim, const wkv_rotary_t *rotary,
+                              int64_t num_tokens, void *stream) {
+  WKV_CHECK_ARG(rotary != nullptr, "rotary must be given");
+  return norm_rotary_call(dtype, q, q_stride_t, q_stride_h, q_out, qo_stride_t, qo_stride_h, num_q_heads, k, k_stride_t,
+                          k_stride_h, k_out, ko_stride_t, ko_stride_h, num_k_heads, head_dim, nullptr, rotary,
+                          num_tokens, stream);
 }
 
 namespace {

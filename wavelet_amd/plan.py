@@ -339,11 +339,10 @@ class GraphDecodeStep:
     default). Every call on a GPU shares that GPU's scratch: two plans' replays must
     not overlap (one stream, or ordered). Geometries whose partials exceed the scratch
     (``wkv_decode_workspace_size`` > ``WKV_NOALLOC_SCRATCH_BYTES``) are refused. The
-    group-aware decode is not captured here. A plan with ``heads`` that are normed is captured with its queries and
-    keys normed and turned in place before the fused append (so ``key`` is refilled for every replay, as ``q`` is); the
-    cache then holds what the plan's own ``run`` leaves, bit for bit, and the attention takes the new token's key and
-    value from their buffers in the place of the cache (``out`` within its rounding). Heads that are turned alone are
-    captured as ``run`` launches them.
+    group-aware decode is not captured here. A plan with ``heads`` is captured with its queries and keys normed and
+    turned in place before the fused append (so ``key`` is refilled for every replay, as ``q`` is): queries and cache are
+    then what the plan's own ``run`` leaves, bit for bit, and the attention takes the new token's key and value from
+    their buffers in the place of the cache (``out`` within its rounding).
     """
 
     def __init__(self, step: DecodeStep, *, shared_blocks: bool | None = None) -> None:
@@ -387,10 +386,6 @@ class GraphDecodeStep:
         # zero-length call validates the arguments and launches nothing)
         first = calls(torch.cuda.current_stream(dev).cuda_stream)[0]
         _lib.check(fn(*first[:17], 0, *first[18:]), "allocation-free decode (set-up)")
-        # heads that are turned and not normed go as the plan runs them, through a workspace of the graph's own:
-        # what turns keys in place (wkv_rotary_axes) rounds their angles in another way than the append
-        turned_alone = step.heads is not None and step.heads.eps is None
-        self.workspace = torch.empty_like(step.workspace) if turned_alone else None
         self.graph = torch.cuda.CUDAGraph()
         capture = torch.cuda.Stream(dev)
         capture.wait_stream(torch.cuda.current_stream(dev))
@@ -399,20 +394,14 @@ class GraphDecodeStep:
             if step.ordered:
                 _lib.check(lib.wkv_decode_order(sl.data_ptr(), batch, step.order.data_ptr(), cur), "decode order")
             for layer, args in enumerate(calls(cur)):
-                heads = step.heads
-                if turned_alone:
-                    c = step.calls[layer]
-                    _lib.check(c.append_fn(*c.append_args[:-1], cur), f"rotary append layer {layer}")
-                    attend = c.decode_args[c.shared_default if shared_blocks is None else bool(shared_blocks)]
-                    _lib.check(lib.wkv_paged_decode_gqa(*attend[:-4], self.workspace.data_ptr(), *attend[-3:-1], cur),
-                               f"decode layer {layer}")
-                    continue
-                if heads is not None:
-                    qq, kk = q[layer], key[layer]
-                    _lib.check(lib.wkv_norm_rotary(1, *_rows(qq, qq), qq.shape[1], *_rows(kk, kk), kk.shape[1], qq.shape[2],
-                                                   heads.norm(layer, len(caches), qq, kk),
-                                                   heads.rotation(batch, qq.shape[2], dev), batch, cur),
-                               f"heads of layer {layer}")
+                if step.heads is not None:
+                    qq, kk, h = q[layer], key[layer], step.heads
+                    rows = (1, *_rows(qq, qq), qq.shape[1], *_rows(kk, kk), kk.shape[1], qq.shape[2])
+                    how = h.rotation(batch, qq.shape[2], dev)
+                    norm = h.norm(layer, len(caches), qq, kk)
+                    # (without a norm by the append's angles, not wkv_rotary_axes's)
+                    _lib.check(lib.wkv_turn_heads(*rows, how, batch, cur) if norm is None
+                               else lib.wkv_norm_rotary(*rows, norm, how, batch, cur), f"heads of layer {layer}")
                 _lib.check(fn(*args), f"allocation-free append+decode layer {layer}")
         torch.cuda.current_stream(dev).wait_stream(capture)
 
