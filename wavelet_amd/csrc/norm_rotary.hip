@@ -11,7 +11,7 @@
 //   dx = r (m - x r^2 mean(m x)),   dw = sum over rows of z x r.
 // A group of lanes keeps its elements of dw in registers over all the rows that it takes; workgroups leave
 // their sums in the workspace, and a second kernel adds them up, in an order that the sizes alone give. Bound by
-// HBM: 16,384 tokens of 40 heads of 128, bf16, 100 us with the sums (503 MB, 5.0 TB/s); 8,191 tokens of 24 heads 36
+// HBM: 16,384 tokens of 40 heads of 128, bf16, 98 us (503 MB, 5.1 TB/s) and 5 for the sums; 8,191 tokens of 24 heads 36
 // (151 MB, 4.2 TB/s) and 4 for the sums.
 #include <algorithm>
 #include <type_traits>
@@ -287,7 +287,8 @@ __global__ __launch_bounds__(64 * kSumWaves) void norm_weight_grad_kernel(Weight
 
 // ---------------------------------------------------------------------------
 // Host. The launches. Heads of 64 and 128 in 16-byte accesses have their lanes as a constant (16,384 tokens of 40
-// heads of 128, bf16: 65.1 us forward, 67.2 without, and 67.2 and 74.5 with each head's weights; backward 119 and 122).
+// heads of 128, bf16: 65.6 us forward, 66.0 without, and 70.9 and 72.1 with each head's weights; forward and backward
+// 166.4 and 168.9).
 template <class T, int V, bool INTER, bool EACH>
 static void launch_norm(const NormRotaryArgs &a, bool far, unsigned grid, size_t lds, hipStream_t s) {
   if (a.r.units > 64) {
@@ -538,8 +539,8 @@ extern "C" int wkv_norm_rotary_backward(int32_t dtype, const void *q, int64_t q_
     fit(num_k_heads, rk, norm->k_weight, norm->k_weight_stride_h);
     a.r = row_units(head_dim, half, w.v);
     const int groups = 64 >> a.r.log_lanes;
-    // Long rows of heads go by ranges with one weight too (16,384 tokens of 40 heads of 128, bf16: 100 us, 110 where a
-    // wave walks a token's heads; fp32 172 and 200), but not short ones (8,191 of 24: 40 and 37.5) or where a token's
+    // Long rows of heads go by ranges with one weight too (16,384 tokens of 40 heads of 128, bf16: 98 us, 106 where a
+    // wave walks a token's heads; fp32 169 and 195), but not short ones (8,191 of 24: 40 and 37.5) or where a token's
     // angles, which each range forms, cost more (32 of 256: 92 and 83). The workgroups are dealt by what a
     // token of a kind costs, in heads: a range costs a whole wave.
     auto in_ranges = [&](int heads, bool each, const GradSums &most) {
@@ -555,7 +556,7 @@ extern "C" int wkv_norm_rotary_backward(int32_t dtype, const void *q, int64_t q_
       if (heads == 0) return k;
       const int64_t wgs = std::min(GradSums::share(kGradWorkgroups * cost, (cost_q + cost_k) * k.ranges), GradSums::most(num_tokens));
       k.wgs = static_cast<int>(std::min(wgs, most.rows / (each ? heads : k.ranges)));  // (what the workspace is for)
-      // Two tokens a block in ranges (16,384 tokens of 40 heads of 128, bf16: 98 us, 105 of one, 103 of four);
+      // Two tokens a block in ranges (16,384 tokens of 40 heads of 128, bf16: 98 us, 104 of one, 105 of four);
       // else as many as give every group of lanes a head (8,192 of 16 + 16 heads of 256: one 83, two 99).
       const int64_t waves = static_cast<int64_t>(k.wgs) * kNormWaves;
       while (split ? k.log_tg < 1 && (num_tokens >> 1) >= waves

@@ -15,7 +15,8 @@
 // walk their heads: a lane's token and unit stay the same, so that its
 // angles and weights are formed once, as the products that y is linear in x by,
 //   y_a = (x_a r) (w_a c) - (x_b r) (w_b s),  y_b = (x_b r) (w_b c) + (x_a r) (w_a s),
-// and a row costs some 7 instructions a value.
+// and a value costs some 14 vector instructions, the angles' among them (counted for 16,384 tokens of 32 + 8 heads
+// of 128).
 #pragma once
 
 #include <cmath>
@@ -46,7 +47,9 @@ __device__ __forceinline__ int64_t position_at(const Angles &a, int64_t t, int i
 // nearest quarter of one in float64, then the Taylor series of that distance, at most pi / 4: to z^4 (sine)
 // and z^5 (cosine) of its square z, whose next terms are below 2^-28 of it and 2^-32. Off by at most 1.3 x
 // 2^-24 (a float32 of half a turn alone by 1.6), 0.3 in the mean, which decides how often a key's last bit,
-// and its code, is the exact one's.
+// and its code, is the exact one's. That is for angles below 2^27; from there on float64's own rounding of
+// the angle, some 2^-52 of it, is the larger part (3.6 x 2^-24 in all at 2^30). The series in float64, rounded once,
+// costs more than it gives: an fp8 append of 8,386 tokens of 28/4 heads 45 us in the place of 38.
 __device__ __forceinline__ float2 angle_of(const Angles &a, int64_t pos, double freq) {
   const double x = static_cast<double>(pos) * freq * 0.15915494309189533577;  // 1 / 2 pi
   const double y = 4. * (x - rint(x)), n = rint(y);
@@ -511,7 +514,7 @@ constexpr int64_t kMaxWorkgroups = (1 << 24) - 1;
 // Waves over the tokens and heads of a kind, four a workgroup: a token a wave (its heads lie together;
 // by_token: as many as the wave's groups, whose stores of one head then lie together in a cache), and with
 // too few tokens for the chip the heads dealt over more waves, down to a round of the wave's groups below
-// 4,096 waves (four a SIMD), to two rounds below 16,384 (4,696 tokens of 128 heads of 64: 38.2 us, 45.4 a
+// 4,096 waves (four a SIMD), to two rounds below 16,384 (4,696 tokens of 128 heads of 64: 38 us, 45 a
 // wave a token; 8,191 of 16 heads of 128, two rounds, lose 1 us in halves).
 struct KindGrid {
   int log_tg = 0, per = 1, splits = 1;
@@ -533,7 +536,9 @@ struct KindGrid {
   }
 };
 
-// The elements of an access: 16 bytes of them, else two, else one, as the layout and every operand allow.
+// The elements of an access: 16 bytes of them, else two, else one, as the layout and every operand allow. The
+// narrow ones are for what models seldom have, half a rotation of no multiple of 16 bytes, and unaligned rows: 16,384
+// tokens of 40 heads of 128, bf16, half 64 / 46 / 45: 65 / 85 / 112 us; with the append 81 / 106 / 156.
 struct Widths {
   int esz, v;
   Widths(int esz, int D, int half, bool inter) : esz(esz), v(16 / esz) {

@@ -10,11 +10,16 @@
 // in the place of values, and its shared key is a kind of one head.
 //
 // Prompts are bound by HBM: 8 of 2,048 tokens, 32/8 heads of 128, bf16: 79 us for 403 MB, 5.1 TB/s, as a
-// large copy (norm_rotary and append in turn: 65 + 34). Into fp8, 8,386 tokens of 28/4 heads take 37, of
-// which the queries alone are 27: a run's keys are a chain of round trips (slots, rows and positions, scale)
+// large copy (norm_rotary and append in turn: 65 + 34). Into fp8 blocks of 16, 8,386 tokens of 28/4 heads take 37,
+// of which the queries alone are 27: a run's keys are a chain of round trips (slots, rows and positions, scale)
 // of 6.5 us in a wave, so the workgroups of keys and values come first and the queries' fill the chip beside
 // them (36.1 so, 41.1 behind them). Few tokens are bound by the launch and that chain (64 tokens bf16: 5.0
 // us; 5 tokens fp8: 6.3).
+//
+// Larger fp8 blocks have longer runs, one wave each, whose pieces of 16 tokens follow each other and are normed and
+// turned twice: those 8,386 tokens take 42, 58, 94 and 154 us in blocks of 32, 64, 128 and 256 (norm_rotary or
+// apply_rotary and append in turn: 64, 71, 99, 150), and 16,384 tokens of 32/8 heads 97, 226 and 632 in blocks of 16,
+// 64 and 256 (in turn 88, 164, 471).
 #include <type_traits>
 
 #include "kv_append_dev.h"
@@ -458,7 +463,7 @@ __device__ __forceinline__ void window_runs(const AppendArgs &a, int wg, F f) {
 }
 
 // fp8: four waves a SIMD (128 registers, 60 bytes of them spilled at D = 128; 143 and three waves otherwise):
-// 38.5 us in the place of 40.4 for 8,386 tokens of 28/4 heads.
+// 38.1 us in the place of 40.2 for 8,386 tokens of 28/4 heads.
 template <int D, int V, bool INTER, bool FP8, bool EACH, bool FAR>
 __global__ __launch_bounds__(kThreads, FP8 ? 4 : 1) void rotary_append_kernel(AppendArgs a) {
   constexpr int UNITS = D / (2 * V), LL = UNITS == 64 ? 6 : UNITS == 32 ? 5 : UNITS == 16 ? 4 : UNITS == 8 ? 3 : 2;
@@ -660,7 +665,7 @@ extern "C" int wkv_rotary_append(const wkv_cache_t *cache, const void *key, int6
   a.k_wgs = static_cast<int>(k_wgs);
   a.v_wgs = static_cast<int>(rest);
   const unsigned grid = static_cast<unsigned>(gq.wgs + k_wgs + rest);
-  // Rows far larger than the caches go past them (8 prompts of 2,048 tokens, 32/8 heads of 128: 82.3 us, 88.7
+  // Rows far larger than the caches go past them (8 prompts of 2,048 tokens, 32/8 heads of 128: 81 us, 88
   // near); the cache's keys and values stay, for the attention.
   const bool far = num_tokens * (num_q_heads + Hk) * D * 2 >= (64 << 20);
   auto s = static_cast<hipStream_t>(stream);

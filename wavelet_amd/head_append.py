@@ -74,8 +74,9 @@ def rotary_append(q: torch.Tensor | None, key: torch.Tensor, value: torch.Tensor
     takes the result and no ``key`` / ``value`` (``paged_decode_gqa``, ``prefill_gqa``, ``paged_tree_gqa``). ``key`` and
     ``value`` are left as they are, and the cache, bf16 or fp8, holds what ``norm_rotary`` and ``cache.append`` would
     leave in it, bit for bit where the key's rows start on 16-byte boundaries (elsewhere they are copied, and then, as
-    where ``apply_rotary`` goes first, a key's last bit may differ). A slot appears once in a call, a block of an fp8 cache in one run of it (as
-    for ``cache.append``).
+    where ``apply_rotary`` goes first, a key's last bit may differ). A slot appears once in a call, a block of an fp8
+    cache in one run of it (as for ``cache.append``). Long prompts into an fp8 cache (16,384 tokens of 8 key heads, or
+    blocks of 256) take less time as ``norm_rotary`` and ``cache.append``.
     """
     if not isinstance(cache, PagedKVCache):
         raise ValueError("cache must be a PagedKVCache (mla_rotary_append appends to latent caches)")
@@ -130,6 +131,8 @@ def mla_rotary_append(q_pe: torch.Tensor | None, kv_c: torch.Tensor, k_pe: torch
 
     bf16; the rotation as for ``apply_rotary``, the norm as ``norm_rotary``'s over a whole entry. The attention
     (``paged_decode_mla``) then takes the result as its ``q_pe`` and no ``kv_c`` / ``k_pe``. A slot appears once in a call.
+    A ``rope_dim`` above 128 needs rows of queries (and, unless ``interleaved``, pairs) in multiples of 2 elements, one
+    above 256 (itself a multiple of 16) in multiples of 8; others are refused.
     """
     if not isinstance(cache, MLALatentCache):
         raise ValueError("cache must be an MLALatentCache (rotary_append appends to key and value caches)")

@@ -253,7 +253,7 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     ``inv_freq`` (float64 ``[R / 2]``, ``R <= D``) and ``scale`` come from ``rotary_frequencies``: pair ``i``
     of a head is turned by ``positions[t] * inv_freq[i]`` and multiplied by ``scale``. A pair is dims ``(i,
     i + R / 2)``, or ``(2 i, 2 i + 1)`` if ``interleaved``; dims from ``R`` on stay as they are. Positions
-    may be any, in any order (a drafted tree's depths; far ones keep their exact angle). ``inverse``
+    may be any, in any order (a drafted tree's depths; far ones keep the angle that float64 gives). ``inverse``
     turns back (the transpose, also by ``scale``). With ``axes`` (int32 ``[R / 2]``, from ``rotary_axes``) the
     positions are int64 ``[A, T]`` and pair ``i`` is turned by those of axis ``axes[i]`` (a pair of an axis outside
     ``[0, A)`` by none). ``out``: the two results' tensors; ``out=(q, k)`` works in
