@@ -67,6 +67,42 @@ def test_the_axes_of_pairs():
     assert scale == 1.0 and torch.equal(freq, rotary_frequencies(16, 1e4, device="cpu")[0])
 
 
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("tokens,hq,hk,d,half,shift", [(37, 8, 2, 128, 64, 0), (5, 3, 1, 64, 10, 0), (130, 4, 2, 80, 13, 0),
+                                                       (300, 2, 0, 64, 32, 1), (4, 1, 3, 512, 255, 2)])
+def test_turn_heads(cuda, tokens, hq, hk, d, half, shift, dtype, inter):
+    """wkv_turn_heads, new rows and in place, and the inverse: the rotation of an append without a norm."""
+    from wavelet_amd import _lib
+    from wavelet_amd.rotary import rotation
+
+    lib = _lib.load()
+    _, _, _, _, pos, freq = _inputs(cuda, tokens, 1, 1, d, half, 3, dtype)
+    axes = (torch.arange(half, device=cuda) % 3).int()
+    x = torch.randn(tokens * (hq + hk) * d + shift, device=cuda).to(dtype)[shift:].view(tokens, hq + hk, d)
+    y, angle = torch.full_like(x, float("nan")), heads.phases(f64(pos), f64(freq), axes.cpu().numpy())
+
+    def rows(a, b):
+        args = []
+        for lo, n in ((0, hq), (hq, hk)):
+            for t in (a, b):
+                args += [t[:, lo:].data_ptr() if n else None, t.stride(0), t.stride(1)]
+            args.append(n)
+        return args
+
+    code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+    stream = torch.cuda.current_stream().cuda_stream
+    for way in (False, True):
+        how = rotation(pos, freq, axes, inter, 1.25, way)
+        _lib.check(lib.wkv_turn_heads(code, *rows(x, y), d, how, tokens, stream), "turn")
+        _check(y, x, -angle if way else angle, inter, 1.25)
+        z = x.clone()
+        _lib.check(lib.wkv_turn_heads(code, *rows(z, z), d, how, tokens, stream), "turn in place")
+        _check(z, x, -angle if way else angle, inter, 1.25)
+        # (fp16 at another alignment: a fused product and conversion rounds some values once, others twice)
+        assert dtype is torch.float16 or torch.equal(y, z)
+
+
 def test_refusals(cuda):
     q, k, _, _, pos, freq = _inputs(cuda, 6, 2, 1, 64, 32, 3, torch.bfloat16)
     axes = rotary_axes((12, 10, 10), device=cuda)
